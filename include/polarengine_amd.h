@@ -429,6 +429,97 @@ int pe_decode_attention(const void* qkv, const float* rope, const int64_t* pos, 
 int pe_lm_head_fits(int64_t M, int64_t N, int K);
 int pe_lm_head(const void* x, const void* w, int64_t M, int64_t N, int K, float* y, void* stream);
 
+/*
+ * A step with several drafted tokens per sequence (speculative decoding), around
+ * the quantized linears; no reference file. n nodes per sequence, 1 <= n <= 64:
+ * node 0 is the sequence's last token, node i > 0 a drafted token that follows
+ * node parents[i] < i. A node whose parent is no earlier existing node is absent
+ * (a padded place). Node i belongs in cache slot lengths[b] + i until the
+ * accepted ones are moved; lengths (int64, on the device) count the cached
+ * positions, and a sequence with lengths[b] < 0 or lengths[b] + n > cap is an
+ * empty slot of the batch. 16-bit tensors are PE_DTYPE_F16 or PE_DTYPE_BF16.
+ *
+ * Caches: element strides of batch, head, position and dimension. Values have
+ * the dimension contiguous; keys the dimension (ks_d = 1) or the position (ks_l
+ * = 1). Where the dimension is contiguous the pointer is 16-byte aligned and
+ * the other strides are multiples of 8.
+ *
+ *   pe_tree_plan: parents int64 [batch, n] (row stride parents_stride, 0: one
+ *       tree for every sequence) -> masks int64 [batch, n] (bit j: j is i or an
+ *       ancestor of i; 0 for absent nodes) and positions int64 [batch, n]
+ *       (lengths[b] + depth; -1 for absent nodes and lengths[b] < 0).
+ *   pe_qk_norm_rope: qkv [rows, (heads + 2 kv_heads) * head_dim], row stride ld
+ *       (a multiple of 8); queries and keys normed per head, x / sqrt(mean(x^2)
+ *       + eps) * weight (no norm where the weight is NULL), then the first rot
+ *       dimensions (a multiple of 16) rotated, pairs (j, j + rot / 2), by row
+ *       positions[row] of rope float32 [rope_rows, rot] (cos, then sin). fp32,
+ *       rounded once. q_out [rows, heads, head_dim], k_out [rows, kv_heads,
+ *       head_dim]; zero rows where positions[row] is outside the table.
+ *   pe_qk_norm_rope_write: the same for batch * n rows (n of any size), keys and
+ *       values written to slots lengths[b] + i of the caches instead; nothing is
+ *       written for a row whose position is outside the table or whose sequence
+ *       is an empty slot.
+ *   pe_tree_attention: out [batch, n, heads, head_dim] = softmax(scale q K^T) V
+ *       over the positions below lengths[b] and the slots lengths[b] + j of
+ *       masks[b][i]'s bits j < n (row stride m_b, 0: one for every sequence). A
+ *       row with nothing to attend to, and an empty slot's, is zero. q: strides
+ *       of batch and node, multiples of 8; heads and dimensions contiguous.
+ *       head_dim 64, 128 or 256.
+ *   pe_verify_drafts: logits [batch, n, vocab] (PE_DTYPE_F32 too; strides of
+ *       batch and node) of the target, tokens int64 [batch, n] (outside 0 ..
+ *       vocab - 1: absent; tokens[b][0] absent: an empty slot), parents as above
+ *       or NULL for a chain, uniforms float32 [batch, n] in [0, 1), temps
+ *       float32 [batch] or NULL for temp, and, for a chain, probs float32
+ *       [batch, n - 1, vocab], row i the distribution that node i + 1 was drawn
+ *       from (NULL: drafts without probabilities). With p = softmax(logits / T)
+ *       of a node (T <= 0 or NaN: all on the first largest logit; NaN logits
+ *       count as -inf) its children are tried in order of their number: child c
+ *       of token x is accepted if uniforms[c] * r < p(x), r what earlier
+ *       rejections left of p in all, and a rejection takes x from p; with probs q
+ *       if uniforms[c] * q(x) < p(x), and a rejection leaves max(p - q, 0).
+ *       Where no child is left the next token is the first v whose running sum of
+ *       what is left passes uniforms[0] of the whole (of p, where nothing is left;
+ *       -1 where p has no finite logit). count int64 [batch]: accepted nodes,
+ *       node 0 among them (0 for an empty slot); path int64 [batch, n]: those
+ *       nodes; out int64 [batch, n]: their tokens without node 0's, then the next
+ *       token; both -1 past count. Sums and comparisons in 64 bits.
+ *   pe_keep_accepted: slots lengths[b] + j of cache [layers, batch, heads, cap,
+ *       dim] take the rows of slots lengths[b] + path[b][j], j < count[b], in
+ *       place (16-bit values; strides as above, s_d = 1 or s_l = 1). Only an
+ *       ascending path within the n slots is followed.
+ */
+int pe_tree_plan(const int64_t* parents, int64_t parents_stride, const int64_t* lengths,
+                 int64_t batch, int n, int64_t* positions, int64_t* masks, void* stream);
+int pe_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t ld, int heads, int kv_heads,
+                    int head_dim, const float* rope, int64_t rope_rows, int rot,
+                    const int64_t* positions, const void* q_weight, const void* k_weight, float eps,
+                    void* q_out, void* k_out, void* stream);
+int pe_qk_norm_rope_write(const void* qkv, int dtype, int64_t batch, int64_t n, int64_t ld,
+                          int heads, int kv_heads, int head_dim, const float* rope,
+                          int64_t rope_rows, int rot, const int64_t* positions,
+                          const void* q_weight, const void* k_weight, float eps, void* q_out,
+                          void* k_cache, int64_t ks_b, int64_t ks_h, int64_t ks_l, int64_t ks_d,
+                          void* v_cache, int64_t vs_b, int64_t vs_h, int64_t vs_l,
+                          const int64_t* lengths, int64_t cap, void* stream);
+size_t pe_tree_attention_workspace_size(int64_t batch, int n, int heads, int kv_heads, int head_dim,
+                                        int64_t cap);
+int pe_tree_attention(const void* q, int dtype, int64_t q_b, int64_t q_n, const void* k_cache,
+                      int64_t ks_b, int64_t ks_h, int64_t ks_l, int64_t ks_d, const void* v_cache,
+                      int64_t vs_b, int64_t vs_h, int64_t vs_l, const int64_t* lengths,
+                      const int64_t* masks, int64_t m_b, void* out, int64_t batch, int n, int heads,
+                      int kv_heads, int head_dim, int64_t cap, float scale, void* workspace,
+                      size_t workspace_bytes, void* stream);
+size_t pe_verify_drafts_workspace_size(int64_t batch, int n, int64_t vocab);
+int pe_verify_drafts(const void* logits, int dtype, int64_t l_b, int64_t l_n, int64_t batch, int n,
+                     int64_t vocab, const int64_t* tokens, const int64_t* parents, int64_t p_b,
+                     const float* uniforms, const float* temps, float temp, const float* probs,
+                     int64_t q_b, int64_t q_n, int64_t* out, int64_t* path, int64_t* count,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int64_t cap, int dim,
+                     int64_t s_layer, int64_t s_b, int64_t s_h, int64_t s_l, int64_t s_d,
+                     const int64_t* lengths, const int64_t* path, const int64_t* count, int n,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

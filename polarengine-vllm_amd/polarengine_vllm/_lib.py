@@ -30,6 +30,7 @@ PE_DTYPE_F16, PE_DTYPE_BF16, PE_DTYPE_F32 = 0, 1, 2
 PE_XTF_F32, PE_XTF_F16, PE_XTF_PAIR_F16, PE_XTF_BF16 = 0, 1, 2, 3
 
 _c_int, _c_i64, _c_sz, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+_c_float = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/polarengine_amd.h
 _SIGNATURES = {
@@ -85,6 +86,23 @@ _SIGNATURES = {
                                      _c_i64, ctypes.c_float, _vp, _c_sz, _vp]),
     "pe_lm_head_fits": (_c_int, [_c_i64, _c_i64, _c_int]),
     "pe_lm_head": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_int, _vp, _vp]),
+    "pe_tree_plan": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_int, _vp, _vp, _vp]),
+    "pe_qk_norm_rope": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _vp, _c_i64,
+                                 _c_int, _vp, _vp, _vp, _c_float, _vp, _vp, _vp]),
+    "pe_qk_norm_rope_write": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_int,
+                                       _vp, _c_i64, _c_int, _vp, _vp, _vp, _c_float, _vp,
+                                       _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                       _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp]),
+    "pe_tree_attention_workspace_size": (_c_sz, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64]),
+    "pe_tree_attention": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                   _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _c_int,
+                                   _c_int, _c_int, _c_int, _c_i64, _c_float, _vp, _c_sz, _vp]),
+    "pe_verify_drafts_workspace_size": (_c_sz, [_c_i64, _c_int, _c_i64]),
+    "pe_verify_drafts": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _vp, _vp,
+                                  _c_i64, _vp, _vp, _c_float, _vp, _c_i64, _c_i64, _vp, _vp, _vp,
+                                  _vp, _c_sz, _vp]),
+    "pe_keep_accepted": (_c_int, [_vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_i64, _c_i64, _c_i64,
+                                  _c_i64, _c_i64, _vp, _vp, _vp, _c_int, _vp]),
 }
 
 # measurement helpers (include/polarengine_amd_bench.h)
