@@ -7,6 +7,8 @@ namespace pe {
 
 constexpr int kTreeMax = 64;  // nodes of a tree: one bit each of a 64-bit mask, one lane each
 
+constexpr int64_t kTreeMaxStride = (int64_t)1 << 26;  // elements, of positions and dimensions
+
 // Ancestor mask (itself among them) of node i = lane of a wave, from its parent:
 // node 0 is the root, whatever its parent says; node i > 0 exists if 0 <= parent
 // < i and the parent exists, else its mask is 0. All 64 lanes call. Pointer
@@ -31,6 +33,8 @@ inline int cache_strides(const void* k, int64_t ks_b, int64_t ks_h, int64_t ks_l
   if (ks_b < 0 || ks_h < 0 || ks_l < 0 || ks_d < 0 || vs_b < 0 || vs_h < 0 || vs_l < 0)
     return PE_ERR_DIMS;
   if (ks_d != 1 && ks_l != 1) return PE_ERR_DIMS;
+  // a workgroup's rows lie within 32-bit byte offsets of one another
+  if (ks_l >= kTreeMaxStride || ks_d >= kTreeMaxStride || vs_l >= kTreeMaxStride) return PE_ERR_DIMS;
   if (!aligned16(v) || (vs_b | vs_h | vs_l) % 8) return PE_ERR_ALIGN;
   if (ks_d == 1 && (!aligned16(k) || (ks_b | ks_h | ks_l) % 8)) return PE_ERR_ALIGN;
   return PE_OK;

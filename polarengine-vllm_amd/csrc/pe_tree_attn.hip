@@ -6,7 +6,8 @@
 // cores together, so a key or value is read from memory once for all of them.
 // A workgroup of four waves takes RB = 16 RT WR rows and a run of tiles of 64
 // positions:
-//  * a tile of keys and values is staged in LDS, the next one in registers;
+//  * tiles of keys and values go straight to LDS, two buffers, the next tile under
+//    way while one is worked on, one barrier a tile;
 //  * scores S^T = K Q^T (v_mfma_f32_16x16x32, keys as A, so a lane holds four
 //    keys of one row and the row's maximum needs two exchanges), Q in registers;
 //  * one pass with running maximum and sum in fp32; the probabilities, rounded to
@@ -19,6 +20,8 @@
 // keys (few rows): those join their sums in LDS at the end.
 // Tiles are divided over workgroups by the lengths, read on the device; a second
 // launch joins the parts of a sequence.
+
+#include <type_traits>
 
 #include "pe_tree.h"
 
@@ -98,11 +101,15 @@ __device__ __forceinline__ float4v mfma16(u32x2v a, u32x2v b, float4v c) {
 }
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
+typedef __attribute__((address_space(1))) const unsigned char glb_byte;
 __device__ __forceinline__ u32x2v lds_tr(const lds_byte* p) {
   return __builtin_bit_cast(u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
 }
 __device__ __forceinline__ u32x4v lds_ld16(const lds_byte* p) {
   return *reinterpret_cast<const __attribute__((address_space(3))) u32x4v*>(p);
+}
+__device__ __forceinline__ void lds_st16v(lds_byte* p, u32x4v v) {
+  *reinterpret_cast<__attribute__((address_space(3))) u32x4v*>(p) = v;
 }
 // whether one of the eight 16-bit values is infinite or NaN
 template <bool BF>
@@ -116,7 +123,8 @@ __device__ __forceinline__ bool not_finite8(u32x4v u) {
 }
 
 template <int D, bool BF, bool KCOL, int RT, int WR>
-__global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) void tree_attn_kernel(
+    const TreeAttnArgs a) {
   constexpr int WK = 4 / WR;         // waves that share the rows and differ in keys
   constexpr int RB = 16 * RT * WR;   // rows of the workgroup
   constexpr int NKT = 4 / WK;        // 16-key blocks of a wave in a tile
@@ -125,10 +133,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
   constexpr int NCH = D / 32;        // 16-byte chunks of a tile per thread
   constexpr int CPR = D / 8;         // chunks of a row
   constexpr int KPI = 256 / CPR;     // rows per pass of the workgroup
-  __shared__ __align__(16) unsigned char smem[2 * kTile * ROW];
+  constexpr int VT = kTile * ROW;    // a buffer: keys, then values
+  // two objects, so that the compiler knows that a tile on its way into one is not
+  // what is read from the other
+  __shared__ __align__(16) unsigned char buf0[2 * VT];
+  __shared__ __align__(16) unsigned char buf1[2 * VT];
   __shared__ float mx[4][16 * RT], lx[4][16 * RT];
-  lds_byte* const kt_lds = (lds_byte*)smem;
-  lds_byte* const vt_lds = kt_lds + kTile * ROW;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -172,66 +182,54 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
   const uint16_t* kb = a.k + (int64_t)b * a.ks_b + kvh * a.ks_h;
   const uint16_t* vb = a.v + (int64_t)b * a.vs_b + kvh * a.vs_h;
 
-  // staging: chunk c = tid + 256 i; by position: row c / CPR, chunk c % CPR; keys by
-  // dimension: dimension c / 8, eight positions c % 8
-  const int srow = tid / CPR, sch = tid % CPR;
-  const uint16_t* vp = vb + srow * a.vs_l + sch * 8;
-  const uint16_t* kp = KCOL ? kb + (tid >> 3) * a.ks_d + (tid & 7) * 8 : kb + srow * a.ks_l + sch * 8;
-  u32x4v kr[NCH], vr[NCH];
-  auto load_tile = [&](int t) {
-    const int64_t p0 = (int64_t)t * kTile;
-    if (p0 + kTile <= end) {
-#pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        if constexpr (KCOL)
-          __builtin_memcpy(&kr[i], kp + i * 32 * a.ks_d + p0, 16);
-        else
-          kr[i] = *reinterpret_cast<const u32x4v*>(kp + (p0 + i * KPI) * a.ks_l);
-        vr[i] = *reinterpret_cast<const u32x4v*>(vp + (p0 + i * KPI) * a.vs_l);
-      }
-      return;
-    }
-    // the last tile: rows from `end` on are not read; values there are zeros
-    const int left = (int)(end - p0);
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int row = srow + i * KPI;
-      vr[i] = u32x4v{0, 0, 0, 0};
-      if (row < left) vr[i] = *reinterpret_cast<const u32x4v*>(vp + (p0 + i * KPI) * a.vs_l);
-      if constexpr (KCOL) {
-        const uint16_t* s = kp + i * 32 * a.ks_d + p0;
-        const int here = left - (tid & 7) * 8;  // positions of this chunk before `end`
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < here) w[e / 2] |= (uint32_t)s[e] << (16 * (e & 1));
-        kr[i] = u32x4v{w[0], w[1], w[2], w[3]};
-      } else {
-        kr[i] = u32x4v{0, 0, 0, 0};
-        if (row < left) kr[i] = *reinterpret_cast<const u32x4v*>(kp + (p0 + i * KPI) * a.ks_l);
-      }
-    }
-  };
-  // LDS places: chunks are permuted within rows so that the reads below, 16 bytes of
-  // 16 rows or 32 bytes of 8 rows at a time, touch every bank once
+  // Staging, straight into LDS: pass i of thread tid fills chunk tid + 256 i of a
+  // tile, row c / CPR. Chunks are permuted within rows (by the source address) so
+  // that the reads below, 16 bytes of 16 rows or 32 bytes of 8 rows at a time, touch
+  // every bank once; the permutations are linear in the bits of the row, so pass i
+  // adds a constant. Addresses are a uniform 64-bit base and the thread's 32-bit
+  // offset (strides below 2^26). Rows from `end` on repeat the last one. Keys by
+  // dimension have any alignment and go through registers: chunk c is dimension
+  // c / 8, eight positions c % 8.
   auto k_swz = [](int key) { return D == 64 ? key >> 1 & 7 : key & 15; };
   auto v_swz = [](int key) { return D == 64 ? key >> 1 & 3 : key & 7; };
   auto kc_swz = [](int d) { return (d >> 1 & 1) | (d >> 3 & 1) << 1; };
-  auto store_tile = [&]() {
+  const int srow = tid / CPR, sch = tid % CPR;
+  const int vch = ((sch >> 1 ^ v_swz(srow)) << 1 | (sch & 1)) * 16, kch = (sch ^ k_swz(srow)) * 16;
+  const int kst = (tid >> 3) * 128 + ((((tid & 7) >> 1) ^ kc_swz(tid >> 3)) << 5) + (tid & 1) * 16;
+  u32x4v kr[KCOL ? NCH : 1];
+  auto issue = [&](lds_byte* to, int t) {
+    const int64_t p0 = (int64_t)t * kTile;
+    const bool whole = p0 + kTile <= end;
+    const int left = whole ? kTile : (int)(end - p0);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int row = srow + i * KPI;
-      lds_byte* vd = vt_lds + row * ROW + ((sch >> 1 ^ v_swz(row)) << 5) + (sch & 1) * 16;
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4v*>(vd) = vr[i];
-      lds_byte* kd;
-      if constexpr (KCOL) {
-        const int d = (tid >> 3) + 32 * i, c = tid & 7;
-        kd = kt_lds + d * 128 + ((c >> 1 ^ kc_swz(d)) << 5) + (c & 1) * 16;
+      const int row = whole ? srow : min(srow + i * KPI, left - 1) - i * KPI;
+      const char* v = reinterpret_cast<const char*>(vb + (p0 + i * KPI) * a.vs_l) +
+                      ((int64_t)row * (int)a.vs_l * 2 + (vch ^ v_swz(i * KPI) << 5));
+      __builtin_amdgcn_global_load_lds((const glb_byte*)v, to + VT + (i * 4 + wave) * 1024, 16, 0, 0);
+      if constexpr (!KCOL) {
+        const char* k = reinterpret_cast<const char*>(kb + (p0 + i * KPI) * a.ks_l) +
+                        ((int64_t)row * (int)a.ks_l * 2 + (kch ^ k_swz(i * KPI) << 4));
+        __builtin_amdgcn_global_load_lds((const glb_byte*)k, to + (i * 4 + wave) * 1024, 16, 0, 0);
       } else {
-        kd = kt_lds + row * ROW + ((sch ^ k_swz(row)) << 4);
+        const char* k = reinterpret_cast<const char*>(kb + i * 32 * a.ks_d + p0) +
+                        ((uint32_t)(tid >> 3) * (uint32_t)a.ks_d * 2u + (tid & 7) * 16);
+        if (whole) {
+          __builtin_memcpy(&kr[i], k, 16);
+        } else {
+          kr[i] = u32x4v{0, 0, 0, 0};
+          const uint16_t* s = reinterpret_cast<const uint16_t*>(k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((tid & 7) * 8 + e < left) kr[i][e / 2] |= (uint32_t)s[e] << (16 * (e & 1));
+        }
       }
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4v*>(kd) = kr[i];
     }
+  };
+  auto store_k = [&](lds_byte* to) {
+    if constexpr (KCOL)
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) lds_st16v(to + kst + i * 32 * 128, kr[i]);
   };
 
   // Q fragments (B operand: lane = row li, dimensions 32 ks + 8 lg ..) and the
@@ -239,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
   u32x4v qf[RT][KS];
   uint64_t mask[RT];
   const uint64_t all = a.n == 64 ? ~0ull : (1ull << a.n) - 1;
-  if (t0 < t1) load_tile(t0);
+  if (t0 < t1) issue((lds_byte*)buf0, t0);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = rblk * RB + (wr * RT + rt) * 16 + li;
@@ -263,33 +261,35 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
   }
   const float c = a.scale * kTreeLog2e;
-  // the lane's bases in the tiles
+  // the lane's places in a buffer
   const int kfirst = wk * (kTile / WK);  // the wave's first key
-  const lds_byte* kl = KCOL ? kt_lds + (8 * lg + (li >> 2)) * 128 + (li & 3) * 8
-                            : kt_lds + (kfirst + li) * ROW;
+  const int kat = KCOL ? (8 * lg + (li >> 2)) * 128 + (li & 3) * 8 : (kfirst + li) * ROW;
   const int kx = KCOL ? kc_swz(8 * lg + (li >> 2)) : k_swz(li);
   const int vrow = 4 * lg + (li >> 2);
-  const lds_byte* vl = vt_lds + (kfirst + vrow) * ROW + (li & 3) * 8;
+  const int vat = VT + (kfirst + vrow) * ROW + (li & 3) * 8;
   const int vx = v_swz(vrow);
 
-  for (int t = t0; t < t1; ++t) {
+  // one tile from `cur`, the next on its way to `nxt`
+  auto step = [&](lds_byte* __restrict__ cur, lds_byte* __restrict__ nxt, int t, auto tail_) {
+    constexpr bool kTail = decltype(tail_)::value;  // holds drafted tokens, or the end
     const int64_t p0 = (int64_t)t * kTile;
-    const bool tail = p0 + kTile > len;
-    __syncthreads();  // the tile before is done with
-    store_tile();
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the tile is in LDS
+    __syncthreads();                // everybody's is, and `nxt` is done with
     bool slow = false;
-    if (!tail) {
-      __syncthreads();
-    } else {
-      // a drafted token's value that is infinite or NaN must not reach, as 0 x inf,
-      // the rows that do not see it
+    if constexpr (kTail) {
+      // Rows from `end` on become zeros. A drafted token's value that is infinite or
+      // NaN must not reach, as 0 x inf, the rows that do not see it.
       bool bad = false;
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
-        bad |= p0 + srow + i * KPI >= len && not_finite8<BF>(vr[i]);
+      for (int i = 0; i < NCH; ++i) {
+        lds_byte* at = cur + VT + (i * 256 + tid) * 16;
+        const int64_t pos = p0 + srow + i * KPI;
+        if (pos >= end) lds_st16v(at, u32x4v{0, 0, 0, 0});
+        else if (pos >= len) bad |= not_finite8<BF>(lds_ld16(at));
+      }
       slow = __syncthreads_or(bad);
     }
-    if (t + 1 < t1) load_tile(t + 1);
+    if (t + 1 < t1) issue(nxt, t + 1);
 
     float4v s[NKT][RT];
 #pragma unroll
@@ -300,11 +300,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
       for (int ks = 0; ks < KS; ++ks) {
         u32x4v kf;
         if constexpr (KCOL) {
-          const lds_byte* p = kl + ks * 32 * 128 + ((wk * NKT + kt ^ kx) << 5);
+          const lds_byte* p = cur + kat + ks * 32 * 128 + ((wk * NKT + kt ^ kx) << 5);
           const u32x2v lo = lds_tr(p), hi = lds_tr(p + 4 * 128);
           kf = u32x4v{lo[0], lo[1], hi[0], hi[1]};
         } else {
-          kf = lds_ld16(kl + kt * 16 * ROW + ((4 * ks + lg ^ kx) << 4));
+          kf = lds_ld16(cur + kat + kt * 16 * ROW + ((4 * ks + lg ^ kx) << 4));
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[kt][rt] = mfma32<BF>(kf, qf[rt][ks], s[kt][rt]);
@@ -314,18 +314,23 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
     u32x2v pf[NKT][RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+      if constexpr (kTail) {
+        const int r0 = (int)(p0 - len) + kfirst + 4 * lg;  // above -64
+#pragma unroll
+        for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int rel = r0 + 16 * kt + e;
+            if (rel >= 0 && (rel >= 64 || !(mask[rt] >> rel & 1))) s[kt][rt][e] = -__builtin_inff();
+          }
+      }
       float top = -__builtin_inff();
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = s[kt][rt][e] * c;
-          if (tail) {
-            const int64_t rel = p0 - len + kfirst + 16 * kt + 4 * lg + e;
-            if (rel >= 0 && (rel >= 64 || !(mask[rt] >> rel & 1))) x = -__builtin_inff();
-          }
-          s[kt][rt][e] = x;
-          top = fmaxf(top, x);
+          s[kt][rt][e] = kTail && s[kt][rt][e] == -__builtin_inff() ? s[kt][rt][e] : s[kt][rt][e] * c;
+          top = fmaxf(top, s[kt][rt][e]);
         }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -349,10 +354,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
         pf[kt][rt] = u32x2v{pack16x2(p[0], p[1], BF), pack16x2(p[2], p[3], BF)};
       }
     }
-    if (__builtin_expect(!slow, 1)) {
+    if (!kTail || !slow) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const lds_byte* p = vl + ((dt ^ vx) << 5);
+        const lds_byte* p = cur + vat + ((dt ^ vx) << 5);
         if constexpr (NKT == 1) {
           const u32x2v vf = lds_tr(p);
 #pragma unroll
@@ -370,32 +375,53 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
         }
       }
     } else {
-      // key by key, skipping what a row does not see
+      // key by key, skipping what a row does not see; the probabilities take the
+      // place of the keys, 64-lane words of one 16-key block after the other
+      __syncthreads();
+      lds_byte* const pw = cur + wave * (NKT * 512);
 #pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-        for (int key = 0; key < 16; ++key) {
-          const int at = kfirst + 16 * kt + key;
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int kt = 0; kt < NKT; ++kt)
+          *reinterpret_cast<lds_u32x2*>(pw + (kt * 64 + lane) * 8) = pf[kt][rt];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int key = 0; key < 16 * NKT; ++key) {
+          const int at = kfirst + key;
           const int64_t rel = p0 - len + at;
+          const float p = f16or_bf(*reinterpret_cast<const lds_u16*>(
+              pw + ((key >> 4) * 64 + (key >> 2 & 3) * 16 + li) * 8 + (key & 3) * 2), BF);
+          if (rel < 0 || (rel < 64 && (mask[rt] >> rel & 1))) {
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const uint32_t two = (key & 2) ? pf[kt][rt][1] : pf[kt][rt][0];
-            const uint32_t got = __shfl(two, li | (key >> 2) << 4, 64);
-            const float p = f16or_bf((uint16_t)((key & 1) ? got >> 16 : got & 0xffff), BF);
-            if (rel < 0 || (rel < 64 && (mask[rt] >> rel & 1))) {
+            for (int dt = 0; dt < DT; ++dt) {
+              const u32x2v w = *reinterpret_cast<const lds_u32x2*>(
+                  cur + VT + at * ROW + ((dt ^ v_swz(at)) << 5) + lg * 8);
 #pragma unroll
-              for (int dt = 0; dt < DT; ++dt) {
-                const u32x2v w = *reinterpret_cast<const lds_u32x2*>(
-                    vt_lds + at * ROW + ((dt ^ v_swz(at)) << 5) + lg * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  o[rt][dt][e] = __builtin_fmaf(
-                      p, f16or_bf((uint16_t)(w[e / 2] >> (16 * (e & 1))), BF), o[rt][dt][e]);
-              }
+              for (int e = 0; e < 4; ++e)
+                o[rt][dt][e] = __builtin_fmaf(
+                    p, f16or_bf((uint16_t)(w[e / 2] >> (16 * (e & 1))), BF), o[rt][dt][e]);
             }
           }
         }
+        __builtin_amdgcn_wave_barrier();
+      }
     }
+    if (t + 1 < t1) store_k(nxt);
+  };
+  if (t0 < t1) store_k((lds_byte*)buf0);
+  const int full = min(t1, (int)(len / kTile));  // tiles before it hold cached positions alone
+  int t = t0;
+  for (; t + 1 < full; t += 2) {
+    step((lds_byte*)buf0, (lds_byte*)buf1, t, std::false_type{});
+    step((lds_byte*)buf1, (lds_byte*)buf0, t + 1, std::false_type{});
   }
+  bool odd = false;
+  if (t < full) {
+    step((lds_byte*)buf0, (lds_byte*)buf1, t++, std::false_type{});
+    odd = true;
+  }
+  for (; t < t1; ++t, odd = !odd)
+    step((lds_byte*)(odd ? buf1 : buf0), (lds_byte*)(odd ? buf0 : buf1), t, std::true_type{});
 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -407,7 +433,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(const TreeAttnArgs a)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) mx[wave][rt * 16 + li] = m[rt];
     __syncthreads();
-    float4v* buf = reinterpret_cast<float4v*>(smem);
+    float4v* buf = reinterpret_cast<float4v*>(buf0);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float top = mx[wr * WK][rt * 16 + li];
@@ -514,7 +540,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, in
 }
 
 // rows of a workgroup: as many as the rows of a KV head fill
-static int tree_rows(int rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : 128; }
+static int tree_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 struct TreePlanHost {
   int rb, blocks;
@@ -550,7 +576,8 @@ static void launch_main(const TreePlanHost& p, const TreeAttnArgs& a, hipStream_
   const unsigned grid = (unsigned)((p.units + 7) / 8 * 8 * p.blocks);
   switch (p.rb) {
     case 16: tree_attn_kernel<D, BF, KCOL, 1, 1><<<grid, 256, 0, st>>>(a); break;
-    case 64: tree_attn_kernel<D, BF, KCOL, 2, 2><<<grid, 256, 0, st>>>(a); break;
+    case 32: tree_attn_kernel<D, BF, KCOL, 1, 2><<<grid, 256, 0, st>>>(a); break;
+    case 64: tree_attn_kernel<D, BF, KCOL, 1, 4><<<grid, 256, 0, st>>>(a); break;
     default: tree_attn_kernel<D, BF, KCOL, 2, 4><<<grid, 256, 0, st>>>(a); break;
   }
 }
