@@ -18,18 +18,18 @@
 //    row i / 4 and gets column i of the 4 x 16 block.
 // WR waves share a tile's keys and differ in their rows, 4 / WR differ in their
 // keys (few rows): those join their sums in LDS at the end.
-// Tiles are divided over workgroups by the lengths, read on the device; a second
-// launch joins the parts of a sequence.
+// The tiles of all sequences and KV heads form one line, cut into equal runs, one a
+// workgroup, by the lengths read on the device; a second launch joins the parts of a
+// sequence that a cut divides.
 
 #include <type_traits>
+
 
 #include "pe_tree.h"
 
 namespace pe {
 
 constexpr int kTile = 64;          // positions of a tile
-constexpr int kTreeTarget = 512;   // workgroups wanted
-constexpr int kTreeMinTiles = 2;   // least tiles of a part
 constexpr float kTreeLog2e = 1.4426950408889634f;
 
 struct TreeAttnArgs {
@@ -44,17 +44,17 @@ struct TreeAttnArgs {
   int blocks;                           // row blocks of one KV head
   int64_t cap;
   float scale;
-  float* parts;  // null: no sequence is divided
+  int runs;      // workgroups of one row block
+  float* parts;  // [runs][blocks][2]: a run divides at most its first and its last sequence
 };
 
 // fp32 words of one part: RB x D sums, RB maxima, RB sums
 __host__ __device__ inline int64_t part_words(int rb, int dim) { return (int64_t)rb * (dim + 2); }
 
 // ---------------------------------------------------------------------------
-// Division of the tiles, from the lengths alone, so that both launches and every
-// workgroup arrive at the same one. A sequence of t tiles is cut into ceil(t / C)
-// equal parts, C such that all parts together give about kTreeTarget workgroups;
-// a unit is one part of one KV head. Every wave does this for itself.
+// The line of tiles: sequence after sequence, within one KV head after KV head.
+// An empty slot of the batch has one tile, without positions, for its zeros. Both
+// launches and every wave find their way by themselves, from the lengths alone.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int wave_sum_i32(int v) {
 #pragma unroll
@@ -65,17 +65,41 @@ __device__ __forceinline__ bool tree_active(const TreeAttnArgs& a, int64_t len) 
   return len >= 0 && len <= a.cap - a.n;
 }
 __device__ __forceinline__ int tree_tiles(const TreeAttnArgs& a, int b) {
-  const int64_t len = b < a.batch ? a.lengths[b] : -1;
-  return tree_active(a, len) ? (int)((len + a.n + kTile - 1) / kTile) : 0;
+  if (b >= a.batch) return 0;
+  const int64_t len = a.lengths[b];
+  return tree_active(a, len) ? (int)((len + a.n + kTile - 1) / kTile) : 1;
 }
-__device__ __forceinline__ int tree_part_tiles(const TreeAttnArgs& a, int lane) {
+// tiles before sequence `upto`, one KV head of each (lanes take sequences)
+__device__ __forceinline__ int tree_tiles_before(const TreeAttnArgs& a, int upto, int lane) {
   int total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) total += tree_tiles(a, b0 + lane);
-  total = wave_sum_i32(total) * a.kv_heads * a.blocks;
-  return max(kTreeMinTiles, (total + kTreeTarget - 1) / kTreeTarget);
+  for (int b = lane; b < upto; b += 64) total += tree_tiles(a, b);
+  return wave_sum_i32(total);
 }
-__device__ __forceinline__ int tree_parts(int tiles, int part) {
-  return tiles > part ? (tiles + part - 1) / part : 1;
+// the sequence that holds place `at` of the line, and the tiles before it
+struct TreePlace {
+  int b, tiles, before;
+};
+__device__ __forceinline__ TreePlace tree_find(const TreeAttnArgs& a, int at, int lane) {
+  TreePlace p{-1, 0, 0};
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int t = tree_tiles(a, b0 + lane);
+    int scan = t;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(scan, off, 64);
+      if (lane >= off) scan += o;
+    }
+    const uint64_t hit = __ballot((p.before + scan) * a.kv_heads > at);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      p.b = b0 + l;
+      p.before += __builtin_amdgcn_readlane(scan - t, l);
+      p.tiles = __builtin_amdgcn_readlane(t, l);
+      return p;
+    }
+    p.before += __builtin_amdgcn_readlane(scan, 63);
+  }
+  return p;
 }
 
 // MFMA and conversions of the 16-bit type
@@ -123,7 +147,7 @@ __device__ __forceinline__ bool not_finite8(u32x4v u) {
 }
 
 template <int D, bool BF, bool KCOL, int RT, int WR>
-__global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) void tree_attn_kernel(
+__global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) void tree_attn_kernel(
     const TreeAttnArgs a) {
   constexpr int WK = 4 / WR;         // waves that share the rows and differ in keys
   constexpr int RB = 16 * RT * WR;   // rows of the workgroup
@@ -140,45 +164,31 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
   __shared__ __align__(16) unsigned char buf1[2 * VT];
   __shared__ float mx[4][16 * RT], lx[4][16 * RT];
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave / WK, wk = wave % WK;
-  const int li = lane & 15, lg = lane >> 4;
 
-  // this workgroup's unit; the row blocks of a unit sit 8 apart, on one XCD
+  // this workgroup's run; the row blocks of a run sit 8 apart, on one XCD
   const int span = 8 * a.blocks;
   const int rem = (int)blockIdx.x % span;
-  const int unit = (int)blockIdx.x / span * 8 + rem % 8;
+  const int run = (int)blockIdx.x / span * 8 + rem % 8;
   const int rblk = rem / 8;
-  const int part = tree_part_tiles(a, lane);
-  int first = 0, b = -1, tiles = 0, parts = 1;  // units before b
-  for (int b0 = 0; b0 < a.batch && b < 0; b0 += 64) {
-    const int t = tree_tiles(a, b0 + lane);
-    const int p = tree_parts(t, part);
-    const int u = b0 + lane < a.batch ? p * a.kv_heads : 0;
-    int scan = u;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(scan, off, 64);
-      if (lane >= off) scan += o;
-    }
-    const uint64_t hit = __ballot(unit < first + scan);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      b = b0 + l;
-      first += __builtin_amdgcn_readlane(scan - u, l);
-      tiles = __builtin_amdgcn_readlane(t, l);
-      parts = __builtin_amdgcn_readlane(p, l);
-    } else {
-      first += __builtin_amdgcn_readlane(scan, 63);
-    }
-  }
-  if (b < 0) return;
-  const int kvh = (unit - first) % a.kv_heads, piece = (unit - first) / a.kv_heads;
-  const int per = (tiles + parts - 1) / parts;
-  const int t0 = piece * per, t1 = min(tiles, t0 + per);
-
-  const int64_t len = tiles ? a.lengths[b] : 0, end = len + a.n;
+  const int total = tree_tiles_before(a, a.batch, threadIdx.x & 63) * a.kv_heads;
+  const int size = (total + a.runs - 1) / a.runs;
+  const int line_end = min(total, (run + 1) * size);
+  for (int at = run * size; at < line_end;) {
+  int tid = threadIdx.x;
+  // what follows from the lane is worked out anew for each sequence: kept across
+  // them it would not leave registers enough for the tiles
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const TreePlace place = tree_find(a, at, lane);
+  const int b = place.b, tiles = place.tiles;
+  const int kvh = (at - place.before * a.kv_heads) / tiles;
+  const int t0 = at - place.before * a.kv_heads - kvh * tiles;
+  const int t1 = min(tiles, t0 + line_end - at);
+  at += t1 - t0;
+  const bool live = tree_active(a, a.lengths[b]);
+  const int64_t len = live ? a.lengths[b] : 0, end = len + a.n;
   const uint16_t* kb = a.k + (int64_t)b * a.ks_b + kvh * a.ks_h;
   const uint16_t* vb = a.v + (int64_t)b * a.vs_b + kvh * a.vs_h;
 
@@ -196,33 +206,43 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
   const int srow = tid / CPR, sch = tid % CPR;
   const int vch = ((sch >> 1 ^ v_swz(srow)) << 1 | (sch & 1)) * 16, kch = (sch ^ k_swz(srow)) * 16;
   const int kst = (tid >> 3) * 128 + ((((tid & 7) >> 1) ^ kc_swz(tid >> 3)) << 5) + (tid & 1) * 16;
+  const uint32_t voff = (uint32_t)srow * (uint32_t)a.vs_l * 2u + vch;
+  const uint32_t koff = KCOL ? (uint32_t)(tid >> 3) * (uint32_t)a.ks_d * 2u + (tid & 7) * 16
+                             : (uint32_t)srow * (uint32_t)a.ks_l * 2u + kch;
+  const uint32_t koff1 = koff - kch + (kch ^ k_swz(KPI) << 4);  // of odd passes
   u32x4v kr[KCOL ? NCH : 1];
   auto issue = [&](lds_byte* to, int t) {
     const int64_t p0 = (int64_t)t * kTile;
-    const bool whole = p0 + kTile <= end;
-    const int left = whole ? kTile : (int)(end - p0);
+    auto v_base = [&](int i) { return reinterpret_cast<const char*>(vb + (p0 + i * KPI) * a.vs_l); };
+    auto k_base = [&](int i) {
+      return reinterpret_cast<const char*>(kb + (KCOL ? i * 32 * a.ks_d + p0 : (p0 + i * KPI) * a.ks_l));
+    };
+    auto dma = [&](const char* from, int i, int plane) {
+      __builtin_amdgcn_global_load_lds((const glb_byte*)from, to + plane + (i * 4 + wave) * 1024, 16,
+                                       0, 0);
+    };
+    if (p0 + kTile <= end) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        if constexpr (KCOL) __builtin_memcpy(&kr[i], k_base(i) + koff, 16);
+        else dma(k_base(i) + (i & 1 ? koff1 : koff), i, 0);
+        dma(v_base(i) + voff, i, VT);
+      }
+      return;
+    }
+    const int left = (int)(end - p0);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int row = whole ? srow : min(srow + i * KPI, left - 1) - i * KPI;
-      const char* v = reinterpret_cast<const char*>(vb + (p0 + i * KPI) * a.vs_l) +
-                      ((int64_t)row * (int)a.vs_l * 2 + (vch ^ v_swz(i * KPI) << 5));
-      __builtin_amdgcn_global_load_lds((const glb_byte*)v, to + VT + (i * 4 + wave) * 1024, 16, 0, 0);
-      if constexpr (!KCOL) {
-        const char* k = reinterpret_cast<const char*>(kb + (p0 + i * KPI) * a.ks_l) +
-                        ((int64_t)row * (int)a.ks_l * 2 + (kch ^ k_swz(i * KPI) << 4));
-        __builtin_amdgcn_global_load_lds((const glb_byte*)k, to + (i * 4 + wave) * 1024, 16, 0, 0);
-      } else {
-        const char* k = reinterpret_cast<const char*>(kb + i * 32 * a.ks_d + p0) +
-                        ((uint32_t)(tid >> 3) * (uint32_t)a.ks_d * 2u + (tid & 7) * 16);
-        if (whole) {
-          __builtin_memcpy(&kr[i], k, 16);
-        } else {
-          kr[i] = u32x4v{0, 0, 0, 0};
-          const uint16_t* s = reinterpret_cast<const uint16_t*>(k);
+      const int row = min(srow + i * KPI, left - 1) - i * KPI;  // may lie before the pass
+      dma(v_base(i) + ((int64_t)row * (int)a.vs_l * 2 + vch), i, VT);
+      if constexpr (KCOL) {
+        kr[i] = u32x4v{0, 0, 0, 0};
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(k_base(i) + koff);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if ((tid & 7) * 8 + e < left) kr[i][e / 2] |= (uint32_t)s[e] << (16 * (e & 1));
-        }
+        for (int e = 0; e < 8; ++e)
+          if ((tid & 7) * 8 + e < left) kr[i][e / 2] |= (uint32_t)s[e] << (16 * (e & 1));
+      } else {
+        dma(k_base(i) + ((int64_t)row * (int)a.ks_l * 2 + (kch ^ k_swz(i * KPI) << 4)), i, 0);
       }
     }
   };
@@ -237,7 +257,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
   u32x4v qf[RT][KS];
   uint64_t mask[RT];
   const uint64_t all = a.n == 64 ? ~0ull : (1ull << a.n) - 1;
-  if (t0 < t1) issue((lds_byte*)buf0, t0);
+  if (live) issue((lds_byte*)buf0, t0);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = rblk * RB + (wr * RT + rt) * 16 + li;
@@ -260,7 +280,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
   }
-  const float c = a.scale * kTreeLog2e;
+  const float c = fmaxf(a.scale * kTreeLog2e, 1e-30f);  // above 0: a masked -inf stays one
   // the lane's places in a buffer
   const int kfirst = wk * (kTile / WK);  // the wave's first key
   const int kat = KCOL ? (8 * lg + (li >> 2)) * 128 + (li & 3) * 8 : (kfirst + li) * ROW;
@@ -304,7 +324,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
           const u32x2v lo = lds_tr(p), hi = lds_tr(p + 4 * 128);
           kf = u32x4v{lo[0], lo[1], hi[0], hi[1]};
         } else {
-          kf = lds_ld16(cur + kat + kt * 16 * ROW + ((4 * ks + lg ^ kx) << 4));
+          kf = lds_ld16(cur + kat + kt * 16 * ROW + ((4 * (ks & 3) + lg ^ kx) << 4) + (ks >> 2) * 256);
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[kt][rt] = mfma32<BF>(kf, qf[rt][ks], s[kt][rt]);
@@ -328,13 +348,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[kt][rt][e] = kTail && s[kt][rt][e] == -__builtin_inff() ? s[kt][rt][e] : s[kt][rt][e] * c;
+        for (int e = 0; e < 4; ++e)
           top = fmaxf(top, s[kt][rt][e]);
-        }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(m[rt], top);
+      const float mn = fmaxf(m[rt], top * c);
       const float base = mn == -__builtin_inff() ? 0.f : mn;
       if (__any(mn > m[rt])) {
         const float al = __builtin_amdgcn_exp2f(m[rt] - base);
@@ -348,7 +366,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(s[kt][rt][e] - base);
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][rt][e], c, -base));
           l[rt] += p[e];
         }
         pf[kt][rt] = u32x2v{pack16x2(p[0], p[1], BF), pack16x2(p[2], p[3], BF)};
@@ -357,7 +375,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
     if (!kTail || !slow) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const lds_byte* p = cur + vat + ((dt ^ vx) << 5);
+        const lds_byte* p = cur + vat + (((dt & 7) ^ vx) << 5) + (dt >> 3) * 256;
         if constexpr (NKT == 1) {
           const u32x2v vf = lds_tr(p);
 #pragma unroll
@@ -408,19 +426,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
     }
     if (t + 1 < t1) store_k(nxt);
   };
-  if (t0 < t1) store_k((lds_byte*)buf0);
+  if (live) store_k((lds_byte*)buf0);
   const int full = min(t1, (int)(len / kTile));  // tiles before it hold cached positions alone
-  int t = t0;
+  int t = live ? t0 : t1;
   for (; t + 1 < full; t += 2) {
     step((lds_byte*)buf0, (lds_byte*)buf1, t, std::false_type{});
     step((lds_byte*)buf1, (lds_byte*)buf0, t + 1, std::false_type{});
   }
-  bool odd = false;
-  if (t < full) {
-    step((lds_byte*)buf0, (lds_byte*)buf1, t++, std::false_type{});
-    odd = true;
-  }
-  for (; t < t1; ++t, odd = !odd)
+  for (bool odd = false; t < t1; ++t, odd = !odd)  // an odd full tile too
     step((lds_byte*)(odd ? buf1 : buf0), (lds_byte*)(odd ? buf0 : buf1), t, std::true_type{});
 
 #pragma unroll
@@ -450,7 +463,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
       }
     }
     __syncthreads();
-    if (wk > 0) return;
+    if (wk == 0)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -461,11 +474,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
           o[rt][dt] += buf[(((wr * (WK - 1) + k - 1) * RT + rt) * DT + dt) * 64 + lane];
       }
   }
+  if (wk == 0)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int local = (wr * RT + rt) * 16 + li;
     const int r = rblk * RB + local;
-    if (parts == 1) {
+    if (t0 == 0 && t1 == tiles) {
       if (r >= a.rows) continue;
       const int node = r / a.group, g = r - node * a.group;
       uint16_t* dst = a.out + (((int64_t)b * a.n + node) * a.kv_heads * a.group +
@@ -477,7 +491,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
             make_uint2(pack16x2(o[rt][dt][0] * inv, o[rt][dt][1] * inv, BF),
                        pack16x2(o[rt][dt][2] * inv, o[rt][dt][3] * inv, BF));
     } else {
-      float* dst = a.parts + ((int64_t)unit * a.blocks + rblk) * part_words(RB, D);
+      // the run's first sequence, begun before it, or its last, which goes on behind it
+      float* dst = a.parts + (((int64_t)run * a.blocks + rblk) * 2 + (t0 == 0)) * part_words(RB, D);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         *reinterpret_cast<float4v*>(dst + local * D + 16 * dt + 4 * lg) = o[rt][dt];
@@ -486,6 +501,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 4) vo
         dst[RB * D + RB + local] = l[rt];
       }
     }
+  }
+  __syncthreads();  // the buffers are free
   }
 }
 
@@ -498,19 +515,19 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, in
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63;
   const int r = (int)blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
-  const int part = tree_part_tiles(a, lane);
-  int first = 0;
-  for (int b0 = 0; b0 < b; b0 += 64)
-    first += b0 + lane < b ? tree_parts(tree_tiles(a, b0 + lane), part) : 0;
-  first = wave_sum_i32(first) * a.kv_heads;
-  const int parts = tree_parts(tree_tiles(a, b), part);
+  const int total = tree_tiles_before(a, a.batch, lane) * a.kv_heads;
+  const int size = (total + a.runs - 1) / a.runs;
+  const int tiles = __builtin_amdgcn_readfirstlane(tree_tiles(a, b));
+  const int start = tree_tiles_before(a, b, lane) * a.kv_heads + kvh * tiles;
+  const int run0 = start / size, parts = (start + tiles - 1) / size - run0 + 1;
   if (parts == 1 || r >= a.rows) return;
-  const int64_t words = part_words(rb, D);
+  const int64_t words = part_words(rb, D), step = 2 * a.blocks * words;  // to the next run
   const int local = r % rb;
-  const float* base = a.parts + ((int64_t)(first + kvh) * a.blocks + r / rb) * words;
-  const int64_t step = (int64_t)a.kv_heads * a.blocks * words;  // to the next part
+  // the first part is its run's last, the others are their runs' first
+  const float* base = a.parts + ((int64_t)run0 * a.blocks + r / rb) * 2 * words;
+  auto part = [&](int s) { return base + s * step + (s == 0 ? words : 0); };
   float m = -__builtin_inff();
-  for (int s = lane; s < parts; s += 64) m = fmaxf(m, base[s * step + rb * D + local]);
+  for (int s = lane; s < parts; s += 64) m = fmaxf(m, part(s)[rb * D + local]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   if (m == -__builtin_inff()) m = 0.f;
@@ -518,14 +535,14 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, in
   for (int s0 = 0; s0 < parts; s0 += 64) {
     float w = 0.f;
     if (s0 + lane < parts) {
-      const float* p = base + (s0 + lane) * step + rb * D + local;
+      const float* p = part(s0 + lane) + rb * D + local;
       w = __builtin_amdgcn_exp2f(p[0] - m);
       l += w * p[rb];
     }
     const int here = min(64, parts - s0);
     for (int s = 0; s < here; ++s) {
       const float ws = __shfl(w, s, 64);
-      const float* p = base + (s0 + s) * step + local * D + lane * E;
+      const float* p = part(s0 + s) + local * D + lane * E;
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(ws, p[e], o[e]);
     }
@@ -544,20 +561,21 @@ static int tree_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows
 
 struct TreePlanHost {
   int rb, blocks;
-  int64_t units;  // at most
-  bool split;     // a sequence may be divided
+  int runs;
+  bool split;  // a sequence may be divided
 };
-static TreePlanHost tree_host(int64_t batch, int n, int heads, int kv_heads, int64_t cap) {
+static TreePlanHost tree_host(int64_t batch, int n, int heads, int kv_heads, int dim, int64_t cap) {
   TreePlanHost p;
   const int rows = n * (heads / kv_heads);
   p.rb = tree_rows(rows);
   p.blocks = (rows + p.rb - 1) / p.rb;
   const int64_t tiles = (cap + kTile - 1) / kTile;
-  const int64_t most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;  // parts of a sequence
-  p.split = most > 1;
-  // sum over b of ceil(t_b / C) parts, C >= total tiles / (target / (KV heads, blocks))
-  p.units = (batch + kTreeTarget / p.blocks / kv_heads + 1) * kv_heads;
-  if (p.units > batch * most * kv_heads) p.units = batch * most * kv_heads;
+  // as many workgroups as the LDS of the CUs holds at a time, each an equal run
+  const int per_cu = dim == 256 ? 1 : dim == 128 ? 2 : 4;
+  const int64_t wanted = (int64_t)num_cus() * per_cu / p.blocks;
+  const int64_t most = batch * kv_heads * tiles;
+  p.runs = (int)(wanted < 1 ? 1 : wanted < most ? wanted : most);
+  p.split = tiles > 1 && p.runs > 1;
   return p;
 }
 
@@ -566,14 +584,12 @@ static bool tree_attn_shape_ok(int64_t batch, int n, int heads, int kv_heads, in
       heads < 1 || heads > 65536 || heads % kv_heads || (dim != 64 && dim != 128 && dim != 256) ||
       cap < 1 || cap > INT32_MAX)
     return false;
-  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, cap);
-  return (double)batch * kv_heads * p.blocks * ((cap + kTile - 1) / kTile) <= 2e9 &&
-         (double)(p.units + 8) * p.blocks <= 2e9;
+  return (double)batch * kv_heads * ((cap + kTile - 1) / kTile) <= 1e9;
 }
 
 template <int D, bool BF, bool KCOL>
 static void launch_main(const TreePlanHost& p, const TreeAttnArgs& a, hipStream_t st) {
-  const unsigned grid = (unsigned)((p.units + 7) / 8 * 8 * p.blocks);
+  const unsigned grid = (unsigned)((p.runs + 7) / 8 * 8 * p.blocks);
   switch (p.rb) {
     case 16: tree_attn_kernel<D, BF, KCOL, 1, 1><<<grid, 256, 0, st>>>(a); break;
     case 32: tree_attn_kernel<D, BF, KCOL, 1, 2><<<grid, 256, 0, st>>>(a); break;
@@ -600,8 +616,8 @@ using namespace pe;
 extern "C" size_t pe_tree_attention_workspace_size(int64_t batch, int n, int heads, int kv_heads,
                                                    int head_dim, int64_t cap) {
   if (!tree_attn_shape_ok(batch, n, heads, kv_heads, head_dim, cap)) return 0;
-  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, cap);
-  return p.split ? (size_t)p.units * p.blocks * part_words(p.rb, head_dim) * 4 : 0;
+  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, head_dim, cap);
+  return p.split ? (size_t)p.runs * p.blocks * 2 * part_words(p.rb, head_dim) * 4 : 0;
 }
 
 extern "C" int pe_tree_attention(const void* q, int dtype, int64_t q_b, int64_t q_n,
@@ -615,7 +631,8 @@ extern "C" int pe_tree_attention(const void* q, int dtype, int64_t q_b, int64_t 
   const int bf = bf16_flag(dtype);
   if (bf < 0) return PE_ERR_DTYPE;
   if (batch == 0) return PE_OK;
-  if (!tree_attn_shape_ok(batch, n, heads, kv_heads, head_dim, cap) || q_b < 0 || q_n < 0 || m_b < 0)
+  if (!tree_attn_shape_ok(batch, n, heads, kv_heads, head_dim, cap) || q_b < 0 || q_n < 0 || m_b < 0 ||
+      !(scale >= 0.f && scale <= 3e38f))
     return PE_ERR_DIMS;
   if (!aligned16(q) || (q_b | q_n) % 8 || !aligned16(out)) return PE_ERR_ALIGN;
   const int ok = cache_strides(k_cache, ks_b, ks_h, ks_l, ks_d, v_cache, vs_b, vs_h, vs_l);
@@ -623,12 +640,12 @@ extern "C" int pe_tree_attention(const void* q, int dtype, int64_t q_b, int64_t 
   const size_t need = pe_tree_attention_workspace_size(batch, n, heads, kv_heads, head_dim, cap);
   if (need && (!workspace || workspace_bytes < need)) return PE_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return PE_ERR_ALIGN;
-  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, cap);
+  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, head_dim, cap);
   TreeAttnArgs a{reinterpret_cast<const uint16_t*>(q), q_b, q_n,
                  reinterpret_cast<const uint16_t*>(k_cache),
                  reinterpret_cast<const uint16_t*>(v_cache), ks_b, ks_h, ks_l, ks_d, vs_b, vs_h, vs_l,
                  lengths, masks, m_b, reinterpret_cast<uint16_t*>(out), (int)batch, n,
-                 heads / kv_heads, kv_heads, n * (heads / kv_heads), p.blocks, cap, scale,
+                 heads / kv_heads, kv_heads, n * (heads / kv_heads), p.blocks, cap, scale, p.runs,
                  reinterpret_cast<float*>(workspace)};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (head_dim) {
