@@ -10,7 +10,7 @@
 // Two launches. The first reads every logit once, 8192 of a row per workgroup, and
 // leaves each piece's maximum, its place and its sum of exp((x - max) / T). In the
 // second every workgroup of a sequence walks the tree for itself (64 nodes: one
-// wave, lane = node; 19 KB of sums from L2), then sums the weights of 4096 tokens
+// wave, lane = node; 19 KB of sums from L2), then sums the weights of 2048 tokens
 // of the node that the walk ends in; the last one to finish finds the piece and
 // the token in it. The counters of that hand-over are cleared by the first
 // launch, so the workspace needs no state between calls.
@@ -20,7 +20,7 @@
 namespace pe {
 
 constexpr int kStatChunk = 8192;
-constexpr int kPickChunk = 4096;
+constexpr int kPickChunk = 2048;
 
 struct RowStat {
   float max;
@@ -55,13 +55,59 @@ __device__ __forceinline__ float logit(const void* p, int64_t i) {
   return fmaxf(x, -__builtin_inff());
 }
 
-// exp((x - m) / T), 1 at the maximum itself (also where that is infinite)
-__device__ __forceinline__ double weight(float x, float m, double inv_t) {
-  return x == m ? 1.0 : exp(((double)x - (double)m) * inv_t);
+// 2^z for z <= 0, relative error 2e-14: z = k + f with |f| <= 1/2, 2^f by its
+// interpolation of degree 9 at the Chebyshev nodes of [-1/2, 1/2]. About 18 64-bit
+// instructions; at the rate of 64-bit fma a card passes 2.1e12 values a second, what
+// it reads of 32-bit logits in the same time.
+__device__ __forceinline__ double exp2_f64(double z) {
+  z = fmax(z, -1100.0);  // 0, also for -inf and NaN
+  constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are rint(z)
+  const double t = z + kRound;
+  const double f = z - (t - kRound);
+  double p = 1.0205905413765595e-07;
+  p = __builtin_fma(p, f, 1.325964524488711e-06);
+  p = __builtin_fma(p, f, 1.5252672924850737e-05);
+  p = __builtin_fma(p, f, 0.0001540343375125101);
+  p = __builtin_fma(p, f, 0.0013333558200794592);
+  p = __builtin_fma(p, f, 0.009618129193934313);
+  p = __builtin_fma(p, f, 0.05550410866465167);
+  p = __builtin_fma(p, f, 0.2402265069564034);
+  p = __builtin_fma(p, f, 0.6931471805599462);
+  p = __builtin_fma(p, f, 1.0000000000000135);
+  return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, t));
+}
+// exp((x - m) / T) with the scale log2(e) / T, 1 at the maximum itself (also where
+// that is infinite)
+__device__ __forceinline__ double weight(float x, float m, double scale) {
+  const double e = exp2_f64(((double)x - (double)m) * scale);
+  return x == m ? 1.0 : e;
+}
+// log2(e) / T, above 0 also for an infinite T (a product with -inf stays -inf)
+__device__ __forceinline__ double weight_scale(float t) {
+  return fmax(1.4426950408889634 / (double)t, 1e-300);
 }
 
-// 1 / T, above 0 also for an infinite T (a product with -inf stays -inf)
-__device__ __forceinline__ double inverse(float t) { return fmax(1.0 / (double)t, 1e-300); }
+// VE consecutive logits (16 bytes) from place v on, -inf from V on
+template <int DT>
+__device__ __forceinline__ void logits16(const void* row, int v, int V,
+                                         float (&x)[DT == PE_DTYPE_F32 ? 4 : 8]) {
+  constexpr int VE = DT == PE_DTYPE_F32 ? 4 : 8;
+  if (v + VE <= V) {  // rows have any alignment
+    u32x4v u;
+    __builtin_memcpy(&u, reinterpret_cast<const char*>(row) + (int64_t)v * (16 / VE), 16);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const uint32_t w = u[VE == 4 ? j : j / 2];
+      if constexpr (DT == PE_DTYPE_F32) x[j] = __builtin_bit_cast(float, w);
+      else x[j] = f16or_bf((uint16_t)(w >> (16 * (j & 1))), DT == PE_DTYPE_BF16);
+      x[j] = fmaxf(x[j], -__builtin_inff());
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      x[j] = v + j < V ? logit<DT>(row, v + j) : -__builtin_inff();
+  }
+}
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
@@ -75,11 +121,18 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
+// sums of two pieces of a row: (max, first, sum) each, sums relative to their maxima
+__device__ __forceinline__ void join_stats(float& m, int& first, double& s, float om, int of,
+                                           double os, double scale) {
+  const float mn = fmaxf(m, om);
+  first = om > m ? of : om == m ? min(first, of) : first;
+  s = (s > 0.0 ? s * weight(m, mn, scale) : 0.0) + (os > 0.0 ? os * weight(om, mn, scale) : 0.0);
+  m = mn;
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
-  __shared__ float wm[4];
-  __shared__ int wi[4];
-  __shared__ double ws[4];
+  __shared__ RowStat ws[4];
   const int64_t row = blockIdx.x / a.nc;
   const int piece = (int)(blockIdx.x - row * a.nc);
   const int64_t b = row / a.n;
@@ -93,45 +146,50 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
                      (b * a.l_b + node * a.l_n) * (DT == PE_DTYPE_F32 ? 4 : 2);
   const int v0 = piece * kStatChunk;
   const float t = a.temps ? a.temps[b] : a.temp;
-  constexpr int E = kStatChunk / 256;
-  float x[E];
+  constexpr int VE = DT == PE_DTYPE_F32 ? 4 : 8;
+  constexpr int G = kStatChunk / 256 / VE;  // loads of 16 bytes
+  float x[G][VE];
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int v = v0 + i * 256 + tid;
-    x[i] = v < a.V ? logit<DT>(base, v) : -__builtin_inff();
-  }
-  float m = x[0];
+  for (int i = 0; i < G; ++i) logits16<DT>(base, v0 + (i * 256 + tid) * VE, a.V, x[i]);
+  float m = -__builtin_inff();
 #pragma unroll
-  for (int i = 1; i < E; ++i) m = fmaxf(m, x[i]);
+  for (int i = 0; i < G; ++i)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) m = fmaxf(m, x[i][j]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  if (lane == 0) wm[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-  double s = 0.0;
+  // sums relative to the wave's own maximum, so that no wave waits for another
+  double s = 0.0, scale = 0.0;
   int first = a.V;
   if (t > 0.f) {
+    scale = weight_scale(t);
     if (m != -__builtin_inff()) {
-      const double inv_t = inverse(t);
 #pragma unroll
-      for (int i = 0; i < E; ++i) s += weight(x[i], m, inv_t);
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) s += weight(x[i][j], m, scale);
     }
     s = wave_sum_f64(s);
   } else {
 #pragma unroll
-    for (int i = E - 1; i >= 0; --i)
-      if (x[i] == m && v0 + i * 256 + tid < a.V) first = v0 + i * 256 + tid;
+    for (int i = G - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = VE - 1; j >= 0; --j) {
+        const int v = v0 + (i * 256 + tid) * VE + j;
+        if (x[i][j] == m && v < a.V) first = v;
+      }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) first = min(first, __shfl_xor(first, off, 64));
   }
-  if (lane == 0) {
-    ws[wave] = s;
-    wi[wave] = first;
-  }
+  if (lane == 0) ws[wave] = RowStat{m, first, s};
   __syncthreads();
-  if (tid == 0)
-    a.stats[blockIdx.x] = RowStat{m, min(min(wi[0], wi[1]), min(wi[2], wi[3])),
-                                  (ws[0] + ws[1]) + (ws[2] + ws[3])};
+  if (wave > 0) return;
+  RowStat r = ws[lane & 3];
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1)
+    join_stats(r.max, r.first, r.sum, __shfl_xor(r.max, off, 64), __shfl_xor(r.first, off, 64),
+               __shfl_xor(r.sum, off, 64), scale);
+  if (lane == 0) a.stats[blockIdx.x] = r;
 }
 
 __device__ __forceinline__ void st_dev64(double* p, double v) {
@@ -169,7 +227,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
   const float t = a.temps ? a.temps[b] : a.temp;
   const bool greedy = !(t > 0.f);
   if (greedy && blockIdx.x > 0) return;
-  const double inv_t = greedy ? 0.0 : inverse(t);
+  const double scale = greedy ? 0.0 : weight_scale(t);
 
   // the rows' maxima and sums, from their pieces: a few lanes a row
   const int tpr = n > 32 ? 4 : n > 16 ? 8 : 16;
@@ -181,27 +239,21 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
     double s = 0.0;
     if (there) {
       const RowStat* st = a.stats + (b * n + r) * a.nc;
-      for (int c = c0; c < a.nc; c += tpr) {
-        const RowStat p = st[c];
-        if (p.max > m || (p.max == m && p.first < first)) first = p.first;
-        const float mn = fmaxf(m, p.max);
-        if (!greedy && mn != -__builtin_inff())
-          s = (s > 0.0 ? s * weight(m, mn, inv_t) : 0.0) +
-              (p.sum > 0.0 ? p.sum * weight(p.max, mn, inv_t) : 0.0);
-        m = mn;
+      constexpr int kBatch = 8;  // pieces on their way at once
+      for (int c = c0; c < a.nc; c += kBatch * tpr) {
+        RowStat p[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (c + k * tpr < a.nc) p[k] = st[c + k * tpr];
+          else p[k] = RowStat{-__builtin_inff(), V, 0.0};
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (c + k * tpr < a.nc) join_stats(m, first, s, p[k].max, p[k].first, p[k].sum, scale);
       }
     }
-    for (int off = 1; off < tpr; off <<= 1) {
-      const float om = __shfl_xor(m, off, 64);
-      const int of = __shfl_xor(first, off, 64);
-      const double os = __shfl_xor(s, off, 64);
-      const float mn = fmaxf(m, om);
-      first = om > m ? of : om == m ? min(first, of) : first;
-      if (!greedy && mn != -__builtin_inff())
-        s = (s > 0.0 ? s * weight(m, mn, inv_t) : 0.0) +
-            (os > 0.0 ? os * weight(om, mn, inv_t) : 0.0);
-      m = mn;
-    }
+    for (int off = 1; off < tpr; off <<= 1)
+      join_stats(m, first, s, __shfl_xor(m, off, 64), __shfl_xor(first, off, 64),
+                 __shfl_xor(s, off, 64), scale);
     if (r < n && c0 == 0) {
       rmax[r] = m;
       rfirst[r] = first;
@@ -225,7 +277,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
   if (there) {
     const float m = rmax[p];
     if (greedy) px = x == rfirst[p] && m != -__builtin_inff() ? 1.0 : 0.0;
-    else if (m != -__builtin_inff()) px = weight(logit<DT>(lrow, x), m, inv_t) / rsum[p];
+    else if (m != -__builtin_inff()) px = weight(logit<DT>(lrow, x), m, scale) / rsum[p];
     u = a.uniforms[b * n + i];
     if (a.probs) {
       const float q = a.probs[b * a.q_b + p * a.q_n + x];
@@ -285,26 +337,48 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
     if (!a.probs && wave == 0 && child && x / kPickChunk == piece)
       atomicOr(&gone[(x % kPickChunk) / 32], 1u << (x & 31));
   };
-  auto weights = [&](int v, double& w, double& alt) {
-    w = alt = 0.0;
-    if (v >= V) return;
-    alt = weight(logit<DT>(row, v), m, inv_t) / total_e;
-    w = alt;
+  // what is left of tokens v .. v + 7, times the row's sum, and the row's own weights
+  auto weights = [&](int v, double (&w)[E], double (&own)[E]) {
+    float x[E], qv[E];
+    constexpr int VE = DT == PE_DTYPE_F32 ? 4 : 8;
+#pragma unroll
+    for (int g = 0; g < E; g += VE) {
+      float y[VE];
+      logits16<DT>(row, v + g, V, y);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) x[g + j] = y[j];
+    }
     if (residual) {
-      const float qv = q[v];
-      w = fmax(alt - (qv > 0.f && qv < __builtin_inff() ? (double)qv : 0.0), 0.0);
-    } else if (gone[(v % kPickChunk) / 32] >> (v & 31) & 1) {
-      w = 0.0;
+#pragma unroll
+      for (int g = 0; g < E; g += 4) {
+        float y[4];
+        logits16<PE_DTYPE_F32>(q, v + g, V, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qv[g + j] = y[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      own[j] = v + j < V ? weight(x[j], m, scale) : 0.0;
+      w[j] = own[j];
+      if (residual)
+        w[j] = fmax(__builtin_fma(-(qv[j] > 0.f && qv[j] < __builtin_inff() ? (double)qv[j] : 0.0),
+                                  total_e, own[j]), 0.0);
+      else if (gone[((v + j) % kPickChunk) / 32] >> ((v + j) & 31) & 1)
+        w[j] = 0.0;
     }
   };
   mark(blockIdx.x);
   __syncthreads();
   double s0 = 0.0, s1 = 0.0;
-  for (int k = 0; k < E; ++k) {
-    double w, alt;
-    weights((int)blockIdx.x * kPickChunk + k * 256 + tid, w, alt);
-    s0 += w;
-    s1 += alt;
+  {
+    double w[E], own[E];
+    weights((int)blockIdx.x * kPickChunk + tid * E, w, own);
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      s0 += w[k];
+      s1 += own[k];
+    }
   }
   s0 = wave_sum_f64(s0);
   s1 = wave_sum_f64(s1);
@@ -369,12 +443,11 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
   mark(piece);
   __syncthreads();
   // each thread takes consecutive tokens; running sums over the workgroup
-  double w[E], mine = 0.0;
+  double w[E], own[E], mine = 0.0;
+  weights(piece * kPickChunk + tid * E, w, own);
 #pragma unroll
   for (int k = 0; k < E; ++k) {
-    double alt;
-    weights(piece * kPickChunk + tid * E + k, w[k], alt);
-    if (s_alt) w[k] = alt;
+    if (s_alt) w[k] = own[k];
     mine += w[k];
   }
   double scan = mine;
