@@ -7,13 +7,13 @@
 // a vocabulary of 150,000 an error of 1e-7 in a cumulative sum moves about one
 // sampled token in a hundred.
 //
-// Two launches. The first reads every logit once, 8192 of a row per workgroup, and
-// leaves each piece's maximum, its place and its sum of exp((x - max) / T). In the
-// second every workgroup of a sequence walks the tree for itself (64 nodes: one
-// wave, lane = node; 19 KB of sums from L2), then sums the weights of 2048 tokens
-// of the node that the walk ends in; the last one to finish finds the piece and
-// the token in it. The counters of that hand-over are cleared by the first
-// launch, so the workspace needs no state between calls.
+// Three launches. The first reads every logit once, 8192 of a row per workgroup, and
+// leaves each piece's maximum, its place and its sum of exp((x - max) / T). The
+// second joins the pieces of every row and walks the trees, one workgroup a sequence
+// (64 nodes: one wave, lane = node). In the third the workgroups of a sequence sum
+// the weights of 2048 tokens each at the node that the walk ends in; the last one to
+// finish finds the piece and the token in it. The counters of that hand-over are
+// cleared by the second launch, so the workspace needs no state between calls.
 
 #include "pe_tree.h"
 
@@ -26,6 +26,15 @@ struct RowStat {
   float max;
   int first;  // lowest place of the maximum
   double sum;
+};
+
+// where a sequence's walk ends
+struct WalkEnd {
+  int node, count;
+  float max;         // of the node's logits
+  int done;          // the next token is known (or the slot empty): nothing to draw
+  double sum;        // of exp((x - max) / T)
+  uint64_t children; // of the node: all rejected
 };
 
 struct VerifyArgs {
@@ -43,6 +52,7 @@ struct VerifyArgs {
   int n, V, nc, np;
   RowStat* stats;   // [batch * n][nc]
   double* sums;     // [batch][np][2]
+  WalkEnd* ends;    // [batch]
   uint32_t* done;   // [batch]
 };
 
@@ -56,11 +66,12 @@ __device__ __forceinline__ float logit(const void* p, int64_t i) {
 }
 
 // 2^z for z <= 0, relative error 2e-14: z = k + f with |f| <= 1/2, 2^f by its
-// interpolation of degree 9 at the Chebyshev nodes of [-1/2, 1/2]. About 18 64-bit
-// instructions; at the rate of 64-bit fma a card passes 2.1e12 values a second, what
-// it reads of 32-bit logits in the same time.
+// interpolation of degree 9 at the Chebyshev nodes of [-1/2, 1/2]. ZERO: 0 where it is
+// below the normal range, for -inf and for NaN; else about 1e-307 there, in one
+// instruction less of the slower kind.
+template <bool ZERO>
 __device__ __forceinline__ double exp2_f64(double z) {
-  z = fmax(z, -1100.0);  // 0, also for -inf and NaN
+  z = fmax(z, ZERO ? -1100.0 : -1020.0);
   constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are rint(z)
   const double t = z + kRound;
   const double f = z - (t - kRound);
@@ -74,12 +85,16 @@ __device__ __forceinline__ double exp2_f64(double z) {
   p = __builtin_fma(p, f, 0.2402265069564034);
   p = __builtin_fma(p, f, 0.6931471805599462);
   p = __builtin_fma(p, f, 1.0000000000000135);
-  return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, t));
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
+  if constexpr (ZERO) return __builtin_ldexp(p, (int)k);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, p);
+  return __builtin_bit_cast(double, (uint64_t)((uint32_t)(bits >> 32) + (k << 20)) << 32 |
+                                        (uint32_t)bits);
 }
 // exp((x - m) / T) with the scale log2(e) / T, 1 at the maximum itself (also where
 // that is infinite)
 __device__ __forceinline__ double weight(float x, float m, double scale) {
-  const double e = exp2_f64(((double)x - (double)m) * scale);
+  const double e = exp2_f64<true>(((double)x - (double)m) * scale);
   return x == m ? 1.0 : e;
 }
 // log2(e) / T, above 0 also for an infinite T (a product with -inf stays -inf)
@@ -87,38 +102,71 @@ __device__ __forceinline__ double weight_scale(float t) {
   return fmax(1.4426950408889634 / (double)t, 1e-300);
 }
 
-// VE consecutive logits (16 bytes) from place v on, -inf from V on
-template <int DT>
-__device__ __forceinline__ void logits16(const void* row, int v, int V,
-                                         float (&x)[DT == PE_DTYPE_F32 ? 4 : 8]) {
-  constexpr int VE = DT == PE_DTYPE_F32 ? 4 : 8;
-  if (v + VE <= V) {  // rows have any alignment
-    u32x4v u;
-    __builtin_memcpy(&u, reinterpret_cast<const char*>(row) + (int64_t)v * (16 / VE), 16);
+// G groups of VE = 4 or 8 logits (16 bytes each), group i from place v + i step on,
+// -inf from V on; `whole`, for the workgroup: none reaches V. All loads go out
+// before the first is waited for. Rows have any alignment.
+template <int DT, int G, int VE>
+__device__ __forceinline__ void logits16(const void* row, int v, int step, int V, bool whole,
+                                         float (&x)[G][VE]) {
+  static_assert(VE == (DT == PE_DTYPE_F32 ? 4 : 8), "16 bytes");
+  if (whole) {
+    u32x4v u[G];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const uint32_t w = u[VE == 4 ? j : j / 2];
-      if constexpr (DT == PE_DTYPE_F32) x[j] = __builtin_bit_cast(float, w);
-      else x[j] = f16or_bf((uint16_t)(w >> (16 * (j & 1))), DT == PE_DTYPE_BF16);
-      x[j] = fmaxf(x[j], -__builtin_inff());
-    }
+    for (int i = 0; i < G; ++i)
+      __builtin_memcpy(&u[i], reinterpret_cast<const char*>(row) + (int64_t)(v + i * step) * (16 / VE), 16);
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const uint32_t w = u[i][VE == 4 ? j : j / 2];
+        if constexpr (DT == PE_DTYPE_F32) x[i][j] = __builtin_bit_cast(float, w);
+        else x[i][j] = f16or_bf((uint16_t)(w >> (16 * (j & 1))), DT == PE_DTYPE_BF16);
+        x[i][j] = fmaxf(x[i][j], -__builtin_inff());
+      }
   } else {
 #pragma unroll
-    for (int j = 0; j < VE; ++j)
-      x[j] = v + j < V ? logit<DT>(row, v + j) : -__builtin_inff();
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const int at = v + i * step + j;
+        x[i][j] = logit<DT>(row, min(at, V - 1));
+        if (at >= V) x[i][j] = -__builtin_inff();
+      }
   }
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
 __device__ __forceinline__ double lane_f64(double v, int lane) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v);
   const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
   const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// lane moves of 64-bit values as two of 32 (DPP control word CTRL; lanes without a
+// source get 0)
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// running sum over the 64 lanes: row_shr 1, 2, 4, 8 within 16 lanes, then the rows
+__device__ __forceinline__ double wave_scan_f64(double v, int lane) {
+  v += dpp_f64<0x111>(v);
+  v += dpp_f64<0x112>(v);
+  v += dpp_f64<0x114>(v);
+  v += dpp_f64<0x118>(v);
+  const double r0 = lane_f64(v, 15), r1 = r0 + lane_f64(v, 31), r2 = r1 + lane_f64(v, 47);
+  const int row = lane >> 4;
+  return v + (row == 0 ? 0.0 : row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+// sum over the 64 lanes, in every lane
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v += dpp_f64<0x111>(v);
+  v += dpp_f64<0x112>(v);
+  v += dpp_f64<0x114>(v);
+  v += dpp_f64<0x118>(v);
+  return (lane_f64(v, 15) + lane_f64(v, 31)) + (lane_f64(v, 47) + lane_f64(v, 63));
 }
 
 // sums of two pieces of a row: (max, first, sum) each, sums relative to their maxima
@@ -137,7 +185,6 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
   const int piece = (int)(blockIdx.x - row * a.nc);
   const int64_t b = row / a.n;
   const int node = (int)(row - b * a.n);
-  if (piece == 0 && node == 0 && threadIdx.x == 0) a.done[b] = 0;
   const int64_t* tok = a.tokens + b * a.n;
   // rows of absent drafts and of empty sequences are not looked at
   if (tok[node] < 0 || tok[node] >= a.V || tok[0] < 0 || tok[0] >= a.V) return;
@@ -149,8 +196,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
   constexpr int VE = DT == PE_DTYPE_F32 ? 4 : 8;
   constexpr int G = kStatChunk / 256 / VE;  // loads of 16 bytes
   float x[G][VE];
-#pragma unroll
-  for (int i = 0; i < G; ++i) logits16<DT>(base, v0 + (i * 256 + tid) * VE, a.V, x[i]);
+  logits16<DT>(base, v0 + tid * VE, 256 * VE, a.V, v0 + kStatChunk <= a.V, x);
   float m = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < G; ++i)
@@ -163,11 +209,18 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
   int first = a.V;
   if (t > 0.f) {
     scale = weight_scale(t);
-    if (m != -__builtin_inff()) {
+    if (__builtin_expect(m == __builtin_inff(), 0)) {  // those share the distribution
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) s += weight(x[i][j], m, scale);
+        for (int j = 0; j < VE; ++j) s += x[i][j] == m ? 1.0 : 0.0;
+    } else if (m != -__builtin_inff()) {
+      const double shift = -(double)m * scale;
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          s += exp2_f64<false>(__builtin_fma((double)x[i][j], scale, shift));
     }
     s = wave_sum_f64(s);
   } else {
@@ -202,31 +255,28 @@ __device__ __forceinline__ double ld_dev64(const double* p) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
+__global__ __launch_bounds__(256) void verify_walk_kernel(const VerifyArgs a) {
   __shared__ float rmax[kTreeMax];
   __shared__ int rfirst[kTreeMax];
   __shared__ double rsum[kTreeMax];
-  __shared__ uint32_t gone[kPickChunk / 32];  // this piece's tokens that were rejected
-  __shared__ double part[2][4];
-  __shared__ int s_piece, s_found;
-  __shared__ double s_before;
-  __shared__ bool s_last, s_alt;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int order[kTreeMax];
+  const int tid = threadIdx.x;
   const int n = a.n, V = a.V;
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.x;
   const int64_t* tok = a.tokens + b * n;
   int64_t *out = a.out + b * n, *path = a.path + b * n;
+  if (tid == 0) a.done[b] = 0;
   const int64_t root = tok[0];
   if (root < 0 || root >= V) {  // an empty slot of the batch
-    if (blockIdx.x == 0) {
-      if (tid < n) out[tid] = path[tid] = -1;
-      if (tid == 0) a.count[b] = 0;
+    if (tid < n) out[tid] = path[tid] = -1;
+    if (tid == 0) {
+      a.count[b] = 0;
+      a.ends[b].done = 1;
     }
     return;
   }
   const float t = a.temps ? a.temps[b] : a.temp;
   const bool greedy = !(t > 0.f);
-  if (greedy && blockIdx.x > 0) return;
   const double scale = greedy ? 0.0 : weight_scale(t);
 
   // the rows' maxima and sums, from their pieces: a few lanes a row
@@ -242,13 +292,24 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
       constexpr int kBatch = 8;  // pieces on their way at once
       for (int c = c0; c < a.nc; c += kBatch * tpr) {
         RowStat p[kBatch];
+        float mn = m;
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
+        for (int k = 0; k < kBatch; ++k) {
+          p[k] = RowStat{-__builtin_inff(), V, 0.0};
           if (c + k * tpr < a.nc) p[k] = st[c + k * tpr];
-          else p[k] = RowStat{-__builtin_inff(), V, 0.0};
+        }
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-          if (c + k * tpr < a.nc) join_stats(m, first, s, p[k].max, p[k].first, p[k].sum, scale);
+        for (int k = 0; k < kBatch; ++k) {
+          if (p[k].max > mn || (p[k].max == mn && p[k].first < first)) first = p[k].first;
+          mn = fmaxf(mn, p[k].max);
+        }
+        if (!greedy && mn != -__builtin_inff()) {
+          s = s > 0.0 ? s * weight(m, mn, scale) : 0.0;
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k)
+            if (p[k].sum > 0.0) s += p[k].sum * weight(p[k].max, mn, scale);
+        }
+        m = mn;
       }
     }
     for (int off = 1; off < tpr; off <<= 1)
@@ -260,11 +321,11 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
       rsum[r] = s;
     }
   }
-  for (int i = tid; i < kPickChunk / 32; i += 256) gone[i] = 0;
   __syncthreads();
+  if (tid >= 64) return;
 
   // the walk: lane = node
-  const int i = lane;
+  const int i = tid;
   const int64_t x = i < n ? tok[i] : -1;
   int64_t par = -1;
   if (i > 0 && i < n && x >= 0 && x < V) par = a.parents ? a.parents[b * a.p_b + i] : i - 1;
@@ -276,210 +337,198 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
   double px = 0.0, qx = 1.0, u = 0.0;
   if (there) {
     const float m = rmax[p];
-    if (greedy) px = x == rfirst[p] && m != -__builtin_inff() ? 1.0 : 0.0;
-    else if (m != -__builtin_inff()) px = weight(logit<DT>(lrow, x), m, scale) / rsum[p];
+    const float lx = logit<DT>(lrow, x);
     u = a.uniforms[b * n + i];
     if (a.probs) {
       const float q = a.probs[b * a.q_b + p * a.q_n + x];
       qx = q > 0.f && q < __builtin_inff() ? q : 0.0;
     }
+    if (greedy) px = x == rfirst[p] && m != -__builtin_inff() ? 1.0 : 0.0;
+    else if (m != -__builtin_inff()) px = weight(lx, m, scale) / rsum[p];
   }
-  bool blocked = false, ok = false;
+  bool blocked = false, ok = there && u * qx < px;
   double rem = 1.0;
-  for (int j = 1; j < n; ++j) {
-    if (i == j) ok = there && (a.probs ? u * qx : u * rem) < px;
-    const bool jt = __builtin_amdgcn_readlane((int)there, j);
-    if (!jt) continue;
-    const int jp = __builtin_amdgcn_readlane(p, j);
-    const int jx = __builtin_amdgcn_readlane((int)x, j);
-    const double jq = lane_f64(px, j);
-    const bool jok = __builtin_amdgcn_readlane((int)ok, j);
-    if (there && i > j && p == jp) {
-      blocked |= jok;
-      if (!a.probs) {
+  if (a.parents) {  // in order of the nodes: what a rejection leaves to later siblings
+    for (uint64_t todo = __ballot(there); todo; todo &= todo - 1) {
+      const int j = __builtin_ctzll(todo);
+      const bool after = there && i > j && p == __builtin_amdgcn_readlane(p, j);
+      if (!__ballot(after)) continue;
+      const int jx = __builtin_amdgcn_readlane((int)x, j);
+      const double jq = lane_f64(px, j);
+      const bool jok = __builtin_amdgcn_readlane((int)ok, j);
+      if (after) {
+        blocked |= jok;
         rem -= jq;
         if ((int)x == jx) px = 0.0;  // rejected once: nothing is left of it
+        ok = u * rem < px;
       }
     }
   }
   const uint64_t taken = __ballot(i == 0 || (ok && !blocked));
   const uint64_t on = __ballot(i < n && mask != 0 && !(mask & ~taken));
   const int last = 63 - __builtin_clzll(on);
-  const bool child = there && p == last;
-  const bool any_child = __ballot(child) != 0;
+  const uint64_t children = __ballot(there && p == last);
   const int count = __popcll(on);
-
-  auto finish = [&](int64_t token) {  // wave 0 of one workgroup; lane = place on the path
-    int at = 0;
-    for (int j = 0; j < n; ++j)
-      if ((on >> j & 1) && __popcll(on & ((1ull << j) - 1)) == i) at = j;
-    const int64_t said = __shfl((long long)x, __shfl(at, (i + 1) & 63, 64), 64);
-    if (i < n) {
-      path[i] = i < count ? at : -1;
-      out[i] = i < count - 1 ? said : i == count - 1 ? token : -1;
-    }
-    if (i == 0) a.count[b] = count;
-  };
   const float m = rmax[last];
-  if (greedy || m == -__builtin_inff()) {
-    if (blockIdx.x == 0 && wave == 0) finish(m == -__builtin_inff() ? -1 : rfirst[last]);
-    return;
-  }
-  const double total_e = rsum[last];
+  const bool none = m == -__builtin_inff();
 
-  // weights of this workgroup's piece
-  const char* row = reinterpret_cast<const char*>(a.logits) +
-                    (b * a.l_b + last * a.l_n) * (DT == PE_DTYPE_F32 ? 4 : 2);
-  const bool residual = a.probs && any_child;
-  const float* q = a.probs + (a.probs ? b * a.q_b + last * a.q_n : 0);
+  // lane = place on the path
+  if (on >> i & 1) order[__popcll(on & ((1ull << i) - 1))] = i;
+  __builtin_amdgcn_wave_barrier();
+  const int at = i < count ? order[i] : 0;
+  const int64_t said = __shfl((long long)x, __shfl(at, (i + 1) & 63, 64), 64);
+  if (i < n) {
+    path[i] = i < count ? at : -1;
+    out[i] = i < count - 1 ? said : i == count - 1 && !none && greedy ? rfirst[last] : -1;
+  }
+  if (i == 0) {
+    a.count[b] = count;
+    a.ends[b] = WalkEnd{last, count, m, greedy || none, rsum[last], children};
+  }
+}
+
+// E consecutive logits of a thread: what is left of them times the row's sum, and the
+// row's own weights
+template <int DT>
+__global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
+  __shared__ uint32_t gone[kPickChunk / 32];  // the piece's tokens that were rejected
+  __shared__ double part[2][4];
+  __shared__ int s_piece, s_found;
+  __shared__ double s_target;
+  __shared__ bool s_last, s_own;
   constexpr int E = kPickChunk / 256;
-  auto mark = [&](int piece) {  // rejected tokens of the piece (drafts without probabilities)
-    if (!a.probs && wave == 0 && child && x / kPickChunk == piece)
-      atomicOr(&gone[(x % kPickChunk) / 32], 1u << (x & 31));
-  };
-  // what is left of tokens v .. v + 7, times the row's sum, and the row's own weights
-  auto weights = [&](int v, double (&w)[E], double (&own)[E]) {
-    float x[E], qv[E];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int V = a.V;
+  const int64_t b = blockIdx.y;
+  const WalkEnd end = a.ends[b];
+  if (end.done) return;
+  const double scale = weight_scale(a.temps ? a.temps[b] : a.temp);
+  const char* row = reinterpret_cast<const char*>(a.logits) +
+                    (b * a.l_b + end.node * a.l_n) * (DT == PE_DTYPE_F32 ? 4 : 2);
+  const bool residual = a.probs && end.children;
+  const float* q = residual ? a.probs + b * a.q_b + end.node * a.q_n : nullptr;
+  double* sums = a.sums + b * a.np * 2;
+
+  int piece = blockIdx.x;
+  for (bool find = false;; find = true) {
+    const int v0 = piece * kPickChunk + tid * E;
     constexpr int VE = DT == PE_DTYPE_F32 ? 4 : 8;
-#pragma unroll
-    for (int g = 0; g < E; g += VE) {
-      float y[VE];
-      logits16<DT>(row, v + g, V, y);
-#pragma unroll
-      for (int j = 0; j < VE; ++j) x[g + j] = y[j];
-    }
-    if (residual) {
-#pragma unroll
-      for (int g = 0; g < E; g += 4) {
-        float y[4];
-        logits16<PE_DTYPE_F32>(q, v + g, V, y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) qv[g + j] = y[j];
+    const bool whole = (piece + 1) * kPickChunk <= V;
+    float x[E / VE][VE], qv[E / 4][4] = {};
+    if (residual) logits16<PE_DTYPE_F32>(q, v0, 4, V, whole, qv);
+    logits16<DT>(row, v0, VE, V, whole, x);
+    if (!residual) {
+      for (int i = tid; i < kPickChunk / 32; i += 256) gone[i] = 0;
+      __syncthreads();
+      if (tid < a.n && (end.children >> tid & 1)) {
+        const int64_t t = a.tokens[b * a.n + tid];
+        if (t / kPickChunk == piece) atomicOr(&gone[t % kPickChunk / 32], 1u << (t & 31));
       }
+      __syncthreads();
     }
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      own[j] = v + j < V ? weight(x[j], m, scale) : 0.0;
-      w[j] = own[j];
-      if (residual)
-        w[j] = fmax(__builtin_fma(-(qv[j] > 0.f && qv[j] < __builtin_inff() ? (double)qv[j] : 0.0),
-                                  total_e, own[j]), 0.0);
-      else if (gone[((v + j) % kPickChunk) / 32] >> ((v + j) & 31) & 1)
-        w[j] = 0.0;
-    }
-  };
-  mark(blockIdx.x);
-  __syncthreads();
-  double s0 = 0.0, s1 = 0.0;
-  {
-    double w[E], own[E];
-    weights((int)blockIdx.x * kPickChunk + tid * E, w, own);
+    double w[E], own[E], s0 = 0.0, s1 = 0.0;
+    const uint32_t lost = residual ? 0 : gone[tid * E / 32] >> (tid * E & 31);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
+      own[k] = v0 + k < V ? weight(x[k / VE][k % VE], end.max, scale) : 0.0;
+      w[k] = own[k];
+      if (residual) {
+        const float qk = qv[k / 4][k % 4];
+        const double qd = qk > 0.f && qk < __builtin_inff() ? (double)qk : 0.0;
+        w[k] = fmax(__builtin_fma(-qd, end.sum, own[k]), 0.0);
+      } else if (lost >> k & 1) {
+        w[k] = 0.0;
+      }
       s0 += w[k];
       s1 += own[k];
     }
-  }
-  s0 = wave_sum_f64(s0);
-  s1 = wave_sum_f64(s1);
-  if (lane == 0) {
-    part[0][wave] = s0;
-    part[1][wave] = s1;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    double* sum = a.sums + (b * a.np + blockIdx.x) * 2;
-    st_dev64(sum, (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]));
-    st_dev64(sum + 1, (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]));
-    __builtin_amdgcn_s_waitcnt(0);
-    s_last = atomicAdd(&a.done[b], 1u) + 1 == (uint32_t)a.np;
-  }
-  __syncthreads();
-  if (!s_last) return;
-
-  // the piece: the first whose running sum passes u_0 of the total
-  const double* sums = a.sums + b * a.np * 2;
-  if (wave == 0) {
-    double total[2] = {0.0, 0.0};
-    for (int c = lane; c < a.np; c += 64) {
-      total[0] += ld_dev64(sums + 2 * c);
-      total[1] += ld_dev64(sums + 2 * c + 1);
-    }
-    total[0] = wave_sum_f64(total[0]);
-    total[1] = wave_sum_f64(total[1]);
-    const int alt = total[0] > 0.0 ? 0 : 1;  // nothing is left: the target's own distribution
-    const double target = fmin(fmax((double)a.uniforms[b * n], 0.0), 1.0) * total[alt];
-    double run = 0.0, before = 0.0;
-    int found = 0;  // without a hit the last piece that has weight
-    for (int c0 = 0; c0 < a.np; c0 += 64) {
-      const double s = c0 + lane < a.np ? ld_dev64(sums + 2 * (c0 + lane) + alt) : 0.0;
-      double scan = s;
+    if (find) {
+      // running sums over the workgroup: the first token that passes the target
+      const bool use_own = s_own;
+      const double mine = use_own ? s1 : s0;
+      const double scan = wave_scan_f64(mine, lane);
+      if (lane == 63) part[0][wave] = scan;
+      __syncthreads();
+      double run = 0.0;
+      for (int k = 0; k < wave; ++k) run += part[0][k];
+      run += scan - mine;
+      int hit = V, any = -1;
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(scan, off, 64);
-        if (lane >= off) scan += o;
+      for (int k = 0; k < E; ++k) {
+        const double wk = use_own ? own[k] : w[k];
+        if (wk > 0.0) {
+          any = v0 + k;
+          run += wk;
+          if (hit == V && run > s_target) hit = any;
+        }
       }
-      const double excl = run + (scan - s);
-      const uint64_t hit = __ballot(s > 0.0 && run + scan > target);
-      const uint64_t some = hit ? hit : __ballot(s > 0.0);
-      if (some) {
-        const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-        found = c0 + l;
-        before = lane_f64(excl, l);
+      if (hit < V) atomicMin(&s_found, hit);
+      __syncthreads();
+      int found = s_found;
+      if (found == V) {  // rounding left the target behind the last weight
+        __syncthreads();
+        if (tid == 0) s_found = -1;
+        __syncthreads();
+        if (any >= 0) atomicMax(&s_found, any);
+        __syncthreads();
+        found = s_found;
       }
-      if (hit) break;
-      run += lane_f64(scan, 63);
+      if (tid == 0) a.out[b * a.n + end.count - 1] = found;
+      return;
     }
+    s0 = wave_sum_f64(s0);
+    s1 = wave_sum_f64(s1);
     if (lane == 0) {
-      s_piece = found;
-      s_before = target - before;
-      s_alt = alt != 0;
-      s_found = V;
+      part[0][wave] = s0;
+      part[1][wave] = s1;
     }
-  }
-  for (int k = tid; k < kPickChunk / 32; k += 256) gone[k] = 0;
-  __syncthreads();
-  const int piece = s_piece;
-  mark(piece);
-  __syncthreads();
-  // each thread takes consecutive tokens; running sums over the workgroup
-  double w[E], own[E], mine = 0.0;
-  weights(piece * kPickChunk + tid * E, w, own);
-#pragma unroll
-  for (int k = 0; k < E; ++k) {
-    if (s_alt) w[k] = own[k];
-    mine += w[k];
-  }
-  double scan = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double o = __shfl_up(scan, off, 64);
-    if (lane >= off) scan += o;
-  }
-  if (lane == 63) part[0][wave] = scan;
-  __syncthreads();
-  double run = 0.0;
-  for (int k = 0; k < wave; ++k) run += part[0][k];
-  run += scan - mine;
-  int hit = V, any = -1;
-#pragma unroll
-  for (int k = 0; k < E; ++k) {
-    if (w[k] > 0.0) {
-      any = piece * kPickChunk + tid * E + k;
-      run += w[k];
-      if (hit == V && run > s_before) hit = any;
+    __syncthreads();
+    if (tid == 0) {
+      st_dev64(sums + 2 * piece, (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]));
+      st_dev64(sums + 2 * piece + 1, (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]));
+      __builtin_amdgcn_s_waitcnt(0);
+      s_last = atomicAdd(&a.done[b], 1u) + 1 == (uint32_t)a.np;
     }
+    __syncthreads();
+    if (!s_last) return;
+
+    // the piece: the first whose running sum passes u_0 of the total
+    if (wave == 0) {
+      double total = 0.0;
+      int use = 0;
+      for (;; use = 1) {
+        total = 0.0;
+        for (int c = lane; c < a.np; c += 64) total += ld_dev64(sums + 2 * c + use);
+        total = wave_sum_f64(total);
+        if (use == 1 || total > 0.0) break;  // nothing is left: the target's own distribution
+      }
+      const double target = fmin(fmax((double)a.uniforms[b * a.n], 0.0), 1.0) * total;
+      double run = 0.0, before = 0.0;
+      int found = 0;  // without a hit the last piece that has weight
+      for (int c0 = 0; c0 < a.np; c0 += 64) {
+        const double s = c0 + lane < a.np ? ld_dev64(sums + 2 * (c0 + lane) + use) : 0.0;
+        const double scan = wave_scan_f64(s, lane);
+        const double excl = run + (scan - s);
+        const uint64_t hit = __ballot(s > 0.0 && run + scan > target);
+        const uint64_t some = hit ? hit : __ballot(s > 0.0);
+        if (some) {
+          const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
+          found = c0 + l;
+          before = lane_f64(excl, l);
+        }
+        if (hit) break;
+        run += lane_f64(scan, 63);
+      }
+      if (lane == 0) {
+        s_piece = found;
+        s_target = target - before;
+        s_own = use == 1;
+        s_found = V;
+      }
+    }
+    __syncthreads();
+    piece = s_piece;
   }
-  if (hit < V) atomicMin(&s_found, hit);
-  __syncthreads();
-  if (s_found == V) {  // rounding left the target behind the last weight
-    __syncthreads();
-    if (tid == 0) s_found = -1;
-    __syncthreads();
-    if (any >= 0) atomicMax(&s_found, any);
-    __syncthreads();
-  }
-  if (wave == 0) finish(s_found);
 }
 
 static int pieces(int64_t V, int chunk) { return (int)((V + chunk - 1) / chunk); }
@@ -496,11 +545,15 @@ static size_t stats_bytes(int64_t batch, int n, int64_t vocab) {
 static size_t sums_bytes(int64_t batch, int64_t vocab) {
   return (size_t)batch * pieces(vocab, kPickChunk) * 16;
 }
+static size_t ends_bytes(int64_t batch) { return round_up((size_t)batch * sizeof(WalkEnd), 16); }
 
 template <int DT>
 static int launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t st) {
   verify_stats_kernel<DT><<<(unsigned)(batch * a.n * a.nc), 256, 0, st>>>(a);
-  const int rc = launch_status();
+  int rc = launch_status();
+  if (rc != PE_OK) return rc;
+  verify_walk_kernel<DT><<<(unsigned)batch, 256, 0, st>>>(a);
+  rc = launch_status();
   if (rc != PE_OK) return rc;
   verify_pick_kernel<DT><<<dim3((unsigned)a.np, (unsigned)batch), 256, 0, st>>>(a);
   return launch_status();
@@ -512,7 +565,8 @@ using namespace pe;
 
 extern "C" size_t pe_verify_drafts_workspace_size(int64_t batch, int n, int64_t vocab) {
   if (!verify_shape_ok(batch, n, vocab)) return 0;
-  return stats_bytes(batch, n, vocab) + sums_bytes(batch, vocab) + round_up((size_t)batch * 4, 16);
+  return stats_bytes(batch, n, vocab) + sums_bytes(batch, vocab) + ends_bytes(batch) +
+         round_up((size_t)batch * 4, 16);
 }
 
 extern "C" int pe_verify_drafts(const void* logits, int dtype, int64_t l_b, int64_t l_n,
@@ -531,12 +585,13 @@ extern "C" int pe_verify_drafts(const void* logits, int dtype, int64_t l_b, int6
     return PE_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PE_ERR_ALIGN;
   char* ws = reinterpret_cast<char*>(workspace);
+  char* sums = ws + stats_bytes(batch, n, vocab);
+  char* ends = sums + sums_bytes(batch, vocab);
   VerifyArgs a{logits, l_b, l_n, tokens, parents, p_b, uniforms, temps, temp, probs, q_b, q_n,
                out, path, count, n, (int)vocab, pieces(vocab, kStatChunk),
                pieces(vocab, kPickChunk), reinterpret_cast<RowStat*>(ws),
-               reinterpret_cast<double*>(ws + stats_bytes(batch, n, vocab)),
-               reinterpret_cast<uint32_t*>(ws + stats_bytes(batch, n, vocab) +
-                                           sums_bytes(batch, vocab))};
+               reinterpret_cast<double*>(sums), reinterpret_cast<WalkEnd*>(ends),
+               reinterpret_cast<uint32_t*>(ends + ends_bytes(batch))};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == PE_DTYPE_F32) return launch_verify<PE_DTYPE_F32>(a, batch, st);
   if (dtype == PE_DTYPE_BF16) return launch_verify<PE_DTYPE_BF16>(a, batch, st);
