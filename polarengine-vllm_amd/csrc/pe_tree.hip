@@ -31,12 +31,24 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(const int64_t* __restrict
 // by the position's angles; values pass as they are. D / 8 lanes a head, one
 // 16-byte load each, so a row is read once and the norm, the rotation and the one
 // rounding happen in registers. Bound by bytes: rows of 16-bit values read and
-// written once.
+// written once. The arithmetic is in 64 bits: it costs no time beside the bytes, and
+// the one rounding is that of the exact value.
+//
+// A workgroup takes a row (or several of a model with few heads), its heads four
+// loads a lane at a time, the row's angles once. Keys that the cache stores by
+// dimension go through LDS instead, 64 rows of a head a workgroup, and leave as 16
+// bytes of eight consecutive positions.
 // ---------------------------------------------------------------------------
+constexpr int kRopeTile = 64;
+
 struct RopeArgs {
   const uint16_t* qkv;
-  int64_t ld, items;
-  int heads, kv_heads, per_row, rot;
+  int64_t ld, rows;
+  int heads, kv_heads, rot;
+  int per_row;        // heads of a row that the row form takes
+  int rows_per_wg;    // of the row form,
+  int parts, part;    // or workgroups per row and heads of each
+  int64_t col_wgs;    // workgroups that take keys by dimension, before those of the row form
   const float* rope;
   int64_t rope_rows;
   const int64_t* positions;
@@ -50,77 +62,220 @@ struct RopeArgs {
   int64_t n, cap;
 };
 
-template <int D, bool BF, bool CACHE>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
-  constexpr int LPG = D / 8;  // lanes per head
-  const int lane = threadIdx.x & (LPG - 1);
-  const int64_t item = (int64_t)blockIdx.x * (256 / LPG) + threadIdx.x / LPG;
-  const bool live = item < a.items;  // the others take part in the exchanges
-  const int64_t row = live ? item / a.per_row : 0;
-  const int head = live ? (int)(item - row * a.per_row) : 0;
-  const int H = a.heads, KVH = a.kv_heads;
+// cosines and sines of a lane's eight dimensions (sines of the lower half negated);
+// lanes past the rotary dimensions have 1 and 0
+struct RopeAngles {
+  double c[8], s[8];
+};
+__device__ __forceinline__ RopeAngles rope_angles(const RopeArgs& a, int64_t pos, int lane) {
+  RopeAngles r;
+  const int hl = a.rot / 16;  // lanes of half the rotary dimensions
+  float c[8] = {1, 1, 1, 1, 1, 1, 1, 1}, s[8] = {};
+  if (lane < 2 * hl && pos >= 0 && pos < a.rope_rows) {
+    const float* t = a.rope + pos * a.rot + 8 * (lane < hl ? lane : lane - hl);
+    load8<PE_DTYPE_F32>(t, c);
+    load8<PE_DTYPE_F32>(t + a.rot / 2, s);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r.c[i] = c[i];
+    r.s[i] = lane < hl ? -s[i] : s[i];
+  }
+  return r;
+}
+
+// 64-bit lane move by a DPP control word
+template <int CTRL>
+__device__ __forceinline__ double dpp_move(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// sum over the D / 8 lanes of a head, in each of them
+template <int D>
+__device__ __forceinline__ double head_sum(double v) {
+  v += dpp_move<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+  v += dpp_move<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  v += dpp_move<0x141>(v);  // row_half_mirror: the other quad of eight
+  if constexpr (D >= 128) v += dpp_move<0x140>(v);  // row_mirror: the other eight of 16
+  if constexpr (D == 256) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+// one head: u (eight 16-bit values of the lane) normed with w, turned, rounded
+template <int D, bool BF>
+__device__ __forceinline__ u32x4v rope_head(const RopeArgs& a, u32x4v u, const uint16_t* w,
+                                            const RopeAngles& r, int lane) {
   float v[8];
-  load8<BF ? PE_DTYPE_BF16 : PE_DTYPE_F16>(a.qkv + row * a.ld + (int64_t)head * D + 8 * lane, v);
-  const int64_t pos = a.positions[row];
-  const bool inside = pos >= 0 && pos < a.rope_rows;
-  if (head < H + KVH) {
-    const uint16_t* w = head < H ? a.qw : a.kw;
-    if (w) {
-      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t two = u[i / 2];
+    v[i] = f16or_bf((uint16_t)(two >> (16 * (i & 1))), BF);
+  }
+  double y = 1.0;
+  if (w) {
+    float g[8], ss = 0.f;
+    load8<BF ? PE_DTYPE_BF16 : PE_DTYPE_F16>(w + 8 * lane, g);
 #pragma unroll
-      for (int off = LPG / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-      const float r = 1.f / __builtin_sqrtf(ss * (1.f / D) + a.eps);
-      float g[8];
-      load8<BF ? PE_DTYPE_BF16 : PE_DTYPE_F16>(w + 8 * lane, g);
+    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+    const double x = head_sum<D>(ss) * (1.0 / D) + (double)a.eps;
+    // 1 / sqrt(x): the instruction's value (relative error below 2^-26) and a Newton step
+    y = __builtin_amdgcn_rsq(x);
+    const double z = y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    y = x < 1e300 ? z : y;  // an infinite square: 0
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= r * g[i];
-    }
-    const int hl = a.rot / 16;  // lanes of half the rotary dimensions
-    const bool lo = lane < hl, in = lane < 2 * hl;
-    const int me = (int)(threadIdx.x & 63);
-    const int other = lo ? me + hl : in ? me - hl : me;
-    float o[8];
+    for (int i = 0; i < 8; ++i) v[i] *= g[i];  // exact: two 16-bit values
+  }
+  float o[8], f[8];
+  if (a.rot == D && D == 128) {  // lane ^ 8
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = lane_xor<8>(v[i]);
+  } else {
+    const int hl = a.rot / 16, me = (int)(threadIdx.x & 63);
+    const int other = lane < hl ? me + hl : lane < 2 * hl ? me - hl : me;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = __shfl(v[i], other, 64);
-    if (in && inside) {
-      const float* t = a.rope + pos * a.rot + 8 * (lo ? lane : lane - hl);
-      float c[8], s[8];
-      load8<PE_DTYPE_F32>(t, c);
-      load8<PE_DTYPE_F32>(t + a.rot / 2, s);
+  }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * c[i] + (lo ? -o[i] : o[i]) * s[i];
+  for (int i = 0; i < 8; ++i) {
+    double t = v[i];
+    // dimensions past the rotary ones keep their value, whatever the other lane holds
+    if (lane < a.rot / 8) t = __builtin_fma(t, r.c[i], (double)o[i] * r.s[i]);
+    f[i] = (float)(t * y);
+    // kept in 32 bits: the direct conversion to 16 takes a dozen instructions more
+    asm("" : "+v"(f[i]));
+  }
+  return u32x4v{pack16x2(f[0], f[1], BF), pack16x2(f[2], f[3], BF), pack16x2(f[4], f[5], BF),
+                pack16x2(f[6], f[7], BF)};
+}
+
+// where row `row` of the step goes in the cache: its sequence and slot, -1 if nowhere
+__device__ __forceinline__ int64_t rope_slot(const RopeArgs& a, int64_t row, int64_t pos, int64_t& b) {
+  b = (uint32_t)row / (uint32_t)a.n;  // below 2^31 both
+  const int64_t len = a.lengths[b];
+  if (pos < 0 || pos >= a.rope_rows || len < 0 || len > a.cap - a.n) return -1;
+  return len + (row - b * a.n);
+}
+
+// ONE: a workgroup takes one row, so that what follows from the row is uniform
+template <int D, bool BF, bool CACHE, bool COL, bool ONE>
+__global__ __launch_bounds__(256, D == 256 ? 4 : 5) void qk_norm_rope_kernel(const RopeArgs a) {
+  constexpr int LPG = D / 8;      // lanes per head
+  constexpr int G = 256 / LPG;    // heads at a time
+  constexpr int U = 4;            // loads of a lane on their way
+  const int lane = threadIdx.x % LPG, grp = threadIdx.x / LPG;
+  const int H = a.heads, KVH = a.kv_heads;
+  if constexpr (COL) {
+    constexpr int PITCH = kRopeTile + 2;  // 16-bit values
+    __shared__ uint16_t tile[D * PITCH];
+    __shared__ int64_t slots[kRopeTile];
+    if ((int64_t)blockIdx.x < a.col_wgs) {  // first: they take longest
+      // keys of one head, rows i0 .. of one sequence
+      constexpr int P = kRopeTile / G;  // passes, their loads all out at once
+      const int per_seq = (int)((a.n + kRopeTile - 1) / kRopeTile);
+      const int kvh = (int)blockIdx.x % KVH, rest = (int)blockIdx.x / KVH;
+      const int64_t b = rest / per_seq, i0 = (int64_t)(rest % per_seq) * kRopeTile;
+      const int count = (int)(a.n - i0 < kRopeTile ? a.n - i0 : kRopeTile);
+      const int64_t first = b * a.n + i0;
+      u32x4v u[P];
+      int64_t pos[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int64_t row = first + min(k * G + grp, count - 1);
+        pos[k] = a.positions[row];
+        u[k] = *reinterpret_cast<const u32x4v*>(a.qkv + row * a.ld + (int64_t)(H + kvh) * D + 8 * lane);
+      }
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int r = k * G + grp;
+        if (k * G >= count) break;
+        const RopeAngles ang = rope_angles(a, pos[k], lane);
+        const u32x4v out = rope_head<D, BF>(a, u[k], a.kw, ang, lane);
+        if (r < count) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t two = out[i / 2];
+            tile[(8 * lane + i) * PITCH + r] = (uint16_t)(two >> (16 * (i & 1)));
+          }
+          int64_t seq;
+          if (lane == 0) slots[r] = rope_slot(a, first + r, pos[k], seq);
+        }
+      }
+      __syncthreads();
+      uint16_t* k = a.kc + b * a.ks_b + kvh * a.ks_h;
+      const int chunks = (count + 7) / 8;
+      for (int t = threadIdx.x; t < D * chunks; t += 256) {
+        const int d = t / chunks, c = t - d * chunks;
+        bool whole = 8 * c + 8 <= count;
+        for (int e = 0; e < 8 && whole; ++e) whole = slots[8 * c + e] >= 0;
+        uint16_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[d * PITCH + 8 * c + e];
+        uint16_t* dst = k + d * a.ks_d;
+        if (whole) {
+          __builtin_memcpy(dst + slots[8 * c], v, 16);  // any alignment
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (8 * c + e < count && slots[8 * c + e] >= 0) dst[slots[8 * c + e]] = v[e];
+        }
+      }
+      return;
     }
   }
-  if (!live) return;
-  uint4 out;
-  out.x = pack16x2(v[0], v[1], BF);
-  out.y = pack16x2(v[2], v[3], BF);
-  out.z = pack16x2(v[4], v[5], BF);
-  out.w = pack16x2(v[6], v[7], BF);
-  if (!inside) out = make_uint4(0, 0, 0, 0);
-  if (head < H) {
-    *reinterpret_cast<uint4*>(a.q_out + (row * H + head) * D + 8 * lane) = out;
-    return;
+  const int wg = blockIdx.x - (COL ? (int)a.col_wgs : 0);
+  const int64_t row0 = ONE ? wg / a.parts : (int64_t)wg * a.rows_per_wg;
+  const int head0 = ONE ? (wg - (int)row0 * a.parts) * a.part : 0;
+  const int here = (int)(a.rows - row0 < a.rows_per_wg ? a.rows - row0 : a.rows_per_wg);
+  const int items = ONE ? min(a.part, a.per_row - head0) : here * a.per_row;
+  RopeAngles ang;
+  int64_t pos = 0, b = 0, slot = 0;
+  if constexpr (ONE) {
+    pos = a.positions[row0];
+    if constexpr (CACHE) slot = rope_slot(a, row0, pos, b);
   }
-  if constexpr (!CACHE) {
-    *reinterpret_cast<uint4*>(a.k_out + (row * KVH + head - H) * D + 8 * lane) = out;
-  } else {
-    const int64_t b = row / a.n, slot = a.lengths[b] + (row - b * a.n);
-    if (!inside || a.lengths[b] < 0 || a.lengths[b] > a.cap - a.n) return;
-    if (head >= H + KVH) {
-      *reinterpret_cast<uint4*>(a.vc + b * a.vs_b + (head - H - KVH) * a.vs_h + slot * a.vs_l +
-                                8 * lane) = out;
-    } else {
-      uint16_t* k = a.kc + b * a.ks_b + (head - H) * a.ks_h + slot * a.ks_l;
-      if (a.ks_d == 1) {
-        *reinterpret_cast<uint4*>(k + 8 * lane) = out;
-      } else {
-        const uint32_t u[4] = {out.x, out.y, out.z, out.w};
+  for (int i0 = 0; i0 < items; i0 += U * G) {
+    u32x4v u[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          k[(8 * lane + i) * a.ks_d] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+    for (int k = 0; k < U; ++k) {
+      const int item = min(i0 + k * G + grp, items - 1);
+      const int local = ONE ? 0 : item / a.per_row;
+      int head = head0 + item - local * a.per_row;
+      if (COL && head >= H) head += KVH;
+      u[k] = *reinterpret_cast<const u32x4v*>(a.qkv + (row0 + local) * a.ld + head * D + 8 * lane);
+    }
+    if (ONE && i0 == 0) ang = rope_angles(a, pos, lane);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int item = i0 + k * G + grp;
+      if (i0 + k * G >= items) break;
+      const bool live = item < items;  // the others take part in the exchanges
+      const int at = live ? item : items - 1;
+      const int local = ONE ? 0 : at / a.per_row;
+      int head = head0 + at - local * a.per_row;
+      if (COL && head >= H) head += KVH;
+      const int64_t row = row0 + local;
+      if constexpr (!ONE) {
+        pos = a.positions[row];
+        if constexpr (CACHE) slot = rope_slot(a, row, pos, b);
+        ang = rope_angles(a, pos, lane);
+      }
+      u32x4v out = u[k];
+      if (__any(head < H + KVH)) {  // a wave of values alone passes them
+        const u32x4v turned = rope_head<D, BF>(a, u[k], head < H ? a.qw : a.kw, ang, lane);
+        if (head < H + KVH) out = turned;
+      }
+      if (!live) continue;
+      if (head < H || !CACHE) {
+        if (pos < 0 || pos >= a.rope_rows) out = u32x4v{0, 0, 0, 0};
+        uint16_t* dst = head < H ? a.q_out + (row * H + head) * D : a.k_out + (row * KVH + head - H) * D;
+        *reinterpret_cast<u32x4v*>(dst + 8 * lane) = out;
+      } else if (slot >= 0) {
+        uint16_t* dst = head < H + KVH
+                            ? a.kc + b * a.ks_b + slot * a.ks_l + (head - H) * a.ks_h
+                            : a.vc + b * a.vs_b + slot * a.vs_l + (head - H - KVH) * a.vs_h;
+        *reinterpret_cast<u32x4v*>(dst + 8 * lane) = out;
       }
     }
   }
@@ -185,22 +340,41 @@ __global__ __launch_bounds__(256) void keep_cols_kernel(const KeepArgs a) {
   c[lane] = v;
 }
 
-template <bool BF, bool CACHE>
-static int launch_rope(int dim, const RopeArgs& a, hipStream_t st) {
-  const int64_t per = 256 / (dim / 8);
-  const int64_t grid = (a.items + per - 1) / per;
-  if (grid > INT32_MAX) return PE_ERR_DIMS;
-  if (dim == 64) qk_norm_rope_kernel<64, BF, CACHE><<<(unsigned)grid, 256, 0, st>>>(a);
-  else if (dim == 128) qk_norm_rope_kernel<128, BF, CACHE><<<(unsigned)grid, 256, 0, st>>>(a);
-  else qk_norm_rope_kernel<256, BF, CACHE><<<(unsigned)grid, 256, 0, st>>>(a);
+template <int D, bool BF, bool ONE>
+static int launch_rope(const RopeArgs& a, bool cache, bool col, int64_t grid, hipStream_t st) {
+  if (!cache) qk_norm_rope_kernel<D, BF, false, false, ONE><<<(unsigned)grid, 256, 0, st>>>(a);
+  else if (col) qk_norm_rope_kernel<D, BF, true, true, ONE><<<(unsigned)grid, 256, 0, st>>>(a);
+  else qk_norm_rope_kernel<D, BF, true, false, ONE><<<(unsigned)grid, 256, 0, st>>>(a);
   return launch_status();
+}
+template <int D, bool BF>
+static int launch_rope(RopeArgs a, bool cache, hipStream_t st) {
+  const bool col = cache && a.ks_d != 1;
+  a.per_row = a.heads + (!cache ? 1 : col ? 1 : 2) * a.kv_heads;
+  const int at_once = 256 / (D / 8);
+  a.rows_per_wg = a.per_row >= at_once ? 1 : at_once / a.per_row;
+  // few rows: a workgroup a pass, so that no pass waits for another
+  const int passes = (a.per_row + at_once - 1) / at_once;
+  a.parts = a.rows * passes <= 8 * (int64_t)num_cus() ? passes : 1;
+  a.part = a.parts > 1 ? at_once : a.per_row;
+  a.col_wgs = col ? a.rows / a.n * a.kv_heads * ((a.n + kRopeTile - 1) / kRopeTile) : 0;
+  const int64_t grid = a.col_wgs + (a.parts > 1 ? a.rows * a.parts
+                                                : (a.rows + a.rows_per_wg - 1) / a.rows_per_wg);
+  if (grid > INT32_MAX) return PE_ERR_DIMS;
+  return a.rows_per_wg == 1 ? launch_rope<D, BF, true>(a, cache, col, grid, st)
+                            : launch_rope<D, BF, false>(a, cache, col, grid, st);
+}
+template <bool BF>
+static int launch_rope(int dim, const RopeArgs& a, bool cache, hipStream_t st) {
+  return dim == 64 ? launch_rope<64, BF>(a, cache, st)
+         : dim == 128 ? launch_rope<128, BF>(a, cache, st) : launch_rope<256, BF>(a, cache, st);
 }
 
 // what both forms check and set
 static int rope_args(const void* qkv, int dtype, int64_t rows, int64_t ld, int heads, int kv_heads,
                      int head_dim, const float* rope, int64_t rope_rows, int rot,
                      const int64_t* positions, const void* q_weight, const void* k_weight, float eps,
-                     void* q_out, bool cache, RopeArgs& a) {
+                     void* q_out, RopeArgs& a) {
   if (!qkv || !rope || !positions || !q_out) return PE_ERR_NULL;
   if (bf16_flag(dtype) < 0) return PE_ERR_DTYPE;
   if (rows < 0 || heads < 1 || kv_heads < 1 || heads > 65536 || kv_heads > 65536 ||
@@ -215,9 +389,8 @@ static int rope_args(const void* qkv, int dtype, int64_t rows, int64_t ld, int h
   a.ld = ld;
   a.heads = heads;
   a.kv_heads = kv_heads;
-  a.per_row = heads + (cache ? 2 : 1) * kv_heads;
-  if (rows > INT64_MAX / 4 / a.per_row) return PE_ERR_DIMS;
-  a.items = rows * a.per_row;
+  if (rows > INT32_MAX) return PE_ERR_DIMS;
+  a.rows = rows;
   a.rot = rot;
   a.rope = rope;
   a.rope_rows = rope_rows;
@@ -251,15 +424,15 @@ extern "C" int pe_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t
                                void* stream) {
   RopeArgs a;
   const int rc = rope_args(qkv, dtype, rows, ld, heads, kv_heads, head_dim, rope, rope_rows, rot,
-                           positions, q_weight, k_weight, eps, q_out, false, a);
+                           positions, q_weight, k_weight, eps, q_out, a);
   if (rc != PE_OK) return rc;
   if (!k_out) return PE_ERR_NULL;
   if (!aligned16(k_out)) return PE_ERR_ALIGN;
   if (rows == 0) return PE_OK;
   a.k_out = reinterpret_cast<uint16_t*>(k_out);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return bf16_flag(dtype) ? launch_rope<true, false>(head_dim, a, st)
-                          : launch_rope<false, false>(head_dim, a, st);
+  return bf16_flag(dtype) ? launch_rope<true>(head_dim, a, false, st)
+                          : launch_rope<false>(head_dim, a, false, st);
 }
 
 extern "C" int pe_qk_norm_rope_write(const void* qkv, int dtype, int64_t batch, int64_t n, int64_t ld,
@@ -271,10 +444,10 @@ extern "C" int pe_qk_norm_rope_write(const void* qkv, int dtype, int64_t batch, 
                                      int64_t vs_h, int64_t vs_l, const int64_t* lengths, int64_t cap,
                                      void* stream) {
   if (!k_cache || !v_cache || !lengths) return PE_ERR_NULL;
-  if (batch < 0 || n < 1 || batch > INT64_MAX / 8 / n || cap < 1) return PE_ERR_DIMS;
+  if (batch < 0 || n < 1 || n > INT32_MAX || batch > INT64_MAX / 8 / n || cap < 1) return PE_ERR_DIMS;
   RopeArgs a;
   const int rc = rope_args(qkv, dtype, batch * n, ld, heads, kv_heads, head_dim, rope, rope_rows, rot,
-                           positions, q_weight, k_weight, eps, q_out, true, a);
+                           positions, q_weight, k_weight, eps, q_out, a);
   if (rc != PE_OK) return rc;
   const int ok = cache_strides(k_cache, ks_b, ks_h, ks_l, ks_d, v_cache, vs_b, vs_h, vs_l);
   if (ok != PE_OK) return ok;
@@ -287,8 +460,8 @@ extern "C" int pe_qk_norm_rope_write(const void* qkv, int dtype, int64_t batch, 
   a.n = n;
   a.cap = cap;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return bf16_flag(dtype) ? launch_rope<true, true>(head_dim, a, st)
-                          : launch_rope<false, true>(head_dim, a, st);
+  return bf16_flag(dtype) ? launch_rope<true>(head_dim, a, true, st)
+                          : launch_rope<false>(head_dim, a, true, st);
 }
 
 extern "C" int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int64_t cap,
