@@ -56,50 +56,62 @@ __host__ __device__ inline int64_t part_words(int rb, int dim) { return (int64_t
 // An empty slot of the batch has one tile, without positions, for its zeros. Both
 // launches and every wave find their way by themselves, from the lengths alone.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int wave_sum_i32(int v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+// running sum over the 64 lanes: DPP row_shr within 16 lanes, then the rows
+__device__ __forceinline__ int wave_scan_i32(int v, int lane) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31);
+  const int r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+  return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
 __device__ __forceinline__ bool tree_active(const TreeAttnArgs& a, int64_t len) {
   return len >= 0 && len <= a.cap - a.n;
 }
-__device__ __forceinline__ int tree_tiles(const TreeAttnArgs& a, int b) {
-  if (b >= a.batch) return 0;
-  const int64_t len = a.lengths[b];
-  return tree_active(a, len) ? (int)((len + a.n + kTile - 1) / kTile) : 1;
+// 64 sequences of the batch, one a lane
+struct TreeChunk {
+  int64_t len;
+  int tiles, scan;  // and their running sum
+};
+__device__ __forceinline__ TreeChunk tree_chunk(const TreeAttnArgs& a, int b0, int lane) {
+  TreeChunk c{-1, 0, 0};
+  if (b0 + lane < a.batch) {
+    c.len = a.lengths[b0 + lane];
+    if (!tree_active(a, c.len)) c.len = -1;
+    c.tiles = c.len >= 0 ? (int)((c.len + a.n + kTile - 1) / kTile) : 1;
+  }
+  c.scan = wave_scan_i32(c.tiles, lane);
+  return c;
 }
-// tiles before sequence `upto`, one KV head of each (lanes take sequences)
-__device__ __forceinline__ int tree_tiles_before(const TreeAttnArgs& a, int upto, int lane) {
-  int total = 0;
-  for (int b = lane; b < upto; b += 64) total += tree_tiles(a, b);
-  return wave_sum_i32(total);
+// tiles of all sequences, one KV head of each; c: the first chunk
+__device__ __forceinline__ int tree_total(const TreeAttnArgs& a, const TreeChunk& c, int lane) {
+  int total = __builtin_amdgcn_readlane(c.scan, 63);
+  for (int b0 = 64; b0 < a.batch; b0 += 64)
+    total += __builtin_amdgcn_readlane(tree_chunk(a, b0, lane).scan, 63);
+  return total;
 }
-// the sequence that holds place `at` of the line, and the tiles before it
+// a sequence: its number, tiles, the tiles before it, and its length (-1: empty slot)
 struct TreePlace {
   int b, tiles, before;
+  int64_t len;
 };
-__device__ __forceinline__ TreePlace tree_find(const TreeAttnArgs& a, int at, int lane) {
-  TreePlace p{-1, 0, 0};
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int t = tree_tiles(a, b0 + lane);
-    int scan = t;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(scan, off, 64);
-      if (lane >= off) scan += o;
-    }
-    const uint64_t hit = __ballot((p.before + scan) * a.kv_heads > at);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      p.b = b0 + l;
-      p.before += __builtin_amdgcn_readlane(scan - t, l);
-      p.tiles = __builtin_amdgcn_readlane(t, l);
-      return p;
-    }
-    p.before += __builtin_amdgcn_readlane(scan, 63);
+__device__ __forceinline__ TreePlace tree_lane(const TreeChunk& c, int b0, int before, int l) {
+  const int t = __builtin_amdgcn_readlane(c.tiles, l);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)c.len, l);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)c.len >> 32), l);
+  return TreePlace{b0 + l, t, before + __builtin_amdgcn_readlane(c.scan, l) - t,
+                   (int64_t)((uint64_t)hi << 32 | lo)};
+}
+// the sequence that holds place `at` of the line (it is on it)
+__device__ __forceinline__ TreePlace tree_find(const TreeAttnArgs& a, TreeChunk c, int at, int lane) {
+  int before = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const uint64_t hit = __ballot((before + c.scan) * a.kv_heads > at);
+    if (hit) return tree_lane(c, b0, before, __builtin_ctzll(hit));
+    before += __builtin_amdgcn_readlane(c.scan, 63);
+    c = tree_chunk(a, b0 + 64, lane);
   }
-  return p;
 }
 
 // MFMA and conversions of the 16-bit type
@@ -172,7 +184,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   const int rem = (int)blockIdx.x % span;
   const int run = (int)blockIdx.x / span * 8 + rem % 8;
   const int rblk = rem / 8;
-  const int total = tree_tiles_before(a, a.batch, threadIdx.x & 63) * a.kv_heads;
+  const TreeChunk chunk = tree_chunk(a, 0, threadIdx.x & 63);
+  const int total = tree_total(a, chunk, threadIdx.x & 63) * a.kv_heads;
   const int size = (total + a.runs - 1) / a.runs;
   const int line_end = min(total, (run + 1) * size);
   for (int at = run * size; at < line_end;) {
@@ -181,14 +194,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   // them it would not leave registers enough for the tiles
   asm volatile("" : "+v"(tid));
   const int lane = tid & 63, li = lane & 15, lg = lane >> 4;
-  const TreePlace place = tree_find(a, at, lane);
+  const TreePlace place = tree_find(a, chunk, at, lane);
   const int b = place.b, tiles = place.tiles;
   const int kvh = (at - place.before * a.kv_heads) / tiles;
   const int t0 = at - place.before * a.kv_heads - kvh * tiles;
   const int t1 = min(tiles, t0 + line_end - at);
   at += t1 - t0;
-  const bool live = tree_active(a, a.lengths[b]);
-  const int64_t len = live ? a.lengths[b] : 0, end = len + a.n;
+  const bool live = place.len >= 0;
+  const int64_t len = live ? place.len : 0, end = len + a.n;
   const uint16_t* kb = a.k + (int64_t)b * a.ks_b + kvh * a.ks_h;
   const uint16_t* vb = a.v + (int64_t)b * a.vs_b + kvh * a.vs_h;
 
@@ -513,47 +526,67 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, int rb) {
   constexpr int E = D / 64;
+  constexpr int U = 8;  // parts on their way
+  typedef float floatE __attribute__((ext_vector_type(E)));
   const int lane = threadIdx.x & 63;
-  const int r = (int)blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
-  const int total = tree_tiles_before(a, a.batch, lane) * a.kv_heads;
+  const int r = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  TreeChunk c = tree_chunk(a, 0, lane);
+  const int total = tree_total(a, c, lane) * a.kv_heads;
   const int size = (total + a.runs - 1) / a.runs;
-  const int tiles = __builtin_amdgcn_readfirstlane(tree_tiles(a, b));
-  const int start = tree_tiles_before(a, b, lane) * a.kv_heads + kvh * tiles;
-  const int run0 = start / size, parts = (start + tiles - 1) / size - run0 + 1;
+  int before = 0;
+  for (int b0 = 0; b0 + 64 <= b; b0 += 64) {
+    before += __builtin_amdgcn_readlane(c.scan, 63);
+    c = tree_chunk(a, b0 + 64, lane);
+  }
+  const TreePlace place = tree_lane(c, b & ~63, before, b & 63);
+  const int start = place.before * a.kv_heads + kvh * place.tiles;
+  const int run0 = start / size, parts = (start + place.tiles - 1) / size - run0 + 1;
   if (parts == 1 || r >= a.rows) return;
   const int64_t words = part_words(rb, D), step = 2 * a.blocks * words;  // to the next run
   const int local = r % rb;
   // the first part is its run's last, the others are their runs' first
   const float* base = a.parts + ((int64_t)run0 * a.blocks + r / rb) * 2 * words;
   auto part = [&](int s) { return base + s * step + (s == 0 ? words : 0); };
-  float m = -__builtin_inff();
-  for (int s = lane; s < parts; s += 64) m = fmaxf(m, part(s)[rb * D + local]);
+  floatE t[U];
+  auto load = [&](int s0) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  if (m == -__builtin_inff()) m = 0.f;
-  float l = 0.f, o[E] = {};
+    for (int u = 0; u < U; ++u)
+      t[u] = reinterpret_cast<const floatE*>(part(min(s0 + u, parts - 1)) + local * D)[lane];
+  };
+  load(0);
+  float m = -__builtin_inff(), l = 0.f;
+  floatE o = 0.f;
   for (int s0 = 0; s0 < parts; s0 += 64) {
-    float w = 0.f;
-    if (s0 + lane < parts) {
-      const float* p = part(s0 + lane) + rb * D + local;
-      w = __builtin_amdgcn_exp2f(p[0] - m);
-      l += w * p[rb];
-    }
     const int here = min(64, parts - s0);
-    for (int s = 0; s < here; ++s) {
-      const float ws = __shfl(w, s, 64);
-      const float* p = part(s0 + s) + local * D + lane * E;
+    const float* p = part(s0 + min(lane, here - 1)) + rb * D + local;
+    const float pm = lane < here ? p[0] : -__builtin_inff(), pl = p[rb];
+    float mn = pm;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(ws, p[e], o[e]);
+    for (int off = 32; off >= 1; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off, 64));
+    mn = fmaxf(mn, m);
+    const float shift = mn == -__builtin_inff() ? 0.f : mn;
+    const float w = __builtin_amdgcn_exp2f(pm - shift), al = __builtin_amdgcn_exp2f(m - shift);
+    m = mn;
+    o *= al;
+    l = l * al + wave_sum_dpp(lane < here ? w * pl : 0.f);
+    for (int s = 0; s < here; s += U) {
+      if (s0 + s > 0) load(s0 + s);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s + u < here)
+          o += t[u] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w),
+                                                                          s + u));
     }
   }
-  l = wave_sum(l);
   const int node = r / a.group, g = r - node * a.group;
   uint16_t* dst = a.out + (((int64_t)b * a.n + node) * a.kv_heads * a.group +
                            (int64_t)kvh * a.group + g) * D + lane * E;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  uint16_t h[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = to16(o[e] * inv, BF);
+  for (int e = 0; e < E; ++e) h[e] = to16(o[e] * inv, BF);
+  __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
 }
 
 // rows of a workgroup: as many as the rows of a KV head fill
