@@ -31,6 +31,7 @@ namespace pe {
 
 constexpr int kTile = 64;          // positions of a tile
 constexpr float kTreeLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;      // powers of two that an exponent may exceed its base by
 
 struct TreeAttnArgs {
   const uint16_t* q;
@@ -147,6 +148,16 @@ __device__ __forceinline__ u32x4v lds_ld16(const lds_byte* p) {
 __device__ __forceinline__ void lds_st16v(lds_byte* p, u32x4v v) {
   *reinterpret_cast<__attribute__((address_space(3))) u32x4v*>(p) = v;
 }
+// maximum over the four lanes li, li + 16, li + 32, li + 48, in each of them
+__device__ __forceinline__ float rows_max(float v) {
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  u = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+  auto b = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
 // whether one of the eight 16-bit values is infinite or NaN
 template <bool BF>
 __device__ __forceinline__ bool not_finite8(u32x4v u) {
@@ -210,7 +221,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   // that the reads below, 16 bytes of 16 rows or 32 bytes of 8 rows at a time, touch
   // every bank once; the permutations are linear in the bits of the row, so pass i
   // adds a constant. Addresses are a uniform 64-bit base and the thread's 32-bit
-  // offset (strides below 2^26). Rows from `end` on repeat the last one. Keys by
+  // offset (strides below 2^26). Rows past the cache repeat the last one. Keys by
   // dimension have any alignment and go through registers: chunk c is dimension
   // c / 8, eight positions c % 8.
   auto k_swz = [](int key) { return D == 64 ? key >> 1 & 7 : key & 15; };
@@ -234,7 +245,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
       __builtin_amdgcn_global_load_lds((const glb_byte*)from, to + plane + (i * 4 + wave) * 1024, 16,
                                        0, 0);
     };
-    if (p0 + kTile <= end) {
+    if (p0 + kTile <= a.cap) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         if constexpr (KCOL) __builtin_memcpy(&kr[i], k_base(i) + koff, 16);
@@ -243,17 +254,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
       }
       return;
     }
-    const int left = (int)(end - p0);
+    const int last = (int)(end - p0) - 1;  // the cache ends within the tile
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int row = min(srow + i * KPI, left - 1) - i * KPI;  // may lie before the pass
+      const int row = min(srow + i * KPI, last) - i * KPI;  // may lie before the pass
       dma(v_base(i) + ((int64_t)row * (int)a.vs_l * 2 + vch), i, VT);
       if constexpr (KCOL) {
-        kr[i] = u32x4v{0, 0, 0, 0};
+        const int first = (tid & 7) * 8;
         const uint16_t* s = reinterpret_cast<const uint16_t*>(k_base(i) + koff);
+        uint32_t h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if ((tid & 7) * 8 + e < left) kr[i][e / 2] |= (uint32_t)s[e] << (16 * (e & 1));
+        for (int e = 0; e < 8; ++e) h[e] = s[min(first + e, last) - first];
+        kr[i] = u32x4v{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
       } else {
         dma(k_base(i) + ((int64_t)row * (int)a.ks_l * 2 + (kch ^ k_swz(i * KPI) << 4)), i, 0);
       }
@@ -363,17 +375,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           top = fmaxf(top, s[kt][rt][e]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(m[rt], top * c);
-      const float base = mn == -__builtin_inff() ? 0.f : mn;
-      if (__any(mn > m[rt])) {
-        const float al = __builtin_amdgcn_exp2f(m[rt] - base);
+      top = rows_max(top) * c;
+      // m is what the exponents are relative to: it moves only where they would pass
+      // kSlack (a factor that neither sums nor 16-bit values mind), so that most tiles
+      // leave the sums alone
+      if (__any(top > m[rt] + kSlack)) {
+        const float mn = fmaxf(m[rt], top);
+        const float al = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
         l[rt] *= al;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
         m[rt] = mn;
       }
+      const float base = m[rt] == -__builtin_inff() ? 0.f : m[rt];
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt) {
         float p[4];
@@ -387,16 +401,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
     }
     if (!kTail || !slow) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const lds_byte* p = cur + vat + (((dt & 7) ^ vx) << 5) + (dt >> 3) * 256;
-        if constexpr (NKT == 1) {
-          const u32x2v vf = lds_tr(p);
+      for (int kt = 0; kt < NKT; kt += 2)
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma16<BF>(vf, pf[0][rt], o[rt][dt]);
-        } else {
+        for (int dt = 0; dt < DT; ++dt) {
+          const lds_byte* p = cur + vat + kt * 16 * ROW + (((dt & 7) ^ vx) << 5) + (dt >> 3) * 256;
+          if constexpr (NKT == 1) {
+            const u32x2v vf = lds_tr(p);
 #pragma unroll
-          for (int kt = 0; kt < NKT; kt += 2) {
-            const u32x2v lo = lds_tr(p + kt * 16 * ROW), hi = lds_tr(p + (kt + 1) * 16 * ROW);
+            for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma16<BF>(vf, pf[0][rt], o[rt][dt]);
+          } else {
+            const u32x2v lo = lds_tr(p), hi = lds_tr(p + 16 * ROW);
             const u32x4v vf{lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -404,7 +418,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
                                                 pf[kt + 1][rt][1]}, o[rt][dt]);
           }
         }
-      }
     } else {
       // key by key, skipping what a row does not see; the probabilities take the
       // place of the keys, 64-lane words of one 16-key block after the other
