@@ -18,20 +18,24 @@ is no scheduler, sampler beyond argmax, paged cache or tokenizer.
 One decode step (``DecodeRunner.step``) takes the batch's current tokens and
 position (device tensors, so the step can be captured in a HIP graph and
 replayed) and returns the logits; ``greedy_tokens_per_s`` replays it with
-the argmax fed back.
+the argmax fed back. ``DecodeRunner.tree_step`` takes several drafted tokens per
+sequence (a chain or a tree, sequences of different lengths) through the same
+layers, ``DecodeRunner.speculative_round`` verifies them, moves what stands to its
+place in the cache and returns the new tokens (kernels.tree_decode).
 """
 
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple, Union
 
 import torch
 
 from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
+from polarengine_vllm.kernels import tree_decode
 from polarengine_vllm.linear_method import PolarQuantLinearMethod
 
 
@@ -46,6 +50,7 @@ class DecoderConfig:
     vocab: int = 151936
     rope_theta: float = 1.0e6
     rms_eps: float = 1e-6
+    qk_norm: bool = False  # RMS norm of every query and key head before the rotation
     # bits per linear: the mixed assignment of one C4 decoder layer
     bits: Dict[str, int] = field(default_factory=lambda: {
         "qkv_proj": 5, "o_proj": 6, "gate_up_proj": 3, "down_proj": 4})
@@ -164,6 +169,10 @@ class DecodeRunner:
             self.layers.append({
                 "in_norm": torch.ones(c.hidden, device=self.dev, dtype=bf),
                 "post_norm": torch.ones(c.hidden, device=self.dev, dtype=bf),
+                # per-head norms of queries and keys, where the model has them
+                **{name: lw[name].to(self.dev, bf) if name in lw
+                   else torch.ones(c.head_dim, device=self.dev, dtype=bf)
+                   for name in ("q_norm", "k_norm") if c.qk_norm},
                 "qkv_proj": mk("qkv_proj", c.hidden, [q_sz, kv_sz, kv_sz]),
                 "o_proj": mk("o_proj", q_sz, [c.hidden]),
                 "gate_up_proj": mk("gate_up_proj", c.hidden, [c.intermediate, c.intermediate]),
@@ -201,9 +210,12 @@ class DecodeRunner:
         """One decode step for the batch: tokens [B] int64, pos [1] int64 (the
         position every sequence of the batch writes); returns fp32 logits
         [B, vocab]."""
+        return self._layers(tokens, self._attention(pos))
+
+    def _layers(self, tokens: torch.Tensor, attend) -> torch.Tensor:
+        """All layers and the lm_head for rows of tokens, with a step's attention."""
         c = self.cfg
         x = self.embed.index_select(0, tokens)  # residual stream, bf16
-        attend = self._attention(pos)
         r = None  # what the last block adds to the residual stream
         for i, ly in enumerate(self.layers):
             x, h = _add_norm(x, r, ly["in_norm"], c.rms_eps)
@@ -211,7 +223,47 @@ class DecodeRunner:
             x, h = _add_norm(x, ly["o_proj"](o), ly["post_norm"], c.rms_eps)
             r = ly["down_proj"](_silu_mul(ly["gate_up_proj"](h)))
         x, h = _add_norm(x, r, self.final_norm, c.rms_eps)
-        return _lm_head(h, self.lm_head)  # [B, vocab]
+        return _lm_head(h, self.lm_head)  # [rows, vocab]
+
+    def tree_step(self, tokens: torch.Tensor, lengths: torch.Tensor,
+                  parents: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One step with n tokens per sequence, 1 <= n <= 64: tokens int64 [B, n],
+        node 0 a sequence's last token, the others drafts that follow node
+        ``parents[i]`` (int64 [B, n] or [n]; a chain without it); lengths int64 [B],
+        the cached positions of each sequence, below 0 for an empty slot. Keys and
+        values go to slots ``lengths[b] + i`` of the cache. Returns fp32 logits
+        [B, n, vocab] after every node (of no meaning for absent nodes: token -1 or
+        no parent). Everything is read on the device, so that a captured step
+        serves every length and tree."""
+        B, n = self.batch, tokens.shape[-1]
+        if tokens.shape != (B, n) or tokens.dtype != torch.int64:
+            raise ValueError(f"tokens must be int64 [{B}, n], got {tokens.dtype} of "
+                             f"{list(tokens.shape)}")
+        if lengths.shape != (B,):
+            raise ValueError(f"lengths must be int64 [{B}], got {list(lengths.shape)}")
+        if parents is None:
+            parents = torch.arange(-1, n - 1, device=self.dev)
+        plan = tree_decode.tree_plan(parents, lengths)
+        attend = self._attention_tree(lengths, plan.positions, plan.masks)
+        return self._layers(tokens.clamp(0, self.cfg.vocab - 1).view(-1), attend).view(B, n, -1)
+
+    def speculative_round(self, tokens: torch.Tensor, lengths: torch.Tensor,
+                          uniforms: torch.Tensor, parents: Optional[torch.Tensor] = None,
+                          draft_probs: Optional[torch.Tensor] = None,
+                          temperature: Union[float, torch.Tensor] = 1.0
+                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``tree_step``, verification of the drafts (``verify_drafts``: uniforms
+        [B, n], draft_probs [B, n - 1, vocab] for a chain that was drawn), and the
+        accepted nodes' keys and values moved to their places in every layer.
+        ``lengths`` grows by ``count`` in place. Returns (out, path, count):
+        ``out[b, :count[b]]`` are the new tokens, the last of them the next round's
+        node 0."""
+        logits = self.tree_step(tokens, lengths, parents)
+        out, path, count = tree_decode.verify_drafts(logits, tokens, uniforms, parents, draft_probs,
+                                                     temperature)
+        tree_decode.keep_accepted(self.k_cache.transpose(-1, -2), self.v_cache, lengths, path, count)
+        lengths.add_(count)
+        return out, path, count
 
     def _attention(self, pos: torch.Tensor):
         """The step's attention, as a function of (layer, qkv rows) -> [B, H * D]:
@@ -220,6 +272,8 @@ class DecodeRunner:
         takes; pos must lie in the cache, which the table lookup checks."""
         c, B = self.cfg, self.batch
         H, KVH, D = c.heads, c.kv_heads, c.head_dim
+        if c.qk_norm:
+            return self._attention_normed(pos)
         ws_bytes = _lib.workspace_size("pe_decode_attention_workspace_size", B, KVH,
                                        H // KVH if H % KVH == 0 else 0, D, self.max_len)
         kc, vc = self.k_cache, self.v_cache
@@ -247,6 +301,31 @@ class DecodeRunner:
 
         return attend
 
+    def _attention_normed(self, pos: torch.Tensor):
+        """The same with per-head norms of queries and keys: a tree of one node."""
+        c = self.cfg
+        if (c.head_dim not in (64, 128, 256) or c.heads % c.kv_heads
+                or not _kernel_operands(self.k_cache, self.v_cache)):
+            return self._attention_torch(pos)
+        lengths = pos.expand(self.batch).contiguous()
+        return self._attention_tree(lengths, lengths, torch.ones_like(lengths)[:, None])
+
+    def _attention_tree(self, lengths: torch.Tensor, positions: torch.Tensor, masks: torch.Tensor):
+        """A step's attention over n nodes per sequence, as a function of (layer, qkv
+        rows) -> [batch * n, H * D]: norms, rotary embedding and cache write in one
+        launch, attention over the cache in one or two."""
+        c, B, n = self.cfg, self.batch, masks.shape[1]
+
+        def attend(i: int, qkv: torch.Tensor) -> torch.Tensor:
+            ly, k, v = self.layers[i], self.k_cache[i].transpose(-1, -2), self.v_cache[i]
+            q = tree_decode.qk_norm_rope_write(
+                qkv, c.heads, c.kv_heads, self.rope, positions, k, v, lengths, ly.get("q_norm"),
+                ly.get("k_norm"), c.rms_eps)
+            o = tree_decode.tree_attention(q.view(B, n, c.heads, c.head_dim), k, v, lengths, masks)
+            return o.view(B * n, c.heads * c.head_dim)
+
+        return attend
+
     def _attention_torch(self, pos: torch.Tensor):
         c, B = self.cfg, self.batch
         H, KVH, D = c.heads, c.kv_heads, c.head_dim
@@ -260,6 +339,10 @@ class DecodeRunner:
         def attend(i: int, qkv: torch.Tensor) -> torch.Tensor:
             # rotate-half RoPE on the q and k heads together
             qk = qkv[:, :(H + KVH) * D].reshape(B, H + KVH, D).float()
+            if c.qk_norm:
+                w = torch.cat([self.layers[i]["q_norm"].expand(H, D),
+                               self.layers[i]["k_norm"].expand(KVH, D)]).float()
+                qk = torch.nn.functional.rms_norm(qk, (D,), eps=c.rms_eps) * w
             x1, x2 = qk[..., :hd], qk[..., hd:]
             qk = torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], -1)
             q = (qk[:, :H] * scale).to(torch.bfloat16).reshape(B, KVH, grp, D)
