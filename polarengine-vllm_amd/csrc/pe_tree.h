@@ -7,6 +7,7 @@ namespace pe {
 
 constexpr int kTreeMax = 64;  // nodes of a tree: one bit each of a 64-bit mask, one lane each
 
+constexpr int64_t kTreeMaxGrid = (1 << 24) - 1;          // workgroups of 256 along x
 constexpr int64_t kTreeMaxStride = (int64_t)1 << 26;  // elements, of positions and dimensions
 
 // Ancestor mask (itself among them) of node i = lane of a wave, from its parent:

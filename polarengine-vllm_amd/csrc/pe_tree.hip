@@ -360,7 +360,7 @@ static int launch_rope(RopeArgs a, bool cache, hipStream_t st) {
   a.col_wgs = col ? a.rows / a.n * a.kv_heads * ((a.n + kRopeTile - 1) / kRopeTile) : 0;
   const int64_t grid = a.col_wgs + (a.parts > 1 ? a.rows * a.parts
                                                 : (a.rows + a.rows_per_wg - 1) / a.rows_per_wg);
-  if (grid > INT32_MAX) return PE_ERR_DIMS;
+  if (grid > kTreeMaxGrid) return PE_ERR_DIMS;
   return a.rows_per_wg == 1 ? launch_rope<D, BF, true>(a, cache, col, grid, st)
                             : launch_rope<D, BF, false>(a, cache, col, grid, st);
 }
@@ -409,7 +409,7 @@ using namespace pe;
 extern "C" int pe_tree_plan(const int64_t* parents, int64_t parents_stride, const int64_t* lengths,
                             int64_t batch, int n, int64_t* positions, int64_t* masks, void* stream) {
   if (!parents || !lengths || !positions || !masks) return PE_ERR_NULL;
-  if (batch < 0 || batch > INT32_MAX || n < 1 || n > kTreeMax || parents_stride < 0)
+  if (batch < 0 || batch > kTreeMaxGrid || n < 1 || n > kTreeMax || parents_stride < 0)
     return PE_ERR_DIMS;
   if (batch == 0) return PE_OK;
   tree_plan_kernel<<<(unsigned)batch, 64, 0, reinterpret_cast<hipStream_t>(stream)>>>(
@@ -479,6 +479,7 @@ extern "C" int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int 
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t items = (int64_t)heads * (s_d == 1 ? dim / 8 : dim);
   const int64_t per = s_d == 1 ? 256 : 4;
+  if ((items + per - 1) / per > kTreeMaxGrid) return PE_ERR_DIMS;
   const dim3 grid((unsigned)((items + per - 1) / per), (unsigned)batch, (unsigned)layers);
   if (s_d == 1) keep_rows_kernel<<<grid, 256, 0, st>>>(a);
   else keep_cols_kernel<<<grid, 256, 0, st>>>(a);

@@ -536,7 +536,7 @@ static int pieces(int64_t V, int chunk) { return (int)((V + chunk - 1) / chunk);
 static bool verify_shape_ok(int64_t batch, int n, int64_t vocab) {
   return batch >= 1 && batch <= 65535 && n >= 1 && n <= kTreeMax && vocab >= 1 &&
          vocab <= (int64_t)1 << 24 &&
-         batch * n * pieces(vocab, kStatChunk) <= INT32_MAX;
+         batch * n * pieces(vocab, kStatChunk) <= kTreeMaxGrid;
 }
 
 static size_t stats_bytes(int64_t batch, int n, int64_t vocab) {

@@ -48,31 +48,35 @@ class TreePlan(NamedTuple):
     masks: torch.Tensor      # bit j of node i's word: j is i or an ancestor of i
 
 
-class _Device:
-    """The tensors' device as the current one, where it is another."""
-
-    def __init__(self, dev: torch.device) -> None:
-        self.dev = dev
-
-    def __enter__(self) -> int:
-        self.back = torch.cuda.current_device()
-        if self.back != self.dev.index:
-            torch.cuda.set_device(self.dev)
-        return _lib.stream_ptr(self.dev)
-
-    def __exit__(self, *exc) -> None:
-        if self.back != self.dev.index:
-            torch.cuda.set_device(self.back)
+def _call(name: str, dev: torch.device, *args) -> None:
+    """One call into the library on the device's current stream, the device made the
+    current one around it where it is another."""
+    lib = _lib.lib()
+    here, index = torch._C._cuda_getDevice(), dev.index
+    if here == index:
+        rc = getattr(lib, name)(*args, _lib.stream_ptr(dev))
+    else:
+        torch._C._cuda_setDevice(index)
+        try:
+            rc = getattr(lib, name)(*args, _lib.stream_ptr(dev))
+        finally:
+            torch._C._cuda_setDevice(here)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _inputs(*tensors: Optional[torch.Tensor]) -> torch.device:
-    dev = _lib.require_device(*tensors)
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
+    """The one GPU of the tensors; refuses others, and inputs that autograd follows."""
+    grad = torch.is_grad_enabled()
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None:
+            if t.get_device() != index or index < 0:
+                _lib.require_device(*tensors)
+            if grad and t.requires_grad:
                 raise RuntimeError("the drafted-token kernels have no backward pass: call them "
                                    "under torch.no_grad() or detach their inputs")
-    return dev
+    return tensors[0].device
 
 
 def _int64(t: torch.Tensor, shape: Tuple[int, ...], name: str) -> torch.Tensor:
@@ -108,7 +112,8 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype: torch.dtype):
                          f"{list(k.shape)} and {list(v.shape)}")
     if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError(f"caches must be {dtype} as the queries, got {k.dtype} and {v.dtype}")
-    ks, vs = k.stride(), v.stride()
+    # a stride along one element says nothing
+    ks, vs = ([0 if n == 1 else st for st, n in zip(t.stride(), t.shape)] for t in (k, v))
     if vs[3] != 1 or (ks[3] != 1 and ks[2] != 1):
         raise ValueError("values must have the dimension contiguous, keys the dimension or the "
                          f"position; got strides {vs} and {ks}")
@@ -117,12 +122,18 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype: torch.dtype):
 
 def _writable(t: torch.Tensor, name: str) -> None:
     """Refuses views whose elements may share memory."""
+    st, n = t.stride(), t.shape
+    if len(n) == 4:  # rows or columns of a head, one head after the other: the usual layouts
+        low, high = (2, 3) if st[2] == 1 else (3, 2)
+        if (st[low] == 1 and st[high] >= n[low] and st[1] >= st[high] * n[high]
+                and st[0] >= st[1] * n[1]):
+            return
     span = 1
-    for stride, size in sorted(zip(t.stride(), t.shape)):
+    for stride, size in sorted(zip(st, n)):
         if size > 1:
             if stride < span:
-                raise ValueError(f"{name} overlaps itself (shape {list(t.shape)}, strides "
-                                 f"{t.stride()}): it cannot be written")
+                raise ValueError(f"{name} overlaps itself (shape {list(n)}, strides {st}): it "
+                                 f"cannot be written")
             span += stride * (size - 1)
 
 
@@ -144,13 +155,12 @@ def tree_plan(parents: torch.Tensor, lengths: torch.Tensor) -> TreePlan:
     _nodes(n)
     parents, stride = _per_node(parents, batch, n, "parents")
     lengths = _int64(lengths, (batch,), "lengths")
-    positions, masks = torch.empty(2, batch, n, dtype=torch.int64, device=dev)
+    positions = torch.empty(batch, n, dtype=torch.int64, device=dev)
+    masks = torch.empty(batch, n, dtype=torch.int64, device=dev)
     if not batch:
         return TreePlan(positions, masks)
-    with _Device(dev) as st:
-        _lib.check(_lib.lib().pe_tree_plan(parents.data_ptr(), stride, lengths.data_ptr(), batch, n,
-                                           positions.data_ptr(), masks.data_ptr(), st),
-                   "pe_tree_plan")
+    _call("pe_tree_plan", dev, parents.data_ptr(), stride, lengths.data_ptr(), batch, n,
+          positions.data_ptr(), masks.data_ptr())
     return TreePlan(positions, masks)
 
 
@@ -204,11 +214,9 @@ def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, rope: torch.Tenso
     k = torch.empty(rows, kv_heads, dim, dtype=qkv.dtype, device=dev)
     if not rows:
         return q, k
-    with _Device(dev) as st:
-        _lib.check(_lib.lib().pe_qk_norm_rope(
-            qkv.data_ptr(), code, rows, qkv.stride(0), heads, kv_heads, dim, rope.data_ptr(),
-            rope.shape[0], rope.shape[1], positions.data_ptr(), _lib.ptr(qw), _lib.ptr(kw), eps,
-            q.data_ptr(), k.data_ptr(), st), "pe_qk_norm_rope")
+    _call("pe_qk_norm_rope", dev, qkv.data_ptr(), code, rows, qkv.stride(0), heads, kv_heads, dim,
+          rope.data_ptr(), rope.shape[0], rope.shape[1], positions.data_ptr(), _lib.ptr(qw),
+          _lib.ptr(kw), eps, q.data_ptr(), k.data_ptr())
     return q, k
 
 
@@ -232,14 +240,14 @@ def qk_norm_rope_write(qkv: torch.Tensor, heads: int, kv_heads: int, rope: torch
         raise ValueError(f"{rows} rows do not go into {batch} sequences")
     _writable(k_cache, "k_cache")
     _writable(v_cache, "v_cache")
+    if k_cache.data_ptr() == v_cache.data_ptr() and rows:
+        raise ValueError("k_cache and v_cache are the same memory")
     q = torch.empty(rows, heads, dim, dtype=qkv.dtype, device=dev)
     if rows:
-        with _Device(dev) as st:
-            _lib.check(_lib.lib().pe_qk_norm_rope_write(
-                qkv.data_ptr(), code, batch, rows // batch, qkv.stride(0), heads, kv_heads, dim,
-                rope.data_ptr(), rope.shape[0], rope.shape[1], positions.data_ptr(), _lib.ptr(qw),
-                _lib.ptr(kw), eps, q.data_ptr(), k_cache.data_ptr(), *ks, v_cache.data_ptr(),
-                *vs[:3], lengths.data_ptr(), shape[2], st), "pe_qk_norm_rope_write")
+        _call("pe_qk_norm_rope_write", dev, qkv.data_ptr(), code, batch, rows // batch,
+              qkv.stride(0), heads, kv_heads, dim, rope.data_ptr(), rope.shape[0], rope.shape[1],
+              positions.data_ptr(), _lib.ptr(qw), _lib.ptr(kw), eps, q.data_ptr(),
+              k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs[:3], lengths.data_ptr(), shape[2])
         _written(k_cache, v_cache)
     return q
 
@@ -274,12 +282,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ws_bytes = _lib.workspace_size("pe_tree_attention_workspace_size", batch, n, heads, shape[1],
                                    dim, shape[2])
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with _Device(dev) as st:
-        _lib.check(_lib.lib().pe_tree_attention(
-            q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs[:3],
-            lengths.data_ptr(), masks.data_ptr(), m_b, out.data_ptr(), batch, n, heads, shape[1],
-            dim, shape[2], 1.0 / math.sqrt(dim) if scale is None else scale, _lib.ptr(ws), ws_bytes,
-            st), "pe_tree_attention")
+    _call("pe_tree_attention", dev, q.data_ptr(), code, qs[0], qs[1], k_cache.data_ptr(), *ks,
+          v_cache.data_ptr(), *vs[:3], lengths.data_ptr(), masks.data_ptr(), m_b, out.data_ptr(),
+          batch, n, heads, shape[1], dim, shape[2], 1.0 / math.sqrt(dim) if scale is None else
+          scale, _lib.ptr(ws), ws_bytes)
     return out
 
 
@@ -352,18 +358,17 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
             raise ValueError(f"temperature must be 0 or more, got {temp}")
     if vocab > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
-    out, path = torch.empty(2, batch, n, dtype=torch.int64, device=dev)
+    out = torch.empty(batch, n, dtype=torch.int64, device=dev)
+    path = torch.empty(batch, n, dtype=torch.int64, device=dev)
     count = torch.empty(batch, dtype=torch.int64, device=dev)
     if not batch:
         return out, path, count
     ws_bytes = _lib.workspace_size("pe_verify_drafts_workspace_size", batch, n, vocab)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _Device(dev) as st:
-        _lib.check(_lib.lib().pe_verify_drafts(
-            logits.data_ptr(), code, logits.stride(0), logits.stride(1), batch, n, vocab,
-            tokens.data_ptr(), _lib.ptr(parents), p_b, uniforms.data_ptr(), _lib.ptr(temps), temp,
-            _lib.ptr(draft_probs), q_b, q_n, out.data_ptr(), path.data_ptr(), count.data_ptr(),
-            ws.data_ptr(), ws_bytes, st), "pe_verify_drafts")
+    _call("pe_verify_drafts", dev, logits.data_ptr(), code, logits.stride(0), logits.stride(1),
+          batch, n, vocab, tokens.data_ptr(), _lib.ptr(parents), p_b, uniforms.data_ptr(),
+          _lib.ptr(temps), temp, _lib.ptr(draft_probs), q_b, q_n, out.data_ptr(), path.data_ptr(),
+          count.data_ptr(), ws.data_ptr(), ws_bytes)
     return out, path, count
 
 
@@ -390,11 +395,9 @@ def keep_accepted(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.T
             raise ValueError(f"{name} must be [(layers,) {batch}, kv_heads, positions, head_dim], "
                              f"got {list(cache.shape)}")
         views.append(c)
-    with _Device(dev) as st:
-        for c in views:
-            if c.numel():
-                layers, _, heads, cap, dim = c.shape
-                _lib.check(_lib.lib().pe_keep_accepted(
-                    c.data_ptr(), layers, batch, heads, cap, dim, *c.stride(), lengths.data_ptr(),
-                    path.data_ptr(), count.data_ptr(), n, st), "pe_keep_accepted")
+    for c in views:
+        if c.numel():
+            layers, _, heads, cap, dim = c.shape
+            _call("pe_keep_accepted", dev, c.data_ptr(), layers, batch, heads, cap, dim, *c.stride(),
+                  lengths.data_ptr(), path.data_ptr(), count.data_ptr(), n)
     _written(k_cache, v_cache)

@@ -836,3 +836,25 @@ def test_refusals():
     assert td.tree_attention(q[:0], k[:0], k[:0], lengths[:0], masks[:0]).shape == (0, n, heads, dim)
     assert [t.shape[0] for t in td.verify_drafts(logits[:0], tok[:0], u[:0])] == [0, 0, 0]
     assert td.tree_plan(tok[:0], lengths[:0]).masks.shape == (0, n)
+
+
+@pytest.mark.parametrize("heads,kv,dim,layout", [(4, 4, 128, "col"), (8, 2, 256, "row"), (16, 1, 64, "row")])
+def test_attention_many_sequences(heads, kv, dim, layout):
+    """More sequences than a wave has lanes, empty slots among them, several to a
+    workgroup."""
+    say(f"attention many sequences {heads}/{kv} dim={dim} {layout}")
+    rng, n = random.Random(dim), 3
+    lens = [rng.choice([-1, 0, 1, 5, 61, 62, 100, 200]) for _ in range(200)]
+    q, k, v, lengths, masks = _attention_case(dim, lens, n, heads, kv, dim, torch.bfloat16, layout,
+                                              cap=203)
+    got = _attend(q, k, v, lengths, masks, layout)
+    _check_attention(got, _attend_ref(q, k, v, lengths, masks, dim ** -0.5), "attention")
+
+
+def test_strides_along_one_element_are_not_looked_at():
+    say("strides along one element")
+    q, k, v, lengths, masks = _attention_case(3, [20], 2, 2, 1, 64, torch.bfloat16, "row")
+    want = _attend(q, k, v, lengths, masks)
+    kd, vd = (t.to(DEV).as_strided(t.shape, (3, 5, 64, 1)) for t in (k, v))
+    qd = q.to(DEV).as_strided(q.shape, (7, 128, 64, 1))
+    assert torch.equal(_td().tree_attention(qd, kd, vd, lengths.to(DEV), masks.to(DEV)), want)
