@@ -136,6 +136,15 @@ __device__ __forceinline__ float4v mfma16(u32x2v a, u32x2v b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4v, a),
                                                  __builtin_bit_cast(half4v, b), c, 0, 0, 0);
 }
+// two values rounded to the 16-bit type, in one instruction
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const float2v v{lo, hi};
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2v));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2v));
+}
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 typedef __attribute__((address_space(1))) const unsigned char glb_byte;
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
           p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][rt][e], c, -base));
           l[rt] += p[e];
         }
-        pf[kt][rt] = u32x2v{pack16x2(p[0], p[1], BF), pack16x2(p[2], p[3], BF)};
+        pf[kt][rt] = u32x2v{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3])};
       }
     }
     if (!kTail || !slow) {
@@ -514,8 +523,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         *reinterpret_cast<uint2*>(dst + 16 * dt) =
-            make_uint2(pack16x2(o[rt][dt][0] * inv, o[rt][dt][1] * inv, BF),
-                       pack16x2(o[rt][dt][2] * inv, o[rt][dt][3] * inv, BF));
+            make_uint2(pack2<BF>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
+                       pack2<BF>(o[rt][dt][2] * inv, o[rt][dt][3] * inv));
     } else {
       // the run's first sequence, begun before it, or its last, which goes on behind it
       float* dst = a.parts + (((int64_t)run * a.blocks + rblk) * 2 + (t0 == 0)) * part_words(RB, D);
