@@ -55,7 +55,8 @@ __host__ __device__ inline int64_t part_words(int rb, int dim) { return (int64_t
 // ---------------------------------------------------------------------------
 // The line of tiles: sequence after sequence, within one KV head after KV head.
 // An empty slot of the batch has one tile, without positions, for its zeros. Both
-// launches and every wave find their way by themselves, from the lengths alone.
+// launches find their way from the lengths alone, in a workgroup that works together
+// one wave for all.
 // ---------------------------------------------------------------------------
 // running sum over the 64 lanes: DPP row_shr within 16 lanes, then the rows
 __device__ __forceinline__ int wave_scan_i32(int v, int lane) {
@@ -104,15 +105,17 @@ __device__ __forceinline__ TreePlace tree_lane(const TreeChunk& c, int b0, int b
   return TreePlace{b0 + l, t, before + __builtin_amdgcn_readlane(c.scan, l) - t,
                    (int64_t)((uint64_t)hi << 32 | lo)};
 }
-// the sequence that holds place `at` of the line (it is on it)
+// the sequence that holds place `at` of the line
 __device__ __forceinline__ TreePlace tree_find(const TreeAttnArgs& a, TreeChunk c, int at, int lane) {
   int before = 0;
-  for (int b0 = 0;; b0 += 64) {
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const uint64_t hit = __ballot((before + c.scan) * a.kv_heads > at);
     if (hit) return tree_lane(c, b0, before, __builtin_ctzll(hit));
     before += __builtin_amdgcn_readlane(c.scan, 63);
     c = tree_chunk(a, b0 + 64, lane);
   }
+  // only if the lengths change under the kernel: an empty slot
+  return TreePlace{a.batch - 1, 1, at / a.kv_heads, -1};
 }
 
 // MFMA and conversions of the 16-bit type
@@ -195,6 +198,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   __shared__ __align__(16) unsigned char buf0[2 * VT];
   __shared__ __align__(16) unsigned char buf1[2 * VT];
   __shared__ float mx[4][16 * RT], lx[4][16 * RT];
+  __shared__ TreePlace line_place;
+  __shared__ int line_total;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave / WK, wk = wave % WK;
@@ -204,8 +209,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   const int rem = (int)blockIdx.x % span;
   const int run = (int)blockIdx.x / span * 8 + rem % 8;
   const int rblk = rem / 8;
-  const TreeChunk chunk = tree_chunk(a, 0, threadIdx.x & 63);
-  const int total = tree_total(a, chunk, threadIdx.x & 63) * a.kv_heads;
+  TreeChunk chunk{};
+  if (wave == 0) {
+    chunk = tree_chunk(a, 0, threadIdx.x & 63);
+    const int total = tree_total(a, chunk, threadIdx.x & 63);
+    if (threadIdx.x == 0) line_total = total * a.kv_heads;
+  }
+  __syncthreads();
+  const int total = __builtin_amdgcn_readfirstlane(line_total);
   const int size = (total + a.runs - 1) / a.runs;
   const int line_end = min(total, (run + 1) * size);
   for (int at = run * size; at < line_end;) {
@@ -214,14 +225,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   // them it would not leave registers enough for the tiles
   asm volatile("" : "+v"(tid));
   const int lane = tid & 63, li = lane & 15, lg = lane >> 4;
-  const TreePlace place = tree_find(a, chunk, at, lane);
-  const int b = place.b, tiles = place.tiles;
-  const int kvh = (at - place.before * a.kv_heads) / tiles;
-  const int t0 = at - place.before * a.kv_heads - kvh * tiles;
+  if (wave == 0) {
+    const TreePlace p = tree_find(a, chunk, at, lane);
+    if (lane == 0) line_place = p;
+  }
+  __syncthreads();
+  const int b = __builtin_amdgcn_readfirstlane(line_place.b);
+  const int tiles = __builtin_amdgcn_readfirstlane(line_place.tiles);
+  const int before = __builtin_amdgcn_readfirstlane(line_place.before);
+  const int kvh = (at - before * a.kv_heads) / tiles;
+  const int t0 = at - before * a.kv_heads - kvh * tiles;
   const int t1 = min(tiles, t0 + line_end - at);
   at += t1 - t0;
-  const bool live = place.len >= 0;
-  const int64_t len = live ? place.len : 0, end = len + a.n;
+  const int64_t found = (int64_t)(
+      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)line_place.len >> 32)) << 32 |
+      (uint32_t)__builtin_amdgcn_readfirstlane((int)line_place.len));
+  const bool live = found >= 0;
+  const int64_t len = live ? found : 0, end = len + a.n;
   const uint16_t* kb = a.k + (int64_t)b * a.ks_b + kvh * a.ks_h;
   const uint16_t* vb = a.v + (int64_t)b * a.vs_b + kvh * a.vs_h;
 
@@ -563,7 +583,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, in
   }
   const TreePlace place = tree_lane(c, b & ~63, before, b & 63);
   const int start = place.before * a.kv_heads + kvh * place.tiles;
-  const int run0 = start / size, parts = (start + place.tiles - 1) / size - run0 + 1;
+  const int run0 = min(start / size, a.runs - 1);
+  const int parts = min((start + place.tiles - 1) / size, a.runs - 1) - run0 + 1;
   if (parts == 1 || r >= a.rows) return;
   const int64_t words = part_words(rb, D), step = 2 * a.blocks * words;  // to the next run
   const int local = r % rb;

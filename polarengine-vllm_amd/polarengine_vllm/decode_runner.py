@@ -255,10 +255,13 @@ class DecodeRunner:
         """``tree_step``, verification of the drafts (``verify_drafts``: uniforms
         [B, n], draft_probs [B, n - 1, vocab] for a chain that was drawn), and the
         accepted nodes' keys and values moved to their places in every layer.
-        ``lengths`` grows by ``count`` in place. Returns (out, path, count):
+        ``lengths`` grows by ``count`` in place; a sequence whose cache has no room for
+        n more is left as an empty slot is, with count 0. Returns (out, path, count):
         ``out[b, :count[b]]`` are the new tokens, the last of them the next round's
         node 0."""
         logits = self.tree_step(tokens, lengths, parents)
+        room = (lengths >= 0) & (lengths <= self.max_len - tokens.shape[1])
+        tokens = torch.where(room[:, None], tokens, -1)
         out, path, count = tree_decode.verify_drafts(logits, tokens, uniforms, parents, draft_probs,
                                                      temperature)
         tree_decode.keep_accepted(self.k_cache.transpose(-1, -2), self.v_cache, lengths, path, count)
@@ -302,7 +305,8 @@ class DecodeRunner:
         return attend
 
     def _attention_normed(self, pos: torch.Tensor):
-        """The same with per-head norms of queries and keys: a tree of one node."""
+        """The same with per-head norms of queries and keys: a tree of one node (a
+        position outside the cache attends to nothing and is not stored)."""
         c = self.cfg
         if (c.head_dim not in (64, 128, 256) or c.heads % c.kv_heads
                 or not _kernel_operands(self.k_cache, self.v_cache)):

@@ -171,6 +171,21 @@ def test_round_replays_from_a_graph():
         assert torch.equal(runs[0].k_cache, runs[1].k_cache)
 
 
+def test_round_without_room_in_the_cache():
+    say("round without room")
+    b, n, max_len = 3, 4, 20
+    run = _runner(b, max_len)
+    run.k_cache.normal_()
+    run.v_cache.normal_()
+    before = run.k_cache.clone()
+    lengths = torch.tensor([max_len - n, max_len - n + 1, -1], device=DEV)
+    out, path, count = run.speculative_round(_tokens((b, n)), lengths, torch.rand(b, n, device=DEV))
+    assert int(count[0]) >= 1 and count[1:].tolist() == [0, 0]
+    assert lengths.tolist() == [max_len - n + int(count[0]), max_len - n + 1, -1]
+    assert bool((out[1:] == -1).all()) and bool((path[1:] == -1).all())
+    assert torch.equal(run.k_cache[:, 1:], before[:, 1:])
+
+
 def test_tree_step_refusals():
     say("tree step refusals")
     run = _runner(2, 20)
