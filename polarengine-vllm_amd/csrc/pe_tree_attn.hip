@@ -632,22 +632,35 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, in
   __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
 }
 
-// rows of a workgroup: as many as the rows of a KV head fill
-static int tree_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Rows of a workgroup: as many as the rows of a KV head fill, 128 at most. Heads of 128
+// stay at 64, by four waves of 16: with keys by dimension, whose 128-row form does not
+// fit the registers (8 sequences of up to 8000, 80 rows: 65 us, 128-row form 111; one
+// of 30000, 512 rows: 127 and 145), and up to 192 rows, where the second half of the
+// last block or the larger parts cost more than K and V read from L2 again (96 rows
+// over 8000: 60 and 65 us; 128 over 6000: 56.5 and 59.4; 192 over 8000: 53 and 62; but
+// 256 over 8000: 66 and 63; 512 over 32700: 110 and 94). Heads of 64 and 256 gain by
+// 128 rows from 128 on (64: 65 us, 68 by 64 rows; 256: 129 and 147).
+static int tree_rows(int rows, int dim, bool kcol) {
+  if (rows <= 64) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return dim == 128 && (kcol || rows <= 192) ? 64 : 128;
+}
 
 struct TreePlanHost {
   int rb, blocks;
   int runs;
   bool split;  // a sequence may be divided
 };
-static TreePlanHost tree_host(int64_t batch, int n, int heads, int kv_heads, int dim, int64_t cap) {
+static TreePlanHost tree_host(int64_t batch, int n, int heads, int kv_heads, int dim, int64_t cap,
+                              bool kcol) {
   TreePlanHost p;
   const int rows = n * (heads / kv_heads);
-  p.rb = tree_rows(rows);
+  p.rb = tree_rows(rows, dim, kcol);
   p.blocks = (rows + p.rb - 1) / p.rb;
   const int64_t tiles = (cap + kTile - 1) / kTile;
-  // as many workgroups as the LDS of the CUs holds at a time, each an equal run
-  const int per_cu = dim == 256 ? 1 : dim == 128 ? 2 : 4;
+  // As many workgroups as the CUs hold at a time, each an equal run. Heads of 64 would
+  // fit three or four times; two are faster (32 rows, 16 sequences of up to 8000: 40.5
+  // us, three 41.7, four 43.6; 128 rows: 65, 75 and 78), their parts being fewer.
+  const int per_cu = dim == 256 ? 1 : 2;
   const int64_t wanted = (int64_t)num_cus() * per_cu / p.blocks;
   const int64_t most = batch * kv_heads * tiles;
   p.runs = (int)(wanted < 1 ? 1 : wanted < most ? wanted : most);
@@ -670,7 +683,9 @@ static void launch_main(const TreePlanHost& p, const TreeAttnArgs& a, hipStream_
     case 16: tree_attn_kernel<D, BF, KCOL, 1, 1><<<grid, 256, 0, st>>>(a); break;
     case 32: tree_attn_kernel<D, BF, KCOL, 1, 2><<<grid, 256, 0, st>>>(a); break;
     case 64: tree_attn_kernel<D, BF, KCOL, 1, 4><<<grid, 256, 0, st>>>(a); break;
-    default: tree_attn_kernel<D, BF, KCOL, 2, 4><<<grid, 256, 0, st>>>(a); break;
+    default:
+      if constexpr (D != 128 || !KCOL) tree_attn_kernel<D, BF, KCOL, 2, 4><<<grid, 256, 0, st>>>(a);
+      break;
   }
 }
 
@@ -692,8 +707,13 @@ using namespace pe;
 extern "C" size_t pe_tree_attention_workspace_size(int64_t batch, int n, int heads, int kv_heads,
                                                    int head_dim, int64_t cap) {
   if (!tree_attn_shape_ok(batch, n, heads, kv_heads, head_dim, cap)) return 0;
-  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, head_dim, cap);
-  return p.split ? (size_t)p.runs * p.blocks * 2 * part_words(p.rb, head_dim) * 4 : 0;
+  size_t most = 0;  // of the two layouts of the keys
+  for (int kcol = 0; kcol < 2; ++kcol) {
+    const TreePlanHost p = tree_host(batch, n, heads, kv_heads, head_dim, cap, kcol);
+    const size_t need = p.split ? (size_t)p.runs * p.blocks * 2 * part_words(p.rb, head_dim) * 4 : 0;
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 extern "C" int pe_tree_attention(const void* q, int dtype, int64_t q_b, int64_t q_n,
@@ -716,7 +736,7 @@ extern "C" int pe_tree_attention(const void* q, int dtype, int64_t q_b, int64_t 
   const size_t need = pe_tree_attention_workspace_size(batch, n, heads, kv_heads, head_dim, cap);
   if (need && (!workspace || workspace_bytes < need)) return PE_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return PE_ERR_ALIGN;
-  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, head_dim, cap);
+  const TreePlanHost p = tree_host(batch, n, heads, kv_heads, head_dim, cap, ks_d != 1);
   TreeAttnArgs a{reinterpret_cast<const uint16_t*>(q), q_b, q_n,
                  reinterpret_cast<const uint16_t*>(k_cache),
                  reinterpret_cast<const uint16_t*>(v_cache), ks_b, ks_h, ks_l, ks_d, vs_b, vs_h, vs_l,

@@ -858,3 +858,15 @@ def test_strides_along_one_element_are_not_looked_at():
     kd, vd = (t.to(DEV).as_strided(t.shape, (3, 5, 64, 1)) for t in (k, v))
     qd = q.to(DEV).as_strided(q.shape, (7, 128, 64, 1))
     assert torch.equal(_td().tree_attention(qd, kd, vd, lengths.to(DEV), masks.to(DEV)), want)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("layout", ["row", "col"])
+@pytest.mark.parametrize("n,group", [(5, 13), (32, 4), (28, 7), (25, 8), (64, 7)])
+def test_attention_row_blocks(n, group, dim, layout):
+    """Rows of a KV head around and past a workgroup's: 65, 128, 196, 200, 448."""
+    say(f"attention rows {n * group} dim={dim} {layout}")
+    q, k, v, lengths, masks = _attention_case(n + dim, [190, 0, 700], n, group, 1, dim, torch.bfloat16,
+                                              layout)
+    got = _attend(q, k, v, lengths, masks, layout)
+    _check_attention(got, _attend_ref(q, k, v, lengths, masks, dim ** -0.5), "attention")
