@@ -31,13 +31,16 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(const int64_t* __restrict
 // by the position's angles; values pass as they are. D / 8 lanes a head, one
 // 16-byte load each, so a row is read once and the norm, the rotation and the one
 // rounding happen in registers. Bound by bytes: rows of 16-bit values read and
-// written once. The arithmetic is in 64 bits: it costs no time beside the bytes, and
-// the one rounding is that of the exact value.
+// written once. The arithmetic behind the products of two 16-bit values (exact in 32
+// bits) is in 64, so that the one rounding is that of the exact value; in 32 bits about
+// one value in 65,000 rounds the other way. It is about half of the vector
+// instructions, which now take as long as the bytes: 8192 rows of 48 heads of 128 to a
+// cache 53 us (3.8 TB/s); 16 rows 4.4 us.
 //
 // A workgroup takes a row (or several of a model with few heads), its heads four
 // loads a lane at a time, the row's angles once. Keys that the cache stores by
 // dimension go through LDS instead, 64 rows of a head a workgroup, and leave as 16
-// bytes of eight consecutive positions.
+// bytes of eight consecutive positions (as 2-byte stores the 8192 rows took 101 us).
 // ---------------------------------------------------------------------------
 constexpr int kRopeTile = 64;
 

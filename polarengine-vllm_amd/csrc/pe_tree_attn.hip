@@ -21,6 +21,12 @@
 // The tiles of all sequences and KV heads form one line, cut into equal runs, one a
 // workgroup, by the lengths read on the device; a second launch joins the parts of a
 // sequence that a cut divides.
+//
+// Bound by HBM where a KV head has few rows: 32 sequences x 8 nodes, 32 rows, up to
+// 16,000 positions 261 us, 5.4 TB/s (tiles through registers 493, equal parts of each
+// sequence instead of the line 315). With 512 rows over 32,700 positions 92 us, 0.74
+// PFLOP/s: the softmax between the products keeps the matrix cores busy 29% of the
+// time. One sequence of 777 and 16 rows: 8.0 + 4.3 us, latency.
 
 #include <type_traits>
 
