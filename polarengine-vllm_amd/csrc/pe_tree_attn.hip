@@ -30,7 +30,6 @@
 
 #include <type_traits>
 
-
 #include "pe_tree.h"
 
 namespace pe {
@@ -224,7 +223,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   __syncthreads();
   const int total = __builtin_amdgcn_readfirstlane(line_total);
   const int size = (total + a.runs - 1) / a.runs;
-  const int line_end = min(total, (run + 1) * size);
+  if ((int64_t)run * size >= total) return;
+  const int line_end = (int)min((int64_t)total, (int64_t)(run + 1) * size);
   for (int at = run * size; at < line_end;) {
   int tid = threadIdx.x;
   // what follows from the lane is worked out anew for each sequence: kept across

@@ -870,3 +870,16 @@ def test_attention_row_blocks(n, group, dim, layout):
                                               layout)
     got = _attend(q, k, v, lengths, masks, layout)
     _check_attention(got, _attend_ref(q, k, v, lengths, masks, dim ** -0.5), "attention")
+
+
+def test_attention_more_row_blocks_than_workgroups():
+    """4096 query heads of one KV head: every row block goes through the whole line."""
+    say("attention row blocks")
+    n, dim = 17, 64
+    q, k, v, lengths, masks = _attention_case(2, [100, -1, 70, 0], n, 4, 1, dim, torch.bfloat16, "row",
+                                              cap=120)
+    want = _attend_ref(q, k, v, lengths, masks, dim ** -0.5)
+    got = _attend(q.repeat(1, 1, 1024, 1), k, v, lengths, masks)
+    for h in (0, 1, 7, 2046, 4095):
+        _check_attention(got[:, :, h:h + 1], [t[:, :, h % 4:h % 4 + 1] for t in want], f"head {h}")
+    assert torch.equal(got[:, :, :4].repeat(1, 1, 1024, 1), got)
