@@ -112,12 +112,13 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype: torch.dtype):
                          f"{list(k.shape)} and {list(v.shape)}")
     if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError(f"caches must be {dtype} as the queries, got {k.dtype} and {v.dtype}")
-    # a stride along one element says nothing
-    ks, vs = ([0 if n == 1 else st for st, n in zip(t.stride(), t.shape)] for t in (k, v))
+    ks, vs, shape = k.stride(), v.stride(), k.shape
+    if 1 in shape:  # a stride along one element says nothing
+        ks, vs = ([0 if n == 1 else st for st, n in zip(s, shape)] for s in (ks, vs))
     if vs[3] != 1 or (ks[3] != 1 and ks[2] != 1):
         raise ValueError("values must have the dimension contiguous, keys the dimension or the "
                          f"position; got strides {vs} and {ks}")
-    return k.shape, ks, vs
+    return shape, ks, vs
 
 
 def _writable(t: torch.Tensor, name: str) -> None:
@@ -172,8 +173,10 @@ def _rope_inputs(qkv, heads, kv_heads, rope, positions, q_weight, k_weight):
     if qkv.dim() != 2 or heads < 1 or kv_heads < 1 or qkv.shape[1] % per:
         raise ValueError(f"qkv must be [rows, (heads + 2 kv_heads) * head_dim] for {heads} and "
                          f"{kv_heads} heads, got {list(qkv.shape)}")
-    rows, dim = qkv.shape[0], qkv.shape[1] // per
-    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1] or qkv.data_ptr() % 16:
+    rows, cols = qkv.shape
+    dim = cols // per
+    ld, one = qkv.stride()
+    if one != 1 or ld % 8 or ld < cols or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     if rope.dtype is not torch.float32 or rope.dim() != 2:
         raise TypeError(f"rope must be a float32 [positions, rotary dims] table, got {rope.dtype} "
@@ -182,18 +185,19 @@ def _rope_inputs(qkv, heads, kv_heads, rope, positions, q_weight, k_weight):
         raise TypeError(f"positions must be int64, got {positions.dtype}")
     if positions.numel() != rows:
         raise ValueError(f"positions must name {rows} rows, got {list(positions.shape)}")
-    ws = []
     for w in (q_weight, k_weight):
-        if w is not None:
-            if w.shape != (dim,) or w.dtype is not qkv.dtype:
-                raise ValueError(f"norm weights must be {qkv.dtype} of [{dim}], got {w.dtype} of "
-                                 f"{list(w.shape)}")
-            w = w.contiguous()
-            w = w.clone() if w.data_ptr() % 16 else w
-        ws.append(w)
-    rope = rope.contiguous()
-    return (rows, dim, code, qkv, rope.clone() if rope.data_ptr() % 16 else rope,
-            positions.contiguous(), ws[0], ws[1])
+        if w is not None and (w.dtype is not qkv.dtype or w.shape != (dim,)):
+            raise ValueError(f"norm weights must be {qkv.dtype} of [{dim}], got {w.dtype} of "
+                             f"{list(w.shape)}")
+    return (rows, dim, code, qkv, _whole(rope), positions.contiguous(),
+            None if q_weight is None else _whole(q_weight),
+            None if k_weight is None else _whole(k_weight))
+
+
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, 16-byte aligned."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, rope: torch.Tensor,
