@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(const int64_t* __restrict
 // bits) is in 64, so that the one rounding is that of the exact value; in 32 bits about
 // one value in 65,000 rounds the other way. It is about half of the vector
 // instructions, which now take as long as the bytes: 8192 rows of 48 heads of 128 to a
-// cache 53 us (3.8 TB/s); 16 rows 4.4 us.
+// cache 54 us (3.7 TB/s); 16 rows 4.4 us.
 //
 // A workgroup takes a row (or several of a model with few heads), its heads four
 // loads a lane at a time, the row's angles once. Keys that the cache stores by
@@ -118,10 +118,11 @@ __device__ __forceinline__ u32x4v rope_head(const RopeArgs& a, u32x4v u, const u
   }
   double y = 1.0;
   if (w) {
-    float g[8], ss = 0.f;
+    float g[8];
+    double ss = 0.0;
     load8<BF ? PE_DTYPE_BF16 : PE_DTYPE_F16>(w + 8 * lane, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+    for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)v[i], (double)v[i], ss);
     const double x = head_sum<D>(ss) * (1.0 / D) + (double)a.eps;
     // 1 / sqrt(x): the instruction's value (relative error below 2^-26) and a Newton step
     y = __builtin_amdgcn_rsq(x);
