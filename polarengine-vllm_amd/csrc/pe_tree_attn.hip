@@ -332,11 +332,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
     }
   }
   float4v o[RT][DT];
-  float m[RT], l[RT];
+  // l: the sums of the rounded probabilities, as a product with ones (every register of
+  // it holds the row's sum): what a row's weights are divided by is then their own sum
+  float m[RT];
+  float4v l4[RT];
+  constexpr uint32_t kOnes = BF ? 0x3F803F80u : 0x3C003C00u;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -__builtin_inff();
-    l[rt] = 0.f;
+    l4[rt] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
   }
@@ -417,7 +421,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
       if (__any(top > m[rt] + kSlack)) {
         const float mn = fmaxf(m[rt], top);
         const float al = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
-        l[rt] *= al;
+        l4[rt] *= al;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
         m[rt] = mn;
@@ -427,11 +431,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
       for (int kt = 0; kt < NKT; ++kt) {
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e)
           p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][rt][e], c, -base));
-          l[rt] += p[e];
-        }
         pf[kt][rt] = u32x2v{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3])};
+      }
+      if constexpr (NKT == 1) {
+        l4[rt] = mfma16<BF>(u32x2v{kOnes, kOnes}, pf[0][rt], l4[rt]);
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < NKT; kt += 2)
+          l4[rt] = mfma32<BF>(u32x4v{kOnes, kOnes, kOnes, kOnes},
+                              u32x4v{pf[kt][rt][0], pf[kt][rt][1], pf[kt + 1][rt][0],
+                                     pf[kt + 1][rt][1]}, l4[rt]);
       }
     }
     if (!kTail || !slow) {
@@ -497,11 +508,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
   for (bool odd = false; t < t1; ++t, odd = !odd)  // an odd full tile too
     step((lds_byte*)(odd ? buf1 : buf0), (lds_byte*)(odd ? buf0 : buf1), t, std::true_type{});
 
+  float l[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 16, 64);
-    l[rt] += __shfl_xor(l[rt], 32, 64);
-  }
+  for (int rt = 0; rt < RT; ++rt) l[rt] = l4[rt][0];
   if constexpr (WK > 1) {  // join the waves that share rows, in their order
     if (lg == 0)
 #pragma unroll
