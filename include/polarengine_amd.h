@@ -464,7 +464,8 @@ int pe_lm_head(const void* x, const void* w, int64_t M, int64_t N, int K, float*
  *       masks[b][i]'s bits j < n (row stride m_b, 0: one for every sequence). A
  *       row with nothing to attend to, and an empty slot's, is zero. q: strides
  *       of batch and node, multiples of 8; heads and dimensions contiguous.
- *       head_dim 64, 128 or 256.
+ *       head_dim 64, 128 or 256. Scores and sums in fp32, probabilities rounded to
+ *       the 16-bit type (fp16: those below 2^-32 of a row's largest become zero).
  *   pe_verify_drafts: logits [batch, n, vocab] (PE_DTYPE_F32 too; strides of
  *       batch and node) of the target, tokens int64 [batch, n] (outside 0 ..
  *       vocab - 1: absent; tokens[b][0] absent: an empty slot), parents as above

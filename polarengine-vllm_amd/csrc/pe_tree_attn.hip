@@ -12,7 +12,10 @@
 //    keys of one row and the row's maximum needs two exchanges), Q in registers;
 //  * one pass with running maximum and sum in fp32; the probabilities, rounded to
 //    the cache's 16-bit type, are the B operand of O^T = V^T P^T just as S^T left
-//    them (the order of a product's keys is free as long as V^T has the same);
+//    them (the order of a product's keys is free as long as V^T has the same). The
+//    matrix cores take 16 bits; a second product with what the rounding leaves would
+//    be half as many instructions again. Each probability is off by half a step, in
+//    the sum that divides alike: at most one step of sum p |v| / sum p in all;
 //  * V^T, and K where it is stored by dimension, come out of LDS through
 //    ds_read_b64_tr_b16: within 16 lanes, lane i gives the address of 8 bytes of
 //    row i / 4 and gets column i of the 4 x 16 block.
@@ -37,6 +40,11 @@ namespace pe {
 constexpr int kTile = 64;          // positions of a tile
 constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;      // powers of two that an exponent may exceed its base by
+// fp16 probabilities are 2^7 times as large: the largest lies in 2^7 .. 2^15, what is below
+// 2^-21 of it (2^-29 where the base is behind) loses bits and what is below 2^-32 (2^-40)
+// vanishes. Without it, beside a key 18 above 32,000 others, results were off by 4.2e-4
+// of 5.8e-4. The row's sum has the factor too; no time is lost. bf16 has fp32's exponents.
+constexpr float kLiftF16 = 7.f;
 
 struct TreeAttnArgs {
   const uint16_t* q;
@@ -426,7 +434,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 2 || D == 128 ? 2 : 3) vo
         for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
         m[rt] = mn;
       }
-      const float base = m[rt] == -__builtin_inff() ? 0.f : m[rt];
+      const float base = (m[rt] == -__builtin_inff() ? 0.f : m[rt]) - (BF ? 0.f : kLiftF16);
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt) {
         float p[4];

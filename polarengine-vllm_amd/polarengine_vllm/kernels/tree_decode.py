@@ -263,8 +263,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     multiple of the cache's; head_dim 64, 128 or 256): node i sees the positions
     below ``lengths[b]`` and the slots ``lengths[b] + j`` of the bits j < n of its
     mask (int64 [batch, n], or [n] for all). Scores, softmax statistics and sums in
-    fp32; ``scale`` is 1 / sqrt(head_dim) unless given. A node with nothing to see
-    gets zeros."""
+    fp32; the probabilities are rounded to the queries' type for the product with the
+    values, where fp16 loses bits of those below 2^-21 of a row's largest and all of
+    those below 2^-32. ``scale`` is 1 / sqrt(head_dim) unless given. A node with
+    nothing to see gets zeros."""
     dev = _inputs(q, k_cache, v_cache, lengths, masks)
     code = _lib.act_dtype(q)
     if q.dim() != 4:
