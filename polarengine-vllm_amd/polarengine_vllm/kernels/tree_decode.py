@@ -34,6 +34,7 @@ import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
@@ -66,16 +67,20 @@ def _call(name: str, dev: torch.device, *args) -> None:
 
 
 def _inputs(*tensors: Optional[torch.Tensor]) -> torch.device:
-    """The one GPU of the tensors; refuses others, and inputs that autograd follows."""
+    """The one GPU of the tensors; refuses others, and inputs that autograd follows
+    (reverse mode, or forward mode, which no_grad does not turn off)."""
     grad = torch.is_grad_enabled()
+    dual = fwAD._current_level >= 0  # outside a dual level no tensor has a tangent
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None:
             if t.get_device() != index or index < 0:
                 _lib.require_device(*tensors)
-            if grad and t.requires_grad:
+            if (grad and t.requires_grad) or (
+                    dual and not t.is_inference() and fwAD.unpack_dual(t).tangent is not None):
                 raise RuntimeError("the drafted-token kernels have no backward pass: call them "
-                                   "under torch.no_grad() or detach their inputs")
+                                   "under torch.no_grad(), without forward-mode tangents, or "
+                                   "detach their inputs")
     return tensors[0].device
 
 

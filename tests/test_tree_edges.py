@@ -1,0 +1,56 @@
+"""CPU tests of the drafted-token entry points: calls at the edges of what their
+documentation allows. Nothing here reaches a launch: the device check and the call
+into the library are replaced."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The calls that would go into the library: (name, arguments)."""
+    from polarengine_vllm import _lib
+    from polarengine_vllm.kernels import tree_decode as td
+    made = []
+    monkeypatch.setattr(_lib, "require_device", lambda *t: t[0].device)
+    monkeypatch.setattr(td, "_call", lambda name, dev, *args: made.append((name, args)))
+    return made
+
+
+def _inputs():
+    q = torch.zeros(2, 3, 4, 64, dtype=BF)
+    k = torch.zeros(2, 2, 16, 64, dtype=BF)
+    lengths, masks = torch.zeros(2, dtype=torch.int64), torch.ones(2, 3, dtype=torch.int64)
+    qkv, table = torch.zeros(6, 8 * 64, dtype=BF), torch.zeros(16, 64)
+    pos = torch.zeros(6, dtype=torch.int64)
+    return q, k, lengths, masks, qkv, table, pos
+
+
+def test_forward_mode_tangents_are_refused(calls):
+    """A dual tensor would lose its tangent; no_grad does not turn forward mode off."""
+    from polarengine_vllm.kernels import tree_decode as td
+    q, k, lengths, masks, qkv, table, pos = _inputs()
+    logits, u = torch.zeros(2, 3, 50), torch.zeros(2, 3)
+    with fwAD.dual_level():
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))
+        for call in (lambda: td.tree_attention(dual(q), k, k, lengths, masks),
+                     lambda: td.tree_attention(q, dual(k), k, lengths, masks),
+                     lambda: td.tree_attention(q, k, dual(k), lengths, masks),
+                     lambda: td.qk_norm_rope(dual(qkv), 4, 2, table, pos),
+                     lambda: td.qk_norm_rope(qkv, 4, 2, dual(table), pos),
+                     lambda: td.qk_norm_rope(qkv, 4, 2, table, pos, dual(torch.ones(64, dtype=BF))),
+                     lambda: td.qk_norm_rope_write(qkv, 4, 2, table, pos, dual(k), k.clone(), lengths),
+                     lambda: td.verify_drafts(dual(logits), masks, u),
+                     lambda: td.verify_drafts(logits, masks, dual(u)),
+                     lambda: td.verify_drafts(logits, masks, u, temperature=dual(torch.ones(2))),
+                     lambda: td.keep_accepted(dual(k), k.clone(), lengths, masks, lengths)):
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(RuntimeError, match="no backward pass"):
+                    call()
+        assert not calls
+        td.tree_attention(q, k, k, lengths, masks)  # nothing of it is dual
+    td.tree_attention(fwAD.unpack_dual(q).primal, k, k, lengths, masks)
+    assert [name for name, _ in calls] == ["pe_tree_attention"] * 2
