@@ -110,6 +110,17 @@ def _nodes(n: int) -> None:
         raise ValueError(f"a step takes 1 to {MAX_NODES} nodes per sequence, got {n}")
 
 
+def _strides(t: torch.Tensor):
+    """Element strides of a cache [.., positions, head_dim]. A stride along one element
+    says nothing: 0, but 1 for the one position of keys by dimension."""
+    st, shape = t.stride(), t.shape
+    if 1 in shape:
+        st = [0 if n == 1 else s for s, n in zip(st, shape)]
+        if shape[-2] == 1 and st[-1] != 1:
+            st[-2] = 1
+    return st
+
+
 def _caches(k: torch.Tensor, v: torch.Tensor, dtype: torch.dtype):
     """Shape and element strides of a key and a value cache."""
     if k.dim() != 4 or k.shape != v.shape:
@@ -117,9 +128,7 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype: torch.dtype):
                          f"{list(k.shape)} and {list(v.shape)}")
     if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError(f"caches must be {dtype} as the queries, got {k.dtype} and {v.dtype}")
-    ks, vs, shape = k.stride(), v.stride(), k.shape
-    if 1 in shape:  # a stride along one element says nothing
-        ks, vs = ([0 if n == 1 else st for st, n in zip(s, shape)] for s in (ks, vs))
+    ks, vs, shape = _strides(k), _strides(v), k.shape
     if vs[3] != 1 or (ks[3] != 1 and ks[2] != 1):
         raise ValueError("values must have the dimension contiguous, keys the dimension or the "
                          f"position; got strides {vs} and {ks}")
@@ -409,6 +418,6 @@ def keep_accepted(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.T
     for c in views:
         if c.numel():
             layers, _, heads, cap, dim = c.shape
-            _call("pe_keep_accepted", dev, c.data_ptr(), layers, batch, heads, cap, dim, *c.stride(),
+            _call("pe_keep_accepted", dev, c.data_ptr(), layers, batch, heads, cap, dim, *_strides(c),
                   lengths.data_ptr(), path.data_ptr(), count.data_ptr(), n)
     _written(k_cache, v_cache)

@@ -54,3 +54,25 @@ def test_forward_mode_tangents_are_refused(calls):
         td.tree_attention(q, k, k, lengths, masks)  # nothing of it is dual
     td.tree_attention(fwAD.unpack_dual(q).primal, k, k, lengths, masks)
     assert [name for name, _ in calls] == ["pe_tree_attention"] * 2
+
+
+def test_strides_along_one_element(calls):
+    """Along one element a stride says nothing; the one position of a cache by dimension
+    keeps that layout."""
+    from polarengine_vllm.kernels import tree_decode as td
+    lengths, one = torch.zeros(1, dtype=torch.int64), torch.ones(1, 1, dtype=torch.int64)
+    rows = torch.zeros(1, 1, 8, 64, dtype=BF).as_strided((1, 1, 8, 64), (3, 5, 64, 1))
+    cols = torch.zeros(1, 1, 64, 8, dtype=BF).transpose(-1, -2).as_strided((1, 1, 8, 64), (3, 5, 1, 8))
+    td.keep_accepted(cols, rows, lengths, one, lengths)
+    assert [a[6:11] for _, a in calls] == [(0, 0, 0, 1, 8), (0, 0, 0, 64, 1)]
+    calls.clear()
+    whole = torch.zeros(2, 2, 64, 1, dtype=BF).transpose(-1, -2)
+    first = torch.zeros(2, 2, 64, 9, dtype=BF).transpose(-1, -2)[:, :, :1]
+    v = torch.zeros(2, 2, 1, 64, dtype=BF)
+    lengths, one = torch.zeros(2, dtype=torch.int64), torch.ones(2, 1, dtype=torch.int64)
+    for k, want in ((whole, (128, 64, 0, 1)), (first, (1152, 576, 1, 9))):
+        td.keep_accepted(k, v, lengths, one, lengths)
+        assert calls[0][1][7:11] == want and calls[1][1][7:11] == (128, 64, 0, 1)
+        td.tree_attention(torch.zeros(2, 1, 4, 64, dtype=BF), k, v, lengths, one)
+        assert calls[2][1][5:9] == want
+        calls.clear()
