@@ -245,7 +245,7 @@ class DecodeRunner:
             parents = torch.arange(-1, n - 1, device=self.dev)
         plan = tree_decode.tree_plan(parents, lengths)
         attend = self._attention_tree(lengths, plan.positions, plan.masks)
-        return self._layers(tokens.clamp(0, self.cfg.vocab - 1).view(-1), attend).view(B, n, -1)
+        return self._layers(tokens.clamp(0, self.cfg.vocab - 1).reshape(-1), attend).view(B, n, -1)
 
     def speculative_round(self, tokens: torch.Tensor, lengths: torch.Tensor,
                           uniforms: torch.Tensor, parents: Optional[torch.Tensor] = None,

@@ -65,3 +65,20 @@ def test_runner_of_one_position():
     lengths = torch.zeros(2, dtype=torch.int64, device=DEV)
     out, _, count = run.speculative_round(_tokens((2, 1)), lengths, torch.rand(2, 1, device=DEV))
     assert count.tolist() == [1, 1] and lengths.tolist() == [1, 1] and bool((out >= 0).all())
+
+
+def test_runner_with_strided_tokens():
+    """DecodeRunner: tokens that are no rows of memory."""
+    say("runner strided tokens")
+    from test_gpu_tree_runner import _runner, _tokens
+    tokens, u = _tokens((2, 5)), torch.rand(2, 5, device=DEV)
+    wide = _tokens((2, 11), 1)
+    wide[:, ::2][:, :5] = tokens
+    go = lambda t: _runner(2, 20).speculative_round(t, torch.zeros(2, dtype=torch.int64, device=DEV), u)
+    want = go(tokens)
+    for other in (tokens.t().contiguous().t(), wide[:, ::2][:, :5]):
+        assert all(torch.equal(x, y) for x, y in zip(go(other), want))
+    shared = tokens[:1].expand(2, -1)
+    assert torch.equal(_runner(2, 20).tree_step(shared, torch.zeros(2, dtype=torch.int64, device=DEV)),
+                       _runner(2, 20).tree_step(shared.contiguous(),
+                                                torch.zeros(2, dtype=torch.int64, device=DEV)))
