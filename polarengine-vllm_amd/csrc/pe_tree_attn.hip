@@ -683,8 +683,13 @@ static TreePlanHost tree_host(int64_t batch, int n, int heads, int kv_heads, int
   // As many workgroups as the CUs hold at a time, each an equal run. Heads of 64 would
   // fit three or four times; two are faster (32 rows, 16 sequences of up to 8000: 40.5
   // us, three 41.7, four 43.6; 128 rows: 65, 75 and 78), their parts being fewer.
+  // A run's row blocks share an XCD, so what fits is counted for each of the eight: one
+  // workgroup more than its CUs hold waits for a whole run (heads of 256, 320 rows over
+  // 8000 positions, three blocks: 11 runs an XCD 119 us, 10 runs 89; 768 rows 121 and 86).
   const int per_cu = dim == 256 ? 1 : 2;
-  const int64_t wanted = (int64_t)num_cus() * per_cu / p.blocks;
+  const int64_t slots = (int64_t)num_cus() * per_cu;
+  const int64_t per_xcd = slots / 8 / p.blocks;
+  const int64_t wanted = per_xcd ? per_xcd * 8 : slots / p.blocks;
   const int64_t most = batch * kv_heads * tiles;
   p.runs = (int)(wanted < 1 ? 1 : wanted < most ? wanted : most);
   p.split = tiles > 1 && p.runs > 1;

@@ -76,3 +76,22 @@ def test_strides_along_one_element(calls):
         td.tree_attention(torch.zeros(2, 1, 4, 64, dtype=BF), k, v, lengths, one)
         assert calls[2][1][5:9] == want
         calls.clear()
+
+
+@pytest.mark.parametrize("dim,per_cu", [(64, 2), (256, 1)])
+@pytest.mark.parametrize("n,group", [(1, 1), (40, 8), (48, 8), (64, 10), (64, 12), (64, 40), (64, 100)])
+def test_attention_runs_fit_every_xcd(dim, per_cu, n, group):
+    """The row blocks of a run share an XCD of 32 CUs: no more workgroups there than they
+    hold at a time (the number of runs from the workspace, two parts each)."""
+    from polarengine_vllm import _lib
+    rows = n * group
+    block = 16 if rows <= 16 else 128
+    need = _lib.lib().pe_tree_attention_workspace_size(4, n, 2 * group, 2, dim, 100000)
+    blocks = -(-rows // block)
+    runs, rest = divmod(need, blocks * 2 * block * (dim + 2) * 4)
+    assert runs >= 1 and rest == 0
+    slots = 32 * per_cu
+    if blocks <= slots:
+        assert -(-runs // 8) * blocks <= slots and runs * blocks > 8 * (slots - blocks)
+    else:
+        assert runs * blocks <= 8 * slots or runs == 1
