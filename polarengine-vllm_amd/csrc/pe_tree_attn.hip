@@ -655,17 +655,23 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a, in
   __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
 }
 
-// Rows of a workgroup: as many as the rows of a KV head fill, 128 at most. Heads of 128
-// stay at 64, by four waves of 16: with keys by dimension, whose 128-row form does not
-// fit the registers (8 sequences of up to 8000, 80 rows: 65 us, 128-row form 111; one
-// of 30000, 512 rows: 127 and 145), and up to 192 rows, where the second half of the
-// last block or the larger parts cost more than K and V read from L2 again (96 rows
-// over 8000: 60 and 65 us; 128 over 6000: 56.5 and 59.4; 192 over 8000: 53 and 62; but
-// 256 over 8000: 66 and 63; 512 over 32700: 110 and 94). Heads of 64 and 256 gain by
-// 128 rows from 128 on (64: 65 us, 68 by 64 rows; 256: 129 and 147).
+// Rows of a workgroup: as many as the rows of a KV head fill, 64 up to 192 of them, 128
+// beyond. Up to 192 the second half of the last block, the larger parts and (heads of 256)
+// the 54 to 119 registers that the 128-row form spills cost more than keys and values read
+// from L2 by a block more. Beyond, 128 rows win by their fewer reads where sequences are
+// long, and lose up to a sixth where they are short. Heads of 128 with keys by dimension
+// stay at 64: their 128-row form does not fit the registers (80 rows, 8 sequences of up to
+// 8000: 111 us, by 64 rows 65). Microseconds by 64 and by 128 rows, caches from HBM, one
+// sequence of 8 KV heads (128 rows: four of 4):
+//   head, keys by   66, 8000   128, 6000  192, 8000  192, 30000  256, 8000  512, 30000
+//   64, position    18.1 22.5  23.4 27.8  19.6 24.8  37.2 42.6   21.8 25.5  64.9 60.5
+//   64, dimension   19.2 22.7  25.4 29.7  20.8 26.1  41.9 45.3   23.7 26.9  77.5 64.9
+//   128, position   26.4 27.6  33.4 38.6  26.7 36.0  59.9 65.8   34.1 37.5   112 95.7
+//   256, position   49.5 56.3  65.3 73.2  63.4 69.0   158  152   72.3 71.0   357  261
+//   256, dimension  52.3 62.7  78.2 90.1  69.3 85.0   184  208   79.1 88.3   413  351
 static int tree_rows(int rows, int dim, bool kcol) {
   if (rows <= 64) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  return dim == 128 && (kcol || rows <= 192) ? 64 : 128;
+  return rows <= 192 || (dim == 128 && kcol) ? 64 : 128;
 }
 
 struct TreePlanHost {
