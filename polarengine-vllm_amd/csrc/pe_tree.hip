@@ -162,9 +162,12 @@ __device__ __forceinline__ int64_t rope_slot(const RopeArgs& a, int64_t row, int
   return len + (row - b * a.n);
 }
 
-// ONE: a workgroup takes one row, so that what follows from the row is uniform
+// ONE: a workgroup takes one row, so that what follows from the row is uniform. Five waves
+// a SIMD where the registers allow it: heads of 256 take more, and several rows to a cache
+// would spill two to six of them (4 x 2048 rows of 8 heads of 128, keys by dimension: 20.1
+// us, with four waves 18.2; by position 16.3 and 16.2).
 template <int D, bool BF, bool CACHE, bool COL, bool ONE>
-__global__ __launch_bounds__(256, D == 256 ? 4 : 5) void qk_norm_rope_kernel(const RopeArgs a) {
+__global__ __launch_bounds__(256, D == 256 || (CACHE && !ONE) ? 4 : 5) void qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int LPG = D / 8;      // lanes per head
   constexpr int G = 256 / LPG;    // heads at a time
   constexpr int U = 4;            // loads of a lane on their way
