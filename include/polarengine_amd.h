@@ -452,8 +452,9 @@ int pe_lm_head(const void* x, const void* w, int64_t M, int64_t N, int K, float*
  *       (a multiple of 8); queries and keys normed per head, x / sqrt(mean(x^2)
  *       + eps) * weight (no norm where the weight is NULL), then the first rot
  *       dimensions (a multiple of 16) rotated, pairs (j, j + rot / 2), by row
- *       positions[row] of rope float32 [rope_rows, rot] (cos, then sin). fp32,
- *       rounded once. q_out [rows, heads, head_dim], k_out [rows, kv_heads,
+ *       positions[row] of rope float32 [rope_rows, rot] (cos, then sin). In 64
+ *       bits, rounded once; the products x * weight have to lie in fp32's range.
+ *       q_out [rows, heads, head_dim], k_out [rows, kv_heads,
  *       head_dim]; zero rows where positions[row] is outside the table.
  *   pe_qk_norm_rope_write: the same for batch * n rows (n of any size), keys and
  *       values written to slots lengths[b] + i of the caches instead; nothing is

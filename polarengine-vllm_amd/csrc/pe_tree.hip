@@ -32,10 +32,13 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(const int64_t* __restrict
 // 16-byte load each, so a row is read once and the norm, the rotation and the one
 // rounding happen in registers. Bound by bytes: rows of 16-bit values read and
 // written once. The arithmetic behind the products of two 16-bit values (exact in 32
-// bits) is in 64, so that the one rounding is that of the exact value; in 32 bits about
-// one value in 65,000 rounds the other way. It is about half of the vector
-// instructions, which now take as long as the bytes: 8192 rows of 48 heads of 128 to a
-// cache 54 us (3.7 TB/s); 16 rows 4.4 us.
+// bits) is in 64 and its result is rounded once, so that a value is the exact one rounded
+// (but for one within 2^-45 of the middle between two): keys do not depend on the order
+// of a sum or on which call wrote them. In 32 bits one fp16 value in 5,500 and one bf16
+// value in 53,000 rounds the other way; rounded to 32 bits before the 16, one in 18,000
+// and in 170,000. It is about half of the vector instructions, which now take as long as
+// the bytes: 8192 rows of 48 heads of 128 to a cache 55 us (3.6 TB/s; with two roundings
+// 53); 16 rows 4.2 us.
 //
 // A workgroup takes a row (or several of a model with few heads), its heads four
 // loads a lane at a time, the row's angles once. Keys that the cache stores by
@@ -106,6 +109,14 @@ __device__ __forceinline__ double head_sum(double v) {
   return v;
 }
 
+// fp32 that rounds to 16 bits as v does: v's first 20 fraction bits, the last of them set
+// where anything follows (a bf16 result below 2^-126 is rounded twice all the same)
+__device__ __forceinline__ float to_odd_f32(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t hi = (uint32_t)(u >> 32) | min((uint32_t)u, 1u);
+  return (float)__builtin_bit_cast(double, (uint64_t)hi << 32);
+}
+
 // one head: u (eight 16-bit values of the lane) normed with w, turned, rounded
 template <int D, bool BF>
 __device__ __forceinline__ u32x4v rope_head(const RopeArgs& a, u32x4v u, const uint16_t* w,
@@ -146,7 +157,7 @@ __device__ __forceinline__ u32x4v rope_head(const RopeArgs& a, u32x4v u, const u
     double t = v[i];
     // dimensions past the rotary ones keep their value, whatever the other lane holds
     if (lane < a.rot / 8) t = __builtin_fma(t, r.c[i], (double)o[i] * r.s[i]);
-    f[i] = (float)(t * y);
+    f[i] = to_odd_f32(t * y);
     // kept in 32 bits: the direct conversion to 16 takes a dozen instructions more
     asm("" : "+v"(f[i]));
   }

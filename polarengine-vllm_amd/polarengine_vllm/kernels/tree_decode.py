@@ -223,7 +223,8 @@ def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, rope: torch.Tenso
     256), RMS-normed per head with the weights [head_dim] that are given, then
     rotated: dimensions j and j + r / 2 of the first r by the angles of row
     positions[row] of ``rope`` float32 [table rows, r], cosines then sines, r a
-    multiple of 16. fp32, rounded once; zeros where the position is outside the
+    multiple of 16. In 64 bits, rounded once (the products of a value and its
+    weight have to lie in fp32's range); zeros where the position is outside the
     table. ``positions`` int64, one a row in any shape."""
     dev = _inputs(qkv, rope, positions, q_weight, k_weight)
     rows, dim, code, qkv, rope, positions, qw, kw = _rope_inputs(
