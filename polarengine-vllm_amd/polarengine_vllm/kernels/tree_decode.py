@@ -152,6 +152,11 @@ def _writable(t: torch.Tensor, name: str) -> None:
             span += stride * (size - 1)
 
 
+def _apart(k: torch.Tensor, v: torch.Tensor) -> None:
+    if k.numel() and k.data_ptr() == v.data_ptr():
+        raise ValueError("k_cache and v_cache are the same memory")
+
+
 def _written(*tensors: torch.Tensor) -> None:
     """Counts writes through raw pointers (inference tensors keep no count)."""
     for t in tensors:
@@ -259,8 +264,8 @@ def qk_norm_rope_write(qkv: torch.Tensor, heads: int, kv_heads: int, rope: torch
         raise ValueError(f"{rows} rows do not go into {batch} sequences")
     _writable(k_cache, "k_cache")
     _writable(v_cache, "v_cache")
-    if k_cache.data_ptr() == v_cache.data_ptr() and rows:
-        raise ValueError("k_cache and v_cache are the same memory")
+    if rows:
+        _apart(k_cache, v_cache)
     q = torch.empty(rows, heads, dim, dtype=qkv.dtype, device=dev)
     if rows:
         _call("pe_qk_norm_rope_write", dev, qkv.data_ptr(), code, batch, rows // batch,
@@ -416,6 +421,7 @@ def keep_accepted(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.T
             raise ValueError(f"{name} must be [(layers,) {batch}, kv_heads, positions, head_dim], "
                              f"got {list(cache.shape)}")
         views.append(c)
+    _apart(k_cache, v_cache)  # moved twice, rows would end up elsewhere
     for c in views:
         if c.numel():
             layers, _, heads, cap, dim = c.shape

@@ -95,3 +95,18 @@ def test_attention_runs_fit_every_xcd(dim, per_cu, n, group):
         assert -(-runs // 8) * blocks <= slots and runs * blocks > 8 * (slots - blocks)
     else:
         assert runs * blocks <= 8 * slots or runs == 1
+
+
+def test_one_cache_for_keys_and_values_is_refused(calls):
+    """The accepted rows of one memory would be moved twice."""
+    from polarengine_vllm.kernels import tree_decode as td
+    _, k, lengths, masks, qkv, table, pos = _inputs()
+    for call in (lambda: td.keep_accepted(k, k, lengths, masks, lengths),
+                 lambda: td.keep_accepted(k[None], k[None], lengths, masks, lengths),
+                 lambda: td.qk_norm_rope_write(qkv, 4, 2, table, pos, k, k, lengths)):
+        with pytest.raises(ValueError, match="same memory"):
+            call()
+    assert not calls
+    both = torch.zeros(2, 2, 16, 128, dtype=BF)  # side by side in one tensor
+    td.keep_accepted(both[..., :64], both[..., 64:], lengths, masks, lengths)
+    assert len(calls) == 2
