@@ -422,9 +422,10 @@ def keep_accepted(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.T
                              f"got {list(cache.shape)}")
         views.append(c)
     _apart(k_cache, v_cache)  # moved twice, rows would end up elsewhere
-    for c in views:
-        if c.numel():
-            layers, _, heads, cap, dim = c.shape
-            _call("pe_keep_accepted", dev, c.data_ptr(), layers, batch, heads, cap, dim, *_strides(c),
-                  lengths.data_ptr(), path.data_ptr(), count.data_ptr(), n)
+    args = [(c.data_ptr(), c.shape[0], batch, *c.shape[2:], *_strides(c), lengths.data_ptr(),
+             path.data_ptr(), count.data_ptr(), n) for c in views if c.numel()]
+    if len(args) == 2:  # the values' layout, without layers to move, before the keys move
+        _lib.check(_lib.lib().pe_keep_accepted(args[1][0], 0, *args[1][2:], None), "pe_keep_accepted")
+    for a in args:
+        _call("pe_keep_accepted", dev, *a)
     _written(k_cache, v_cache)

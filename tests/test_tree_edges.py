@@ -110,3 +110,15 @@ def test_one_cache_for_keys_and_values_is_refused(calls):
     both = torch.zeros(2, 2, 16, 128, dtype=BF)  # side by side in one tensor
     td.keep_accepted(both[..., :64], both[..., 64:], lengths, masks, lengths)
     assert len(calls) == 2
+
+
+def test_nothing_moves_if_the_values_cannot(calls):
+    """Values whose layout the library refuses: before the keys have moved."""
+    from polarengine_vllm.kernels import tree_decode as td
+    _, k, lengths, masks, *_ = _inputs()
+    for v in (torch.zeros(2, 2, 16, 68, dtype=BF)[..., 4:],         # rows not 16-byte aligned
+              torch.zeros(2, 2, 16, 132, dtype=BF)[..., ::2][..., :64],  # nothing contiguous
+              torch.zeros(2, 2, 16, 60, dtype=BF)):
+        with pytest.raises(RuntimeError, match="pe_keep_accepted"):
+            td.keep_accepted(k, v, lengths, masks, lengths)
+    assert not calls
