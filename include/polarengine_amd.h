@@ -487,7 +487,8 @@ int pe_lm_head(const void* x, const void* w, int64_t M, int64_t N, int K, float*
  *       token; both -1 past count. Sums and comparisons in 64 bits.
  *   pe_keep_accepted: slots lengths[b] + j of cache [layers, batch, heads, cap,
  *       dim] take the rows of slots lengths[b] + path[b][j], j < count[b], in
- *       place (16-bit values; strides as above, s_d = 1 or s_l = 1). Only an
+ *       place (16-bit values; strides as above, s_d = 1 or s_l = 1; layers 0
+ *       checks the other arguments). Only an
  *       ascending path within the n slots is followed.
  */
 int pe_tree_plan(const int64_t* parents, int64_t parents_stride, const int64_t* lengths,

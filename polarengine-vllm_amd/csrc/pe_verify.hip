@@ -394,8 +394,9 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(const VerifyArgs a) {
   }
 }
 
-// E consecutive logits of a thread: what is left of them times the row's sum, and the
-// row's own weights
+// The next token. A workgroup sums the weights that are left of a piece, and the row's own
+// (for where nothing is left), E consecutive tokens a thread; the last one to finish finds
+// the piece that holds the token and goes through it once more.
 template <int DT>
 __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a) {
   __shared__ uint32_t gone[kPickChunk / 32];  // the piece's tokens that were rejected

@@ -15,9 +15,11 @@ below ``lengths[b]`` hold the sequence so far. In the order of a step:
 
 Everything that differs between sequences is read on the device, so a captured
 step serves every length, tree and outcome. ``lengths[b] < 0``, or too long for the
-cache to hold n more, marks an empty slot of the batch: its outputs are zeros and
-nothing of it is written. A node whose parent is no earlier existing node is
-absent (a padded place of a smaller tree).
+cache to hold n more, marks an empty slot of the batch: the attention gives it
+zeros, and nothing of it is written or moved. (The queries follow the positions
+alone: zeros where the table has none, as for the plan's -1.) ``verify_drafts``
+knows an empty slot by its node 0's token. A node whose parent is no earlier
+existing node is absent (a padded place of a smaller tree).
 
 Caches are [batch, kv_heads, positions, head_dim] views, fp16 or bf16: values with
 the dimension contiguous, keys with the dimension or the position contiguous (the
@@ -45,7 +47,7 @@ MAX_NODES = 64
 class TreePlan(NamedTuple):
     """What the layers of one step share: int64 [batch, n]."""
 
-    positions: torch.Tensor  # of each node; -1 for absent nodes and empty slots
+    positions: torch.Tensor  # of each node; -1 for absent nodes and where lengths[b] < 0
     masks: torch.Tensor      # bit j of node i's word: j is i or an ancestor of i
 
 
@@ -251,7 +253,8 @@ def qk_norm_rope_write(qkv: torch.Tensor, heads: int, kv_heads: int, rope: torch
                        eps: float = 1e-6) -> torch.Tensor:
     """The same for the n rows of each sequence (any n: a step's nodes, a prompt),
     keys and values written to slots ``lengths[b] + i`` of the caches; returns the
-    queries. Rows whose position is outside the table leave their slot as it was."""
+    queries. Rows whose position is outside the table, and those of a sequence whose
+    cache has no room for n more, leave their slots as they were."""
     dev = _inputs(qkv, rope, positions, k_cache, v_cache, lengths, q_weight, k_weight)
     rows, dim, code, qkv, rope, positions, qw, kw = _rope_inputs(
         qkv, heads, kv_heads, rope, positions, q_weight, k_weight)
@@ -285,8 +288,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     mask (int64 [batch, n], or [n] for all). Scores, softmax statistics and sums in
     fp32; the probabilities are rounded to the queries' type for the product with the
     values, where fp16 loses bits of those below 2^-21 of a row's largest and all of
-    those below 2^-32. ``scale`` is 1 / sqrt(head_dim) unless given. A node with
-    nothing to see gets zeros."""
+    those below 2^-32. ``scale``, 0 or more, is 1 / sqrt(head_dim) unless given. A
+    node with nothing to see gets zeros."""
     dev = _inputs(q, k_cache, v_cache, lengths, masks)
     code = _lib.act_dtype(q)
     if q.dim() != 4:
@@ -332,8 +335,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     c, ``uniforms[b, 0]`` the next token. parents int64 [batch, n] or [n]; None
     for a chain. draft_probs float32 [batch, n - 1, vocab], for a chain: row i is
     what node i + 1 was drawn from; None for drafts that are no random draws (the
-    likeliest tokens, a lookup). temperature: a number or float32 [batch]; 0 takes
-    the first largest logit.
+    likeliest tokens, a lookup). temperature: a number or float32 [batch]; 0 (in a
+    tensor, NaN or less than 0 too) takes the first largest logit.
 
     The children of a node are tried in order. With p = softmax(logits /
     temperature) child c of token x is accepted if u_c r < p(x), r being what the
