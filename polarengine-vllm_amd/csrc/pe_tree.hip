@@ -37,8 +37,8 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(const int64_t* __restrict
 // of a sum or on which call wrote them. In 32 bits one fp16 value in 5,500 and one bf16
 // value in 53,000 rounds the other way; rounded to 32 bits before the 16, one in 18,000
 // and in 170,000. It is about half of the vector instructions, which now take as long as
-// the bytes: 8192 rows of 48 heads of 128 to a cache 55 us (3.6 TB/s; with two roundings
-// 53); 16 rows 4.2 us.
+// the bytes: 8192 rows of 48 heads of 128 to a cache 55 to 57 us (3.6 TB/s; with two
+// roundings 53), keys by position 51; 16 rows 4.2 us.
 //
 // A workgroup takes a row (or several of a model with few heads), its heads four
 // loads a lane at a time, the row's angles once. Keys that the cache stores by

@@ -28,10 +28,10 @@
 // sequence that a cut divides.
 //
 // Bound by HBM where a KV head has few rows: 32 sequences x 8 nodes, 32 rows, up to
-// 16,000 positions 261 us, 5.4 TB/s (tiles through registers 493, equal parts of each
-// sequence instead of the line 315). With 512 rows over 32,700 positions 92 us, 0.74
-// PFLOP/s: the softmax between the products keeps the matrix cores busy 29% of the
-// time. One sequence of 777 and 16 rows: 8.0 + 4.3 us, latency.
+// 16,000 positions 262 us for both launches, 5.4 TB/s (tiles through registers 493, equal
+// parts of each sequence instead of the line 315). With 512 rows over 32,700 positions 94
+// us, 0.73 PFLOP/s: the softmax between the products keeps the matrix cores busy 29% of
+// the time. One sequence of 777 and 16 rows: 11.5 us, latency.
 
 #include <type_traits>
 

@@ -15,11 +15,11 @@
 // finish finds the piece and the token in it. The counters of that hand-over are
 // cleared by the second launch, so the workspace needs no state between calls.
 //
-// Measured: 8 x 64 nodes over 151,936 32-bit logits 72.6 + 14.1 + 15.8 us (the read
-// 4.3 TB/s, its exponentials alone 34 us of 64-bit instructions); 32 x 8 nodes over
-// 100,003 16-bit ones 21.0 + 6.0 + 18.8; one sequence of five nodes 7.2 + 5.2 + 10.7,
-// each launch a chain of loads and sums. With the walk in every workgroup of the draw,
-// two launches: 115, 52 and 23 us in all.
+// Measured: 8 x 64 nodes over 151,936 32-bit logits 74.7 + 13.9 + 15.6 us (the read
+// 4.2 TB/s beside 64-bit exponentials; greedy, without them, 55.4 + 13.0 + 4.5); 32 x 8
+// nodes over 100,003 16-bit ones 20.8 + 6.2 + 19.1 (greedy 13.0 + 4.8 + 1.8); one
+// sequence of five nodes 7.5 + 4.9 + 11.1, each launch a chain of loads and sums. With
+// the walk in every workgroup of the draw, two launches: 115, 52 and 23 us in all.
 
 #include "pe_tree.h"
 
