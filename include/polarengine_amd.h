@@ -523,6 +523,84 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
                      const int64_t* lengths, const int64_t* path, const int64_t* count, int n,
                      void* stream);
 
+/*
+ * Serving over a paged cache in 8 bits; no reference file. Sequences of different
+ * lengths share a pool of blocks of block_size positions (16, 32, 64 or 128). A
+ * layer's cache: keys e4m3 [blocks, kv_heads, block_size, head_dim], values e4m3
+ * [blocks, kv_heads, head_dim, block_size], each block and head with a power of two
+ * as scale (e8m0 [blocks, kv_heads]: 2^(byte - 127)); a block's parts are contiguous
+ * and 16-byte aligned, k_b, v_b and s_b are the strides of blocks in bytes.
+ * head_dim 64, 128 or 256. tables int32 [batch, width] (row stride t_b): the blocks
+ * of each sequence in order of position, below 0 where it has none. All sizes that
+ * differ between sequences are read on the device.
+ *   pe_plan_step: room for counts[b] more positions of each sequence of lengths[b]
+ *       (int64; lengths[b] < 0: an empty slot). Rows of the step are packed: those of
+ *       sequence b begin at starts[b] (int64 [batch + 1], the running sum of the
+ *       counts, at most rows). Blocks that a sequence lacks for positions lengths[b]
+ *       .. lengths[b] + counts[b] - 1 are taken from the end of the first
+ *       free_count[0] entries of free_blocks (int32 [free_cap]), sequence after
+ *       sequence, and written to tables; free_count falls. A sequence whose rows pass
+ *       `rows`, whose positions pass its table, or whose blocks and those of the
+ *       sequences before it (in the way or not) pass free_count gets nothing.
+ *       positions and slots int64 [rows]: position of each row and block *
+ *       block_size + position % block_size, -1 for rows of such sequences and behind
+ *       the last; out_lengths int64 [batch]: lengths[b] + counts[b], or -1 where the
+ *       sequence got nothing or is empty. batch <= 4096, rows <= 2^24.
+ *   pe_release_blocks: the blocks of each sequence from position keep[b], rounded up
+ *       to a block, on, up to its first entry below 0, go back to the end of
+ *       free_blocks (the last sequence's last block first, so that a released plan
+ *       leaves the pool as it was) and -1 takes their place; keep[b] < 0: none.
+ *       Nothing moves if they do not fit free_blocks.
+ *   pe_write_blocks: keys and values [rows, kv_heads, head_dim] of 16 bits (strides
+ *       of row and head in elements) to slots[row] of a layer's cache (< 0 or past
+ *       the last block: none). A run, rows whose slots rise by one within a block,
+ *       gives the block the smallest scale 2^e (e >= -100) that holds its largest
+ *       finite |x| as at most 448 2^e, and no smaller one than the block's own unless
+ *       the run begins at the block's first slot; codes already in the block are
+ *       rounded to the new scale where it has grown. Codes are x 2^-e rounded to the
+ *       nearest e4m3 value, ties to even; NaN where x is not finite. Only one run of a
+ *       call may go to a block.
+ *   pe_paged_attention: q [rows, heads, head_dim] (row stride q_r) of sequences whose
+ *       rows begin at starts (int64 [batch + 1]), the last of a sequence at position
+ *       lengths[b] - 1. out [rows, heads, head_dim] = softmax(scale q K^T) V over the
+ *       positions j <= p of a row's position p with j > p - window or j < sinks
+ *       (window 0: all). Rows of a sequence with lengths[b] < 0, before position 0,
+ *       without a block in sight, and outside all sequences get zeros; positions
+ *       whose block is none of the cache's are not seen. Scores, softmax statistics
+ *       and sums in fp32.
+ *   pe_token_logprobs: of logits [rows, vocab] (PE_DTYPE_F32 too; row stride ld) and
+ *       tokens int64 [rows]: logprob float32 = x[t] - log sum exp x, rank int64 = how
+ *       many tokens come before t (larger logit, or as large and of a lower number),
+ *       entropy float32 of softmax(x), and the `top` likeliest tokens in order
+ *       (top_logprobs float32, top_tokens int64, [rows, top], ties by number).
+ *       A token outside the vocabulary: logprob 0, rank -1. top <= 64, vocab >= top.
+ */
+int pe_plan_step(const int64_t* lengths, const int64_t* counts, int32_t* tables, int64_t t_b,
+                 int64_t batch, int64_t width, const int32_t* free_blocks, int64_t free_cap,
+                 int64_t* free_count, int64_t rows, int block_size, int64_t* starts,
+                 int64_t* positions, int64_t* slots, int64_t* out_lengths, void* stream);
+int pe_release_blocks(int32_t* tables, int64_t t_b, int64_t batch, int64_t width,
+                      const int64_t* keep, int32_t* free_blocks, int64_t free_cap,
+                      int64_t* free_count, int block_size, void* stream);
+int pe_write_blocks(const void* k, const void* v, int dtype, int64_t rows, int64_t k_r, int64_t k_h,
+                    int64_t v_r, int64_t v_h, const int64_t* slots, void* k_codes, int64_t k_b,
+                    void* v_codes, int64_t v_b, void* k_scale, void* v_scale, int64_t s_b,
+                    int64_t blocks, int kv_heads, int block_size, int head_dim, void* stream);
+size_t pe_paged_attention_workspace_size(int64_t rows, int64_t batch, int heads, int kv_heads,
+                                         int head_dim, int64_t positions);
+int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t rows, int heads,
+                       const void* k_codes, int64_t k_b, const void* v_codes, int64_t v_b,
+                       const void* k_scale, const void* v_scale, int64_t s_b, int64_t blocks,
+                       int kv_heads, int block_size, int head_dim, const int32_t* tables,
+                       int64_t t_b, int64_t batch, int64_t width, const int64_t* starts,
+                       const int64_t* lengths, int64_t window, int64_t sinks, float scale, void* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t pe_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top);
+int pe_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t ld, int64_t vocab,
+                      const int64_t* tokens, int top, float* logprob, int64_t* rank, float* entropy,
+                      float* top_logprobs, int64_t* top_tokens, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

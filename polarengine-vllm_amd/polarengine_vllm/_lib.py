@@ -103,6 +103,19 @@ _SIGNATURES = {
                                   _vp, _c_sz, _vp]),
     "pe_keep_accepted": (_c_int, [_vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_i64, _c_i64, _c_i64,
                                   _c_i64, _c_i64, _vp, _vp, _vp, _c_int, _vp]),
+    "pe_plan_step": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int,
+                              _vp, _vp, _vp, _vp, _vp]),
+    "pe_release_blocks": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _c_int, _vp]),
+    "pe_write_blocks": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp,
+                                 _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int,
+                                 _c_int, _vp]),
+    "pe_paged_attention_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_int, _c_int, _c_int, _c_i64]),
+    "pe_paged_attention": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_int, _vp, _c_i64, _vp, _c_i64, _vp,
+                                    _vp, _c_i64, _c_i64, _c_int, _c_int, _c_int, _vp, _c_i64, _c_i64,
+                                    _c_i64, _vp, _vp, _c_i64, _c_i64, _c_float, _vp, _vp, _c_sz, _vp]),
+    "pe_token_logprobs_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_int]),
+    "pe_token_logprobs": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_int, _vp, _vp, _vp,
+                                   _vp, _vp, _vp, _c_sz, _vp]),
 }
 
 # measurement helpers (include/polarengine_amd_bench.h)

@@ -36,10 +36,10 @@ import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
-import torch.autograd.forward_ad as fwAD
-from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
+from polarengine_vllm.kernels._calls import (call as _call, inputs as _inputs, int64 as _int64,
+                                             written as _written)
 
 MAX_NODES = 64
 
@@ -49,49 +49,6 @@ class TreePlan(NamedTuple):
 
     positions: torch.Tensor  # of each node; -1 for absent nodes and where lengths[b] < 0
     masks: torch.Tensor      # bit j of node i's word: j is i or an ancestor of i
-
-
-def _call(name: str, dev: torch.device, *args) -> None:
-    """One call into the library on the device's current stream, the device made the
-    current one around it where it is another."""
-    lib = _lib.lib()
-    here, index = torch._C._cuda_getDevice(), dev.index
-    if here == index:
-        rc = getattr(lib, name)(*args, _lib.stream_ptr(dev))
-    else:
-        torch._C._cuda_setDevice(index)
-        try:
-            rc = getattr(lib, name)(*args, _lib.stream_ptr(dev))
-        finally:
-            torch._C._cuda_setDevice(here)
-    if rc:
-        _lib.check(rc, name)
-
-
-def _inputs(*tensors: Optional[torch.Tensor]) -> torch.device:
-    """The one GPU of the tensors; refuses others, and inputs that autograd follows
-    (reverse mode, or forward mode, which no_grad does not turn off)."""
-    grad = torch.is_grad_enabled()
-    dual = fwAD._current_level >= 0  # outside a dual level no tensor has a tangent
-    index = tensors[0].get_device()
-    for t in tensors:
-        if t is not None:
-            if t.get_device() != index or index < 0:
-                _lib.require_device(*tensors)
-            if (grad and t.requires_grad) or (
-                    dual and not t.is_inference() and fwAD.unpack_dual(t).tangent is not None):
-                raise RuntimeError("the drafted-token kernels have no backward pass: call them "
-                                   "under torch.no_grad(), without forward-mode tangents, or "
-                                   "detach their inputs")
-    return tensors[0].device
-
-
-def _int64(t: torch.Tensor, shape: Tuple[int, ...], name: str) -> torch.Tensor:
-    if t.dtype is not torch.int64:
-        raise TypeError(f"{name} must be int64, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    return t.contiguous()
 
 
 def _per_node(t: torch.Tensor, batch: int, n: int, name: str) -> Tuple[torch.Tensor, int]:
@@ -157,13 +114,6 @@ def _writable(t: torch.Tensor, name: str) -> None:
 def _apart(k: torch.Tensor, v: torch.Tensor) -> None:
     if k.numel() and k.data_ptr() == v.data_ptr():
         raise ValueError("k_cache and v_cache are the same memory")
-
-
-def _written(*tensors: torch.Tensor) -> None:
-    """Counts writes through raw pointers (inference tensors keep no count)."""
-    for t in tensors:
-        if not t.is_inference():
-            increment_version(t)
 
 
 def tree_plan(parents: torch.Tensor, lengths: torch.Tensor) -> TreePlan:
