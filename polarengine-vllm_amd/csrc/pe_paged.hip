@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void write_blocks_kernel(const WriteArgs a) {
 static bool plan_shape_ok(int64_t batch, int64_t width, int64_t t_b, int64_t free_cap,
                           int block_size) {
   if (block_size != 16 && block_size != 32 && block_size != 64 && block_size != 128) return false;
-  return batch >= 0 && batch <= kPagedMaxBatch && width >= 1 && width <= INT32_MAX / 128 &&
+  return batch >= 0 && batch <= kPagedMaxBatch && width >= 1 && width <= kPagedMaxWidth &&
          t_b >= width && free_cap >= 1 && free_cap <= INT32_MAX;
 }
 static int log2_of(int block_size) {

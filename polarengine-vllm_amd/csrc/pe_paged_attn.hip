@@ -1,83 +1,698 @@
-// Attention over the paged 8-bit cache: a wave per row and head, 64 positions a
-// step, scores and sums in fp32.
+// Attention over the paged 8-bit cache: packed rows of sequences of different lengths,
+// each row over the positions up to its own, or over a window of them and the first
+// few.
+//
+// The rows of one KV head (new tokens x group query heads) go through the matrix cores
+// together, 16 RT of them. A wave takes 64 positions a step, straight from memory to
+// registers:
+//  * scores S^T = K Q^T (v_mfma_f32_16x16x32, keys as A). Which key is which row of A
+//    is free, so row 4 g + e of product t is position 16 g + 4 t + e: a lane then
+//    holds the scores of 16 neighbouring positions of one row of queries, which lie in
+//    one block, so one scale serves all of them;
+//  * the probabilities, in fp16, are the B operand of O^T = V^T P^T just as the scores'
+//    products left them, and the lane's part of V^T is 16 neighbouring bytes of the
+//    block's values, which are stored by dimension. Nothing goes through LDS;
+//  * e4m3 values are exact in fp16 and bf16 (v_cvt_scalef32_pk, two a instruction).
+//    The keys' scale multiplies the fp32 scores; the values' is applied by the
+//    conversion, relative to the largest that the wave has seen (er: sums are rescaled
+//    when it grows), 2^7 times as large: codes of a scale down to 2^-22 of the largest
+//    stay exact.
+//  * one pass with running maximum and sum in fp32. Probabilities are 2^7 times as
+//    large and relative to a base that moves only when they would pass 2^15, so that
+//    fp16 keeps what is 2^-21 of the largest whole and what is above 2^-32 of it in
+//    part. Rounding them costs half an fp16 step of each (in the sum that divides
+//    alike): less than the rounding of a bf16 result, about that of an fp16 one.
+// The four waves of a workgroup take 64 positions each of a tile of 256 and join their
+// sums in LDS at the end of a row block.
+//
+// The tiles of all sequences, KV heads and row blocks form one line, cut into equal
+// runs, one a workgroup, by the lengths read on the device; a second launch joins the
+// parts of a row block that a cut divides.
 
 #include "pe_paged.h"
 
 namespace pe {
+
+constexpr int kPaTile = 256;       // positions of a step of a workgroup
+constexpr float kPaLog2e = 1.4426950408889634f;
+constexpr float kPaSlack = 8.f;    // powers of two that an exponent may exceed its base by
+constexpr float kPaLift = 7.f;     // and by which probabilities are larger
+constexpr int kPaVLift = 7;        // and values
 
 struct PagedAttnArgs {
   const uint16_t* q;
   int64_t q_r;
   PagedCache c;
   const int32_t* tables;
-  int64_t t_b, width;
+  int64_t t_b;
+  int width;
   const int64_t *starts, *lengths;
   uint16_t* out;
-  int rows, batch, heads, group;
-  int64_t window, sinks;
+  int rows, batch, group;
+  int window;  // 0: none
+  int sinks;
   float scale;
+  int runs;
+  float* parts;  // [runs][2]: a run divides at most its first and its last row block
 };
 
-__device__ __forceinline__ float wave_max64(float v) {
+// fp32 words of one part: RB x D sums, RB maxima, RB sums
+__host__ __device__ inline int64_t pa_part_words(int rb, int dim) { return (int64_t)rb * (dim + 2); }
+
+// ---------------------------------------------------------------------------
+// The line of tiles: sequence after sequence, within one KV head after KV head, within
+// one row block after the other. Rows of an empty sequence and behind the last have a
+// tile without positions, for their zeros.
+// ---------------------------------------------------------------------------
+struct PaSeq {
+  int first, n;    // rows
+  int lead;        // rows before starts[b] (of sequence 0, where starts[0] > 0)
+  int64_t p0;      // position of row `first`; -1 - n and below: none
+  int blocks;      // row blocks of a KV head
+};
+template <int RB>
+__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) {
+  PaSeq s{0, 0, 0, 0, 0};
+  if (b > a.batch) return s;
+  const int64_t rows = a.rows;
+  const int64_t s0 = b == 0 ? 0 : max((int64_t)0, min(a.starts[b], rows));
+  const int64_t end = b == a.batch ? rows : a.starts[b + 1];
+  const int64_t s1 = max(s0, min(end, rows));
+  const int64_t len = b == a.batch ? -1 : a.lengths[b];
+  s.first = (int)s0;
+  s.n = (int)(s1 - s0);
+  s.lead = b == 0 ? (int)max((int64_t)0, min(a.starts[0], rows)) : 0;
+  s.p0 = len >= 0 ? len - (end - s0) : INT64_MIN / 2;
+  s.blocks = (int)(((int64_t)s.n * a.group + RB - 1) / RB);
+  return s;
+}
+// the positions of row block qb: [0, sink) and [lo, hi), in tiles
+struct PaSpan {
+  int lo, hi, sink;
+  int sink_tiles, first_tile, tiles;
+};
+template <int RB>
+__device__ __forceinline__ PaSpan pa_span(const PagedAttnArgs& a, const PaSeq& s, int qb) {
+  PaSpan r;
+  const int cap = a.width << a.c.log_t;
+  const int t0 = (int)((int64_t)qb * RB / a.group);
+  const int t1 = min(s.n - 1, (int)(((int64_t)qb * RB + RB - 1) / a.group));
+  r.hi = (int)max((int64_t)0, min(s.p0 + t1 + 1, (int64_t)cap));
+  r.lo = 0;
+  if (a.window) r.lo = (int)max((int64_t)0, min(s.p0 + t0 - a.window + 1, (int64_t)cap));
+  r.sink = min(a.sinks, r.lo);
+  r.sink_tiles = (r.sink + kPaTile - 1) / kPaTile;
+  r.first_tile = max(r.lo / kPaTile, r.sink_tiles);
+  r.tiles = max(1, r.sink_tiles + max(0, (r.hi + kPaTile - 1) / kPaTile - r.first_tile));
+  return r;
+}
+// tiles of all row blocks of a sequence, one KV head
+template <int RB>
+__device__ __forceinline__ int64_t pa_tiles(const PagedAttnArgs& a, const PaSeq& s) {
+  int64_t sum = 0;
+  for (int qb = 0; qb < s.blocks; ++qb) sum += pa_span<RB>(a, s, qb).tiles;
+  return sum;
+}
+__device__ __forceinline__ int64_t pa_scan(int64_t v, int lane) {
 #pragma unroll
-  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t u = __shfl_up((long long)v, off, 64);
+    if (lane >= off) v += u;
+  }
   return v;
 }
+// a row block's place in the line
+struct PaPlace {
+  int b, kvh, qb, t0;  // and the tile of the row block
+  int tiles;
+};
+// one wave: the length of the line
+template <int RB>
+__device__ __forceinline__ int64_t pa_total(const PagedAttnArgs& a, int lane) {
+  int64_t sum = 0;
+  for (int b0 = 0; b0 <= a.batch; b0 += 64) sum += pa_tiles<RB>(a, pa_seq<RB>(a, b0 + lane));
+#pragma unroll
+  for (int m = 32; m; m >>= 1) sum += __shfl_xor((long long)sum, m, 64);
+  return sum * a.c.kv_heads;
+}
+// one wave: what holds place `at` of the line (all lanes; at below the total)
+template <int RB>
+__device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, int64_t at, int lane) {
+  PaPlace r{-1, 0, 0, 0, 0};
+  int64_t before = 0;
+  for (int b0 = 0; b0 <= a.batch; b0 += 64) {
+    const int64_t mine = pa_tiles<RB>(a, pa_seq<RB>(a, b0 + lane));
+    const int64_t scan = pa_scan(mine, lane);
+    const uint64_t hit = __ballot((before + scan) * a.c.kv_heads > at);
+    if (!hit) {
+      before += __shfl((long long)scan, 63, 64);
+      continue;
+    }
+    const int l = __builtin_ctzll(hit);
+    const int64_t tiles = __shfl((long long)mine, l, 64);
+    at -= (before + __shfl((long long)scan, l, 64) - tiles) * a.c.kv_heads;
+    r.b = b0 + l;
+    r.kvh = (int)(at / tiles);
+    at -= r.kvh * tiles;
+    const PaSeq s = pa_seq<RB>(a, r.b);
+    for (int q0 = 0; q0 < s.blocks; q0 += 64) {
+      const int64_t t = q0 + lane < s.blocks ? pa_span<RB>(a, s, q0 + lane).tiles : 0;
+      const int64_t sc = pa_scan(t, lane);
+      const uint64_t in = __ballot(sc > at);
+      if (in) {
+        const int k = __builtin_ctzll(in);
+        r.qb = q0 + k;
+        r.tiles = (int)__shfl((long long)t, k, 64);
+        r.t0 = (int)(at - (__shfl((long long)sc, k, 64) - r.tiles));
+        return r;
+      }
+      at -= __shfl((long long)sc, 63, 64);
+    }
+    break;
+  }
+  r.b = -1;  // only if the lengths change under the kernel
+  return r;
+}
 
-template <int D, bool BF>
-__global__ __launch_bounds__(64) void paged_attn_kernel(const PagedAttnArgs a) {
-  __shared__ float qs[D];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int T = 1 << a.c.log_t;
-  int lo = 0, hi = a.batch;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.starts[mid + 1] > row) hi = mid;
-    else lo = mid + 1;
+// ---------------------------------------------------------------------------
+// MFMA operands
+// ---------------------------------------------------------------------------
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+template <bool BF>
+__device__ __forceinline__ float4v pa_mfma(u32x4v a, u32x4v b, float4v c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, a),
+                                                   __builtin_bit_cast(bf16x8v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, a),
+                                                  __builtin_bit_cast(half8v, b), c, 0, 0, 0);
+}
+// eight e4m3 values times a power of two, as bf16 or fp16
+template <bool BF>
+__device__ __forceinline__ u32x4v pa_unpack(uint32_t lo, uint32_t hi, float s) {
+  if constexpr (BF)
+    return u32x4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true))};
+  else
+    return u32x4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, true)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, true))};
+}
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{lo, hi}), half2v));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pa_pack16(float lo, float hi) {
+  const float2v v{lo, hi};
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2v));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2v));
+}
+// maximum over the four lanes li, li + 16, li + 32, li + 48, in each of them
+__device__ __forceinline__ float pa_rows_max(float v) {
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t x0 = x[0], x1 = x[1];
+  u = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1)));
+  auto y = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t y0 = y[0], y1 = y[1];
+  return fmaxf(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1));
+}
+// bit 7 of each byte that is a NaN code
+__device__ __forceinline__ uint32_t pa_nan(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
+// the bits of positions below n, of 16
+__device__ __forceinline__ uint32_t pa_below(int n) { return (1u << min(max(n, 0), 16)) - 1; }
+
+template <int D, bool BF, int RT>
+__global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
+  constexpr int RB = 16 * RT;      // rows of a row block
+  constexpr int KS = D / 32;       // products of 32 dimensions
+  constexpr int KL = D / 64;       // 16-byte loads of a key row's part
+  constexpr int DT = D / 16;       // products of 16 dimensions of values
+  __shared__ __align__(16) float4v join[2][RT * DT * 64];
+  __shared__ float join_m[4][RB], join_l[4][RB];
+  __shared__ PaPlace place;
+  __shared__ int64_t line;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  if (wave == 0) {
+    const int64_t total = pa_total<RB>(a, lane);
+    if (lane == 0) line = total;
   }
-  uint16_t* out = a.out + ((int64_t)row * a.heads + h) * D;
-  float o[D / 64] = {};
-  float m = -__builtin_inff(), l = 0.f;
-  int64_t p = -1;
-  const int b = lo;
-  if (b < a.batch && row >= a.starts[b] && a.lengths[b] >= 0)
-    p = a.lengths[b] - (a.starts[b + 1] - row);
-  const uint16_t* q = a.q + row * a.q_r + (int64_t)h * D;
-  for (int d = lane; d < D; d += 64) qs[d] = f16or_bf(q[d], BF) * a.scale;
   __syncthreads();
-  const int kvh = h / a.group;
-  const int64_t end = min(p + 1, a.width << a.c.log_t);
-  for (int64_t j0 = 0; j0 < end; j0 += 64) {
-    if (a.window && j0 + 63 <= p - a.window && j0 >= a.sinks) continue;
-    const int64_t j = j0 + lane;
-    bool seen = j < end && (!a.window || j > p - a.window || j < a.sinks);
-    const int64_t block = seen ? a.tables[b * a.t_b + (j >> a.c.log_t)] : -1;
-    seen = block >= 0 && block < a.c.blocks;
-    float s = -__builtin_inff();
-    if (seen) {
-      const uint8_t* k = a.c.k + block * a.c.k_b + ((int64_t)kvh * T + (j & (T - 1))) * D;
-      s = 0.f;
-      for (int d = 0; d < D; ++d) s += qs[d] * __builtin_amdgcn_cvt_f32_fp8(k[d], 0);
-      s *= e8m0(a.c.ks[block * a.c.s_b + kvh]);
+  const int64_t total = line;
+  const int64_t size = (total + a.runs - 1) / a.runs;
+  // the runs of an XCD are neighbours, which share keys and values
+  const int64_t active = (total + size - 1) / size, per = (active + 7) / 8;
+  const int64_t run = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int64_t)(blockIdx.x >> 3) >= per || run >= active) return;
+  const int64_t line_end = min(total, (run + 1) * size);
+  const int H = a.c.kv_heads * a.group;
+  const int T1 = (1 << a.c.log_t) - 1;
+
+  for (int64_t at = run * size; at < line_end;) {
+    if (wave == 0) {
+      const PaPlace p = pa_find<RB>(a, at, lane);
+      if (lane == 0) place = p;
     }
-    const float top = fmaxf(m, wave_max64(s));
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    const float al = expf(m - base);
-    const float w = expf(s - base);
-    m = top;
-    l = l * al + wave_sum(w);
-    for (int i = 0; i < D / 64; ++i) o[i] *= al;
-    for (int i = 0; i < 64; ++i) {
-      const int64_t blk = __shfl(seen ? (int)block : -1, i, 64);
-      if (blk < 0) continue;
-      const float pw = __shfl(w, i, 64) * e8m0(a.c.vs[blk * a.c.s_b + kvh]);
-      const uint8_t* v = a.c.v + blk * a.c.v_b + (int64_t)kvh * T * D + ((j0 + i) & (T - 1));
-      for (int u = 0; u < D / 64; ++u)
-        o[u] += pw * __builtin_amdgcn_cvt_f32_fp8(v[(lane + 64 * u) * T], 0);
+    __syncthreads();
+    const int b = __builtin_amdgcn_readfirstlane(place.b);
+    const int kvh = __builtin_amdgcn_readfirstlane(place.kvh);
+    const int qb = __builtin_amdgcn_readfirstlane(place.qb);
+    const int t0 = __builtin_amdgcn_readfirstlane(place.t0);
+    const int tiles = __builtin_amdgcn_readfirstlane(place.tiles);
+    if (b < 0) return;
+    const int t1 = (int)min((int64_t)tiles, t0 + (line_end - at));
+    at += t1 - t0;
+    const PaSeq seq = pa_seq<RB>(a, b);
+    const PaSpan span = pa_span<RB>(a, seq, qb);
+    const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
+    const int t_first = (int)((int64_t)qb * RB / a.group);
+    // positions of the block's first and last row (of fewer rows, if some are absent)
+    const int64_t p_low = seq.lead ? -1 : seq.p0 + t_first;
+    const int64_t p_high = seq.p0 + (int)(((int64_t)qb * RB + RB - 1) / a.group);
+
+    // queries (B operand: lane = row li, dimensions 64 j + 16 lg + 8 h of product 2 j + h)
+    // and the position of the lane's rows
+    u32x4v qf[RT][KS];
+    int pos[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int64_t r = (int64_t)qb * RB + rt * 16 + li;
+      const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+      const bool there = token < seq.n;
+      pos[rt] = there && token >= seq.lead
+                    ? (int)max((int64_t)-1, min(seq.p0 + token, (int64_t)INT32_MAX / 2)) : -1;
+      const uint16_t* q = a.q + (int64_t)(seq.first + token) * a.q_r +
+                          (int64_t)(kvh * a.group + g) * D + 16 * lg;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qf[rt][ks] = u32x4v{0, 0, 0, 0};
+        if (there) qf[rt][ks] = *reinterpret_cast<const u32x4v*>(q + 64 * (ks >> 1) + 8 * (ks & 1));
+      }
+    }
+    float4v o[RT][DT];
+    float m[RT], l[RT];
+    int er = 0;  // the values' scale (exponent byte) that sums are relative to
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = -__builtin_inff();
+      l[rt] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+    const float c = a.scale * kPaLog2e;
+
+    // the wave's 64 positions of tile i of the row block, and whether any row sees one
+    auto first_pos = [&](int i) {
+      return (i < span.sink_tiles ? i : span.first_tile + i - span.sink_tiles) * kPaTile + wave * 64;
+    };
+    auto in_sight = [&](int p) { return p < span.hi && (p + 63 >= span.lo || p < span.sink); };
+    auto next_tile = [&](int i) {  // the first from i on of which the wave sees something
+      while (i < t1 && !in_sight(first_pos(i))) ++i;
+      return i;
+    };
+    // blocks of positions p + 16 (li / 4) (the lane's keys) and p + 16 lg (its values and
+    // scales), -1 where there is none
+    struct Blocks {
+      int k, v;
+    };
+    auto blocks_of = [&](int p) {
+      Blocks r;
+      const int ik = (p + 16 * (li >> 2)) >> a.c.log_t, iv = (p + 16 * lg) >> a.c.log_t;
+      r.k = table[min(ik, a.width - 1)];
+      r.v = table[min(iv, a.width - 1)];
+      if (ik >= a.width || r.k >= a.c.blocks) r.k = -1;
+      if (iv >= a.width || r.v >= a.c.blocks) r.v = -1;
+      return r;
+    };
+    u32x4v kr[4][KL], vr[DT];
+    uint32_t ksb, vsb;
+    auto load_k = [&](int p, Blocks bl) {
+      const uint8_t* k = a.c.k + (int64_t)max(bl.k, 0) * a.c.k_b +
+                         (((int64_t)kvh << a.c.log_t) + ((p + 16 * (li >> 2)) & T1) + (li & 3)) * D + 16 * lg;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < KL; ++j)
+          kr[t][j] = *reinterpret_cast<const u32x4v*>(k + 4 * t * D + 64 * j);
+      ksb = a.c.ks[(int64_t)max(bl.v, 0) * a.c.s_b + kvh];
+    };
+    auto load_v = [&](int p, Blocks bl) {
+      const uint8_t* v = a.c.v + (int64_t)max(bl.v, 0) * a.c.v_b +
+                         ((((int64_t)kvh * D + li) << a.c.log_t) + ((p + 16 * lg) & T1));
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        vr[dt] = *reinterpret_cast<const u32x4v*>(v + ((int64_t)(16 * dt) << a.c.log_t));
+      vsb = a.c.vs[(int64_t)max(bl.v, 0) * a.c.s_b + kvh];
+    };
+
+    int i = next_tile(t0);
+    Blocks cur{-1, -1}, nxt{-1, -1};
+    if (i < t1) {
+      cur = blocks_of(first_pos(i));
+      load_k(first_pos(i), cur);
+      load_v(first_pos(i), cur);
+    }
+    while (i < t1) {
+      const int p = first_pos(i);
+      const int in = next_tile(i + 1);
+      if (in < t1) nxt = blocks_of(first_pos(in));
+      // whether all rows see all of it
+      const bool full = p + 63 <= p_low && !__any(cur.v < 0) &&
+                        (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
+      float4v s[RT][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4v kf = pa_unpack<BF>(kr[t][ks >> 1][2 * (ks & 1)], kr[t][ks >> 1][2 * (ks & 1) + 1], 1.f);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = pa_mfma<BF>(kf, qf[rt][ks], s[rt][t]);
+        }
+      }
+      // above 0: a masked -inf stays one
+      const float kc = fmaxf(e8m0(ksb) * c, 1e-37f);
+      if (in < t1) load_k(first_pos(in), nxt);
+      uint32_t seen[RT];  // bit j: row sees the lane's position j of 16
+      bool slow = false;
+      if (!full) {
+        const int x = p + 16 * lg;
+        const uint32_t there = cur.v >= 0 ? 0xFFFFu : 0u;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          uint32_t hidden = 0;
+          if (a.window) hidden = pa_below(pos[rt] - a.window + 1 - x) & ~pa_below(a.sinks - x);
+          seen[rt] = pa_below(pos[rt] + 1 - x) & ~hidden & there;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[rt][t][e] = seen[rt] & (1u << (4 * t + e)) ? s[rt][t][e] : -__builtin_inff();
+        }
+        // values that no row sees become zeros; what is NaN among the others must not
+        // reach, as 0 x NaN, the rows that do not see it
+        const uint32_t any = pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
+        uint32_t keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) keep[w] = (((any >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu;
+        uint32_t bad = 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            vr[dt][w] &= keep[w];
+            bad |= pa_nan(vr[dt][w]);
+          }
+        slow = __any(bad != 0);
+      }
+      // the values' scale, relative to the largest so far
+      const uint32_t vb = cur.v >= 0 ? vsb : 0;
+      if (__any((int)vb > er)) {
+        int top = (int)vb;
+#pragma unroll
+        for (int k = 32; k; k >>= 1) top = max(top, __shfl_xor(top, k, 64));
+        top = __builtin_amdgcn_readfirstlane(top);
+        const float f = __builtin_ldexpf(1.f, max(er - top, -200));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
+        er = top;
+      }
+      const float vscale = e8m0((uint32_t)max(127 + kPaVLift + (int)vb - er, 1));
+
+      u32x4v pf[RT][2];  // 8 neighbouring positions each
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[rt][t][e]);
+        top *= kc;
+        if (__any(top > m[rt] + kPaSlack)) {
+          const float mn = fmaxf(m[rt], pa_rows_max(top));
+          const float al = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
+          l[rt] *= al;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
+          m[rt] = mn;
+        }
+        const float base = (m[rt] == -__builtin_inff() ? 0.f : m[rt]) - kPaLift;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][e], kc, -base));
+          const uint32_t w0 = pa_pack(w[0], w[1]), w1 = pa_pack(w[2], w[3]);
+          // the sum is that of the rounded probabilities
+          const half2v ones{(_Float16)1.f, (_Float16)1.f};
+          l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w0), ones, l[rt], false);
+          l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w1), ones, l[rt], false);
+          pf[rt][t >> 1][2 * (t & 1)] = w0;
+          pf[rt][t >> 1][2 * (t & 1) + 1] = w1;
+        }
+      }
+      if (__builtin_expect(slow, 0)) {
+        // NaN codes become zeros, and a product of where they are with what each row
+        // sees says which sums are NaN
+        u32x4v sf[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              sf[rt][h][w] = (seen[rt] >> (8 * h + 2 * w) & 1u) * 0x3C00u |
+                             (seen[rt] >> (8 * h + 2 * w + 1) & 1u) * 0x3C000000u;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          float4v hit[RT];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) hit[rt] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // e4m3 1.0 is 0x38: bits 3, 4 and 5
+            const uint32_t n0 = pa_nan(vr[dt][2 * h]), n1 = pa_nan(vr[dt][2 * h + 1]);
+            const u32x4v nf = pa_unpack<false>((n0 >> 2) | (n0 >> 3) | (n0 >> 4),
+                                               (n1 >> 2) | (n1 >> 3) | (n1 >> 4), 1.f);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) hit[rt] = pa_mfma<false>(nf, sf[rt][h], hit[rt]);
+            vr[dt][2 * h] &= ~((n0 >> 7) * 0xFFu);
+            vr[dt][2 * h + 1] &= ~((n1 >> 7) * 0xFFu);
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (hit[rt][e] > 0.f) o[rt][dt][e] = __builtin_nanf("");
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4v vf = pa_unpack<false>(vr[dt][2 * h], vr[dt][2 * h + 1], vscale);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(vf, pf[rt][h], o[rt][dt]);
+        }
+      if (in < t1) load_v(first_pos(in), nxt);
+      cur = nxt;
+      i = in;
+    }
+
+    // the four waves' sums, in the order (0 + 2) + (1 + 3)
+    const float unit = __builtin_ldexpf(1.f, er - 127 - kPaVLift);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+      if (lg == 0) join_m[wave][rt * 16 + li] = m[rt];
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = rt * 16 + li;
+      const float top = fmaxf(fmaxf(join_m[0][r], join_m[1][r]), fmaxf(join_m[2][r], join_m[3][r]));
+      const float al = __builtin_amdgcn_exp2f(m[rt] - (top == -__builtin_inff() ? 0.f : top));
+      m[rt] = top;
+      l[rt] *= al;
+      l[rt] += __shfl_xor(l[rt], 16, 64);
+      l[rt] += __shfl_xor(l[rt], 32, 64);
+      if (lg == 0) join_l[wave][r] = l[rt];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        o[rt][dt] *= al * unit;
+        if (wave >= 2) join[wave - 2][(rt * DT + dt) * 64 + lane] = o[rt][dt];
+      }
+    }
+    __syncthreads();
+    if (wave < 2)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] += join[wave][(rt * DT + dt) * 64 + lane];
+    __syncthreads();
+    if (wave == 1)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) join[0][(rt * DT + dt) * 64 + lane] = o[rt][dt];
+    __syncthreads();
+    if (wave == 0)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int local = rt * 16 + li;
+        const float sum = (join_l[0][local] + join_l[1][local]) + (join_l[2][local] + join_l[3][local]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] += join[0][(rt * DT + dt) * 64 + lane];
+        if (t0 == 0 && t1 == tiles) {
+          const int64_t r = (int64_t)qb * RB + local;
+          const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+          if (token >= seq.n) continue;
+          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+          uint16_t* dst = a.out + ((int64_t)(seq.first + token) * H + kvh * a.group + g) * D + 4 * lg;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            *reinterpret_cast<uint2*>(dst + 16 * dt) =
+                make_uint2(pa_pack16<BF>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
+                           pa_pack16<BF>(o[rt][dt][2] * inv, o[rt][dt][3] * inv));
+        } else {
+          // the run's first row block, begun before it, or its last, which goes on
+          float* dst = a.parts + (run * 2 + (t0 == 0)) * pa_part_words(RB, D);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            *reinterpret_cast<float4v*>(dst + local * D + 16 * dt + 4 * lg) = o[rt][dt];
+          if (lg == 0) {
+            dst[RB * D + local] = m[rt];
+            dst[RB * D + RB + local] = sum;
+          }
+        }
+      }
+    __syncthreads();  // the buffers are free
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The row block that begins in a run and goes on behind it: out = sum of its parts,
+// each weighted exp2(m_part - m) / l, in order. A wave a row, lane = dimensions.
+// ---------------------------------------------------------------------------
+template <int D, bool BF, int RT>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
+  constexpr int RB = 16 * RT, E = D / 64, U = 8;
+  typedef float floatE __attribute__((ext_vector_type(E)));
+  __shared__ PaPlace place;
+  __shared__ int64_t line;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (wave == 0) {
+    const int64_t t = pa_total<RB>(a, lane);
+    const int64_t size = (t + a.runs - 1) / a.runs, end = ((int64_t)blockIdx.x + 1) * size;
+    PaPlace p{-1, 0, 0, 0, 0};
+    if (end < t) {
+      p = pa_find<RB>(a, end, lane);
+      // the block that holds the next run's first tile: begun in this run?
+      if (p.t0 == 0 || end - p.t0 < (int64_t)blockIdx.x * size) p.b = -1;
+    }
+    if (lane == 0) {
+      place = p;
+      line = size;
     }
   }
-  for (int u = 0; u < D / 64; ++u)
-    out[lane + 64 * u] = to16(l > 0.f || l != l ? o[u] / l : 0.f, BF);
+  __syncthreads();
+  if (place.b < 0) return;
+  const int64_t size = line, run = blockIdx.x;
+  const int64_t start = (run + 1) * size - place.t0;
+  const int parts = (int)((start + place.tiles - 1) / size - run) + 1;
+  const PaSeq seq = pa_seq<RB>(a, place.b);
+  const int64_t words = pa_part_words(RB, D);
+  const float* base = a.parts + run * 2 * words;
+  // the first part is its run's last, the others are their runs' first
+  auto part = [&](int s) { return base + s * 2 * words + (s == 0 ? words : 0); };
+  for (int local = blockIdx.y * 4 + wave; local < RB; local += 4 * gridDim.y) {
+    const int64_t r = (int64_t)place.qb * RB + local;
+    const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+    if (token >= seq.n) return;
+    float m = -__builtin_inff(), l = 0.f;
+    floatE o = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+      const int here = min(64, parts - s0);
+      const float* p = part(s0 + min(lane, here - 1)) + RB * D + local;
+      const float pm = lane < here ? p[0] : -__builtin_inff(), pl = p[RB];
+      float mn = pm;
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off, 64));
+      mn = fmaxf(mn, m);
+      const float shift = mn == -__builtin_inff() ? 0.f : mn;
+      const float w = __builtin_amdgcn_exp2f(pm - shift), al = __builtin_amdgcn_exp2f(m - shift);
+      m = mn;
+      o *= al;
+      l = l * al + wave_sum(lane < here ? w * pl : 0.f);
+      for (int s = 0; s < here; s += U) {
+        floatE t[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          t[u] = reinterpret_cast<const floatE*>(part(s0 + min(s + u, here - 1)) + local * D)[lane];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (s + u < here)
+            o += t[u] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + u));
+      }
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    uint16_t h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = to16(o[e] * inv, BF);
+    uint16_t* dst = a.out + ((int64_t)(seq.first + token) * a.c.kv_heads * a.group +
+                             place.kvh * a.group + g) * D + lane * E;
+    __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
+  }
+}
+
+struct PaPlan {
+  int rt, runs;
+  bool split;  // a row block may be divided
+};
+static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int dim, int64_t positions) {
+  PaPlan p;
+  const int group = heads / kv_heads;
+  // rows of a KV head that a sequence has in the mean
+  const int64_t mean = (rows + batch - 1) / batch * group;
+  p.rt = mean <= 16 ? 1 : mean <= 32 || dim == 256 ? 2 : 4;
+  const int64_t tiles = (positions + kPaTile - 1) / kPaTile;
+  const int64_t most = (rows * group / (16 * p.rt) + batch + 1) * kv_heads * tiles;
+  const int64_t wanted = (int64_t)num_cus() * (p.rt == 1 && dim != 256 ? 2 : 1);
+  p.runs = (int)(wanted < most ? wanted : most);
+  p.split = tiles > 1 && p.runs > 1;
+  return p;
+}
+
+static bool pa_shape_ok(int64_t rows, int64_t batch, int heads, int kv_heads, int dim) {
+  return rows >= 0 && rows <= kPagedMaxRows && batch >= 0 && batch <= kPagedMaxBatch &&
+         kv_heads >= 1 && heads >= 1 && heads <= 65535 && heads % kv_heads == 0 &&
+         (dim == 64 || dim == 128 || dim == 256);
+}
+
+template <int D, bool BF, int RT>
+static int launch_rt(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
+  paged_attn_kernel<D, BF, RT><<<(unsigned)((p.runs + 7) / 8 * 8), 256, 0, st>>>(a);
+  const int rc = launch_status();
+  if (rc != PE_OK || !p.split) return rc;
+  paged_join_kernel<D, BF, RT><<<dim3((unsigned)p.runs, 4), 256, 0, st>>>(a);
+  return launch_status();
+}
+template <int D, bool BF>
+static int launch_pa(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
+  if (p.rt == 1) return launch_rt<D, BF, 1>(p, a, st);
+  if (D == 256 || p.rt == 2) return launch_rt<D, BF, 2>(p, a, st);
+  if constexpr (D != 256) return launch_rt<D, BF, 4>(p, a, st);
+  return PE_ERR_DIMS;
 }
 
 }  // namespace pe
@@ -86,7 +701,10 @@ using namespace pe;
 
 extern "C" size_t pe_paged_attention_workspace_size(int64_t rows, int64_t batch, int heads,
                                                     int kv_heads, int head_dim, int64_t positions) {
-  return 0;
+  if (!pa_shape_ok(rows, batch, heads, kv_heads, head_dim) || rows < 1 || batch < 1 || positions < 1)
+    return 0;
+  const PaPlan p = pa_plan(rows, batch, heads, kv_heads, head_dim, positions);
+  return p.split ? (size_t)p.runs * 2 * pa_part_words(16 * p.rt, head_dim) * 4 : 0;
 }
 
 extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t rows, int heads,
@@ -104,36 +722,41 @@ extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t
   const int ok = paged_cache(a.c, k_codes, k_b, v_codes, v_b, k_scale, v_scale, s_b, blocks, kv_heads,
                              block_size, head_dim);
   if (ok != PE_OK) return ok;
-  if (rows < 0 || rows > kPagedMaxRows || batch < 0 || batch > kPagedMaxBatch || width < 1 ||
-      width > INT32_MAX / 128 || t_b < width || heads < 1 || heads > 65535 || heads % kv_heads ||
-      q_r < 0 || window < 0 || sinks < 0 || !(scale >= 0.f && scale <= 3e38f))
+  if (!pa_shape_ok(rows, batch, heads, kv_heads, head_dim) || width < 1 || width > kPagedMaxWidth ||
+      t_b < width || q_r < 0 || window < 0 || sinks < 0 || !(scale >= 0.f && scale <= 3e38f))
     return PE_ERR_DIMS;
   if (!aligned16(q) || q_r % 8 || !aligned16(out)) return PE_ERR_ALIGN;
   if (rows == 0) return PE_OK;
+  if (batch == 0) return PE_ERR_DIMS;
+  const PaPlan p = pa_plan(rows, batch, heads, kv_heads, head_dim, width * block_size);
+  const size_t need = pe_paged_attention_workspace_size(rows, batch, heads, kv_heads, head_dim,
+                                                        width * block_size);
+  if (need && (!workspace || workspace_bytes < need)) return PE_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return PE_ERR_ALIGN;
   a.q = reinterpret_cast<const uint16_t*>(q);
   a.q_r = q_r;
   a.tables = tables;
   a.t_b = t_b;
-  a.width = width;
+  a.width = (int)width;
   a.starts = starts;
   a.lengths = lengths;
   a.out = reinterpret_cast<uint16_t*>(out);
   a.rows = (int)rows;
   a.batch = (int)batch;
-  a.heads = heads;
   a.group = heads / kv_heads;
-  a.window = window;
-  a.sinks = sinks;
+  // past every position there is no difference
+  a.window = (int)(window < kPagedMaxPositions ? window : 0);
+  a.sinks = a.window ? (int)(sinks < kPagedMaxPositions ? sinks : kPagedMaxPositions) : 0;
   a.scale = scale;
-  const dim3 grid((unsigned)rows, (unsigned)heads);
+  a.runs = p.runs;
+  a.parts = reinterpret_cast<float*>(workspace);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (head_dim * 2 + bf) {
-    case 128: paged_attn_kernel<64, false><<<grid, 64, 0, st>>>(a); break;
-    case 129: paged_attn_kernel<64, true><<<grid, 64, 0, st>>>(a); break;
-    case 256: paged_attn_kernel<128, false><<<grid, 64, 0, st>>>(a); break;
-    case 257: paged_attn_kernel<128, true><<<grid, 64, 0, st>>>(a); break;
-    case 512: paged_attn_kernel<256, false><<<grid, 64, 0, st>>>(a); break;
-    default: paged_attn_kernel<256, true><<<grid, 64, 0, st>>>(a); break;
+    case 128: return launch_pa<64, false>(p, a, st);
+    case 129: return launch_pa<64, true>(p, a, st);
+    case 256: return launch_pa<128, false>(p, a, st);
+    case 257: return launch_pa<128, true>(p, a, st);
+    case 512: return launch_pa<256, false>(p, a, st);
+    default: return launch_pa<256, true>(p, a, st);
   }
-  return launch_status();
 }
