@@ -33,7 +33,6 @@
 
 namespace pe {
 
-constexpr int kPaTile = 256;       // positions of a step of a workgroup
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaSlack = 8.f;    // powers of two that an exponent may exceed its base by
 constexpr float kPaLift = 7.f;     // and by which probabilities are larger
@@ -91,7 +90,7 @@ struct PaSpan {
   int lo, hi, sink;
   int sink_tiles, first_tile, tiles;
 };
-template <int RB>
+template <int RB, int TILE>
 __device__ __forceinline__ PaSpan pa_span(const PagedAttnArgs& a, const PaSeq& s, int qb) {
   PaSpan r;
   const int cap = a.width << a.c.log_t;
@@ -101,16 +100,16 @@ __device__ __forceinline__ PaSpan pa_span(const PagedAttnArgs& a, const PaSeq& s
   r.lo = 0;
   if (a.window) r.lo = (int)max((int64_t)0, min(s.p0 + t0 - a.window + 1, (int64_t)cap));
   r.sink = min(a.sinks, r.lo);
-  r.sink_tiles = (r.sink + kPaTile - 1) / kPaTile;
-  r.first_tile = max(r.lo / kPaTile, r.sink_tiles);
-  r.tiles = max(1, r.sink_tiles + max(0, (r.hi + kPaTile - 1) / kPaTile - r.first_tile));
+  r.sink_tiles = (r.sink + TILE - 1) / TILE;
+  r.first_tile = max(r.lo / TILE, r.sink_tiles);
+  r.tiles = max(1, r.sink_tiles + max(0, (r.hi + TILE - 1) / TILE - r.first_tile));
   return r;
 }
 // tiles of all row blocks of a sequence, one KV head
-template <int RB>
+template <int RB, int TILE>
 __device__ __forceinline__ int64_t pa_tiles(const PagedAttnArgs& a, const PaSeq& s) {
   int64_t sum = 0;
-  for (int qb = 0; qb < s.blocks; ++qb) sum += pa_span<RB>(a, s, qb).tiles;
+  for (int qb = 0; qb < s.blocks; ++qb) sum += pa_span<RB, TILE>(a, s, qb).tiles;
   return sum;
 }
 __device__ __forceinline__ int64_t pa_scan(int64_t v, int lane) {
@@ -127,21 +126,21 @@ struct PaPlace {
   int tiles;
 };
 // one wave: the length of the line
-template <int RB>
+template <int RB, int TILE>
 __device__ __forceinline__ int64_t pa_total(const PagedAttnArgs& a, int lane) {
   int64_t sum = 0;
-  for (int b0 = 0; b0 <= a.batch; b0 += 64) sum += pa_tiles<RB>(a, pa_seq<RB>(a, b0 + lane));
+  for (int b0 = 0; b0 <= a.batch; b0 += 64) sum += pa_tiles<RB, TILE>(a, pa_seq<RB>(a, b0 + lane));
 #pragma unroll
   for (int m = 32; m; m >>= 1) sum += __shfl_xor((long long)sum, m, 64);
   return sum * a.c.kv_heads;
 }
 // one wave: what holds place `at` of the line (all lanes; at below the total)
-template <int RB>
+template <int RB, int TILE>
 __device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, int64_t at, int lane) {
   PaPlace r{-1, 0, 0, 0, 0};
   int64_t before = 0;
   for (int b0 = 0; b0 <= a.batch; b0 += 64) {
-    const int64_t mine = pa_tiles<RB>(a, pa_seq<RB>(a, b0 + lane));
+    const int64_t mine = pa_tiles<RB, TILE>(a, pa_seq<RB>(a, b0 + lane));
     const int64_t scan = pa_scan(mine, lane);
     const uint64_t hit = __ballot((before + scan) * a.c.kv_heads > at);
     if (!hit) {
@@ -156,7 +155,7 @@ __device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, int64_t at, i
     at -= r.kvh * tiles;
     const PaSeq s = pa_seq<RB>(a, r.b);
     for (int q0 = 0; q0 < s.blocks; q0 += 64) {
-      const int64_t t = q0 + lane < s.blocks ? pa_span<RB>(a, s, q0 + lane).tiles : 0;
+      const int64_t t = q0 + lane < s.blocks ? pa_span<RB, TILE>(a, s, q0 + lane).tiles : 0;
       const int64_t sc = pa_scan(t, lane);
       const uint64_t in = __ballot(sc > at);
       if (in) {
@@ -229,12 +228,251 @@ __device__ __forceinline__ uint32_t pa_nan(uint32_t w) {
 // the bits of positions below n, of 16
 __device__ __forceinline__ uint32_t pa_below(int n) { return (1u << min(max(n, 0), 16)) - 1; }
 
+// The runs of a launch: this workgroup's, in tiles of the line. The runs of an XCD are
+// neighbours, which share keys and values.
+struct PaRun {
+  int64_t run, at, end;  // at >= end: none
+};
+__device__ __forceinline__ PaRun pa_run(const PagedAttnArgs& a, int64_t total) {
+  const int64_t size = (total + a.runs - 1) / a.runs;
+  const int64_t active = (total + size - 1) / size, per = (active + 7) / 8;
+  const int64_t run = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int64_t)(blockIdx.x >> 3) >= per || run >= active) return PaRun{0, 0, 0};
+  return PaRun{run, run * size, min(total, (run + 1) * size)};
+}
+
+// What a wave keeps of RT products of 16 rows.
+template <int D, int RT>
+struct PaRows {
+  static constexpr int KS = D / 32, DT = D / 16;
+  u32x4v q[RT][KS];  // B operand: lane = row li, dimensions 64 j + 16 lg + 8 h of product 2 j + h
+  int pos[RT];       // of the lane's rows, below 0: sees nothing
+  float4v o[RT][DT];
+  float m[RT], l[RT];
+  int er;            // the values' scale (exponent byte) that o is relative to
+
+  // rows first .. first + 16 RT - 1 of the row block
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PaSeq& seq, int kvh, int64_t first,
+                                        int li, int lg) {
+    er = 0;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int64_t r = first + rt * 16 + li;
+      const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+      const bool there = token < seq.n;
+      pos[rt] = there && token >= seq.lead
+                    ? (int)max((int64_t)-1, min(seq.p0 + token, (int64_t)INT32_MAX / 2)) : -1;
+      const uint16_t* src = a.q + (int64_t)(seq.first + token) * a.q_r +
+                            (int64_t)(kvh * a.group + g) * D + 16 * lg;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        q[rt][ks] = u32x4v{0, 0, 0, 0};
+        if (there) q[rt][ks] = *reinterpret_cast<const u32x4v*>(src + 64 * (ks >> 1) + 8 * (ks & 1));
+      }
+      m[rt] = -__builtin_inff();
+      l[rt] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // scores of positions that a row does not see; bit j of seen: the lane's position
+  // x + j of 16
+  __device__ __forceinline__ void mask(const PagedAttnArgs& a, float4v (&s)[RT][4], uint32_t (&seen)[RT],
+                                       int x, uint32_t there) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      uint32_t hidden = 0;
+      if (a.window) hidden = pa_below(pos[rt] - a.window + 1 - x) & ~pa_below(a.sinks - x);
+      seen[rt] = pa_below(pos[rt] + 1 - x) & ~hidden & there;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[rt][t][e] = seen[rt] & (1u << (4 * t + e)) ? s[rt][t][e] : -__builtin_inff();
+    }
+  }
+  // vb: exponent byte of the values of the lane's 16 positions (0: none there); the
+  // factor that the conversion gives them
+  __device__ __forceinline__ float value_scale(int vb) {
+    if (__any(vb > er)) {
+      int top = vb;
+#pragma unroll
+      for (int k = 32; k; k >>= 1) top = max(top, __shfl_xor(top, k, 64));
+      top = __builtin_amdgcn_readfirstlane(top);
+      const float f = __builtin_ldexpf(1.f, max(er - top, -200));
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
+      er = top;
+    }
+    return e8m0((uint32_t)max(127 + kPaVLift + vb - er, 1));
+  }
+  // p: B operands of two products, 8 neighbouring positions each. kc: what the scores
+  // of the lane are multiplied by
+  __device__ __forceinline__ void softmax(const float4v (&s)[RT][4], float kc, u32x4v (&p)[RT][2]) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[rt][t][e]);
+      top *= kc;
+      if (__any(top > m[rt] + kPaSlack)) {
+        const float mn = fmaxf(m[rt], pa_rows_max(top));
+        const float al = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
+        l[rt] *= al;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
+        m[rt] = mn;
+      }
+      const float base = (m[rt] == -__builtin_inff() ? 0.f : m[rt]) - kPaLift;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][e], kc, -base));
+        const uint32_t w0 = pa_pack(w[0], w[1]), w1 = pa_pack(w[2], w[3]);
+        // the sum is that of the rounded probabilities
+        const half2v ones{(_Float16)1.f, (_Float16)1.f};
+        l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w0), ones, l[rt], false);
+        l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w1), ones, l[rt], false);
+        p[rt][t >> 1][2 * (t & 1)] = w0;
+        p[rt][t >> 1][2 * (t & 1) + 1] = w1;
+      }
+    }
+  }
+  // NaN among the values of 16 dimensions, where some row does not see it: sums of rows
+  // that do become NaN (a product of where it is with what each row sees says which),
+  // the codes become zeros
+  __device__ __forceinline__ void nan_values(u32x4v& v, int dt, const uint32_t (&seen)[RT]) {
+    float4v hit[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) hit[rt] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // e4m3 1.0 is 0x38: bits 3, 4 and 5
+      const uint32_t n0 = pa_nan(v[2 * h]), n1 = pa_nan(v[2 * h + 1]);
+      const u32x4v nf = pa_unpack<false>((n0 >> 2) | (n0 >> 3) | (n0 >> 4),
+                                         (n1 >> 2) | (n1 >> 3) | (n1 >> 4), 1.f);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        u32x4v sf;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          sf[w] = (seen[rt] >> (8 * h + 2 * w) & 1u) * 0x3C00u |
+                  (seen[rt] >> (8 * h + 2 * w + 1) & 1u) * 0x3C000000u;
+        hit[rt] = pa_mfma<false>(nf, sf, hit[rt]);
+      }
+      v[2 * h] &= ~((n0 >> 7) * 0xFFu);
+      v[2 * h + 1] &= ~((n1 >> 7) * 0xFFu);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (hit[rt][e] > 0.f) o[rt][dt][e] = __builtin_nanf("");
+  }
+  __device__ __forceinline__ void values(u32x4v v, int dt, float scale, const u32x4v (&p)[RT][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4v vf = pa_unpack<false>(v[2 * h], v[2 * h + 1], scale);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(vf, p[rt][h], o[rt][dt]);
+    }
+  }
+  // the row's whole sum in all of its lanes, sums in units of 1
+  __device__ __forceinline__ void finish() {
+    const float unit = __builtin_ldexpf(1.f, er - 127 - kPaVLift);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] += __shfl_xor(l[rt], 16, 64);
+      l[rt] += __shfl_xor(l[rt], 32, 64);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= unit;
+    }
+  }
+  // result or part (of RB rows) of rows first .. of the row block
+  template <bool BF, int RB>
+  __device__ __forceinline__ void store(const PagedAttnArgs& a, const PaSeq& seq, int kvh, int qb,
+                                        int first, float* part, int li, int lg) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int local = first + rt * 16 + li;
+      if (!part) {
+        const int64_t r = (int64_t)qb * RB + local;
+        const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+        if (token >= seq.n) continue;
+        const float inv = l[rt] > 0.f || l[rt] != l[rt] ? 1.f / l[rt] : 0.f;
+        uint16_t* dst = a.out + ((int64_t)(seq.first + token) * (a.c.kv_heads * a.group) + kvh * a.group + g) * D +
+                        4 * lg;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          *reinterpret_cast<uint2*>(dst + 16 * dt) =
+              make_uint2(pa_pack16<BF>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
+                         pa_pack16<BF>(o[rt][dt][2] * inv, o[rt][dt][3] * inv));
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          *reinterpret_cast<float4v*>(part + local * D + 16 * dt + 4 * lg) = o[rt][dt];
+        if (lg == 0) {
+          part[RB * D + local] = m[rt];
+          part[RB * D + RB + local] = l[rt];
+        }
+      }
+    }
+  }
+};
+
+// blocks of positions p + 16 (li / 4) (the lane's keys) and p + 16 lg (its values and
+// scales), -1 where there is none
+struct PaBlocks {
+  int k, v;
+};
+__device__ __forceinline__ PaBlocks pa_blocks(const PagedAttnArgs& a, const int32_t* table, int p, int li,
+                                              int lg) {
+  PaBlocks r;
+  const int ik = (p + 16 * (li >> 2)) >> a.c.log_t, iv = (p + 16 * lg) >> a.c.log_t;
+  r.k = table[min(ik, a.width - 1)];
+  r.v = table[min(iv, a.width - 1)];
+  if (ik >= a.width || r.k >= a.c.blocks) r.k = -1;
+  if (iv >= a.width || r.v >= a.c.blocks) r.v = -1;
+  return r;
+}
+// the lane's part of the keys (rows 4 t and 16-byte chunks 4 j behind it) and values
+// (16 dimensions behind it) of 64 positions from p on
+template <int D>
+__device__ __forceinline__ const uint8_t* pa_keys(const PagedAttnArgs& a, int kvh, int p, int block, int li,
+                                                  int lg) {
+  return a.c.k + (int64_t)max(block, 0) * a.c.k_b +
+         (((int64_t)kvh << a.c.log_t) + ((p + 16 * (li >> 2)) & ((1 << a.c.log_t) - 1)) + (li & 3)) * D + 16 * lg;
+}
+template <int D>
+__device__ __forceinline__ const uint8_t* pa_values(const PagedAttnArgs& a, int kvh, int p, int block, int li,
+                                                    int lg) {
+  return a.c.v + (int64_t)max(block, 0) * a.c.v_b +
+         ((((int64_t)kvh * D + li) << a.c.log_t) + ((p + 16 * lg) & ((1 << a.c.log_t) - 1)));
+}
+// bytes of the lane's 16 positions from x on that some row of the block sees
+__device__ __forceinline__ u32x4v pa_keep(const PaSpan& span, int x, uint32_t there) {
+  const uint32_t any = pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
+  u32x4v keep;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) keep[w] = (((any >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu;
+  return keep;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the four waves of a workgroup take 64 positions each of a tile of 256,
+// straight from memory to registers, and join their sums in LDS at the end of a row
+// block.
+// ---------------------------------------------------------------------------
 template <int D, bool BF, int RT>
 __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
-  constexpr int RB = 16 * RT;      // rows of a row block
-  constexpr int KS = D / 32;       // products of 32 dimensions
-  constexpr int KL = D / 64;       // 16-byte loads of a key row's part
-  constexpr int DT = D / 16;       // products of 16 dimensions of values
+  constexpr int RB = 16 * RT, TILE = 256;
+  constexpr int KS = D / 32, KL = D / 64, DT = D / 16;
   __shared__ __align__(16) float4v join[2][RT * DT * 64];
   __shared__ float join_m[4][RB], join_l[4][RB];
   __shared__ PaPlace place;
@@ -242,23 +480,15 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   if (wave == 0) {
-    const int64_t total = pa_total<RB>(a, lane);
+    const int64_t total = pa_total<RB, TILE>(a, lane);
     if (lane == 0) line = total;
   }
   __syncthreads();
-  const int64_t total = line;
-  const int64_t size = (total + a.runs - 1) / a.runs;
-  // the runs of an XCD are neighbours, which share keys and values
-  const int64_t active = (total + size - 1) / size, per = (active + 7) / 8;
-  const int64_t run = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || run >= active) return;
-  const int64_t line_end = min(total, (run + 1) * size);
-  const int H = a.c.kv_heads * a.group;
-  const int T1 = (1 << a.c.log_t) - 1;
+  const PaRun run = pa_run(a, line);
 
-  for (int64_t at = run * size; at < line_end;) {
+  for (int64_t at = run.at; at < run.end;) {
     if (wave == 0) {
-      const PaPlace p = pa_find<RB>(a, at, lane);
+      const PaPlace p = pa_find<RB, TILE>(a, at, lane);
       if (lane == 0) place = p;
     }
     __syncthreads();
@@ -268,75 +498,33 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     const int t0 = __builtin_amdgcn_readfirstlane(place.t0);
     const int tiles = __builtin_amdgcn_readfirstlane(place.tiles);
     if (b < 0) return;
-    const int t1 = (int)min((int64_t)tiles, t0 + (line_end - at));
+    const int t1 = (int)min((int64_t)tiles, t0 + (run.end - at));
     at += t1 - t0;
     const PaSeq seq = pa_seq<RB>(a, b);
-    const PaSpan span = pa_span<RB>(a, seq, qb);
+    const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
-    const int t_first = (int)((int64_t)qb * RB / a.group);
     // positions of the block's first and last row (of fewer rows, if some are absent)
-    const int64_t p_low = seq.lead ? -1 : seq.p0 + t_first;
+    const int64_t p_low = seq.lead ? -1 : seq.p0 + (int)((int64_t)qb * RB / a.group);
     const int64_t p_high = seq.p0 + (int)(((int64_t)qb * RB + RB - 1) / a.group);
-
-    // queries (B operand: lane = row li, dimensions 64 j + 16 lg + 8 h of product 2 j + h)
-    // and the position of the lane's rows
-    u32x4v qf[RT][KS];
-    int pos[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int64_t r = (int64_t)qb * RB + rt * 16 + li;
-      const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
-      const bool there = token < seq.n;
-      pos[rt] = there && token >= seq.lead
-                    ? (int)max((int64_t)-1, min(seq.p0 + token, (int64_t)INT32_MAX / 2)) : -1;
-      const uint16_t* q = a.q + (int64_t)(seq.first + token) * a.q_r +
-                          (int64_t)(kvh * a.group + g) * D + 16 * lg;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        qf[rt][ks] = u32x4v{0, 0, 0, 0};
-        if (there) qf[rt][ks] = *reinterpret_cast<const u32x4v*>(q + 64 * (ks >> 1) + 8 * (ks & 1));
-      }
-    }
-    float4v o[RT][DT];
-    float m[RT], l[RT];
-    int er = 0;  // the values' scale (exponent byte) that sums are relative to
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = -__builtin_inff();
-      l[rt] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
-    }
+    PaRows<D, RT> w;
+    w.begin(a, seq, kvh, (int64_t)qb * RB, li, lg);
     const float c = a.scale * kPaLog2e;
 
     // the wave's 64 positions of tile i of the row block, and whether any row sees one
     auto first_pos = [&](int i) {
-      return (i < span.sink_tiles ? i : span.first_tile + i - span.sink_tiles) * kPaTile + wave * 64;
+      return (i < span.sink_tiles ? i : span.first_tile + i - span.sink_tiles) * TILE + wave * 64;
     };
-    auto in_sight = [&](int p) { return p < span.hi && (p + 63 >= span.lo || p < span.sink); };
     auto next_tile = [&](int i) {  // the first from i on of which the wave sees something
-      while (i < t1 && !in_sight(first_pos(i))) ++i;
+      for (; i < t1; ++i) {
+        const int p = first_pos(i);
+        if (p < span.hi && (p + 63 >= span.lo || p < span.sink)) break;
+      }
       return i;
-    };
-    // blocks of positions p + 16 (li / 4) (the lane's keys) and p + 16 lg (its values and
-    // scales), -1 where there is none
-    struct Blocks {
-      int k, v;
-    };
-    auto blocks_of = [&](int p) {
-      Blocks r;
-      const int ik = (p + 16 * (li >> 2)) >> a.c.log_t, iv = (p + 16 * lg) >> a.c.log_t;
-      r.k = table[min(ik, a.width - 1)];
-      r.v = table[min(iv, a.width - 1)];
-      if (ik >= a.width || r.k >= a.c.blocks) r.k = -1;
-      if (iv >= a.width || r.v >= a.c.blocks) r.v = -1;
-      return r;
     };
     u32x4v kr[4][KL], vr[DT];
     uint32_t ksb, vsb;
-    auto load_k = [&](int p, Blocks bl) {
-      const uint8_t* k = a.c.k + (int64_t)max(bl.k, 0) * a.c.k_b +
-                         (((int64_t)kvh << a.c.log_t) + ((p + 16 * (li >> 2)) & T1) + (li & 3)) * D + 16 * lg;
+    auto load_k = [&](int p, PaBlocks bl) {
+      const uint8_t* k = pa_keys<D>(a, kvh, p, bl.k, li, lg);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -344,9 +532,8 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
           kr[t][j] = *reinterpret_cast<const u32x4v*>(k + 4 * t * D + 64 * j);
       ksb = a.c.ks[(int64_t)max(bl.v, 0) * a.c.s_b + kvh];
     };
-    auto load_v = [&](int p, Blocks bl) {
-      const uint8_t* v = a.c.v + (int64_t)max(bl.v, 0) * a.c.v_b +
-                         ((((int64_t)kvh * D + li) << a.c.log_t) + ((p + 16 * lg) & T1));
+    auto load_v = [&](int p, PaBlocks bl) {
+      const uint8_t* v = pa_values<D>(a, kvh, p, bl.v, li, lg);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         vr[dt] = *reinterpret_cast<const u32x4v*>(v + ((int64_t)(16 * dt) << a.c.log_t));
@@ -354,16 +541,16 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     };
 
     int i = next_tile(t0);
-    Blocks cur{-1, -1}, nxt{-1, -1};
+    PaBlocks cur{-1, -1}, nxt{-1, -1};
     if (i < t1) {
-      cur = blocks_of(first_pos(i));
+      cur = pa_blocks(a, table, first_pos(i), li, lg);
       load_k(first_pos(i), cur);
       load_v(first_pos(i), cur);
     }
     while (i < t1) {
       const int p = first_pos(i);
       const int in = next_tile(i + 1);
-      if (in < t1) nxt = blocks_of(first_pos(in));
+      if (in < t1) nxt = pa_blocks(a, table, first_pos(in), li, lg);
       // whether all rows see all of it
       const bool full = p + 63 <= p_low && !__any(cur.v < 0) &&
                         (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
@@ -376,161 +563,60 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
         for (int ks = 0; ks < KS; ++ks) {
           const u32x4v kf = pa_unpack<BF>(kr[t][ks >> 1][2 * (ks & 1)], kr[t][ks >> 1][2 * (ks & 1) + 1], 1.f);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][t] = pa_mfma<BF>(kf, qf[rt][ks], s[rt][t]);
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = pa_mfma<BF>(kf, w.q[rt][ks], s[rt][t]);
         }
       }
       // above 0: a masked -inf stays one
       const float kc = fmaxf(e8m0(ksb) * c, 1e-37f);
       if (in < t1) load_k(first_pos(in), nxt);
-      uint32_t seen[RT];  // bit j: row sees the lane's position j of 16
+      uint32_t seen[RT];
       bool slow = false;
       if (!full) {
-        const int x = p + 16 * lg;
         const uint32_t there = cur.v >= 0 ? 0xFFFFu : 0u;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          uint32_t hidden = 0;
-          if (a.window) hidden = pa_below(pos[rt] - a.window + 1 - x) & ~pa_below(a.sinks - x);
-          seen[rt] = pa_below(pos[rt] + 1 - x) & ~hidden & there;
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[rt][t][e] = seen[rt] & (1u << (4 * t + e)) ? s[rt][t][e] : -__builtin_inff();
-        }
-        // values that no row sees become zeros; what is NaN among the others must not
-        // reach, as 0 x NaN, the rows that do not see it
-        const uint32_t any = pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
-        uint32_t keep[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) keep[w] = (((any >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu;
+        w.mask(a, s, seen, p + 16 * lg, there);
+        // NaN codes of positions that a row does not see must not reach it as 0 x NaN
         uint32_t bad = 0;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            vr[dt][w] &= keep[w];
-            bad |= pa_nan(vr[dt][w]);
-          }
+          bad |= pa_nan(vr[dt][0]) | pa_nan(vr[dt][1]) | pa_nan(vr[dt][2]) | pa_nan(vr[dt][3]);
         slow = __any(bad != 0);
       }
-      // the values' scale, relative to the largest so far
-      const uint32_t vb = cur.v >= 0 ? vsb : 0;
-      if (__any((int)vb > er)) {
-        int top = (int)vb;
-#pragma unroll
-        for (int k = 32; k; k >>= 1) top = max(top, __shfl_xor(top, k, 64));
-        top = __builtin_amdgcn_readfirstlane(top);
-        const float f = __builtin_ldexpf(1.f, max(er - top, -200));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-        er = top;
-      }
-      const float vscale = e8m0((uint32_t)max(127 + kPaVLift + (int)vb - er, 1));
-
-      u32x4v pf[RT][2];  // 8 neighbouring positions each
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float top = -__builtin_inff();
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[rt][t][e]);
-        top *= kc;
-        if (__any(top > m[rt] + kPaSlack)) {
-          const float mn = fmaxf(m[rt], pa_rows_max(top));
-          const float al = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
-          l[rt] *= al;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
-          m[rt] = mn;
-        }
-        const float base = (m[rt] == -__builtin_inff() ? 0.f : m[rt]) - kPaLift;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][e], kc, -base));
-          const uint32_t w0 = pa_pack(w[0], w[1]), w1 = pa_pack(w[2], w[3]);
-          // the sum is that of the rounded probabilities
-          const half2v ones{(_Float16)1.f, (_Float16)1.f};
-          l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w0), ones, l[rt], false);
-          l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w1), ones, l[rt], false);
-          pf[rt][t >> 1][2 * (t & 1)] = w0;
-          pf[rt][t >> 1][2 * (t & 1) + 1] = w1;
-        }
-      }
+      const float vscale = w.value_scale(cur.v >= 0 ? (int)vsb : 0);
+      u32x4v pf[RT][2];
+      w.softmax(s, kc, pf);
       if (__builtin_expect(slow, 0)) {
-        // NaN codes become zeros, and a product of where they are with what each row
-        // sees says which sums are NaN
-        u32x4v sf[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-              sf[rt][h][w] = (seen[rt] >> (8 * h + 2 * w) & 1u) * 0x3C00u |
-                             (seen[rt] >> (8 * h + 2 * w + 1) & 1u) * 0x3C000000u;
+        const u32x4v keep = pa_keep(span, p + 16 * lg, cur.v >= 0 ? 0xFFFFu : 0u);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          float4v hit[RT];
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) hit[rt] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // e4m3 1.0 is 0x38: bits 3, 4 and 5
-            const uint32_t n0 = pa_nan(vr[dt][2 * h]), n1 = pa_nan(vr[dt][2 * h + 1]);
-            const u32x4v nf = pa_unpack<false>((n0 >> 2) | (n0 >> 3) | (n0 >> 4),
-                                               (n1 >> 2) | (n1 >> 3) | (n1 >> 4), 1.f);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) hit[rt] = pa_mfma<false>(nf, sf[rt][h], hit[rt]);
-            vr[dt][2 * h] &= ~((n0 >> 7) * 0xFFu);
-            vr[dt][2 * h + 1] &= ~((n1 >> 7) * 0xFFu);
-          }
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (hit[rt][e] > 0.f) o[rt][dt][e] = __builtin_nanf("");
+          vr[dt] &= keep;
+          w.nan_values(vr[dt], dt, seen);
         }
       }
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const u32x4v vf = pa_unpack<false>(vr[dt][2 * h], vr[dt][2 * h + 1], vscale);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(vf, pf[rt][h], o[rt][dt]);
-        }
+      for (int dt = 0; dt < DT; ++dt) w.values(vr[dt], dt, vscale, pf);
       if (in < t1) load_v(first_pos(in), nxt);
       cur = nxt;
       i = in;
     }
 
     // the four waves' sums, in the order (0 + 2) + (1 + 3)
-    const float unit = __builtin_ldexpf(1.f, er - 127 - kPaVLift);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
-      if (lg == 0) join_m[wave][rt * 16 + li] = m[rt];
+      if (lg == 0) join_m[wave][rt * 16 + li] = w.m[rt];
+    w.finish();
     __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = rt * 16 + li;
       const float top = fmaxf(fmaxf(join_m[0][r], join_m[1][r]), fmaxf(join_m[2][r], join_m[3][r]));
-      const float al = __builtin_amdgcn_exp2f(m[rt] - (top == -__builtin_inff() ? 0.f : top));
-      m[rt] = top;
-      l[rt] *= al;
-      l[rt] += __shfl_xor(l[rt], 16, 64);
-      l[rt] += __shfl_xor(l[rt], 32, 64);
-      if (lg == 0) join_l[wave][r] = l[rt];
+      const float al = __builtin_amdgcn_exp2f(w.m[rt] - (top == -__builtin_inff() ? 0.f : top));
+      w.m[rt] = top;
+      w.l[rt] *= al;
+      if (lg == 0) join_l[wave][r] = w.l[rt];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        o[rt][dt] *= al * unit;
-        if (wave >= 2) join[wave - 2][(rt * DT + dt) * 64 + lane] = o[rt][dt];
+        w.o[rt][dt] *= al;
+        if (wave >= 2) join[wave - 2][(rt * DT + dt) * 64 + lane] = w.o[rt][dt];
       }
     }
     __syncthreads();
@@ -538,44 +624,208 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] += join[wave][(rt * DT + dt) * 64 + lane];
+        for (int dt = 0; dt < DT; ++dt) w.o[rt][dt] += join[wave][(rt * DT + dt) * 64 + lane];
     __syncthreads();
     if (wave == 1)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) join[0][(rt * DT + dt) * 64 + lane] = o[rt][dt];
+        for (int dt = 0; dt < DT; ++dt) join[0][(rt * DT + dt) * 64 + lane] = w.o[rt][dt];
     __syncthreads();
-    if (wave == 0)
+    if (wave == 0) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int local = rt * 16 + li;
-        const float sum = (join_l[0][local] + join_l[1][local]) + (join_l[2][local] + join_l[3][local]);
+        const int r = rt * 16 + li;
+        w.l[rt] = (join_l[0][r] + join_l[1][r]) + (join_l[2][r] + join_l[3][r]);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] += join[0][(rt * DT + dt) * 64 + lane];
-        if (t0 == 0 && t1 == tiles) {
-          const int64_t r = (int64_t)qb * RB + local;
-          const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
-          if (token >= seq.n) continue;
-          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-          uint16_t* dst = a.out + ((int64_t)(seq.first + token) * H + kvh * a.group + g) * D + 4 * lg;
+        for (int dt = 0; dt < DT; ++dt) w.o[rt][dt] += join[0][(rt * DT + dt) * 64 + lane];
+      }
+      // a part: the run's first row block, begun before it, or its last, which goes on
+      float* part = t0 == 0 && t1 == tiles ? nullptr
+                                           : a.parts + (run.run * 2 + (t0 == 0)) * pa_part_words(RB, D);
+      w.template store<BF, RB>(a, seq, kvh, qb, 0, part, li, lg);
+    }
+    __syncthreads();  // the buffers are free
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (chunks of prompts): the four waves of a workgroup take 16 RT rows each and
+// share 64 positions a step, which go straight to LDS in the order in which lanes read
+// them (64 lanes x 16 bytes an operand, the addresses that the other form loads from),
+// two buffers, the next tile under way while one is worked on, one barrier a tile.
+// ---------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) unsigned char pa_lds;
+typedef __attribute__((address_space(1))) const unsigned char pa_glb;
+
+template <int D, bool BF, int RT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(const PagedAttnArgs a) {
+  constexpr int RB = 64 * RT, TILE = 64;
+  constexpr int KL = D / 64, DT = D / 16;
+  constexpr int KF = 4 * KL;             // operands of keys, 1 KB each, then DT of values
+  constexpr int PER = (KF + DT) / 4;     // operands that a wave brings
+  __shared__ __align__(16) unsigned char buf0[(KF + DT) * 1024];
+  __shared__ __align__(16) unsigned char buf1[(KF + DT) * 1024];
+  __shared__ PaPlace place;
+  __shared__ int64_t line;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  if (wave == 0) {
+    const int64_t total = pa_total<RB, TILE>(a, lane);
+    if (lane == 0) line = total;
+  }
+  __syncthreads();
+  const PaRun run = pa_run(a, line);
+
+  for (int64_t at = run.at; at < run.end;) {
+    if (wave == 0) {
+      const PaPlace p = pa_find<RB, TILE>(a, at, lane);
+      if (lane == 0) place = p;
+    }
+    __syncthreads();
+    const int b = __builtin_amdgcn_readfirstlane(place.b);
+    const int kvh = __builtin_amdgcn_readfirstlane(place.kvh);
+    const int qb = __builtin_amdgcn_readfirstlane(place.qb);
+    const int t0 = __builtin_amdgcn_readfirstlane(place.t0);
+    const int tiles = __builtin_amdgcn_readfirstlane(place.tiles);
+    if (b < 0) return;
+    const int t1 = (int)min((int64_t)tiles, t0 + (run.end - at));
+    at += t1 - t0;
+    const PaSeq seq = pa_seq<RB>(a, b);
+    const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
+    const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
+    // the wave's rows, and positions of the first and the last of them
+    const int64_t first = (int64_t)qb * RB + wave * 16 * RT;
+    const int token0 = (int)(first / a.group), token1 = (int)((first + 16 * RT - 1) / a.group);
+    const int64_t p_low = seq.lead ? -1 : seq.p0 + token0;
+    const int64_t p_high = seq.p0 + min(token1, seq.n - 1);
+    const bool idle = token0 >= seq.n;
+    PaRows<D, RT> w;
+    w.begin(a, seq, kvh, first, li, lg);
+    const float c = a.scale * kPaLog2e;
+
+    auto first_pos = [&](int i) {
+      return (i < span.sink_tiles ? i : span.first_tile + i - span.sink_tiles) * TILE;
+    };
+    auto in_sight = [&](int i) {  // of the row block
+      const int p = first_pos(i);
+      return p < span.hi && (p + 63 >= span.lo || p < span.sink);
+    };
+    struct Scales {
+      uint32_t k, v;
+      int block;
+    };
+    PaBlocks nb;
+    auto issue = [&](unsigned char* to, int p, PaBlocks bl) {
+      const uint8_t* k = pa_keys<D>(a, kvh, p, bl.k, li, lg);
+      const uint8_t* v = pa_values<D>(a, kvh, p, bl.v, li, lg);
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-            *reinterpret_cast<uint2*>(dst + 16 * dt) =
-                make_uint2(pa_pack16<BF>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
-                           pa_pack16<BF>(o[rt][dt][2] * inv, o[rt][dt][3] * inv));
+      for (int n = 0; n < PER; ++n) {
+        const int f = wave * PER + n;  // waves 0 and 1 bring keys, 2 and 3 values
+        const uint8_t* src = f < KF ? k + 4 * (f / KL) * D + 64 * (f % KL)
+                                    : v + ((int64_t)(16 * (f - KF)) << a.c.log_t);
+        __builtin_amdgcn_global_load_lds((const pa_glb*)src, (pa_lds*)to + f * 1024, 16, 0, 0);
+      }
+      const int64_t sc = (int64_t)max(bl.v, 0) * a.c.s_b + kvh;
+      return Scales{a.c.ks[sc], a.c.vs[sc], bl.v};
+    };
+    Scales cur{0, 0, -1}, nxt{0, 0, -1};
+    int i = t0;
+    while (i < t1 && !in_sight(i)) ++i;
+    if (i < t1) cur = issue(buf0, first_pos(i), pa_blocks(a, table, first_pos(i), li, lg));
+    int in = i + 1;
+    while (in < t1 && !in_sight(in)) ++in;
+    if (in < t1) nb = pa_blocks(a, table, first_pos(in), li, lg);
+    auto step = [&](const unsigned char* from, unsigned char* to) {
+      const int p = first_pos(i);
+      __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the tile is in LDS
+      __syncthreads();                // everybody's is, and `to` is done with
+      int after = in + 1;
+      if (in < t1) {
+        nxt = issue(to, first_pos(in), nb);
+        while (after < t1 && !in_sight(after)) ++after;
+        if (after < t1) nb = pa_blocks(a, table, first_pos(after), li, lg);
+      }
+      // a wave whose rows see nothing of the tile leaves it
+      const bool none = idle || p > p_high ||
+                        (a.window && p + 63 <= max(p_low, (int64_t)-1) - a.window && p >= a.sinks);
+      if (!none) {
+        const bool full = p + 63 <= p_low && !__any(cur.block < 0) &&
+                          (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
+        const u32x4v* kf = reinterpret_cast<const u32x4v*>(from) + lane;
+        const u32x4v* vf = kf + KF * 64;
+        // operands one ahead of their products; the fences keep the compiler from
+        // bringing them all at once, for which there are no registers
+        float4v s[RT][4];
+        u32x4v raw[2][KL];
+#pragma unroll
+        for (int j = 0; j < KL; ++j) raw[0][j] = kf[j * 64];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (t < 3)
+#pragma unroll
+            for (int j = 0; j < KL; ++j) raw[(t + 1) & 1][j] = kf[((t + 1) * KL + j) * 64];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < KL; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const u32x4v kk = pa_unpack<BF>(raw[t & 1][j][2 * h], raw[t & 1][j][2 * h + 1], 1.f);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) s[rt][t] = pa_mfma<BF>(kk, w.q[rt][2 * j + h], s[rt][t]);
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const float kc = fmaxf(e8m0(cur.k) * c, 1e-37f);
+        const float vscale = w.value_scale(cur.block >= 0 ? (int)cur.v : 0);
+        const uint32_t there = cur.block >= 0 ? 0xFFFFu : 0u;
+        uint32_t seen[RT];
+        bool slow = false;
+        if (!full) {
+          w.mask(a, s, seen, p + 16 * lg, there);
+          uint32_t bad = 0;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const u32x4v v = vf[dt * 64];
+            bad |= pa_nan(v[0]) | pa_nan(v[1]) | pa_nan(v[2]) | pa_nan(v[3]);
+          }
+          slow = __any(bad != 0);
+        }
+        u32x4v pf[RT][2];
+        w.softmax(s, kc, pf);
+        if (__builtin_expect(slow, 0)) {
+          const u32x4v keep = pa_keep(span, p + 16 * lg, there);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            u32x4v v = vf[dt * 64] & keep;
+            w.nan_values(v, dt, seen);
+            w.values(v, dt, vscale, pf);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         } else {
-          // the run's first row block, begun before it, or its last, which goes on
-          float* dst = a.parts + (run * 2 + (t0 == 0)) * pa_part_words(RB, D);
+          u32x4v v = vf[0];
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-            *reinterpret_cast<float4v*>(dst + local * D + 16 * dt + 4 * lg) = o[rt][dt];
-          if (lg == 0) {
-            dst[RB * D + local] = m[rt];
-            dst[RB * D + RB + local] = sum;
+          for (int dt = 0; dt < DT; ++dt) {
+            const u32x4v next = vf[min(dt + 1, DT - 1) * 64];
+            w.values(v, dt, vscale, pf);
+            v = next;
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
+      cur = nxt;
+      i = in;
+      in = after;
+    };
+    while (i < t1) {
+      step(buf0, buf1);
+      if (i < t1) step(buf1, buf0);
+    }
+    w.finish();
+    float* part = t0 == 0 && t1 == tiles ? nullptr
+                                         : a.parts + (run.run * 2 + (t0 == 0)) * pa_part_words(RB, D);
+    w.template store<BF, RB>(a, seq, kvh, qb, wave * 16 * RT, part, li, lg);
     __syncthreads();  // the buffers are free
   }
 }
@@ -584,19 +834,19 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 // The row block that begins in a run and goes on behind it: out = sum of its parts,
 // each weighted exp2(m_part - m) / l, in order. A wave a row, lane = dimensions.
 // ---------------------------------------------------------------------------
-template <int D, bool BF, int RT>
+template <int D, bool BF, int RB, int TILE>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
-  constexpr int RB = 16 * RT, E = D / 64, U = 8;
+  constexpr int E = D / 64, U = 8;
   typedef float floatE __attribute__((ext_vector_type(E)));
   __shared__ PaPlace place;
   __shared__ int64_t line;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (wave == 0) {
-    const int64_t t = pa_total<RB>(a, lane);
+    const int64_t t = pa_total<RB, TILE>(a, lane);
     const int64_t size = (t + a.runs - 1) / a.runs, end = ((int64_t)blockIdx.x + 1) * size;
     PaPlace p{-1, 0, 0, 0, 0};
     if (end < t) {
-      p = pa_find<RB>(a, end, lane);
+      p = pa_find<RB, TILE>(a, end, lane);
       // the block that holds the next run's first tile: begun in this run?
       if (p.t0 == 0 || end - p.t0 < (int64_t)blockIdx.x * size) p.b = -1;
     }
@@ -656,7 +906,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 }
 
 struct PaPlan {
-  int rt, runs;
+  int rb;      // rows of a row block: 16 and 32 in the form for few rows, else 128
+  int runs;
   bool split;  // a row block may be divided
 };
 static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int dim, int64_t positions) {
@@ -664,10 +915,11 @@ static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int 
   const int group = heads / kv_heads;
   // rows of a KV head that a sequence has in the mean
   const int64_t mean = (rows + batch - 1) / batch * group;
-  p.rt = mean <= 16 ? 1 : mean <= 32 || dim == 256 ? 2 : 4;
-  const int64_t tiles = (positions + kPaTile - 1) / kPaTile;
-  const int64_t most = (rows * group / (16 * p.rt) + batch + 1) * kv_heads * tiles;
-  const int64_t wanted = (int64_t)num_cus() * (p.rt == 1 && dim != 256 ? 2 : 1);
+  p.rb = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+  const int tile = p.rb == 128 ? 64 : 256;
+  const int64_t tiles = (positions + tile - 1) / tile;
+  const int64_t most = (rows * group / p.rb + batch + 1) * kv_heads * tiles;
+  const int64_t wanted = (int64_t)num_cus() * ((p.rb == 16 || p.rb == 128) && dim != 256 ? 2 : 1);
   p.runs = (int)(wanted < most ? wanted : most);
   p.split = tiles > 1 && p.runs > 1;
   return p;
@@ -679,20 +931,23 @@ static bool pa_shape_ok(int64_t rows, int64_t batch, int heads, int kv_heads, in
          (dim == 64 || dim == 128 || dim == 256);
 }
 
-template <int D, bool BF, int RT>
-static int launch_rt(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
-  paged_attn_kernel<D, BF, RT><<<(unsigned)((p.runs + 7) / 8 * 8), 256, 0, st>>>(a);
-  const int rc = launch_status();
-  if (rc != PE_OK || !p.split) return rc;
-  paged_join_kernel<D, BF, RT><<<dim3((unsigned)p.runs, 4), 256, 0, st>>>(a);
-  return launch_status();
-}
 template <int D, bool BF>
 static int launch_pa(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
-  if (p.rt == 1) return launch_rt<D, BF, 1>(p, a, st);
-  if (D == 256 || p.rt == 2) return launch_rt<D, BF, 2>(p, a, st);
-  if constexpr (D != 256) return launch_rt<D, BF, 4>(p, a, st);
-  return PE_ERR_DIMS;
+  const unsigned grid = (unsigned)((p.runs + 7) / 8 * 8);
+  const dim3 join((unsigned)p.runs, 4);
+  switch (p.rb) {
+    case 16: paged_attn_kernel<D, BF, 1><<<grid, 256, 0, st>>>(a); break;
+    case 32: paged_attn_kernel<D, BF, 2><<<grid, 256, 0, st>>>(a); break;
+    default: paged_chunk_kernel<D, BF, 2><<<grid, 256, 0, st>>>(a); break;
+  }
+  const int rc = launch_status();
+  if (rc != PE_OK || !p.split) return rc;
+  switch (p.rb) {
+    case 16: paged_join_kernel<D, BF, 16, 256><<<join, 256, 0, st>>>(a); break;
+    case 32: paged_join_kernel<D, BF, 32, 256><<<join, 256, 0, st>>>(a); break;
+    default: paged_join_kernel<D, BF, 128, 64><<<join, 256, 0, st>>>(a); break;
+  }
+  return launch_status();
 }
 
 }  // namespace pe
@@ -704,7 +959,7 @@ extern "C" size_t pe_paged_attention_workspace_size(int64_t rows, int64_t batch,
   if (!pa_shape_ok(rows, batch, heads, kv_heads, head_dim) || rows < 1 || batch < 1 || positions < 1)
     return 0;
   const PaPlan p = pa_plan(rows, batch, heads, kv_heads, head_dim, positions);
-  return p.split ? (size_t)p.runs * 2 * pa_part_words(16 * p.rt, head_dim) * 4 : 0;
+  return p.split ? (size_t)p.runs * 2 * pa_part_words(p.rb, head_dim) * 4 : 0;
 }
 
 extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t rows, int heads,
