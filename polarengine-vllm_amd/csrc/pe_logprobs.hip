@@ -1,17 +1,25 @@
 // Log probabilities of given tokens, their ranks, the entropy and the likeliest
-// alternatives: a workgroup a row.
+// alternatives, in one pass over the logits:
+//
+//   lse = m + log z, z = sum e^(x - m), entropy = log z - (sum (x - m) e^(x - m)) / z
+//
+// Bound by reading the logits; a row is cut into pieces, a workgroup each, where there
+// are few rows, and a second launch joins them. A wave reads chunks of eight values a
+// lane, the next one's loads under way. A lane's sums are relative to its own maximum,
+// eight values at a time in fp32 and those in 64 bits, so that a row of 200,000 tokens
+// is no less exact than one of a thousand. Ranks are counted by ballots. The wave's
+// likeliest tokens so far lie sorted across its lanes; a chunk is looked through only
+// if one of its values passes the last of them, which is rare behind the first chunks.
 
 #include "pe_internal.h"
 
 namespace pe {
 
-constexpr int kTopMax = 64;
-
-template <int DT>
-__device__ __forceinline__ float logit(const void* p, int64_t i) {
-  if constexpr (DT == PE_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
-  else return f16or_bf(reinterpret_cast<const uint16_t*>(p)[i], DT == PE_DTYPE_BF16);
-}
+constexpr int kTopMax = 64;        // a lane each
+constexpr int kLpThreads = 256;
+constexpr int kLpWaves = kLpThreads / 64;
+constexpr float kLpLog2e = 1.4426950408889634f;
+constexpr int kLpLowest = 0x7FFFFFFF;  // no token
 
 struct LogprobArgs {
   const void* logits;
@@ -23,111 +31,331 @@ struct LogprobArgs {
   float* entropy;
   float* top_logprobs;
   int64_t* top_tokens;
+  int pieces;    // of a row
+  int granules;  // of 16 bytes of a piece, a multiple of a chunk's
+  char* parts;   // [rows][pieces]: LpSums, then [rows][pieces][waves][top]: LpTop
+};
+struct LpSums {
+  double z, e;
+  float m;
+  int rank;
+};
+struct LpTop {
+  float x;
+  int i;
 };
 
 template <int DT>
-__global__ __launch_bounds__(1024) void logprob_kernel(const LogprobArgs a) {
-  __shared__ double rd[16];
-  __shared__ float rf[16];
-  __shared__ int ri[16];
-  const int row = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
-  const int64_t base = row * a.ld;
-  auto best = [&](float v, int i) {  // the largest, the first of equals
+__device__ __forceinline__ float lp_logit(const void* p, int64_t i) {
+  if constexpr (DT == PE_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+  else return f16or_bf(reinterpret_cast<const uint16_t*>(p)[i], DT == PE_DTYPE_BF16);
+}
+
+__device__ __forceinline__ bool lp_before(float x, int i, float y, int j) {
+  return x > y || (x == y && i < j);
+}
+__device__ __forceinline__ float lp_lane(float v, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+
+// The wave's `top` likeliest tokens, the l-th in lane l, -inf and no token at first.
+struct LpList {
+  float x;
+  int i;
+  float last_x;  // of lane top - 1, uniform
+  int last_i;
+  __device__ __forceinline__ void begin() {
+    x = last_x = -__builtin_inff();
+    i = last_i = kLpLowest;
+  }
+  // candidates (v, at), one a lane; NaN: none
+  __device__ __forceinline__ void offer(float v, int at, int lane, int top) {
+    uint64_t left = __ballot(lp_before(v, at, last_x, last_i));
+    while (left) {
+      const int l = __builtin_ctzll(left);
+      const float nv = lp_lane(v, l);
+      const int ni = __builtin_amdgcn_readlane(at, l);
+      const bool mine = lp_before(x, i, nv, ni);  // stays before it
+      const float ux = __shfl_up(x, 1, 64);
+      const int ui = __shfl_up(i, 1, 64);
+      const bool above = lane > 0 && lp_before(ux, ui, nv, ni);
+      if (!mine) {
+        x = lane == 0 || above ? nv : ux;
+        i = lane == 0 || above ? ni : ui;
+      }
+      last_x = lp_lane(x, top - 1);
+      last_i = __builtin_amdgcn_readlane(i, top - 1);
+      left &= left - 1;
+      left &= __ballot(lp_before(v, at, last_x, last_i));
+    }
+  }
+};
+
+// A workgroup's sums, in every thread.
+__device__ __forceinline__ LpSums lp_join(LpSums s, LpSums* shared, int lane, int wave) {
+  float m = s.m;
 #pragma unroll
-    for (int m = 32; m; m >>= 1) {
-      const float ov = __shfl_xor(v, m, 64);
-      const int oi = __shfl_xor(i, m, 64);
-      if (ov > v || (ov == v && oi < i)) {
-        v = ov;
-        i = oi;
-      }
-    }
-    __syncthreads();
-    if ((tid & 63) == 0) {
-      rf[wave] = v;
-      ri[wave] = i;
-    }
-    __syncthreads();
-    v = rf[0];
-    i = ri[0];
-    for (int w = 1; w < 16; ++w)
-      if (rf[w] > v || (rf[w] == v && ri[w] < i)) {
-        v = rf[w];
-        i = ri[w];
-      }
-  return make_float2(v, __builtin_bit_cast(float, i));
+  for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+  auto onto = [](LpSums v, float to) {  // relative to `to`
+    const float d = v.m - to;
+    const double f = v.z > 0 ? (double)__builtin_amdgcn_exp2f(d * kLpLog2e) : 0.0;
+    v.e = v.z > 0 ? f * (v.e + d * v.z) : 0.0;
+    v.z *= f;
+    v.m = to;
+    return v;
   };
-  auto sum = [&](double v) {
+  s = onto(s, m);
 #pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
-    __syncthreads();
-    if ((tid & 63) == 0) rd[wave] = v;
-    __syncthreads();
-    double t = 0;
-    for (int w = 0; w < 16; ++w) t += rd[w];
-    return t;
+  for (int k = 32; k; k >>= 1) {
+    s.z += __shfl_xor(s.z, k, 64);
+    s.e += __shfl_xor(s.e, k, 64);
+    s.rank += __shfl_xor(s.rank, k, 64);
+  }
+  if (lane == 0) shared[wave] = s;
+  __syncthreads();
+  for (int w = 0; w < kLpWaves; ++w) m = fmaxf(m, shared[w].m);
+  LpSums t{0, 0, m, 0};
+  for (int w = 0; w < kLpWaves; ++w) {
+    const LpSums o = onto(shared[w], m);
+    t.z += o.z;
+    t.e += o.e;
+    t.rank += o.rank;
+  }
+  return t;
+}
+
+// The row's answers, by one wave that holds its list. xt: the token's logit.
+template <int DT>
+__device__ __forceinline__ void lp_answer(const LogprobArgs& a, int row, const LpSums& s, const LpList& list,
+                                          int lane) {
+  const double lz = log(s.z);
+  if (lane < a.top) {
+    const bool any = list.i != kLpLowest;
+    a.top_logprobs[(int64_t)row * a.top + lane] = (float)((double)(list.x - s.m) - lz);
+    a.top_tokens[(int64_t)row * a.top + lane] = any ? list.i : -1;
+  }
+  if (lane == 0) {
+    const int64_t tok = a.tokens[row];
+    float lp = 0.f;
+    int64_t rank = -1;
+    if (tok >= 0 && tok < a.vocab) {
+      const float xt = lp_logit<DT>(a.logits, row * a.ld + tok);
+      lp = (float)((double)(xt - s.m) - lz);
+      rank = s.rank;
+    }
+    a.logprob[row] = lp;
+    a.rank[row] = rank;
+    a.entropy[row] = (float)(lz - s.e / s.z);
+  }
+}
+
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
+  constexpr int SZ = DT == PE_DTYPE_F32 ? 4 : 2, PER = 16 / SZ;  // values of a granule
+  constexpr int U = 8 / PER;                                    // granules of a lane and chunk
+  __shared__ LpSums sums[kLpWaves];
+  __shared__ LpTop tops[kLpWaves][kTopMax];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x, piece = blockIdx.y;
+  // 16-byte granules from the one that holds the row's first value; value j of granule g
+  // is token g PER + j - off
+  const char* start = reinterpret_cast<const char*>(a.logits) + row * a.ld * SZ;
+  const int off = (int)(reinterpret_cast<uintptr_t>(start) & 15) / SZ;
+  const u32x4v* base = reinterpret_cast<const u32x4v*>(start - off * SZ);
+  const int all = (a.vocab + off + PER - 1) / PER;
+  const int g0 = piece * a.granules, g1 = min(all, g0 + a.granules);
+  const int64_t tok64 = a.tokens[row];
+  const bool there = tok64 >= 0 && tok64 < a.vocab;
+  const int tok = there ? (int)tok64 : 0;
+  const float xt = there ? lp_logit<DT>(a.logits, row * a.ld + tok) : __builtin_nanf("");
+
+  LpList list;
+  list.begin();
+  float m = -__builtin_inff();
+  double z = 0, e = 0;
+  int rank = 0;
+  constexpr int STEP = kLpWaves * 64 * U;  // granules of the workgroup's chunks
+  u32x4v nxt[U];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) nxt[u] = base[min(c + u * 64 + lane, all - 1)];
   };
-  const int64_t tok = a.tokens[row];
-  const bool there = tok >= 0 && tok < a.vocab;
-  const float xt = there ? logit<DT>(a.logits, base + tok) : 0.f;
-  float mx = -__builtin_inff();
-  int mi = a.vocab;
-  for (int i = tid; i < a.vocab; i += 1024) {
-    const float x = logit<DT>(a.logits, base + i);
-    if (x > mx || (x == mx && i < mi)) {
-      mx = x;
-      mi = i;
+  int c = g0 + wave * 64 * U;
+  if (c < g1) load(c);
+  for (; c < g1; c += STEP) {
+    u32x4v cur[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+    if (c + STEP < g1) load(c + STEP);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = cur[j / PER][j % PER * SZ / 4];
+      if constexpr (DT == PE_DTYPE_F32) x[j] = __builtin_bit_cast(float, w);
+      else if constexpr (DT == PE_DTYPE_BF16)
+        x[j] = __builtin_bit_cast(float, j & 1 ? w & 0xFFFF0000u : w << 16);
+      else x[j] = h2f((uint16_t)(w >> (16 * (j & 1))));
     }
-  }
-  float2 w = best(mx, mi);
-  const float top = w.x;
-  double z = 0, e = 0, r = 0;
-  for (int i = tid; i < a.vocab; i += 1024) {
-    const float x = logit<DT>(a.logits, base + i), d = x - top;
-    const float p = expf(d);
-    z += p;
-    if (p > 0.f || p != p) e += (double)p * d;
-    r += x > xt || (x == xt && i < tok);
-  }
-  z = sum(z);
-  e = sum(e);
-  r = sum(r);
-  const double lz = log(z);
-  if (tid == 0) {
-    a.logprob[row] = there ? (float)((double)(xt - top) - lz) : 0.f;
-    a.rank[row] = there ? (int64_t)r : -1;
-    a.entropy[row] = (float)(lz - e / z);
-  }
-  int last = -1;  // the one taken before
-  float lv = 0.f;
-  for (int k = 0; k < a.top; ++k) {
-    if (k) {
-      mx = -__builtin_inff();
-      mi = a.vocab;
-      for (int i = tid; i < a.vocab; i += 1024) {
-        const float x = logit<DT>(a.logits, base + i);
-        if (!(x < lv || (x == lv && i > last))) continue;
-        if (x > mx || (x == mx && i < mi)) {
-          mx = x;
-          mi = i;
-        }
+    auto index = [&](int j) { return (c + (j / PER) * 64 + lane) * PER + j % PER - off; };
+    // outside the row and past the piece: NaN, which no comparison holds for
+    if (c == 0 || c + 64 * U > g1 || c + 64 * U >= all) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool out = ((uint32_t)index(j) >= (uint32_t)a.vocab) | (c + (j / PER) * 64 + lane >= g1);
+        x[j] = out ? __builtin_nanf("") : x[j];
       }
-      w = best(mx, mi);
     }
-    lv = w.x;
-    last = __builtin_bit_cast(int, w.y);
-    if (tid == 0) {
-      a.top_logprobs[(int64_t)row * a.top + k] = (float)((double)(lv - top) - lz);
-      a.top_tokens[(int64_t)row * a.top + k] = last < a.vocab ? last : -1;
+    float cm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__any(cm > m)) {
+      const float mn = fmaxf(m, cm);
+      if (mn > m) {
+        const float d = m - mn;
+        const double f = m == -__builtin_inff() ? 0.0 : (double)__builtin_amdgcn_exp2f(d * kLpLog2e);
+        e = m == -__builtin_inff() ? 0.0 : f * (e + d * z);
+        z *= f;
+        m = mn;
+      }
     }
+    const float sub = m == -__builtin_inff() ? 0.f : m;
+    float zs = 0.f, es = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = fmaxf(x[j] - sub, -1e4f);  // -inf and NaN: a weight of 0
+      const float w = __builtin_amdgcn_exp2f(d * kLpLog2e);
+      zs += w;
+      es = __builtin_fmaf(w, d, es);
+    }
+    z += zs;
+    e += es;
+    // ties count where they come before the token; its own granule is looked at below
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t before = __ballot((c + u * 64 + lane) * PER + PER - 1 - off < tok);
+#pragma unroll
+      for (int j = u * PER; j < u * PER + PER; ++j)
+        rank += __builtin_popcountll(__ballot(x[j] > xt) | (__ballot(x[j] == xt) & before));
+    }
+    if constexpr (TOP)
+      if (__any(cm > list.last_x) || (list.last_i == kLpLowest && __any(cm == list.last_x)))
+#pragma unroll
+        for (int j = 0; j < 8; ++j) list.offer(x[j], index(j), lane, a.top);
   }
+  rank = lane == 0 ? rank : 0;
+  if (there && piece == 0 && wave == 0 && lane < PER) {
+    // ties before the token in its granule
+    const int i = (tok + off) / PER * PER - off + lane;
+    rank += i >= 0 && i < tok && lp_logit<DT>(a.logits, row * a.ld + i) == xt;
+  }
+  const LpSums s = lp_join(LpSums{z, e, m, rank}, sums, lane, wave);
+  if (a.pieces > 1) {
+    const int64_t part = (int64_t)row * a.pieces + piece;
+    if (threadIdx.x == 0) reinterpret_cast<LpSums*>(a.parts)[part] = s;
+    if (TOP && lane < a.top)
+      reinterpret_cast<LpTop*>(reinterpret_cast<LpSums*>(a.parts) + (int64_t)a.rows * a.pieces)
+          [(part * kLpWaves + wave) * a.top + lane] = LpTop{list.x, list.i};
+    return;
+  }
+  if constexpr (TOP) {
+    tops[wave][lane] = LpTop{list.x, list.i};
+    __syncthreads();
+    if (wave == 0)
+      for (int w = 1; w < kLpWaves; ++w) {
+        const LpTop t = tops[w][lane];
+        list.offer(lane < a.top && t.i != kLpLowest ? t.x : __builtin_nanf(""), t.i, lane, a.top);
+      }
+  }
+  if (wave == 0) lp_answer<DT>(a, row, s, list, lane);
+}
+
+// a workgroup a row: its pieces' sums and lists
+template <int DT>
+__global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobArgs a) {
+  __shared__ LpSums sums[kLpWaves];
+  __shared__ LpTop tops[kLpWaves][kTopMax];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x;
+  const LpSums* parts = reinterpret_cast<const LpSums*>(a.parts) + (int64_t)row * a.pieces;
+  const int count = a.pieces * kLpWaves * a.top;
+  const LpTop* cand = reinterpret_cast<const LpTop*>(reinterpret_cast<const LpSums*>(a.parts) +
+                                                     (int64_t)a.rows * a.pieces) + (int64_t)row * count;
+  LpSums s{0, 0, -__builtin_inff(), 0};
+  if ((int)threadIdx.x < a.pieces) s = parts[threadIdx.x];
+  s = lp_join(s, sums, lane, wave);
+  LpList list;
+  list.begin();
+  // a chunk: eight candidates a lane
+  for (int c = wave * 512; c < count; c += kLpWaves * 512) {
+    LpTop t[8];
+    float cm = __builtin_nanf("");
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = c + j * 64 + lane;
+      t[j] = cand[min(i, count - 1)];
+      if (i >= count || t[j].i == kLpLowest) t[j].x = __builtin_nanf("");
+      cm = fmaxf(cm, t[j].x);
+    }
+    // equal ones may come before those of an earlier chunk
+    if (__any(cm >= list.last_x))
+#pragma unroll
+      for (int j = 0; j < 8; ++j) list.offer(t[j].x, t[j].i, lane, a.top);
+  }
+  if (a.top) {
+    tops[wave][lane] = LpTop{list.x, list.i};
+    __syncthreads();
+    if (wave == 0)
+      for (int w = 1; w < kLpWaves; ++w) {
+        const LpTop t = tops[w][lane];
+        list.offer(lane < a.top && t.i != kLpLowest ? t.x : __builtin_nanf(""), t.i, lane, a.top);
+      }
+  }
+  if (wave == 0) lp_answer<DT>(a, row, s, list, lane);
+}
+
+// Pieces of a row: one where the rows alone fill the card, else as many as make about
+// kLpTarget workgroups, of at least a chunk of the workgroup's.
+constexpr int kLpTarget = 1024;
+constexpr int kLpMaxPieces = kLpThreads;  // a thread each in the join
+struct LpPlan {
+  int pieces, granules;
+};
+static LpPlan lp_plan(int64_t rows, int64_t vocab, int dtype) {
+  const int per = dtype == PE_DTYPE_F32 ? 4 : 8, step = kLpWaves * 64 * (8 / per);
+  const int64_t all = (vocab + 2 * per - 2) / per;  // at most, wherever the row begins
+  int64_t n = (kLpTarget + rows - 1) / rows;
+  n = n < kLpMaxPieces ? n : kLpMaxPieces;
+  int64_t granules = ((all + n - 1) / n + step - 1) / step * step;
+  return LpPlan{(int)((all + granules - 1) / granules), (int)granules};
+}
+static size_t lp_bytes(const LpPlan& p, int64_t rows, int top) {
+  return p.pieces == 1 ? 0 : (size_t)rows * p.pieces * (sizeof(LpSums) + kLpWaves * (size_t)top * sizeof(LpTop));
+}
+static bool lp_shape_ok(int64_t rows, int64_t vocab, int top) {
+  return rows >= 0 && rows <= (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && top >= 0 && top <= kTopMax &&
+         top <= vocab;
+}
+
+template <int DT>
+static int launch_lp(const LogprobArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.rows, (unsigned)a.pieces);
+  if (a.top) logprob_kernel<DT, true><<<grid, kLpThreads, 0, st>>>(a);
+  else logprob_kernel<DT, false><<<grid, kLpThreads, 0, st>>>(a);
+  const int rc = launch_status();
+  if (rc != PE_OK || a.pieces == 1) return rc;
+  logprob_join_kernel<DT><<<(unsigned)a.rows, kLpThreads, 0, st>>>(a);
+  return launch_status();
 }
 
 }  // namespace pe
 
 using namespace pe;
 
-extern "C" size_t pe_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top) { return 0; }
+extern "C" size_t pe_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top) {
+  if (!lp_shape_ok(rows, vocab, top) || rows == 0) return 0;
+  // of the types, the one with more pieces
+  const size_t a = lp_bytes(lp_plan(rows, vocab, PE_DTYPE_F32), rows, top);
+  const size_t b = lp_bytes(lp_plan(rows, vocab, PE_DTYPE_F16), rows, top);
+  return a > b ? a : b;
+}
 
 extern "C" int pe_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t ld,
                                  int64_t vocab, const int64_t* tokens, int top, float* logprob,
@@ -137,15 +365,17 @@ extern "C" int pe_token_logprobs(const void* logits, int dtype, int64_t rows, in
   if (!logits || !tokens || !logprob || !rank || !entropy || (top > 0 && (!top_logprobs || !top_tokens)))
     return PE_ERR_NULL;
   if (dtype != PE_DTYPE_F32 && bf16_flag(dtype) < 0) return PE_ERR_DTYPE;
-  if (rows < 0 || rows > kTopMax * (int64_t)(1 << 18) || vocab < 1 || vocab > (1 << 24) || ld < vocab ||
-      top < 0 || top > kTopMax || top > vocab)
-    return PE_ERR_DIMS;
+  if (!lp_shape_ok(rows, vocab, top) || ld < vocab) return PE_ERR_DIMS;
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == PE_DTYPE_F32 ? 4 : 2)) return PE_ERR_ALIGN;
   if (rows == 0) return PE_OK;
+  const LpPlan p = lp_plan(rows, vocab, dtype);
+  const size_t need = lp_bytes(p, rows, top);
+  if (need && (!workspace || workspace_bytes < need)) return PE_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return PE_ERR_ALIGN;
   const LogprobArgs a{logits, ld, tokens, (int)rows, (int)vocab, top, logprob, rank, entropy,
-                      top_logprobs, top_tokens};
+                      top_logprobs, top_tokens, p.pieces, p.granules, reinterpret_cast<char*>(workspace)};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == PE_DTYPE_F32) logprob_kernel<PE_DTYPE_F32><<<(unsigned)rows, 1024, 0, st>>>(a);
-  else if (dtype == PE_DTYPE_BF16) logprob_kernel<PE_DTYPE_BF16><<<(unsigned)rows, 1024, 0, st>>>(a);
-  else logprob_kernel<PE_DTYPE_F16><<<(unsigned)rows, 1024, 0, st>>>(a);
-  return launch_status();
+  if (dtype == PE_DTYPE_F32) return launch_lp<PE_DTYPE_F32>(a, st);
+  if (dtype == PE_DTYPE_BF16) return launch_lp<PE_DTYPE_BF16>(a, st);
+  return launch_lp<PE_DTYPE_F16>(a, st);
 }
