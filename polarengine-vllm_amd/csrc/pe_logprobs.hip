@@ -19,7 +19,6 @@ constexpr int kTopMax = 64;        // a lane each
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
 constexpr float kLpLog2e = 1.4426950408889634f;
-constexpr int kLpLowest = 0x7FFFFFFF;  // no token
 
 struct LogprobArgs {
   const void* logits;
@@ -33,16 +32,12 @@ struct LogprobArgs {
   int64_t* top_tokens;
   int pieces;    // of a row
   int granules;  // of 16 bytes of a piece, a multiple of a chunk's
-  char* parts;   // [rows][pieces]: LpSums, then [rows][pieces][waves][top]: LpTop
+  char* parts;   // [rows][pieces]: LpSums, then [rows][pieces][top]: LpKey
 };
 struct LpSums {
   double z, e;
   float m;
   int rank;
-};
-struct LpTop {
-  float x;
-  int i;
 };
 
 template <int DT>
@@ -51,45 +46,118 @@ __device__ __forceinline__ float lp_logit(const void* p, int64_t i) {
   else return f16or_bf(reinterpret_cast<const uint16_t*>(p)[i], DT == PE_DTYPE_BF16);
 }
 
-__device__ __forceinline__ bool lp_before(float x, int i, float y, int j) {
-  return x > y || (x == y && i < j);
+// A token as one number: the larger the logit the larger, of equal logits the lower
+// token; 0: none.
+typedef uint64_t LpKey;
+__device__ __forceinline__ LpKey lp_key(float x, int i) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);  // -0 is 0
+  const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return x != x ? 0 : (uint64_t)o << 32 | ~(uint32_t)i;
 }
-__device__ __forceinline__ float lp_lane(float v, int l) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+__device__ __forceinline__ float lp_value(LpKey k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return k ? __builtin_bit_cast(float, o & 0x80000000u ? o ^ 0x80000000u : ~o) : -__builtin_inff();
+}
+__device__ __forceinline__ int lp_token(LpKey k) { return k ? (int)~(uint32_t)k : -1; }
+
+template <int M>
+__device__ __forceinline__ uint32_t lp_xor32(uint32_t v, int lane) {
+  if constexpr (M <= 8) {
+    return __builtin_bit_cast(uint32_t, lane_xor<M>(__builtin_bit_cast(float, v)));
+  } else if constexpr (M == 16) {
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    return lane & 16 ? r0 : r1;
+  } else {
+    auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    return lane & 32 ? r0 : r1;
+  }
+}
+template <int M>
+__device__ __forceinline__ LpKey lp_xor(LpKey k, int lane) {
+  return (uint64_t)lp_xor32<M>((uint32_t)(k >> 32), lane) << 32 | lp_xor32<M>((uint32_t)k, lane);
+}
+// one step of a bitonic network: the larger of lanes l and l ^ M in the one where
+// lane & M is not set, unless `up`
+template <int M>
+__device__ __forceinline__ LpKey lp_step(LpKey k, bool up, int lane) {
+  const LpKey o = lp_xor<M>(k, lane);
+  const bool low = ((lane & M) == 0) != up;
+  return (o > k) == low ? o : k;
+}
+// a bitonic sequence in order, falling unless `up`
+template <int M>
+__device__ __forceinline__ LpKey lp_merge(LpKey k, bool up, int lane) {
+  k = lp_step<M>(k, up, lane);
+  if constexpr (M > 1) k = lp_merge<M / 2>(k, up, lane);
+  return k;
+}
+// rising over the 64 lanes
+__device__ __forceinline__ LpKey lp_sort(LpKey k, int lane) {
+  k = lp_merge<1>(k, (lane & 2) == 0, lane);
+  k = lp_merge<2>(k, (lane & 4) == 0, lane);
+  k = lp_merge<4>(k, (lane & 8) == 0, lane);
+  k = lp_merge<8>(k, (lane & 16) == 0, lane);
+  k = lp_merge<16>(k, (lane & 32) == 0, lane);
+  return lp_merge<32>(k, true, lane);
 }
 
-// The wave's `top` likeliest tokens, the l-th in lane l, -inf and no token at first.
+// The wave's 64 likeliest tokens, falling over the lanes; `last`, uniform, is the
+// top-th of them, which a candidate has to pass.
 struct LpList {
-  float x;
-  int i;
-  float last_x;  // of lane top - 1, uniform
-  int last_i;
+  LpKey k, last;
+  float last_x;
   __device__ __forceinline__ void begin() {
-    x = last_x = -__builtin_inff();
-    i = last_i = kLpLowest;
+    k = last = 0;
+    last_x = -__builtin_inff();
   }
-  // candidates (v, at), one a lane; NaN: none
-  __device__ __forceinline__ void offer(float v, int at, int lane, int top) {
-    uint64_t left = __ballot(lp_before(v, at, last_x, last_i));
-    while (left) {
-      const int l = __builtin_ctzll(left);
-      const float nv = lp_lane(v, l);
-      const int ni = __builtin_amdgcn_readlane(at, l);
-      const bool mine = lp_before(x, i, nv, ni);  // stays before it
-      const float ux = __shfl_up(x, 1, 64);
-      const int ui = __shfl_up(i, 1, 64);
-      const bool above = lane > 0 && lp_before(ux, ui, nv, ni);
-      if (!mine) {
-        x = lane == 0 || above ? nv : ux;
-        i = lane == 0 || above ? ni : ui;
+  __device__ __forceinline__ void set_last(int top) {
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), top - 1);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)k, top - 1);
+    last = (uint64_t)hi << 32 | lo;
+    last_x = lp_value(last);
+  }
+  // 64 more, rising over the lanes: the larger of each pair are the 64 likeliest of both
+  __device__ __forceinline__ void join(LpKey rising, int lane, int top) {
+    k = lp_merge<32>(rising > k ? rising : k, false, lane);
+    set_last(top);
+  }
+  // eight candidates a lane: the best of each lane at a time, as long as some pass
+  __device__ __forceinline__ void offer(LpKey (&c)[8], int lane, int top) {
+    for (int round = 0; round < 8; ++round) {
+      LpKey best = c[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) best = c[j] > best ? c[j] : best;
+      uint64_t pass = __ballot(best > last);
+      if (!pass) return;
+      if (__builtin_popcountll(pass) > 3) {
+        join(lp_sort(best > last ? best : 0, lane), lane, top);
+      } else {
+        while (pass) {  // one by one: the lanes behind its place move by one
+          const int l = __builtin_ctzll(pass);
+          const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), l);
+          const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)best, l);
+          const LpKey n = (uint64_t)hi << 32 | lo;
+          const LpKey up = __shfl_up((unsigned long long)k, 1, 64);
+          k = k > n ? k : lane == 0 || up > n ? n : up;
+          pass &= pass - 1;
+        }
+        set_last(top);
       }
-      last_x = lp_lane(x, top - 1);
-      last_i = __builtin_amdgcn_readlane(i, top - 1);
-      left &= left - 1;
-      left &= __ballot(lp_before(v, at, last_x, last_i));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = c[j] == best ? 0 : c[j];
     }
   }
 };
+
+// The lists of a workgroup's waves, in the first wave's.
+__device__ __forceinline__ void lp_join_lists(LpList& list, LpKey (*shared)[64], int lane, int wave, int top) {
+  shared[wave][lane] = list.k;
+  __syncthreads();
+  if (wave == 0)
+    for (int w = 1; w < kLpWaves; ++w) list.join(shared[w][63 - lane], lane, top);
+}
 
 // A workgroup's sums, in every thread.
 __device__ __forceinline__ LpSums lp_join(LpSums s, LpSums* shared, int lane, int wave) {
@@ -130,9 +198,8 @@ __device__ __forceinline__ void lp_answer(const LogprobArgs& a, int row, const L
                                           int lane) {
   const double lz = log(s.z);
   if (lane < a.top) {
-    const bool any = list.i != kLpLowest;
-    a.top_logprobs[(int64_t)row * a.top + lane] = (float)((double)(list.x - s.m) - lz);
-    a.top_tokens[(int64_t)row * a.top + lane] = any ? list.i : -1;
+    a.top_logprobs[(int64_t)row * a.top + lane] = (float)((double)(lp_value(list.k) - s.m) - lz);
+    a.top_tokens[(int64_t)row * a.top + lane] = lp_token(list.k);
   }
   if (lane == 0) {
     const int64_t tok = a.tokens[row];
@@ -154,7 +221,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
   constexpr int SZ = DT == PE_DTYPE_F32 ? 4 : 2, PER = 16 / SZ;  // values of a granule
   constexpr int U = 8 / PER;                                    // granules of a lane and chunk
   __shared__ LpSums sums[kLpWaves];
-  __shared__ LpTop tops[kLpWaves][kTopMax];
+  __shared__ LpKey tops[kLpWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x, piece = blockIdx.y;
   // 16-byte granules from the one that holds the row's first value; value j of granule g
@@ -236,9 +303,12 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         rank += __builtin_popcountll(__ballot(x[j] > xt) | (__ballot(x[j] == xt) & before));
     }
     if constexpr (TOP)
-      if (__any(cm > list.last_x) || (list.last_i == kLpLowest && __any(cm == list.last_x)))
+      if (__any(cm > list.last_x) || (list.last == 0 && __any(cm == list.last_x))) {
+        LpKey k[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) list.offer(x[j], index(j), lane, a.top);
+        for (int j = 0; j < 8; ++j) k[j] = lp_key(x[j], index(j));
+        list.offer(k, lane, a.top);
+      }
   }
   rank = lane == 0 ? rank : 0;
   if (there && piece == 0 && wave == 0 && lane < PER) {
@@ -247,67 +317,46 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     rank += i >= 0 && i < tok && lp_logit<DT>(a.logits, row * a.ld + i) == xt;
   }
   const LpSums s = lp_join(LpSums{z, e, m, rank}, sums, lane, wave);
-  if (a.pieces > 1) {
-    const int64_t part = (int64_t)row * a.pieces + piece;
-    if (threadIdx.x == 0) reinterpret_cast<LpSums*>(a.parts)[part] = s;
-    if (TOP && lane < a.top)
-      reinterpret_cast<LpTop*>(reinterpret_cast<LpSums*>(a.parts) + (int64_t)a.rows * a.pieces)
-          [(part * kLpWaves + wave) * a.top + lane] = LpTop{list.x, list.i};
+  if constexpr (TOP) lp_join_lists(list, tops, lane, wave, a.top);
+  if (wave) return;
+  if (a.pieces == 1) {
+    lp_answer<DT>(a, row, s, list, lane);
     return;
   }
-  if constexpr (TOP) {
-    tops[wave][lane] = LpTop{list.x, list.i};
-    __syncthreads();
-    if (wave == 0)
-      for (int w = 1; w < kLpWaves; ++w) {
-        const LpTop t = tops[w][lane];
-        list.offer(lane < a.top && t.i != kLpLowest ? t.x : __builtin_nanf(""), t.i, lane, a.top);
-      }
-  }
-  if (wave == 0) lp_answer<DT>(a, row, s, list, lane);
+  const int64_t part = (int64_t)row * a.pieces + piece;
+  if (lane == 0) reinterpret_cast<LpSums*>(a.parts)[part] = s;
+  if (TOP && lane < a.top)
+    reinterpret_cast<LpKey*>(reinterpret_cast<LpSums*>(a.parts) + (int64_t)a.rows * a.pieces)
+        [part * a.top + lane] = list.k;
 }
 
 // a workgroup a row: its pieces' sums and lists
 template <int DT>
 __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobArgs a) {
   __shared__ LpSums sums[kLpWaves];
-  __shared__ LpTop tops[kLpWaves][kTopMax];
+  __shared__ LpKey tops[kLpWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x;
   const LpSums* parts = reinterpret_cast<const LpSums*>(a.parts) + (int64_t)row * a.pieces;
-  const int count = a.pieces * kLpWaves * a.top;
-  const LpTop* cand = reinterpret_cast<const LpTop*>(reinterpret_cast<const LpSums*>(a.parts) +
+  const int count = a.pieces * a.top;
+  const LpKey* cand = reinterpret_cast<const LpKey*>(reinterpret_cast<const LpSums*>(a.parts) +
                                                      (int64_t)a.rows * a.pieces) + (int64_t)row * count;
   LpSums s{0, 0, -__builtin_inff(), 0};
   if ((int)threadIdx.x < a.pieces) s = parts[threadIdx.x];
-  s = lp_join(s, sums, lane, wave);
   LpList list;
   list.begin();
-  // a chunk: eight candidates a lane
   for (int c = wave * 512; c < count; c += kLpWaves * 512) {
-    LpTop t[8];
-    float cm = __builtin_nanf("");
+    LpKey k[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int i = c + j * 64 + lane;
-      t[j] = cand[min(i, count - 1)];
-      if (i >= count || t[j].i == kLpLowest) t[j].x = __builtin_nanf("");
-      cm = fmaxf(cm, t[j].x);
+      k[j] = cand[min(i, count - 1)];
+      k[j] = i < count ? k[j] : 0;
     }
-    // equal ones may come before those of an earlier chunk
-    if (__any(cm >= list.last_x))
-#pragma unroll
-      for (int j = 0; j < 8; ++j) list.offer(t[j].x, t[j].i, lane, a.top);
+    list.offer(k, lane, a.top);
   }
-  if (a.top) {
-    tops[wave][lane] = LpTop{list.x, list.i};
-    __syncthreads();
-    if (wave == 0)
-      for (int w = 1; w < kLpWaves; ++w) {
-        const LpTop t = tops[w][lane];
-        list.offer(lane < a.top && t.i != kLpLowest ? t.x : __builtin_nanf(""), t.i, lane, a.top);
-      }
-  }
+  s = lp_join(s, sums, lane, wave);
+  if (a.top) lp_join_lists(list, tops, lane, wave, a.top);
   if (wave == 0) lp_answer<DT>(a, row, s, list, lane);
 }
 
@@ -327,7 +376,7 @@ static LpPlan lp_plan(int64_t rows, int64_t vocab, int dtype) {
   return LpPlan{(int)((all + granules - 1) / granules), (int)granules};
 }
 static size_t lp_bytes(const LpPlan& p, int64_t rows, int top) {
-  return p.pieces == 1 ? 0 : (size_t)rows * p.pieces * (sizeof(LpSums) + kLpWaves * (size_t)top * sizeof(LpTop));
+  return p.pieces == 1 ? 0 : (size_t)rows * p.pieces * (sizeof(LpSums) + (size_t)top * sizeof(LpKey));
 }
 static bool lp_shape_ok(int64_t rows, int64_t vocab, int top) {
   return rows >= 0 && rows <= (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && top >= 0 && top <= kTopMax &&
