@@ -5,8 +5,6 @@
 
 namespace pe {
 
-typedef float float2v __attribute__((ext_vector_type(2)));
-
 constexpr int kPlanThreads = 1024;
 
 // Running sums over a workgroup of 1024 in order of thread; `total` in every thread.
@@ -32,18 +30,43 @@ __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t* waves, uint3
 }
 
 // ---------------------------------------------------------------------------
-// One workgroup: a thread a sequence, then a thread a row.
+// The plan, one workgroup: a thread a sequence, then a thread a row. What bounds it is
+// the chain of loads: lengths, table entries, free blocks, the rows' entries. A
+// sequence's first kPlanShort entries are its thread's, at once; of longer ones a wave
+// takes 64 at a time.
 // ---------------------------------------------------------------------------
+constexpr int kPlanShort = 4;
+constexpr int kPlanWaves = kPlanThreads / 64;
+
+// sequences of a round that have more than kPlanShort entries to look at
+struct PlanLong {
+  uint32_t count;
+  uint16_t of[kPlanThreads];
+};
+__device__ __forceinline__ void plan_long(PlanLong& l, bool mine) {
+  __syncthreads();
+  if (threadIdx.x == 0) l.count = 0;
+  __syncthreads();
+  if (mine) l.of[atomicAdd(&l.count, 1u)] = (uint16_t)threadIdx.x;  // in any order
+  __syncthreads();
+}
+
 __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
     const int64_t* __restrict__ lengths, const int64_t* __restrict__ counts, int32_t* tables,
     int64_t t_b, int batch, int64_t width, const int32_t* __restrict__ free_blocks, int64_t free_cap,
-    int64_t* free_count, int rows, int log_t, int64_t* starts, int64_t* __restrict__ positions,
-    int64_t* __restrict__ slots, int64_t* out_lengths) {
-  __shared__ uint32_t waves[kPlanThreads / 64];
+    int64_t* free_count, int rows, int log_t, int64_t* __restrict__ starts,
+    int64_t* __restrict__ positions, int64_t* __restrict__ slots, int64_t* __restrict__ out_lengths) {
+  __shared__ uint32_t waves[kPlanWaves];
   __shared__ uint32_t used;
-  const int tid = threadIdx.x;
-  const int64_t have0 = *free_count;
-  const uint32_t have = (uint32_t)max((int64_t)0, min(have0, free_cap));
+  __shared__ PlanLong longs;
+  __shared__ uint32_t needs[kPlanThreads];
+  __shared__ int64_t firsts[kPlanThreads], lasts[kPlanThreads];
+  // of the step: each sequence's end among the rows, and position minus row (kNone: it
+  // got nothing)
+  constexpr int kNone = INT32_MIN;
+  __shared__ int ends[kPagedMaxBatch], offsets[kPagedMaxBatch];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t have = (uint32_t)max((int64_t)0, min(*free_count, free_cap));
   if (tid == 0) {
     starts[0] = 0;
     used = 0;
@@ -57,90 +80,191 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
     uint32_t total;
     const uint32_t end = min(row0 + plan_scan(n, waves, total), (uint32_t)rows + 1);
     row0 = min(row0 + total, (uint32_t)rows + 1);
-    if (b < batch) starts[b + 1] = min(end, (uint32_t)rows);
     const bool fits = len >= 0 && len <= (width << log_t) - (int64_t)n && end <= (uint32_t)rows;
-    uint32_t need = 0;
     const int64_t j0 = len >> log_t, j1 = fits && n ? (len + n - 1) >> log_t : j0 - 1;
     int32_t* row = tables + (int64_t)b * t_b;
-    for (int64_t j = j0; j <= j1; ++j) need += row[j] < 0;
+    uint32_t need = 0;
+    int32_t entry[kPlanShort];
+#pragma unroll
+    for (int i = 0; i < kPlanShort; ++i) entry[i] = j0 + i <= j1 ? row[j0 + i] : 0;
+#pragma unroll
+    for (int i = 0; i < kPlanShort; ++i) need += entry[i] < 0;
+    const bool is_long = j1 - j0 >= kPlanShort;
+    firsts[tid] = j0;
+    lasts[tid] = j1;
+    plan_long(longs, is_long);
+    for (uint32_t k = wave; k < longs.count; k += kPlanWaves) {
+      const int t = longs.of[k];
+      const int32_t* r = tables + (int64_t)(b0 + t) * t_b;
+      uint32_t lacks = 0;
+      for (int64_t j = firsts[t] + lane; j - lane <= lasts[t]; j += 64)
+        lacks += __builtin_popcountll(__ballot(j <= lasts[t] && r[min(j, lasts[t])] < 0));
+      if (lane == 0) needs[t] = lacks;
+    }
+    __syncthreads();
+    if (is_long) need = needs[tid];
     const uint32_t cum = need0 + plan_scan(need, waves, total);
-    need0 += total;
+    need0 = min(need0 + total, kPlanCap);
     const bool taken = fits && (need == 0 || cum <= have);
-    if (b < batch) out_lengths[b] = taken ? len + n : -1;
-    if (taken && need) {
+    if (b < batch) {
+      starts[b + 1] = min(end, (uint32_t)rows);
+      out_lengths[b] = taken ? len + n : -1;
+      ends[b] = (int)min(end, (uint32_t)rows);
+      offsets[b] = taken ? (int)len - (int)(end - n) : kNone;
+    }
+    if (taken && need && !is_long) {
       uint32_t at = cum - need;
-      for (int64_t j = j0; j <= j1; ++j)
-        if (row[j] < 0) row[j] = free_blocks[have - 1 - at++];
-      atomicMax(&used, cum);
+#pragma unroll
+      for (int i = 0; i < kPlanShort; ++i)
+        if (entry[i] < 0) row[j0 + i] = free_blocks[have - 1 - at++];
     }
+    needs[tid] = taken && need ? cum - need : UINT32_MAX;  // rank of the first block
+    if (taken && need) atomicMax(&used, cum);
+    __syncthreads();
+    for (uint32_t k = wave; k < longs.count; k += kPlanWaves) {
+      const int t = longs.of[k];
+      if (needs[t] == UINT32_MAX) continue;
+      int32_t* r = tables + (int64_t)(b0 + t) * t_b;
+      uint32_t at = needs[t];
+      for (int64_t j = firsts[t] + lane; j - lane <= lasts[t]; j += 64) {
+        const bool lacks = j <= lasts[t] && r[min(j, lasts[t])] < 0;
+        const uint64_t all = __ballot(lacks);
+        if (lacks) r[j] = free_blocks[have - 1 - (at + __builtin_popcountll(all & ((1ull << lane) - 1)))];
+        at += __builtin_popcountll(all);
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (tid == 0) *free_count = (int64_t)have - used;
-  for (int r = tid; r < rows; r += kPlanThreads) {
-    int lo = 0, hi = batch;  // the first sequence that ends behind row r
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (starts[mid + 1] > r) hi = mid;
-      else lo = mid + 1;
+  // four rows a thread at a time, so that their entries' loads go out together
+  constexpr int R = 4;
+  for (int r0 = tid; r0 < rows; r0 += R * kPlanThreads) {
+    int64_t pos[R], slot[R];
+    int32_t block[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = min(r0 + i * kPlanThreads, rows - 1);
+      int lo = 0, hi = batch;  // the first sequence that ends behind row r
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (ends[mid] > r) hi = mid;
+        else lo = mid + 1;
+      }
+      const int off = lo < batch ? offsets[lo] : kNone;
+      pos[i] = off != kNone ? off + r : -1;
+      block[i] = off != kNone ? tables[lo * t_b + (pos[i] >> log_t)] : 0;
     }
-    int64_t pos = -1, slot = -1;
-    if (lo < batch && out_lengths[lo] >= 0) {
-      pos = lengths[lo] + r - starts[lo];
-      slot = ((int64_t)tables[lo * t_b + (pos >> log_t)] << log_t) + (pos & ((1 << log_t) - 1));
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + i * kPlanThreads;
+      slot[i] = pos[i] >= 0 ? ((int64_t)block[i] << log_t) + (pos[i] & ((1 << log_t) - 1)) : -1;
+      if (r < rows) {
+        positions[r] = pos[i];
+        slots[r] = slot[i];
+      }
     }
-    positions[r] = pos;
-    slots[r] = slot;
   }
 }
 
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(
-    int32_t* __restrict__ tables, int64_t t_b, int batch, int64_t width,
-    const int64_t* __restrict__ keep, int32_t* __restrict__ free_blocks, int64_t free_cap,
-    int64_t* free_count, int log_t) {
-  __shared__ uint32_t waves[kPlanThreads / 64];
-  const int tid = threadIdx.x;
+    int32_t* tables, int64_t t_b, int batch, int64_t width, const int64_t* __restrict__ keep,
+    int32_t* __restrict__ free_blocks, int64_t free_cap, int64_t* free_count, int log_t) {
+  __shared__ uint32_t waves[kPlanWaves];
+  __shared__ PlanLong longs;
+  __shared__ uint32_t ns[kPlanThreads], ats[kPlanThreads];
+  __shared__ int64_t firsts[kPlanThreads];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t have = max((int64_t)0, min(*free_count, free_cap));
-  uint32_t all = 0;
-  auto count = [&](int b, int64_t& first) {
-    uint32_t n = 0;
-    first = width;
+  int64_t first;
+  int32_t entry[kPlanShort];
+  bool is_long;
+  // how many blocks of sequence b0 + tid go back; `longs` has those of more than kPlanShort
+  auto count = [&](int b0) {
+    const int b = b0 + tid;
     const int64_t k = b < batch ? keep[b] : -1;
-    if (k >= 0) {
-      first = min(width, (k >> log_t) + ((k & ((1 << log_t) - 1)) != 0));
-      while (first + n < width && tables[b * t_b + first + n] >= 0) ++n;
+    first = k < 0 ? width : min(width, (k >> log_t) + ((k & ((1 << log_t) - 1)) != 0));
+#pragma unroll
+    for (int i = 0; i < kPlanShort; ++i)
+      entry[i] = first + i < width ? tables[b * t_b + first + i] : -1;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanShort; ++i) n += n == (uint32_t)i && entry[i] >= 0;
+    is_long = n == kPlanShort;
+    firsts[tid] = first;
+    plan_long(longs, is_long);
+    for (uint32_t l = wave; l < longs.count; l += kPlanWaves) {
+      const int t = longs.of[l];
+      const int32_t* r = tables + (int64_t)(b0 + t) * t_b;
+      uint32_t m = 0;
+      for (int64_t j = firsts[t] + lane;; j += 64) {
+        const uint64_t there = __ballot(j < width && r[min(j, width - 1)] >= 0);
+        m += ~there ? __builtin_ctzll(~there) : 64;
+        if (~there) break;
+      }
+      if (lane == 0) ns[t] = m;
     }
+    __syncthreads();
+    if (is_long) n = ns[tid];
     return n;
   };
+  uint32_t all = 0, total, n = 0;
   for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
-    int64_t first;
-    uint32_t total;
-    plan_scan(count(b0 + tid, first), waves, total);
+    n = count(b0);
+    plan_scan(n, waves, total);
     all += total;
   }
   if (have + all > free_cap) return;
   uint32_t before = 0;
   for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
-    int64_t first;
-    uint32_t total;
-    const uint32_t n = count(b0 + tid, first);
+    if (batch > kPlanThreads) n = count(b0);
     const uint32_t at = before + plan_scan(n, waves, total) - n;
     before += total;
-    for (uint32_t i = 0; i < n; ++i) {
-      int32_t* e = tables + (b0 + tid) * t_b + first + i;
-      free_blocks[have + all - 1 - (at + i)] = *e;
-      *e = -1;
+    int32_t* row = tables + (int64_t)(b0 + tid) * t_b + first;
+    // from the stack's new end on, downwards
+    int32_t* top = free_blocks + have + all - 1;
+    if (!is_long) {
+#pragma unroll
+      for (int i = 0; i < kPlanShort; ++i)
+        if ((uint32_t)i < n) {
+          top[-(int64_t)(at + i)] = entry[i];
+          row[i] = -1;
+        }
     }
+    ats[tid] = at;
+    ns[tid] = n;
+    __syncthreads();
+    for (uint32_t l = wave; l < longs.count; l += kPlanWaves) {
+      const int t = longs.of[l];
+      int32_t* r = tables + (int64_t)(b0 + t) * t_b + firsts[t];
+      for (uint32_t i = lane; i < ns[t]; i += 64) {
+        top[-(int64_t)(ats[t] + i)] = r[i];
+        r[i] = -1;
+      }
+    }
+    __syncthreads();
   }
   if (tid == 0) *free_count = have + all;
 }
 
 // ---------------------------------------------------------------------------
-// The write: one workgroup per row, KV head, and keys or values; it works if its
-// row begins a run. The run's largest |x| gives the scale, codes go out one by one.
+// The write. A workgroup looks for runs that begin among its `per` rows (one in a
+// decode step, so that every token has a workgroup; 16 in a prompt) and takes those of
+// one KV head, keys or values, one after the other. A thread holds 4 slots x 8
+// dimensions: the run is read once, its largest |x| gives the scale, then codes go out.
+// Threads of a wave run over dimensions first for keys (rows of the block) and over
+// slots first for values (which the block stores by dimension), so that either writes
+// neighbouring bytes.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint8_t f8_code(float x) {
-  if (!(fabsf(x) <= 3.4e38f)) return 0x7F;
-  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
+// four codes; NaN where a value is not finite (the conversion itself would saturate)
+__device__ __forceinline__ uint32_t f8_codes(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+  uint32_t u = (uint32_t)r;
+  u = fabsf(a) <= 3.4e38f ? u : u | 0x7Fu;
+  u = fabsf(b) <= 3.4e38f ? u : u | 0x7F00u;
+  u = fabsf(c) <= 3.4e38f ? u : u | 0x7F0000u;
+  u = fabsf(d) <= 3.4e38f ? u : u | 0x7F000000u;
+  return u;
 }
 // the smallest e with amax <= 448 2^e
 __device__ __forceinline__ int f8_exp(float amax) {
@@ -156,51 +280,138 @@ struct WriteArgs {
   int64_t k_r, k_h, v_r, v_h;
   const int64_t* slots;
   PagedCache c;
-  int rows;
+  int rows, per, log_d;
 };
 
-template <int D, bool BF>
+template <int G, bool BF>
 __global__ __launch_bounds__(256) void write_blocks_kernel(const WriteArgs a) {
   __shared__ float red[4];
-  const int row = blockIdx.x, h = blockIdx.y;
+  const int h = blockIdx.y;
   const bool val = blockIdx.z;
-  const int T = 1 << a.c.log_t, tid = threadIdx.x;
-  const int64_t slot = a.slots[row];
-  if (slot < 0 || slot >= a.c.blocks << a.c.log_t) return;
-  const int off = (int)(slot & (T - 1));
-  if (off && row && a.slots[row - 1] == slot - 1) return;  // within a run
-  int n = 1;
-  while (off + n < T && row + n < a.rows && a.slots[row + n] == slot + n) ++n;
-  const int64_t block = slot >> a.c.log_t;
-  const uint16_t* src = val ? a.v + row * a.v_r + h * a.v_h : a.k + row * a.k_r + h * a.k_h;
-  const int64_t s_r = val ? a.v_r : a.k_r;
-  uint8_t* dst = (val ? a.c.v + block * a.c.v_b : a.c.k + block * a.c.k_b) + (int64_t)h * T * D;
-  uint8_t* scale = (val ? a.c.vs : a.c.ks) + block * a.c.s_b + h;
-  float amax = 0.f;
-  for (int i = tid; i < n * D; i += 256) {
-    const float x = fabsf(f16or_bf(src[(i / D) * s_r + i % D], BF));
-    if (x <= 3.4e38f) amax = fmaxf(amax, x);
+  const int log_t = a.c.log_t, T = 1 << log_t, log_d = a.log_d, D = 1 << log_d;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int row0 = blockIdx.x * a.per;
+  const int64_t n_slots = a.c.blocks << log_t;
+  // rows that begin a run, a lane each
+  uint64_t begins;
+  {
+    const int r = min(row0 + lane, a.rows - 1);
+    const int64_t slot = a.slots[r], prev = a.slots[max(r - 1, 0)];
+    const bool within = r > 0 && prev == slot - 1 && (slot & (T - 1));
+    begins = __ballot(lane < a.per && row0 + lane < a.rows && slot >= 0 && slot < n_slots && !within);
   }
-#pragma unroll
-  for (int m = 32; m; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = amax;
-  const int old = (int)*scale - 127;
-  __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int e = off ? max(old, f8_exp(amax)) : f8_exp(amax);
-  if (off && e > old)
-    for (int i = tid; i < T * D; i += 256) {
-      const float f = __builtin_amdgcn_cvt_f32_fp8(dst[i], 0);
-      dst[i] = f8_code(__builtin_ldexpf(f, old - e));
+  for (; begins; begins &= begins - 1) {
+    const int row = row0 + __builtin_ctzll(begins);
+    const int64_t slot = a.slots[row];
+    const int off = (int)(slot & (T - 1));
+    int n = 1;  // rows of the run
+    for (int i0 = 1; n == i0 && off + n < T; i0 += 64) {
+      const int i = i0 + lane;
+      const uint64_t on = __ballot(off + i < T && row + i < a.rows &&
+                                   a.slots[min(row + i, a.rows - 1)] == slot + i);
+      n += ~on ? __builtin_ctzll(~on) : 64;
     }
-  __syncthreads();
-  if (tid == 0) *scale = (uint8_t)(e + 127);
-  for (int i = tid; i < n * D; i += 256) {
-    const int t = i / D, d = i % D;
-    const uint8_t code = f8_code(__builtin_ldexpf(f16or_bf(src[t * s_r + d], BF), -e));
-    dst[val ? d * T + off + t : (off + t) * D + d] = code;
+    const int64_t block = slot >> log_t;
+    const uint16_t* src = val ? a.v + row * a.v_r + h * a.v_h : a.k + row * a.k_r + h * a.k_h;
+    const int64_t s_r = val ? a.v_r : a.k_r;
+    uint8_t* dst = (val ? a.c.v + block * a.c.v_b : a.c.k + block * a.c.k_b) + ((int64_t)h << (log_t + log_d));
+    uint8_t* scale = (val ? a.c.vs : a.c.ks) + block * a.c.s_b + h;
+    const int old = (int)*scale - 127;
+    // the thread's groups: slots 4 sg .. + 3 and dimensions 8 ch .. + 7
+    int sg[G], ch[G];
+    u32x4v x[G][4];
+    float amax = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int i = tid + g * (int)blockDim.x;
+      sg[g] = val ? i & ((T >> 2) - 1) : i >> (log_d - 3);
+      ch[g] = val ? i >> (log_t - 2) : i & ((D >> 3) - 1);
+      const bool in = i < T * D / 32;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int rel = 4 * sg[g] + t - off;
+        x[g][t] = u32x4v{0, 0, 0, 0};
+        if (in && rel >= 0 && rel < n)
+          x[g][t] = *reinterpret_cast<const u32x4v*>(src + rel * s_r + 8 * ch[g]);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t u = x[g][t][w];
+          const float lo = fabsf(f16or_bf((uint16_t)u, BF)), hi = fabsf(f16or_bf((uint16_t)(u >> 16), BF));
+          amax = fmaxf(amax, lo <= 3.4e38f ? lo : 0.f);
+          amax = fmaxf(amax, hi <= 3.4e38f ? hi : 0.f);
+        }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
+    __syncthreads();  // the last run's sums and stores are done with
+    if (lane == 0) red[tid >> 6] = amax;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) amax = fmaxf(amax, red[w]);
+    const int e = off ? max(old, f8_exp(amax)) : f8_exp(amax);
+    if (off && e > old) {
+      uint32_t* codes = reinterpret_cast<uint32_t*>(dst);
+      for (int i = tid; i < T * D / 4; i += blockDim.x) {
+        const uint32_t u = codes[i];
+        float f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t one = u >> (8 * k);
+          f[k] = __builtin_ldexpf(__builtin_amdgcn_cvt_f32_fp8(one, 0), old - e);
+        }
+        codes[i] = f8_codes(f[0], f[1], f[2], f[3]);
+      }
+      __syncthreads();
+    }
+    if (tid == 0) *scale = (uint8_t)(e + 127);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int s0 = 4 * sg[g] - off;  // of the run's rows
+      if (s0 + 3 < 0 || s0 >= n || tid + g * (int)blockDim.x >= T * D / 32) continue;
+      uint32_t code[4][2];  // of each slot, eight dimensions
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t u = x[g][t][2 * w], v = x[g][t][2 * w + 1];
+          code[t][w] = f8_codes(__builtin_ldexpf(f16or_bf((uint16_t)u, BF), -e),
+                                __builtin_ldexpf(f16or_bf((uint16_t)(u >> 16), BF), -e),
+                                __builtin_ldexpf(f16or_bf((uint16_t)v, BF), -e),
+                                __builtin_ldexpf(f16or_bf((uint16_t)(v >> 16), BF), -e));
+        }
+      if (!val) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (s0 + t >= 0 && s0 + t < n)
+            *reinterpret_cast<uint2*>(dst + ((4 * sg[g] + t) << log_d) + 8 * ch[g]) =
+                make_uint2(code[t][0], code[t][1]);
+      } else {
+        const bool whole = s0 >= 0 && s0 + 3 < n;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          uint32_t u = 0;  // four slots of a dimension
+#pragma unroll
+          for (int t = 0; t < 4; ++t) u |= (code[t][d >> 2] >> (8 * (d & 3)) & 0xFFu) << (8 * t);
+          uint8_t* to = dst + ((8 * ch[g] + d) << log_t) + 4 * sg[g];
+          if (whole) {
+            *reinterpret_cast<uint32_t*>(to) = u;
+          } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              if (s0 + t >= 0 && s0 + t < n) to[t] = (uint8_t)(u >> (8 * t));
+          }
+        }
+      }
+    }
   }
 }
+
+// up to how many (row, KV head, keys or values) every row has a workgroup
+constexpr int64_t kWriteSingle = 8192;
 
 static bool plan_shape_ok(int64_t batch, int64_t width, int64_t t_b, int64_t free_cap,
                           int block_size) {
@@ -267,15 +478,21 @@ extern "C" int pe_write_blocks(const void* k, const void* v, int dtype, int64_t 
   a.v_h = v_h;
   a.slots = slots;
   a.rows = (int)rows;
-  const dim3 grid((unsigned)rows, (unsigned)kv_heads, 2);
+  a.log_d = head_dim == 64 ? 6 : head_dim == 128 ? 7 : 8;
+  a.per = rows * kv_heads * 2 <= kWriteSingle ? 1 : 16;
+  const dim3 grid((unsigned)((rows + a.per - 1) / a.per), (unsigned)kv_heads, 2);
+  const int groups = block_size * head_dim / 32;  // of 4 slots x 8 dimensions
+  const unsigned threads = groups < 64 ? 64 : groups < 256 ? groups : 256;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  switch (head_dim * 2 + bf) {
-    case 128: write_blocks_kernel<64, false><<<grid, 256, 0, st>>>(a); break;
-    case 129: write_blocks_kernel<64, true><<<grid, 256, 0, st>>>(a); break;
-    case 256: write_blocks_kernel<128, false><<<grid, 256, 0, st>>>(a); break;
-    case 257: write_blocks_kernel<128, true><<<grid, 256, 0, st>>>(a); break;
-    case 512: write_blocks_kernel<256, false><<<grid, 256, 0, st>>>(a); break;
-    default: write_blocks_kernel<256, true><<<grid, 256, 0, st>>>(a); break;
+  if (groups <= 256) {
+    if (bf) write_blocks_kernel<1, true><<<grid, threads, 0, st>>>(a);
+    else write_blocks_kernel<1, false><<<grid, threads, 0, st>>>(a);
+  } else if (groups <= 512) {
+    if (bf) write_blocks_kernel<2, true><<<grid, threads, 0, st>>>(a);
+    else write_blocks_kernel<2, false><<<grid, threads, 0, st>>>(a);
+  } else {
+    if (bf) write_blocks_kernel<4, true><<<grid, threads, 0, st>>>(a);
+    else write_blocks_kernel<4, false><<<grid, threads, 0, st>>>(a);
   }
   return launch_status();
 }
