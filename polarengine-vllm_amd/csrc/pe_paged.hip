@@ -1,13 +1,15 @@
 // The paged 8-bit cache: block tables and slot maps of a step, blocks back to the
 // pool, and the quantizing write of keys and values.
 
+#include <type_traits>
+
 #include "pe_paged.h"
 
 namespace pe {
 
 constexpr int kPlanThreads = 1024;
 
-// Running sums over a workgroup of 1024 in order of thread; `total` in every thread.
+// Running sums over a workgroup in order of thread; `total` in every thread.
 // Values and sums stop at kPlanCap, which is past any number of rows or blocks.
 constexpr uint32_t kPlanCap = 1u << 30;
 __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t* waves, uint32_t& total) {
@@ -22,7 +24,7 @@ __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t* waves, uint3
   __syncthreads();
   uint32_t before = 0;
   total = 0;
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
+  for (int w = 0; w < (int)blockDim.x / 64; ++w) {
     if (w < wave) before = min(before + waves[w], kPlanCap);
     total = min(total + waves[w], kPlanCap);
   }
@@ -36,19 +38,19 @@ __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t* waves, uint3
 // takes 64 at a time.
 // ---------------------------------------------------------------------------
 constexpr int kPlanShort = 4;
-constexpr int kPlanWaves = kPlanThreads / 64;
 
 // sequences of a round that have more than kPlanShort entries to look at
 struct PlanLong {
   uint32_t count;
   uint16_t of[kPlanThreads];
 };
-__device__ __forceinline__ void plan_long(PlanLong& l, bool mine) {
-  __syncthreads();
+__device__ __forceinline__ bool plan_long(PlanLong& l, bool mine) {
+  if (!__syncthreads_or(mine)) return false;
   if (threadIdx.x == 0) l.count = 0;
   __syncthreads();
   if (mine) l.of[atomicAdd(&l.count, 1u)] = (uint16_t)threadIdx.x;  // in any order
   __syncthreads();
+  return true;
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
     int64_t t_b, int batch, int64_t width, const int32_t* __restrict__ free_blocks, int64_t free_cap,
     int64_t* free_count, int rows, int log_t, int64_t* __restrict__ starts,
     int64_t* __restrict__ positions, int64_t* __restrict__ slots, int64_t* __restrict__ out_lengths) {
-  __shared__ uint32_t waves[kPlanWaves];
+  __shared__ uint32_t waves[kPlanThreads / 64];
   __shared__ uint32_t used;
   __shared__ PlanLong longs;
   __shared__ uint32_t needs[kPlanThreads];
@@ -66,13 +68,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
   constexpr int kNone = INT32_MIN;
   __shared__ int ends[kPagedMaxBatch], offsets[kPagedMaxBatch];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int threads = blockDim.x, n_waves = threads / 64;
   const uint32_t have = (uint32_t)max((int64_t)0, min(*free_count, free_cap));
   if (tid == 0) {
     starts[0] = 0;
     used = 0;
   }
   uint32_t row0 = 0, need0 = 0;  // of the sequences before this round's
-  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < batch; b0 += threads) {
     const int b = b0 + tid;
     const int64_t len = b < batch ? lengths[b] : -1;
     // a count past the rows is as good as one row more
@@ -92,8 +95,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
     const bool is_long = j1 - j0 >= kPlanShort;
     firsts[tid] = j0;
     lasts[tid] = j1;
-    plan_long(longs, is_long);
-    for (uint32_t k = wave; k < longs.count; k += kPlanWaves) {
+    const bool any_long = plan_long(longs, is_long);
+    for (uint32_t k = wave; any_long && k < longs.count; k += n_waves) {
       const int t = longs.of[k];
       const int32_t* r = tables + (int64_t)(b0 + t) * t_b;
       uint32_t lacks = 0;
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
         lacks += __builtin_popcountll(__ballot(j <= lasts[t] && r[min(j, lasts[t])] < 0));
       if (lane == 0) needs[t] = lacks;
     }
-    __syncthreads();
+    if (any_long) __syncthreads();
     if (is_long) need = needs[tid];
     const uint32_t cum = need0 + plan_scan(need, waves, total);
     need0 = min(need0 + total, kPlanCap);
@@ -121,7 +124,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
     needs[tid] = taken && need ? cum - need : UINT32_MAX;  // rank of the first block
     if (taken && need) atomicMax(&used, cum);
     __syncthreads();
-    for (uint32_t k = wave; k < longs.count; k += kPlanWaves) {
+    for (uint32_t k = wave; any_long && k < longs.count; k += n_waves) {
       const int t = longs.of[k];
       if (needs[t] == UINT32_MAX) continue;
       int32_t* r = tables + (int64_t)(b0 + t) * t_b;
@@ -133,51 +136,55 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
         at += __builtin_popcountll(all);
       }
     }
-    __syncthreads();
+    if (any_long) __syncthreads();
   }
   if (tid == 0) *free_count = (int64_t)have - used;
-  // four rows a thread at a time, so that their entries' loads go out together
-  constexpr int R = 4;
-  for (int r0 = tid; r0 < rows; r0 += R * kPlanThreads) {
-    int64_t pos[R], slot[R];
-    int32_t block[R];
+  // R rows a thread at a time, so that their entries' loads go out together
+  auto place = [&](auto R_) {
+    constexpr int R = decltype(R_)::value;
+    for (int r0 = tid; r0 < rows; r0 += R * threads) {
+      int64_t pos[R];
+      int32_t block[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = min(r0 + i * kPlanThreads, rows - 1);
-      int lo = 0, hi = batch;  // the first sequence that ends behind row r
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (ends[mid] > r) hi = mid;
-        else lo = mid + 1;
+      for (int i = 0; i < R; ++i) {
+        const int r = min(r0 + i * threads, rows - 1);
+        int lo = 0, hi = batch;  // the first sequence that ends behind row r
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (ends[mid] > r) hi = mid;
+          else lo = mid + 1;
+        }
+        const int off = lo < batch ? offsets[lo] : kNone;
+        pos[i] = off != kNone ? off + r : -1;
+        block[i] = off != kNone ? tables[lo * t_b + (pos[i] >> log_t)] : 0;
       }
-      const int off = lo < batch ? offsets[lo] : kNone;
-      pos[i] = off != kNone ? off + r : -1;
-      block[i] = off != kNone ? tables[lo * t_b + (pos[i] >> log_t)] : 0;
-    }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + i * kPlanThreads;
-      slot[i] = pos[i] >= 0 ? ((int64_t)block[i] << log_t) + (pos[i] & ((1 << log_t) - 1)) : -1;
-      if (r < rows) {
-        positions[r] = pos[i];
-        slots[r] = slot[i];
+      for (int i = 0; i < R; ++i) {
+        const int r = r0 + i * threads;
+        if (r < rows) {
+          positions[r] = pos[i];
+          slots[r] = pos[i] >= 0 ? ((int64_t)block[i] << log_t) + (pos[i] & ((1 << log_t) - 1)) : -1;
+        }
       }
     }
-  }
+  };
+  if (rows <= threads) place(std::integral_constant<int, 1>{});
+  else place(std::integral_constant<int, 8>{});
 }
 
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(
     int32_t* tables, int64_t t_b, int batch, int64_t width, const int64_t* __restrict__ keep,
     int32_t* __restrict__ free_blocks, int64_t free_cap, int64_t* free_count, int log_t) {
-  __shared__ uint32_t waves[kPlanWaves];
+  __shared__ uint32_t waves[kPlanThreads / 64];
   __shared__ PlanLong longs;
   __shared__ uint32_t ns[kPlanThreads], ats[kPlanThreads];
   __shared__ int64_t firsts[kPlanThreads];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int threads = blockDim.x, n_waves = threads / 64;
   const int64_t have = max((int64_t)0, min(*free_count, free_cap));
   int64_t first;
   int32_t entry[kPlanShort];
-  bool is_long;
+  bool is_long, any_long = false;
   // how many blocks of sequence b0 + tid go back; `longs` has those of more than kPlanShort
   auto count = [&](int b0) {
     const int b = b0 + tid;
@@ -191,8 +198,8 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(
     for (int i = 0; i < kPlanShort; ++i) n += n == (uint32_t)i && entry[i] >= 0;
     is_long = n == kPlanShort;
     firsts[tid] = first;
-    plan_long(longs, is_long);
-    for (uint32_t l = wave; l < longs.count; l += kPlanWaves) {
+    any_long = plan_long(longs, is_long);
+    for (uint32_t l = wave; any_long && l < longs.count; l += n_waves) {
       const int t = longs.of[l];
       const int32_t* r = tables + (int64_t)(b0 + t) * t_b;
       uint32_t m = 0;
@@ -203,20 +210,20 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(
       }
       if (lane == 0) ns[t] = m;
     }
-    __syncthreads();
+    if (any_long) __syncthreads();
     if (is_long) n = ns[tid];
     return n;
   };
   uint32_t all = 0, total, n = 0;
-  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < batch; b0 += threads) {
     n = count(b0);
     plan_scan(n, waves, total);
     all += total;
   }
   if (have + all > free_cap) return;
   uint32_t before = 0;
-  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
-    if (batch > kPlanThreads) n = count(b0);
+  for (int b0 = 0; b0 < batch; b0 += threads) {
+    if (batch > threads) n = count(b0);
     const uint32_t at = before + plan_scan(n, waves, total) - n;
     before += total;
     int32_t* row = tables + (int64_t)(b0 + tid) * t_b + first;
@@ -230,10 +237,11 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(
           row[i] = -1;
         }
     }
+    if (!any_long) continue;
     ats[tid] = at;
     ns[tid] = n;
     __syncthreads();
-    for (uint32_t l = wave; l < longs.count; l += kPlanWaves) {
+    for (uint32_t l = wave; l < longs.count; l += n_waves) {
       const int t = longs.of[l];
       int32_t* r = tables + (int64_t)(b0 + t) * t_b + firsts[t];
       for (uint32_t i = lane; i < ns[t]; i += 64) {
@@ -248,8 +256,8 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(
 
 // ---------------------------------------------------------------------------
 // The write. A workgroup looks for runs that begin among its `per` rows (one in a
-// decode step, so that every token has a workgroup; 16 in a prompt) and takes those of
-// one KV head, keys or values, one after the other. A thread holds 4 slots x 8
+// decode step, so that every token has a workgroup; up to 32 in a prompt) and takes
+// those of one KV head, keys or values, one after the other. A thread holds 4 slots x 8
 // dimensions: the run is read once, its largest |x| gives the scale, then codes go out.
 // Threads of a wave run over dimensions first for keys (rows of the block) and over
 // slots first for values (which the block stores by dimension), so that either writes
@@ -283,33 +291,40 @@ struct WriteArgs {
   int rows, per, log_d;
 };
 
-template <int G, bool BF>
-__global__ __launch_bounds__(256) void write_blocks_kernel(const WriteArgs a) {
-  __shared__ float red[4];
+template <bool BF, int THREADS>
+__global__ __launch_bounds__(THREADS, THREADS <= 256 ? 6 : 4) void write_blocks_kernel(const WriteArgs a) {
+  __shared__ float red[THREADS / 64];
   const int h = blockIdx.y;
   const bool val = blockIdx.z;
   const int log_t = a.c.log_t, T = 1 << log_t, log_d = a.log_d, D = 1 << log_d;
   const int tid = threadIdx.x, lane = tid & 63;
   const int row0 = blockIdx.x * a.per;
   const int64_t n_slots = a.c.blocks << log_t;
-  // rows that begin a run, a lane each
-  uint64_t begins;
-  {
-    const int r = min(row0 + lane, a.rows - 1);
-    const int64_t slot = a.slots[r], prev = a.slots[max(r - 1, 0)];
-    const bool within = r > 0 && prev == slot - 1 && (slot & (T - 1));
-    begins = __ballot(lane < a.per && row0 + lane < a.rows && slot >= 0 && slot < n_slots && !within);
-  }
+  // the thread's part of a block: slots 4 sg .. + 3 and dimensions 8 ch .. + 7
+  const int sg = val ? tid & ((T >> 2) - 1) : tid >> (log_d - 3);
+  const int ch = val ? tid >> (log_t - 2) : tid & ((D >> 3) - 1);
+  const bool in = tid < T * D / 32;
+  // 64 rows' slots, a lane each: which of the first `per` rows begin a run
+  const int64_t mine = a.slots[min(row0 + lane, a.rows - 1)];
+  int64_t prev = __shfl_up((long long)mine, 1, 64);
+  if (lane == 0) prev = row0 ? a.slots[row0 - 1] : -1;
+  const bool within = row0 + lane > 0 && prev == mine - 1 && (mine & (T - 1));
+  const bool valid = row0 + lane < a.rows && mine >= 0 && mine < n_slots;
+  uint64_t begins = __ballot(lane < a.per && valid && !within);
+  const uint64_t on = __ballot(valid && within);  // goes on what the row before it does
   for (; begins; begins &= begins - 1) {
-    const int row = row0 + __builtin_ctzll(begins);
-    const int64_t slot = a.slots[row];
+    const int l = __builtin_ctzll(begins), row = row0 + l;
+    const int64_t slot = __shfl((long long)mine, l, 64);
     const int off = (int)(slot & (T - 1));
-    int n = 1;  // rows of the run
-    for (int i0 = 1; n == i0 && off + n < T; i0 += 64) {
+    const uint64_t rest = l < 63 ? ~(on >> (l + 1)) : ~0ull;
+    int n = 1 + (rest ? __builtin_ctzll(rest) : 64);  // rows of the run
+    n = min(n, 64 - l);
+    // on behind the 64
+    for (int i0 = 64 - l; n == i0 && off + n < T; i0 += 64) {
       const int i = i0 + lane;
-      const uint64_t on = __ballot(off + i < T && row + i < a.rows &&
-                                   a.slots[min(row + i, a.rows - 1)] == slot + i);
-      n += ~on ? __builtin_ctzll(~on) : 64;
+      const uint64_t more = __ballot(off + i < T && row + i < a.rows &&
+                                     a.slots[min(row + i, a.rows - 1)] == slot + i);
+      n += ~more ? __builtin_ctzll(~more) : 64;
     }
     const int64_t block = slot >> log_t;
     const uint16_t* src = val ? a.v + row * a.v_r + h * a.v_h : a.k + row * a.k_r + h * a.k_h;
@@ -317,35 +332,26 @@ __global__ __launch_bounds__(256) void write_blocks_kernel(const WriteArgs a) {
     uint8_t* dst = (val ? a.c.v + block * a.c.v_b : a.c.k + block * a.c.k_b) + ((int64_t)h << (log_t + log_d));
     uint8_t* scale = (val ? a.c.vs : a.c.ks) + block * a.c.s_b + h;
     const int old = (int)*scale - 127;
-    // the thread's groups: slots 4 sg .. + 3 and dimensions 8 ch .. + 7
-    int sg[G], ch[G];
-    u32x4v x[G][4];
+    const int s0 = 4 * sg - off;  // of the run's rows
+    const bool act = in && s0 + 3 >= 0 && s0 < n;
+    u32x4v x[4];
     float amax = 0.f;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int i = tid + g * (int)blockDim.x;
-      sg[g] = val ? i & ((T >> 2) - 1) : i >> (log_d - 3);
-      ch[g] = val ? i >> (log_t - 2) : i & ((D >> 3) - 1);
-      const bool in = i < T * D / 32;
+    if (act) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int rel = 4 * sg[g] + t - off;
-        x[g][t] = u32x4v{0, 0, 0, 0};
-        if (in && rel >= 0 && rel < n)
-          x[g][t] = *reinterpret_cast<const u32x4v*>(src + rel * s_r + 8 * ch[g]);
+        x[t] = u32x4v{0, 0, 0, 0};
+        if (s0 + t >= 0 && s0 + t < n) x[t] = *reinterpret_cast<const u32x4v*>(src + (s0 + t) * s_r + 8 * ch);
       }
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t u = x[g][t][w];
+          const uint32_t u = x[t][w];
           const float lo = fabsf(f16or_bf((uint16_t)u, BF)), hi = fabsf(f16or_bf((uint16_t)(u >> 16), BF));
           amax = fmaxf(amax, lo <= 3.4e38f ? lo : 0.f);
           amax = fmaxf(amax, hi <= 3.4e38f ? hi : 0.f);
         }
+    }
 #pragma unroll
     for (int m = 32; m; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
     __syncthreads();  // the last run's sums and stores are done with
@@ -368,50 +374,45 @@ __global__ __launch_bounds__(256) void write_blocks_kernel(const WriteArgs a) {
       __syncthreads();
     }
     if (tid == 0) *scale = (uint8_t)(e + 127);
+    if (!act) continue;
+    uint32_t code[4][2];  // of each slot, eight dimensions
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int s0 = 4 * sg[g] - off;  // of the run's rows
-      if (s0 + 3 < 0 || s0 >= n || tid + g * (int)blockDim.x >= T * D / 32) continue;
-      uint32_t code[4][2];  // of each slot, eight dimensions
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t u = x[t][2 * w], v = x[t][2 * w + 1];
+        code[t][w] = f8_codes(__builtin_ldexpf(f16or_bf((uint16_t)u, BF), -e),
+                              __builtin_ldexpf(f16or_bf((uint16_t)(u >> 16), BF), -e),
+                              __builtin_ldexpf(f16or_bf((uint16_t)v, BF), -e),
+                              __builtin_ldexpf(f16or_bf((uint16_t)(v >> 16), BF), -e));
+      }
+    if (!val) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
+        if (s0 + t >= 0 && s0 + t < n)
+          *reinterpret_cast<uint2*>(dst + ((4 * sg + t) << log_d) + 8 * ch) = make_uint2(code[t][0], code[t][1]);
+    } else {
+      const bool whole = s0 >= 0 && s0 + 3 < n;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t u = x[g][t][2 * w], v = x[g][t][2 * w + 1];
-          code[t][w] = f8_codes(__builtin_ldexpf(f16or_bf((uint16_t)u, BF), -e),
-                                __builtin_ldexpf(f16or_bf((uint16_t)(u >> 16), BF), -e),
-                                __builtin_ldexpf(f16or_bf((uint16_t)v, BF), -e),
-                                __builtin_ldexpf(f16or_bf((uint16_t)(v >> 16), BF), -e));
-        }
-      if (!val) {
+      for (int d = 0; d < 8; ++d) {
+        uint32_t u = 0;  // four slots of a dimension
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (s0 + t >= 0 && s0 + t < n)
-            *reinterpret_cast<uint2*>(dst + ((4 * sg[g] + t) << log_d) + 8 * ch[g]) =
-                make_uint2(code[t][0], code[t][1]);
-      } else {
-        const bool whole = s0 >= 0 && s0 + 3 < n;
+        for (int t = 0; t < 4; ++t) u |= (code[t][d >> 2] >> (8 * (d & 3)) & 0xFFu) << (8 * t);
+        uint8_t* to = dst + ((8 * ch + d) << log_t) + 4 * sg;
+        if (whole) {
+          *reinterpret_cast<uint32_t*>(to) = u;
+        } else {
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          uint32_t u = 0;  // four slots of a dimension
-#pragma unroll
-          for (int t = 0; t < 4; ++t) u |= (code[t][d >> 2] >> (8 * (d & 3)) & 0xFFu) << (8 * t);
-          uint8_t* to = dst + ((8 * ch[g] + d) << log_t) + 4 * sg[g];
-          if (whole) {
-            *reinterpret_cast<uint32_t*>(to) = u;
-          } else {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-              if (s0 + t >= 0 && s0 + t < n) to[t] = (uint8_t)(u >> (8 * t));
-          }
+          for (int t = 0; t < 4; ++t)
+            if (s0 + t >= 0 && s0 + t < n) to[t] = (uint8_t)(u >> (8 * t));
         }
       }
     }
   }
 }
 
-// up to how many (row, KV head, keys or values) every row has a workgroup
-constexpr int64_t kWriteSingle = 8192;
+// workgroups that a write is cut into, by giving each of them up to 32 rows
+constexpr int64_t kWriteWgs = 4096;
 
 static bool plan_shape_ok(int64_t batch, int64_t width, int64_t t_b, int64_t free_cap,
                           int block_size) {
@@ -419,6 +420,8 @@ static bool plan_shape_ok(int64_t batch, int64_t width, int64_t t_b, int64_t fre
   return batch >= 0 && batch <= kPagedMaxBatch && width >= 1 && width <= kPagedMaxWidth &&
          t_b >= width && free_cap >= 1 && free_cap <= INT32_MAX;
 }
+// a small plan's barriers are cheaper among four waves
+static unsigned plan_threads(int64_t items) { return items <= 256 ? 256 : kPlanThreads; }
 static int log2_of(int block_size) {
   return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
 }
@@ -438,7 +441,7 @@ extern "C" int pe_plan_step(const int64_t* lengths, const int64_t* counts, int32
   if (!plan_shape_ok(batch, width, t_b, free_cap, block_size) || rows < 0 || rows > kPagedMaxRows)
     return PE_ERR_DIMS;
   if (batch == 0) return PE_OK;
-  plan_step_kernel<<<1, kPlanThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(
+  plan_step_kernel<<<1, plan_threads(batch > rows ? batch : rows), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       lengths, counts, tables, t_b, (int)batch, width, free_blocks, free_cap, free_count, (int)rows,
       log2_of(block_size), starts, positions, slots, out_lengths);
   return launch_status();
@@ -450,7 +453,7 @@ extern "C" int pe_release_blocks(int32_t* tables, int64_t t_b, int64_t batch, in
   if (!tables || !keep || !free_blocks || !free_count) return PE_ERR_NULL;
   if (!plan_shape_ok(batch, width, t_b, free_cap, block_size)) return PE_ERR_DIMS;
   if (batch == 0) return PE_OK;
-  release_kernel<<<1, kPlanThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(
+  release_kernel<<<1, plan_threads(batch), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       tables, t_b, (int)batch, width, keep, free_blocks, free_cap, free_count, log2_of(block_size));
   return launch_status();
 }
@@ -479,20 +482,18 @@ extern "C" int pe_write_blocks(const void* k, const void* v, int dtype, int64_t 
   a.slots = slots;
   a.rows = (int)rows;
   a.log_d = head_dim == 64 ? 6 : head_dim == 128 ? 7 : 8;
-  a.per = rows * kv_heads * 2 <= kWriteSingle ? 1 : 16;
+  const int64_t per = (rows * kv_heads * 2 + kWriteWgs - 1) / kWriteWgs;
+  a.per = (int)(per < 32 ? per : 32);
   const dim3 grid((unsigned)((rows + a.per - 1) / a.per), (unsigned)kv_heads, 2);
-  const int groups = block_size * head_dim / 32;  // of 4 slots x 8 dimensions
-  const unsigned threads = groups < 64 ? 64 : groups < 256 ? groups : 256;
+  const int parts = block_size * head_dim / 32;  // of 4 slots x 8 dimensions: a thread each
+  const unsigned threads = parts < 64 ? 64 : parts;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (groups <= 256) {
-    if (bf) write_blocks_kernel<1, true><<<grid, threads, 0, st>>>(a);
-    else write_blocks_kernel<1, false><<<grid, threads, 0, st>>>(a);
-  } else if (groups <= 512) {
-    if (bf) write_blocks_kernel<2, true><<<grid, threads, 0, st>>>(a);
-    else write_blocks_kernel<2, false><<<grid, threads, 0, st>>>(a);
+  if (threads <= 256) {
+    if (bf) write_blocks_kernel<true, 256><<<grid, threads, 0, st>>>(a);
+    else write_blocks_kernel<false, 256><<<grid, threads, 0, st>>>(a);
   } else {
-    if (bf) write_blocks_kernel<4, true><<<grid, threads, 0, st>>>(a);
-    else write_blocks_kernel<4, false><<<grid, threads, 0, st>>>(a);
+    if (bf) write_blocks_kernel<true, 1024><<<grid, threads, 0, st>>>(a);
+    else write_blocks_kernel<false, 1024><<<grid, threads, 0, st>>>(a);
   }
   return launch_status();
 }

@@ -53,6 +53,7 @@ struct PagedAttnArgs {
   float scale;
   int runs;
   float* parts;  // [runs][2]: a run divides at most its first and its last row block
+  struct PaCut* cuts;  // [runs], behind the parts
 };
 
 // fp32 words of one part: RB x D sums, RB maxima, RB sums
@@ -124,53 +125,80 @@ __device__ __forceinline__ int64_t pa_scan(int64_t v, int lane) {
 struct PaPlace {
   int b, kvh, qb, t0;  // and the tile of the row block
   int tiles;
+  PaSeq seq;
 };
-// one wave: the length of the line
+// 64 sequences, one a lane: tiles of a KV head
+template <int RB>
+struct PaChunk {
+  PaSeq seq;
+  int64_t tiles;
+};
 template <int RB, int TILE>
-__device__ __forceinline__ int64_t pa_total(const PagedAttnArgs& a, int lane) {
-  int64_t sum = 0;
-  for (int b0 = 0; b0 <= a.batch; b0 += 64) sum += pa_tiles<RB, TILE>(a, pa_seq<RB>(a, b0 + lane));
+__device__ __forceinline__ PaChunk<RB> pa_chunk(const PagedAttnArgs& a, int b0, int lane) {
+  PaChunk<RB> c;
+  c.seq = pa_seq<RB>(a, b0 + lane);
+  c.tiles = pa_tiles<RB, TILE>(a, c.seq);
+  return c;
+}
+__device__ __forceinline__ int64_t pa_from(int64_t v, int lane) { return __shfl((long long)v, lane, 64); }
+// one wave: the length of the line; c: the first chunk
+template <int RB, int TILE>
+__device__ __forceinline__ int64_t pa_total(const PagedAttnArgs& a, const PaChunk<RB>& c, int lane) {
+  int64_t sum = c.tiles;
+  for (int b0 = 64; b0 <= a.batch; b0 += 64) sum += pa_chunk<RB, TILE>(a, b0, lane).tiles;
 #pragma unroll
   for (int m = 32; m; m >>= 1) sum += __shfl_xor((long long)sum, m, 64);
   return sum * a.c.kv_heads;
 }
 // one wave: what holds place `at` of the line (all lanes; at below the total)
 template <int RB, int TILE>
-__device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, int64_t at, int lane) {
-  PaPlace r{-1, 0, 0, 0, 0};
+__device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, PaChunk<RB> c, int64_t at, int lane) {
+  PaPlace r{-1, 0, 0, 0, 0, {}};
   int64_t before = 0;
   for (int b0 = 0; b0 <= a.batch; b0 += 64) {
-    const int64_t mine = pa_tiles<RB, TILE>(a, pa_seq<RB>(a, b0 + lane));
-    const int64_t scan = pa_scan(mine, lane);
+    if (b0) c = pa_chunk<RB, TILE>(a, b0, lane);
+    const int64_t scan = pa_scan(c.tiles, lane);
     const uint64_t hit = __ballot((before + scan) * a.c.kv_heads > at);
     if (!hit) {
-      before += __shfl((long long)scan, 63, 64);
+      before += pa_from(scan, 63);
       continue;
     }
     const int l = __builtin_ctzll(hit);
-    const int64_t tiles = __shfl((long long)mine, l, 64);
-    at -= (before + __shfl((long long)scan, l, 64) - tiles) * a.c.kv_heads;
-    r.b = b0 + l;
+    const int64_t tiles = pa_from(c.tiles, l);
+    at -= (before + pa_from(scan, l) - tiles) * a.c.kv_heads;
     r.kvh = (int)(at / tiles);
     at -= r.kvh * tiles;
-    const PaSeq s = pa_seq<RB>(a, r.b);
+    PaSeq& s = r.seq;
+    s.first = __shfl(c.seq.first, l, 64);
+    s.n = __shfl(c.seq.n, l, 64);
+    s.lead = __shfl(c.seq.lead, l, 64);
+    s.p0 = pa_from(c.seq.p0, l);
+    s.blocks = __shfl(c.seq.blocks, l, 64);
     for (int q0 = 0; q0 < s.blocks; q0 += 64) {
       const int64_t t = q0 + lane < s.blocks ? pa_span<RB, TILE>(a, s, q0 + lane).tiles : 0;
       const int64_t sc = pa_scan(t, lane);
       const uint64_t in = __ballot(sc > at);
       if (in) {
         const int k = __builtin_ctzll(in);
+        r.b = b0 + l;
         r.qb = q0 + k;
-        r.tiles = (int)__shfl((long long)t, k, 64);
-        r.t0 = (int)(at - (__shfl((long long)sc, k, 64) - r.tiles));
+        r.tiles = (int)pa_from(t, k);
+        r.t0 = (int)(at - (pa_from(sc, k) - r.tiles));
         return r;
       }
-      at -= __shfl((long long)sc, 63, 64);
+      at -= pa_from(sc, 63);
     }
-    break;
+    return r;
   }
-  r.b = -1;  // only if the lengths change under the kernel
-  return r;
+  return r;  // only if the lengths change under the kernel
+}
+// a place that one wave found, in every thread
+__device__ __forceinline__ int pa_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ PaPlace pa_place(const PaPlace& p) {
+  const uint32_t lo = pa_uniform((int)(uint32_t)p.seq.p0), hi = pa_uniform((int)(uint32_t)((uint64_t)p.seq.p0 >> 32));
+  return PaPlace{pa_uniform(p.b), pa_uniform(p.kvh), pa_uniform(p.qb), pa_uniform(p.t0), pa_uniform(p.tiles),
+                 PaSeq{pa_uniform(p.seq.first), pa_uniform(p.seq.n), pa_uniform(p.seq.lead),
+                       (int64_t)((uint64_t)hi << 32 | lo), pa_uniform(p.seq.blocks)}};
 }
 
 // ---------------------------------------------------------------------------
@@ -228,17 +256,39 @@ __device__ __forceinline__ uint32_t pa_nan(uint32_t w) {
 // the bits of positions below n, of 16
 __device__ __forceinline__ uint32_t pa_below(int n) { return (1u << min(max(n, 0), 16)) - 1; }
 
+// What the second launch has to know of a run: the row block that begins in it and goes
+// on behind it.
+struct PaCut {
+  int parts;  // runs that it lies in; 0: there is none
+  int first, n;  // rows of its sequence
+  int kvh, qb;
+};
 // The runs of a launch: this workgroup's, in tiles of the line. The runs of an XCD are
 // neighbours, which share keys and values.
 struct PaRun {
-  int64_t run, at, end;  // at >= end: none
+  int64_t run, at, end, size;  // at >= end: none
 };
 __device__ __forceinline__ PaRun pa_run(const PagedAttnArgs& a, int64_t total) {
   const int64_t size = (total + a.runs - 1) / a.runs;
   const int64_t active = (total + size - 1) / size, per = (active + 7) / 8;
-  const int64_t run = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || run >= active) return PaRun{0, 0, 0};
-  return PaRun{run, run * size, min(total, (run + 1) * size)};
+  const int64_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
+  // workgroups that are not needed get the numbers behind
+  const int64_t run = y < per ? x * per + y : 8 * per + (y - per) * 8 + x;
+  if (run < a.runs && threadIdx.x == 0 && a.cuts) a.cuts[run].parts = 0;
+  if (run >= active) return PaRun{run, 0, 0, size};
+  return PaRun{run, run * size, min(total, (run + 1) * size), size};
+}
+// where the row block at tiles t0 .. t1 of `tiles` puts its sums: null if it is whole.
+// A part: the run's first row block, begun before it, or its last, which goes on.
+__device__ __forceinline__ float* pa_part(const PagedAttnArgs& a, const PaRun& run, const PaPlace& p, int t1,
+                                          int64_t words) {
+  if (p.t0 == 0 && t1 == p.tiles) return nullptr;
+  if (p.t0 == 0 && threadIdx.x == 0) {
+    const int64_t start = run.end - t1;
+    a.cuts[run.run] = PaCut{(int)((start + p.tiles - 1) / run.size - run.run) + 1, p.seq.first, p.seq.n,
+                            p.kvh, p.qb};
+  }
+  return a.parts + (run.run * 2 + (p.t0 == 0)) * words;
 }
 
 // What a wave keeps of RT products of 16 rows.
@@ -479,8 +529,10 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
   __shared__ int64_t line;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  PaChunk<RB> chunk{};
   if (wave == 0) {
-    const int64_t total = pa_total<RB, TILE>(a, lane);
+    chunk = pa_chunk<RB, TILE>(a, 0, lane);
+    const int64_t total = pa_total<RB, TILE>(a, chunk, lane);
     if (lane == 0) line = total;
   }
   __syncthreads();
@@ -488,19 +540,16 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 
   for (int64_t at = run.at; at < run.end;) {
     if (wave == 0) {
-      const PaPlace p = pa_find<RB, TILE>(a, at, lane);
+      const PaPlace p = pa_find<RB, TILE>(a, chunk, at, lane);
       if (lane == 0) place = p;
     }
     __syncthreads();
-    const int b = __builtin_amdgcn_readfirstlane(place.b);
-    const int kvh = __builtin_amdgcn_readfirstlane(place.kvh);
-    const int qb = __builtin_amdgcn_readfirstlane(place.qb);
-    const int t0 = __builtin_amdgcn_readfirstlane(place.t0);
-    const int tiles = __builtin_amdgcn_readfirstlane(place.tiles);
+    const PaPlace here = pa_place(place);
+    const int b = here.b, kvh = here.kvh, qb = here.qb, t0 = here.t0;
     if (b < 0) return;
-    const int t1 = (int)min((int64_t)tiles, t0 + (run.end - at));
+    const int t1 = (int)min((int64_t)here.tiles, t0 + (run.end - at));
     at += t1 - t0;
-    const PaSeq seq = pa_seq<RB>(a, b);
+    const PaSeq seq = here.seq;
     const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
     // positions of the block's first and last row (of fewer rows, if some are absent)
@@ -640,9 +689,7 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) w.o[rt][dt] += join[0][(rt * DT + dt) * 64 + lane];
       }
-      // a part: the run's first row block, begun before it, or its last, which goes on
-      float* part = t0 == 0 && t1 == tiles ? nullptr
-                                           : a.parts + (run.run * 2 + (t0 == 0)) * pa_part_words(RB, D);
+      float* part = pa_part(a, run, here, t1, pa_part_words(RB, D));
       w.template store<BF, RB>(a, seq, kvh, qb, 0, part, li, lg);
     }
     __syncthreads();  // the buffers are free
@@ -670,8 +717,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
   __shared__ int64_t line;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  PaChunk<RB> chunk{};
   if (wave == 0) {
-    const int64_t total = pa_total<RB, TILE>(a, lane);
+    chunk = pa_chunk<RB, TILE>(a, 0, lane);
+    const int64_t total = pa_total<RB, TILE>(a, chunk, lane);
     if (lane == 0) line = total;
   }
   __syncthreads();
@@ -679,19 +728,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
 
   for (int64_t at = run.at; at < run.end;) {
     if (wave == 0) {
-      const PaPlace p = pa_find<RB, TILE>(a, at, lane);
+      const PaPlace p = pa_find<RB, TILE>(a, chunk, at, lane);
       if (lane == 0) place = p;
     }
     __syncthreads();
-    const int b = __builtin_amdgcn_readfirstlane(place.b);
-    const int kvh = __builtin_amdgcn_readfirstlane(place.kvh);
-    const int qb = __builtin_amdgcn_readfirstlane(place.qb);
-    const int t0 = __builtin_amdgcn_readfirstlane(place.t0);
-    const int tiles = __builtin_amdgcn_readfirstlane(place.tiles);
+    const PaPlace here = pa_place(place);
+    const int b = here.b, kvh = here.kvh, qb = here.qb, t0 = here.t0;
     if (b < 0) return;
-    const int t1 = (int)min((int64_t)tiles, t0 + (run.end - at));
+    const int t1 = (int)min((int64_t)here.tiles, t0 + (run.end - at));
     at += t1 - t0;
-    const PaSeq seq = pa_seq<RB>(a, b);
+    const PaSeq seq = here.seq;
     const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
     // the wave's rows, and positions of the first and the last of them
@@ -823,8 +869,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
       if (i < t1) step(buf1, buf0);
     }
     w.finish();
-    float* part = t0 == 0 && t1 == tiles ? nullptr
-                                         : a.parts + (run.run * 2 + (t0 == 0)) * pa_part_words(RB, D);
+    float* part = pa_part(a, run, here, t1, pa_part_words(RB, D));
     w.template store<BF, RB>(a, seq, kvh, qb, wave * 16 * RT, part, li, lg);
     __syncthreads();  // the buffers are free
   }
@@ -834,41 +879,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
 // The row block that begins in a run and goes on behind it: out = sum of its parts,
 // each weighted exp2(m_part - m) / l, in order. A wave a row, lane = dimensions.
 // ---------------------------------------------------------------------------
-template <int D, bool BF, int RB, int TILE>
+template <int D, bool BF, int RB>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
   constexpr int E = D / 64, U = 8;
   typedef float floatE __attribute__((ext_vector_type(E)));
-  __shared__ PaPlace place;
-  __shared__ int64_t line;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (wave == 0) {
-    const int64_t t = pa_total<RB, TILE>(a, lane);
-    const int64_t size = (t + a.runs - 1) / a.runs, end = ((int64_t)blockIdx.x + 1) * size;
-    PaPlace p{-1, 0, 0, 0, 0};
-    if (end < t) {
-      p = pa_find<RB, TILE>(a, end, lane);
-      // the block that holds the next run's first tile: begun in this run?
-      if (p.t0 == 0 || end - p.t0 < (int64_t)blockIdx.x * size) p.b = -1;
-    }
-    if (lane == 0) {
-      place = p;
-      line = size;
-    }
-  }
-  __syncthreads();
-  if (place.b < 0) return;
-  const int64_t size = line, run = blockIdx.x;
-  const int64_t start = (run + 1) * size - place.t0;
-  const int parts = (int)((start + place.tiles - 1) / size - run) + 1;
-  const PaSeq seq = pa_seq<RB>(a, place.b);
+  const int64_t run = blockIdx.x;
+  const int local = blockIdx.y * 4 + wave;
+  const PaCut cut = a.cuts[run];
+  const int parts = cut.parts;
+  if (!parts) return;
   const int64_t words = pa_part_words(RB, D);
   const float* base = a.parts + run * 2 * words;
   // the first part is its run's last, the others are their runs' first
   auto part = [&](int s) { return base + s * 2 * words + (s == 0 ? words : 0); };
-  for (int local = blockIdx.y * 4 + wave; local < RB; local += 4 * gridDim.y) {
-    const int64_t r = (int64_t)place.qb * RB + local;
+  {
+    const int64_t r = (int64_t)cut.qb * RB + local;
     const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
-    if (token >= seq.n) return;
+    if (token >= cut.n) return;
     float m = -__builtin_inff(), l = 0.f;
     floatE o = 0.f;
     for (int s0 = 0; s0 < parts; s0 += 64) {
@@ -899,8 +927,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     uint16_t h[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) h[e] = to16(o[e] * inv, BF);
-    uint16_t* dst = a.out + ((int64_t)(seq.first + token) * a.c.kv_heads * a.group +
-                             place.kvh * a.group + g) * D + lane * E;
+    uint16_t* dst = a.out + ((int64_t)(cut.first + token) * a.c.kv_heads * a.group + cut.kvh * a.group + g) * D +
+                    lane * E;
     __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
   }
 }
@@ -934,7 +962,7 @@ static bool pa_shape_ok(int64_t rows, int64_t batch, int heads, int kv_heads, in
 template <int D, bool BF>
 static int launch_pa(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
   const unsigned grid = (unsigned)((p.runs + 7) / 8 * 8);
-  const dim3 join((unsigned)p.runs, 4);
+  const dim3 join((unsigned)p.runs, (unsigned)p.rb / 4);
   switch (p.rb) {
     case 16: paged_attn_kernel<D, BF, 1><<<grid, 256, 0, st>>>(a); break;
     case 32: paged_attn_kernel<D, BF, 2><<<grid, 256, 0, st>>>(a); break;
@@ -943,9 +971,9 @@ static int launch_pa(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
   const int rc = launch_status();
   if (rc != PE_OK || !p.split) return rc;
   switch (p.rb) {
-    case 16: paged_join_kernel<D, BF, 16, 256><<<join, 256, 0, st>>>(a); break;
-    case 32: paged_join_kernel<D, BF, 32, 256><<<join, 256, 0, st>>>(a); break;
-    default: paged_join_kernel<D, BF, 128, 64><<<join, 256, 0, st>>>(a); break;
+    case 16: paged_join_kernel<D, BF, 16><<<join, 256, 0, st>>>(a); break;
+    case 32: paged_join_kernel<D, BF, 32><<<join, 256, 0, st>>>(a); break;
+    default: paged_join_kernel<D, BF, 128><<<join, 256, 0, st>>>(a); break;
   }
   return launch_status();
 }
@@ -959,7 +987,7 @@ extern "C" size_t pe_paged_attention_workspace_size(int64_t rows, int64_t batch,
   if (!pa_shape_ok(rows, batch, heads, kv_heads, head_dim) || rows < 1 || batch < 1 || positions < 1)
     return 0;
   const PaPlan p = pa_plan(rows, batch, heads, kv_heads, head_dim, positions);
-  return p.split ? (size_t)p.runs * 2 * pa_part_words(p.rb, head_dim) * 4 : 0;
+  return p.split ? (size_t)p.runs * (2 * pa_part_words(p.rb, head_dim) * 4 + sizeof(PaCut)) : 0;
 }
 
 extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t rows, int heads,
@@ -1005,6 +1033,8 @@ extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t
   a.scale = scale;
   a.runs = p.runs;
   a.parts = reinterpret_cast<float*>(workspace);
+  a.cuts = p.split ? reinterpret_cast<PaCut*>(a.parts + (int64_t)p.runs * 2 * pa_part_words(p.rb, head_dim))
+                   : nullptr;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (head_dim * 2 + bf) {
     case 128: return launch_pa<64, false>(p, a, st);
