@@ -13,7 +13,7 @@ residual stream, and a bf16 lm_head (vLLM keeps embeddings and lm_head
 unquantized unless a checkpoint quantizes them). Residual add + norm,
 attention (with the rotary embedding and the cache write) and SiLU * up run
 on the library's decode kernels where their shapes fit, else in torch. There
-is no scheduler, sampler beyond argmax, paged cache or tokenizer.
+is no scheduler, sampler beyond argmax or tokenizer.
 
 One decode step (``DecodeRunner.step``) takes the batch's current tokens and
 position (device tensors, so the step can be captured in a HIP graph and
@@ -22,6 +22,9 @@ the argmax fed back. ``DecodeRunner.tree_step`` takes several drafted tokens per
 sequence (a chain or a tree, sequences of different lengths) through the same
 layers, ``DecodeRunner.speculative_round`` verifies them, moves what stands to its
 place in the cache and returns the new tokens (kernels.tree_decode).
+``DecodeRunner.paged_step`` takes chunks of prompts and single tokens of sequences of
+different lengths together, over a paged cache in 8 bits (kernels.paged_cache), and
+``DecodeRunner.score`` the log probabilities of a prompt's tokens (kernels.logprobs).
 """
 
 from __future__ import annotations
@@ -35,7 +38,8 @@ import torch
 from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
-from polarengine_vllm.kernels import tree_decode
+from polarengine_vllm.kernels import paged_cache, tree_decode
+from polarengine_vllm.kernels.logprobs import TokenLogprobs, token_logprobs
 from polarengine_vllm.linear_method import PolarQuantLinearMethod
 
 
@@ -212,8 +216,9 @@ class DecodeRunner:
         [B, vocab]."""
         return self._layers(tokens, self._attention(pos))
 
-    def _layers(self, tokens: torch.Tensor, attend) -> torch.Tensor:
-        """All layers and the lm_head for rows of tokens, with a step's attention."""
+    def _layers(self, tokens: torch.Tensor, attend, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """All layers for rows of tokens, with a step's attention, and the lm_head (of
+        ``rows`` alone if they are given)."""
         c = self.cfg
         x = self.embed.index_select(0, tokens)  # residual stream, bf16
         r = None  # what the last block adds to the residual stream
@@ -222,6 +227,8 @@ class DecodeRunner:
             o = attend(i, ly["qkv_proj"](h))
             x, h = _add_norm(x, ly["o_proj"](o), ly["post_norm"], c.rms_eps)
             r = ly["down_proj"](_silu_mul(ly["gate_up_proj"](h)))
+        if rows is not None:
+            x, r = x.index_select(0, rows), None if r is None else r.index_select(0, rows)
         x, h = _add_norm(x, r, self.final_norm, c.rms_eps)
         return _lm_head(h, self.lm_head)  # [rows, vocab]
 
@@ -267,6 +274,65 @@ class DecodeRunner:
         tree_decode.keep_accepted(self.k_cache.transpose(-1, -2), self.v_cache, lengths, path, count)
         lengths.add_(count)
         return out, path, count
+
+    def paged_pool(self, blocks: int, batch: int, block_size: int = 64) -> paged_cache.PagedPool:
+        """A paged 8-bit cache for this model: ``blocks`` blocks for up to ``batch``
+        sequences of ``max_len`` positions at a time."""
+        c = self.cfg
+        return paged_cache.PagedPool(c.layers, blocks, c.kv_heads, c.head_dim, batch, self.max_len,
+                                     self.dev, block_size)
+
+    def paged_step(self, tokens: torch.Tensor, counts: torch.Tensor, pool: paged_cache.PagedPool,
+                   window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
+        """One step for ``counts[b]`` tokens (int64 [batch]) of each sequence of the pool,
+        packed in ``tokens`` (int64 [rows]; rows behind the last sequence's are left
+        out): chunks of prompts and single tokens together. Their keys and values go to
+        the pool's caches, whose lengths grow; a row attends to the positions up to its
+        own, with a ``window`` to the last of them and the first ``sinks``. Returns fp32
+        logits [batch, vocab] after each sequence's last row (of no meaning where it has
+        none, or found no room: then its length has stayed). Captured, it serves every
+        mix of up to ``rows`` tokens."""
+        plan, attend = self._paged(tokens, counts, pool, window, sinks)
+        return self._layers(tokens.clamp(0, self.cfg.vocab - 1), attend, (plan.starts[1:] - 1).clamp(min=0))
+
+    def score(self, tokens: torch.Tensor, counts: torch.Tensor, pool: paged_cache.PagedPool, top: int = 0,
+              window: Optional[int] = None, sinks: int = 0) -> TokenLogprobs:
+        """``paged_step`` with the log probability of each row's next token (logprob 0 and
+        rank -1 in a sequence's last row of the step, of no meaning in rows that found no
+        room), entropy and ``top`` likeliest tokens of every row."""
+        plan, attend = self._paged(tokens, counts, pool, window, sinks)
+        rows = tokens.shape[0]
+        follow = torch.cat([tokens[1:], tokens[:1]])
+        # rows before another sequence's first, and behind the last sequence
+        last = torch.zeros(rows + 1, dtype=torch.bool, device=self.dev).index_fill_(0, plan.starts, True)[1:]
+        last |= torch.arange(rows, device=self.dev) >= plan.starts[-1]
+        logits = self._layers(tokens.clamp(0, self.cfg.vocab - 1), attend)
+        return token_logprobs(logits, torch.where(last, -1, follow), top)
+
+    def _paged(self, tokens: torch.Tensor, counts: torch.Tensor, pool: paged_cache.PagedPool,
+               window: Optional[int], sinks: int):
+        """A paged step's plan and its attention, as a function of (layer, qkv rows)."""
+        c = self.cfg
+        if tokens.dim() != 1 or tokens.dtype != torch.int64:
+            raise ValueError(f"tokens must be int64 [rows], got {tokens.dtype} of {list(tokens.shape)}")
+        if len(pool.caches) != c.layers:
+            raise ValueError(f"the pool has {len(pool.caches)} layers, the model {c.layers}")
+        if pool.tables.shape[1] * pool.block_size > self.max_len:
+            raise ValueError(f"the pool's sequences pass the {self.max_len} positions of the model")
+        plan = pool.plan(counts, tokens.shape[0])
+        H, KVH, D = c.heads, c.kv_heads, c.head_dim
+
+        def attend(i: int, qkv: torch.Tensor) -> torch.Tensor:
+            ly = self.layers[i]
+            q, k = tree_decode.qk_norm_rope(qkv, H, KVH, self.rope, plan.positions, ly.get("q_norm"),
+                                            ly.get("k_norm"), c.rms_eps)
+            v = qkv.view(-1, H + 2 * KVH, D)[:, H + KVH:]
+            paged_cache.write_blocks(k, v, pool.caches[i], plan.slots)
+            o = paged_cache.paged_attention(q, pool.caches[i], pool.tables, plan.starts, plan.lengths,
+                                            window, sinks)
+            return o.view(-1, H * D)
+
+        return plan, attend
 
     def _attention(self, pos: torch.Tensor):
         """The step's attention, as a function of (layer, qkv rows) -> [B, H * D]:

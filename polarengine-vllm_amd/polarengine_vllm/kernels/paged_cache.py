@@ -68,6 +68,40 @@ def new_cache(blocks: int, kv_heads: int, block_size: int, head_dim: int, device
           for _ in range(2)))
 
 
+class PagedPool:
+    """The caches of a model's layers, which share one set of blocks: tables, the stack
+    of free blocks and the sequences' lengths, for up to ``batch`` sequences of
+    ``max_len`` positions (rounded down to whole blocks) at a time."""
+
+    def __init__(self, layers: int, blocks: int, kv_heads: int, head_dim: int, batch: int,
+                 max_len: int, device, block_size: int = 64) -> None:
+        _block_size(block_size)
+        if batch < 1 or max_len < block_size:
+            raise ValueError(f"a pool has room for at least one sequence of a block, got {batch} of "
+                             f"{max_len}")
+        self.block_size = block_size
+        self.caches = [new_cache(blocks, kv_heads, block_size, head_dim, device) for _ in range(layers)]
+        self.tables = torch.full((batch, max_len // block_size), -1, dtype=torch.int32, device=device)
+        self.free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), blocks, dtype=torch.int64, device=device)
+        self.lengths = torch.full((batch,), -1, dtype=torch.int64, device=device)  # -1: empty slot
+
+    def plan(self, counts: torch.Tensor, rows: int) -> StepPlan:
+        """``plan_step`` for ``counts[b]`` new tokens of each sequence; lengths follow
+        where there was room."""
+        plan = plan_step(self.lengths, counts, self.tables, self.free, self.free_count, rows,
+                         self.block_size)
+        torch.where(plan.lengths >= 0, plan.lengths, self.lengths, out=self.lengths)
+        return plan
+
+    def keep(self, lengths: torch.Tensor) -> None:
+        """Each sequence's first ``lengths[b]`` positions stay (int64 [batch]), as many as
+        it has, and its other blocks are free again: 0 begins a new sequence, below 0
+        leaves an empty slot."""
+        release_blocks(self.tables, lengths.clamp(min=0), self.free, self.free_count, self.block_size)
+        torch.minimum(lengths, self.lengths.clamp(min=0), out=self.lengths)
+
+
 def _block_size(t: int) -> None:
     if t not in BLOCK_SIZES:
         raise ValueError(f"blocks hold {BLOCK_SIZES} positions, got {t}")
