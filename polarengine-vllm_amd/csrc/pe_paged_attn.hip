@@ -83,7 +83,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) {
   s.n = (int)(s1 - s0);
   s.lead = b == 0 ? (int)max((int64_t)0, min(a.starts[0], rows)) : 0;
   s.p0 = len >= 0 ? len - (end - s0) : INT64_MIN / 2;
-  s.blocks = (int)(((int64_t)s.n * a.group + RB - 1) / RB);
+  s.blocks = (s.n * a.group + RB - 1) / RB;
   return s;
 }
 // the positions of row block qb: [0, sink) and [lo, hi), in tiles
@@ -95,8 +95,8 @@ template <int RB, int TILE>
 __device__ __forceinline__ PaSpan pa_span(const PagedAttnArgs& a, const PaSeq& s, int qb) {
   PaSpan r;
   const int cap = a.width << a.c.log_t;
-  const int t0 = (int)((int64_t)qb * RB / a.group);
-  const int t1 = min(s.n - 1, (int)(((int64_t)qb * RB + RB - 1) / a.group));
+  const int t0 = qb * RB / a.group;
+  const int t1 = min(s.n - 1, (qb * RB + RB - 1) / a.group);
   r.hi = (int)max((int64_t)0, min(s.p0 + t1 + 1, (int64_t)cap));
   r.lo = 0;
   if (a.window) r.lo = (int)max((int64_t)0, min(s.p0 + t0 - a.window + 1, (int64_t)cap));
@@ -252,6 +252,10 @@ __device__ __forceinline__ float pa_rows_max(float v) {
 __device__ __forceinline__ uint32_t pa_nan(uint32_t w) {
   return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
+// bit 15 of each fp16 value that is not finite (converted codes: NaN)
+__device__ __forceinline__ uint32_t pa_nan16(uint32_t w) {
+  return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+}
 
 // the bits of positions below n, of 16
 __device__ __forceinline__ uint32_t pa_below(int n) { return (1u << min(max(n, 0), 16)) - 1; }
@@ -291,6 +295,22 @@ __device__ __forceinline__ float* pa_part(const PagedAttnArgs& a, const PaRun& r
   return a.parts + (run.run * 2 + (p.t0 == 0)) * words;
 }
 
+// The largest exponent byte of values so far: vb is that of the lane's 16 positions (0:
+// none there).
+__device__ __forceinline__ int pa_largest(int er, int vb) {
+  if (__any(vb > er)) {
+    int top = vb;
+#pragma unroll
+    for (int k = 32; k; k >>= 1) top = max(top, __shfl_xor(top, k, 64));
+    er = __builtin_amdgcn_readfirstlane(max(top, er));
+  }
+  return er;
+}
+// and the factor that the conversion gives the lane's values
+__device__ __forceinline__ float pa_factor(int vb, int er) {
+  return e8m0((uint32_t)max(127 + kPaVLift + vb - er, 1));
+}
+
 // What a wave keeps of RT products of 16 rows.
 template <int D, int RT>
 struct PaRows {
@@ -302,13 +322,13 @@ struct PaRows {
   int er;            // the values' scale (exponent byte) that o is relative to
 
   // rows first .. first + 16 RT - 1 of the row block
-  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PaSeq& seq, int kvh, int64_t first,
-                                        int li, int lg) {
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PaSeq& seq, int kvh, int first, int li,
+                                        int lg) {
     er = 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int64_t r = first + rt * 16 + li;
-      const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+      const int r = first + rt * 16 + li;
+      const int token = r / a.group, g = r - token * a.group;
       const bool there = token < seq.n;
       pos[rt] = there && token >= seq.lead
                     ? (int)max((int64_t)-1, min(seq.p0 + token, (int64_t)INT32_MAX / 2)) : -1;
@@ -341,22 +361,14 @@ struct PaRows {
           s[rt][t][e] = seen[rt] & (1u << (4 * t + e)) ? s[rt][t][e] : -__builtin_inff();
     }
   }
-  // vb: exponent byte of the values of the lane's 16 positions (0: none there); the
-  // factor that the conversion gives them
-  __device__ __forceinline__ float value_scale(int vb) {
-    if (__any(vb > er)) {
-      int top = vb;
+  // sums relative to another scale of values, `to`, that is larger
+  __device__ __forceinline__ void rescale(int to) {
+    const float f = __builtin_ldexpf(1.f, max(er - to, -200));
 #pragma unroll
-      for (int k = 32; k; k >>= 1) top = max(top, __shfl_xor(top, k, 64));
-      top = __builtin_amdgcn_readfirstlane(top);
-      const float f = __builtin_ldexpf(1.f, max(er - top, -200));
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-      er = top;
-    }
-    return e8m0((uint32_t)max(127 + kPaVLift + vb - er, 1));
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
+    er = to;
   }
   // p: B operands of two products, 8 neighbouring positions each. kc: what the scores
   // of the lane are multiplied by
@@ -394,44 +406,41 @@ struct PaRows {
       }
     }
   }
-  // NaN among the values of 16 dimensions, where some row does not see it: sums of rows
-  // that do become NaN (a product of where it is with what each row sees says which),
-  // the codes become zeros
-  __device__ __forceinline__ void nan_values(u32x4v& v, int dt, const uint32_t (&seen)[RT]) {
-    float4v hit[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) hit[rt] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // e4m3 1.0 is 0x38: bits 3, 4 and 5
-      const uint32_t n0 = pa_nan(v[2 * h]), n1 = pa_nan(v[2 * h + 1]);
-      const u32x4v nf = pa_unpack<false>((n0 >> 2) | (n0 >> 3) | (n0 >> 4),
-                                         (n1 >> 2) | (n1 >> 3) | (n1 >> 4), 1.f);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        u32x4v sf;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          sf[w] = (seen[rt] >> (8 * h + 2 * w) & 1u) * 0x3C00u |
-                  (seen[rt] >> (8 * h + 2 * w + 1) & 1u) * 0x3C000000u;
-        hit[rt] = pa_mfma<false>(nf, sf, hit[rt]);
-      }
-      v[2 * h] &= ~((n0 >> 7) * 0xFFu);
-      v[2 * h + 1] &= ~((n1 >> 7) * 0xFFu);
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (hit[rt][e] > 0.f) o[rt][dt][e] = __builtin_nanf("");
+  // fp16 values of 16 dimensions, positions 8 h .. 8 h + 7 of the lane's 16, where some
+  // are NaN. NaN must not reach, as 0 x NaN, the rows that do not see it: for the product
+  // it is a zero, and a product of where it is with what each row sees says which sums
+  // are NaN. `any`: positions that some row of the block sees; the others hold anything.
+  static __device__ __forceinline__ uint32_t pairs(uint32_t bits, int h, int w) {
+    return (bits >> (8 * h + 2 * w) & 1u) * 0xFFFFu | (bits >> (8 * h + 2 * w + 1) & 1u) * 0xFFFF0000u;
   }
-  __device__ __forceinline__ void values(u32x4v v, int dt, float scale, const u32x4v (&p)[RT][2]) {
+  static __device__ __forceinline__ u32x4v clean(u32x4v v) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x4v vf = pa_unpack<false>(v[2 * h], v[2 * h + 1], scale);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(vf, p[rt][h], o[rt][dt]);
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t u = v[w];
+      v[w] = u & ~((pa_nan16(u) >> 15) * 0xFFFFu);
     }
+    return v;
+  }
+  __device__ __forceinline__ void nan_values(u32x4v v, int dt, int h, const uint32_t (&seen)[RT], uint32_t any) {
+    u32x4v nf;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t u = v[w];
+      nf[w] = (pa_nan16(u) >> 15) * 0xFFFFu & pairs(any, h, w) & 0x3C003C00u;  // 1.0
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      u32x4v sf;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sf[w] = pairs(seen[rt], h, w) & 0x3C003C00u;
+      const float4v hit = pa_mfma<false>(nf, sf, float4v{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[rt][dt][e] = hit[e] > 0.f ? __builtin_nanf("") : o[rt][dt][e];
+    }
+  }
+  __device__ __forceinline__ void values(u32x4v v, int dt, int h, const u32x4v (&p)[RT][2]) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(v, p[rt][h], o[rt][dt]);
   }
   // the row's whole sum in all of its lanes, sums in units of 1
   __device__ __forceinline__ void finish() {
@@ -452,8 +461,8 @@ struct PaRows {
     for (int rt = 0; rt < RT; ++rt) {
       const int local = first + rt * 16 + li;
       if (!part) {
-        const int64_t r = (int64_t)qb * RB + local;
-        const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+        const int r = qb * RB + local;
+        const int token = r / a.group, g = r - token * a.group;
         if (token >= seq.n) continue;
         const float inv = l[rt] > 0.f || l[rt] != l[rt] ? 1.f / l[rt] : 0.f;
         uint16_t* dst = a.out + ((int64_t)(seq.first + token) * (a.c.kv_heads * a.group) + kvh * a.group + g) * D +
@@ -505,13 +514,9 @@ __device__ __forceinline__ const uint8_t* pa_values(const PagedAttnArgs& a, int 
   return a.c.v + (int64_t)max(block, 0) * a.c.v_b +
          ((((int64_t)kvh * D + li) << a.c.log_t) + ((p + 16 * lg) & ((1 << a.c.log_t) - 1)));
 }
-// bytes of the lane's 16 positions from x on that some row of the block sees
-__device__ __forceinline__ u32x4v pa_keep(const PaSpan& span, int x, uint32_t there) {
-  const uint32_t any = pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
-  u32x4v keep;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) keep[w] = (((any >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu;
-  return keep;
+// bits of the lane's 16 positions from x on that some row of the block sees
+__device__ __forceinline__ uint32_t pa_any(const PaSpan& span, int x, uint32_t there) {
+  return pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
 }
 
 // ---------------------------------------------------------------------------
@@ -553,10 +558,10 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
     // positions of the block's first and last row (of fewer rows, if some are absent)
-    const int64_t p_low = seq.lead ? -1 : seq.p0 + (int)((int64_t)qb * RB / a.group);
-    const int64_t p_high = seq.p0 + (int)(((int64_t)qb * RB + RB - 1) / a.group);
+    const int64_t p_low = seq.lead ? -1 : seq.p0 + qb * RB / a.group;
+    const int64_t p_high = seq.p0 + (qb * RB + RB - 1) / a.group;
     PaRows<D, RT> w;
-    w.begin(a, seq, kvh, (int64_t)qb * RB, li, lg);
+    w.begin(a, seq, kvh, qb * RB, li, lg);
     const float c = a.scale * kPaLog2e;
 
     // the wave's 64 positions of tile i of the row block, and whether any row sees one
@@ -630,19 +635,28 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
           bad |= pa_nan(vr[dt][0]) | pa_nan(vr[dt][1]) | pa_nan(vr[dt][2]) | pa_nan(vr[dt][3]);
         slow = __any(bad != 0);
       }
-      const float vscale = w.value_scale(cur.v >= 0 ? (int)vsb : 0);
+      const int vb = cur.v >= 0 ? (int)vsb : 0, er = pa_largest(w.er, vb);
+      if (er != w.er) w.rescale(er);
+      const float vscale = pa_factor(vb, er);
       u32x4v pf[RT][2];
       w.softmax(s, kc, pf);
-      if (__builtin_expect(slow, 0)) {
-        const u32x4v keep = pa_keep(span, p + 16 * lg, cur.v >= 0 ? 0xFFFFu : 0u);
+      auto unpack = [&](int dt, int h) { return pa_unpack<false>(vr[dt][2 * h], vr[dt][2 * h + 1], vscale); };
+      if (__builtin_expect(!slow, 1)) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          vr[dt] &= keep;
-          w.nan_values(vr[dt], dt, seen);
-        }
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w.values(unpack(dt, h), dt, h, pf);
+      } else {
+        const uint32_t any = pa_any(span, p + 16 * lg, cur.v >= 0 ? 0xFFFFu : 0u);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x4v v = unpack(dt, h);
+            w.values(w.clean(v), dt, h, pf);
+            w.nan_values(v, dt, h, seen, any);
+          }
       }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) w.values(vr[dt], dt, vscale, pf);
       if (in < t1) load_v(first_pos(in), nxt);
       cur = nxt;
       i = in;
@@ -698,21 +712,22 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 
 // ---------------------------------------------------------------------------
 // Many rows (chunks of prompts): the four waves of a workgroup take 16 RT rows each and
-// share 64 positions a step, which go straight to LDS in the order in which lanes read
-// them (64 lanes x 16 bytes an operand, the addresses that the other form loads from),
-// two buffers, the next tile under way while one is worked on, one barrier a tile.
+// share 64 positions a step. Two waves bring the keys and two the values, convert them
+// and put them to LDS in the order in which lanes read them (64 lanes x 16 bytes an
+// operand, from the addresses that the other form loads), so that a code is converted
+// once for all rows: the conversions, one instruction for two codes, would otherwise be
+// a third of the vector instructions beside the products. Two buffers: while a step is
+// worked on, the next one's operands are written and the loads of the one behind it are
+// under way; one barrier a step.
 // ---------------------------------------------------------------------------
-typedef __attribute__((address_space(3))) unsigned char pa_lds;
-typedef __attribute__((address_space(1))) const unsigned char pa_glb;
-
 template <int D, bool BF, int RT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(const PagedAttnArgs a) {
   constexpr int RB = 64 * RT, TILE = 64;
   constexpr int KL = D / 64, DT = D / 16;
-  constexpr int KF = 4 * KL;             // operands of keys, 1 KB each, then DT of values
-  constexpr int PER = (KF + DT) / 4;     // operands that a wave brings
-  __shared__ __align__(16) unsigned char buf0[(KF + DT) * 1024];
-  __shared__ __align__(16) unsigned char buf1[(KF + DT) * 1024];
+  constexpr int PER = DT / 2;          // 16-byte loads of a wave; 4 KL = DT of keys and of values
+  constexpr int KF = 2 * DT;           // operands of keys, 1 KB each, then as many of values
+  __shared__ __align__(16) u32x4v buf0[2 * KF * 64];
+  __shared__ __align__(16) u32x4v buf1[2 * KF * 64];
   __shared__ PaPlace place;
   __shared__ int64_t line;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -741,8 +756,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
     const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
     // the wave's rows, and positions of the first and the last of them
-    const int64_t first = (int64_t)qb * RB + wave * 16 * RT;
-    const int token0 = (int)(first / a.group), token1 = (int)((first + 16 * RT - 1) / a.group);
+    const int first = qb * RB + wave * 16 * RT;
+    const int token0 = first / a.group, token1 = (first + 16 * RT - 1) / a.group;
     const int64_t p_low = seq.lead ? -1 : seq.p0 + token0;
     const int64_t p_high = seq.p0 + min(token1, seq.n - 1);
     const bool idle = token0 >= seq.n;
@@ -757,112 +772,155 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
       const int p = first_pos(i);
       return p < span.hi && (p + 63 >= span.lo || p < span.sink);
     };
-    struct Scales {
-      uint32_t k, v;
-      int block;
+    auto next_tile = [&](int i) {
+      while (i < t1 && !in_sight(i)) ++i;
+      return i;
     };
+    // a step on its way: the wave's part of it, the scales of the lane's 16 positions
+    u32x4v raw[PER];
+    uint32_t rk, rv;
+    int rblock;
     PaBlocks nb;
-    auto issue = [&](unsigned char* to, int p, PaBlocks bl) {
-      const uint8_t* k = pa_keys<D>(a, kvh, p, bl.k, li, lg);
-      const uint8_t* v = pa_values<D>(a, kvh, p, bl.v, li, lg);
+    auto load = [&](int p, PaBlocks bl) {
+      if (wave < 2) {
+        const uint8_t* k = pa_keys<D>(a, kvh, p, bl.k, li, lg);
 #pragma unroll
-      for (int n = 0; n < PER; ++n) {
-        const int f = wave * PER + n;  // waves 0 and 1 bring keys, 2 and 3 values
-        const uint8_t* src = f < KF ? k + 4 * (f / KL) * D + 64 * (f % KL)
-                                    : v + ((int64_t)(16 * (f - KF)) << a.c.log_t);
-        __builtin_amdgcn_global_load_lds((const pa_glb*)src, (pa_lds*)to + f * 1024, 16, 0, 0);
+        for (int n = 0; n < PER; ++n) {
+          const int f = wave * PER + n;
+          raw[n] = *reinterpret_cast<const u32x4v*>(k + 4 * (f / KL) * D + 64 * (f % KL));
+        }
+      } else {
+        const uint8_t* v = pa_values<D>(a, kvh, p, bl.v, li, lg) + ((int64_t)((wave - 2) * PER * 16) << a.c.log_t);
+#pragma unroll
+        for (int n = 0; n < PER; ++n)
+          raw[n] = *reinterpret_cast<const u32x4v*>(v + ((int64_t)(16 * n) << a.c.log_t));
       }
       const int64_t sc = (int64_t)max(bl.v, 0) * a.c.s_b + kvh;
-      return Scales{a.c.ks[sc], a.c.vs[sc], bl.v};
+      rk = a.c.ks[sc];
+      rv = a.c.vs[sc];
+      rblock = bl.v;
     };
-    Scales cur{0, 0, -1}, nxt{0, 0, -1};
-    int i = t0;
-    while (i < t1 && !in_sight(i)) ++i;
-    if (i < t1) cur = issue(buf0, first_pos(i), pa_blocks(a, table, first_pos(i), li, lg));
-    int in = i + 1;
-    while (in < t1 && !in_sight(in)) ++in;
-    if (in < t1) nb = pa_blocks(a, table, first_pos(in), li, lg);
-    auto step = [&](const unsigned char* from, unsigned char* to) {
+    // of the step that is worked on
+    int block = -1, er = 0;
+    uint32_t kb = 0;
+    // and of the one whose operands are in LDS next
+    int nblock = -1, ner = 0;
+    uint32_t nkb = 0;
+    auto convert = [&](u32x4v* to) {
+      const int vb = rblock >= 0 ? (int)rv : 0;
+      nblock = rblock;
+      nkb = rk;
+      ner = pa_largest(er, vb);
+      const float f = pa_factor(vb, ner);
+      u32x4v* dst = to + (wave * PER * 2) * 64 + lane;
+#pragma unroll
+      for (int n = 0; n < PER; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          dst[(2 * n + h) * 64] = BF && wave < 2 ? pa_unpack<true>(raw[n][2 * h], raw[n][2 * h + 1], 1.f)
+                                                 : pa_unpack<false>(raw[n][2 * h], raw[n][2 * h + 1],
+                                                                    wave < 2 ? 1.f : f);
+    };
+    int i = next_tile(t0), in = next_tile(i + 1), after = next_tile(in + 1);
+    if (i < t1) {
+      load(first_pos(i), pa_blocks(a, table, first_pos(i), li, lg));
+      convert(buf0);
+      if (in < t1) load(first_pos(in), pa_blocks(a, table, first_pos(in), li, lg));
+      if (after < t1) nb = pa_blocks(a, table, first_pos(after), li, lg);
+    }
+    auto step = [&](const u32x4v* from, u32x4v* to) {
       const int p = first_pos(i);
-      __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the tile is in LDS
-      __syncthreads();                // everybody's is, and `to` is done with
-      int after = in + 1;
+      block = nblock;
+      kb = nkb;
+      er = ner;
+      if (er != w.er) w.rescale(er);
+      __syncthreads();  // the operands are there, and `to` is done with
       if (in < t1) {
-        nxt = issue(to, first_pos(in), nb);
-        while (after < t1 && !in_sight(after)) ++after;
-        if (after < t1) nb = pa_blocks(a, table, first_pos(after), li, lg);
+        convert(to);
+        if (after < t1) {
+          load(first_pos(after), nb);
+          const int behind = next_tile(after + 1);
+          if (behind < t1) nb = pa_blocks(a, table, first_pos(behind), li, lg);
+          i = in;
+          in = after;
+          after = behind;
+        } else {
+          i = in;
+          in = after;
+        }
+      } else {
+        i = in;
       }
-      // a wave whose rows see nothing of the tile leaves it
+      // a wave whose rows see nothing of the step leaves it
       const bool none = idle || p > p_high ||
                         (a.window && p + 63 <= max(p_low, (int64_t)-1) - a.window && p >= a.sinks);
-      if (!none) {
-        const bool full = p + 63 <= p_low && !__any(cur.block < 0) &&
-                          (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
-        const u32x4v* kf = reinterpret_cast<const u32x4v*>(from) + lane;
-        const u32x4v* vf = kf + KF * 64;
-        // operands one ahead of their products; the fences keep the compiler from
-        // bringing them all at once, for which there are no registers
-        float4v s[RT][4];
-        u32x4v raw[2][KL];
+      if (none) return;
+      const bool full = p + 63 <= p_low && !__any(block < 0) &&
+                        (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
+      const u32x4v* kf = from + lane;
+      const u32x4v* vf = kf + KF * 64;
+      // operands A ahead of their products; the fences keep the compiler from bringing
+      // them all at once, for which there are no registers
+      constexpr int A = 4;
+      float4v s[RT][4];
+      {
+        u32x4v g[A];
 #pragma unroll
-        for (int j = 0; j < KL; ++j) raw[0][j] = kf[j * 64];
+        for (int f = 0; f < A; ++f) g[f] = kf[f * 64];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (t < 3)
+        for (int f = 0; f < KF; ++f) {
+          const int t = f / (2 * KL), j = f % (2 * KL);
 #pragma unroll
-            for (int j = 0; j < KL; ++j) raw[(t + 1) & 1][j] = kf[((t + 1) * KL + j) * 64];
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < KL; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const u32x4v kk = pa_unpack<BF>(raw[t & 1][j][2 * h], raw[t & 1][j][2 * h + 1], 1.f);
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt) s[rt][t] = pa_mfma<BF>(kk, w.q[rt][2 * j + h], s[rt][t]);
-            }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        const float kc = fmaxf(e8m0(cur.k) * c, 1e-37f);
-        const float vscale = w.value_scale(cur.block >= 0 ? (int)cur.v : 0);
-        const uint32_t there = cur.block >= 0 ? 0xFFFFu : 0u;
-        uint32_t seen[RT];
-        bool slow = false;
-        if (!full) {
-          w.mask(a, s, seen, p + 16 * lg, there);
-          uint32_t bad = 0;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const u32x4v v = vf[dt * 64];
-            bad |= pa_nan(v[0]) | pa_nan(v[1]) | pa_nan(v[2]) | pa_nan(v[3]);
-          }
-          slow = __any(bad != 0);
-        }
-        u32x4v pf[RT][2];
-        w.softmax(s, kc, pf);
-        if (__builtin_expect(slow, 0)) {
-          const u32x4v keep = pa_keep(span, p + 16 * lg, there);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            u32x4v v = vf[dt * 64] & keep;
-            w.nan_values(v, dt, seen);
-            w.values(v, dt, vscale, pf);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        } else {
-          u32x4v v = vf[0];
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const u32x4v next = vf[min(dt + 1, DT - 1) * 64];
-            w.values(v, dt, vscale, pf);
-            v = next;
-            __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int rt = 0; rt < RT; ++rt)
+            s[rt][t] = pa_mfma<BF>(g[f % A], w.q[rt][j], j ? s[rt][t] : float4v{0.f, 0.f, 0.f, 0.f});
+          if (f + A < KF) g[f % A] = kf[(f + A) * 64];
+          if (f & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      cur = nxt;
-      i = in;
-      in = after;
+      // above 0: a masked -inf stays one
+      const float kc = fmaxf(e8m0(kb) * c, 1e-37f);
+      const uint32_t there = block >= 0 ? 0xFFFFu : 0u;
+      uint32_t seen[RT];
+      bool slow = false;
+      if (!full) {
+        w.mask(a, s, seen, p + 16 * lg, there);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+          const u32x4v v = vf[f * 64];
+          bad |= pa_nan16(v[0]) | pa_nan16(v[1]) | pa_nan16(v[2]) | pa_nan16(v[3]);
+          if ((f & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        slow = __any(bad != 0);
+      }
+      u32x4v pf[RT][2];
+      w.softmax(s, kc, pf);
+      if (__builtin_expect(slow, 0)) {
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+          w.values(w.clean(vf[f * 64]), f >> 1, f & 1, pf);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const uint32_t any = pa_any(span, p + 16 * lg, there);
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+          w.nan_values(vf[f * 64], f >> 1, f & 1, seen, any);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        u32x4v v[A];
+#pragma unroll
+        for (int f = 0; f < A; ++f) v[f] = vf[f * 64];
+#pragma unroll
+        for (int f = 0; f < KF; f += 2) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w.values(v[(f + h) % A], f >> 1, h, pf);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (f + h + A < KF) v[(f + h) % A] = vf[(f + h + A) * 64];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     };
     while (i < t1) {
       step(buf0, buf1);
@@ -894,8 +952,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
   // the first part is its run's last, the others are their runs' first
   auto part = [&](int s) { return base + s * 2 * words + (s == 0 ? words : 0); };
   {
-    const int64_t r = (int64_t)cut.qb * RB + local;
-    const int token = (int)(r / a.group), g = (int)(r - (int64_t)token * a.group);
+    const int r = cut.qb * RB + local;
+    const int token = r / a.group, g = r - token * a.group;
     if (token >= cut.n) return;
     float m = -__builtin_inff(), l = 0.f;
     floatE o = 0.f;
@@ -956,6 +1014,7 @@ static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int 
 static bool pa_shape_ok(int64_t rows, int64_t batch, int heads, int kv_heads, int dim) {
   return rows >= 0 && rows <= kPagedMaxRows && batch >= 0 && batch <= kPagedMaxBatch &&
          kv_heads >= 1 && heads >= 1 && heads <= 65535 && heads % kv_heads == 0 &&
+         (rows + 1) * (heads / kv_heads) <= INT32_MAX - 256 &&  // rows of a KV head
          (dim == 64 || dim == 128 || dim == 256);
 }
 

@@ -57,6 +57,6 @@ def int64(t: torch.Tensor, shape: Tuple[int, ...], name: str) -> torch.Tensor:
 
 def written(*tensors: torch.Tensor) -> None:
     """Counts writes through raw pointers (inference tensors keep no count)."""
-    for t in tensors:
-        if not t.is_inference():
-            increment_version(t)
+    if any(t.is_inference() for t in tensors):
+        tensors = tuple(t for t in tensors if not t.is_inference())
+    increment_version(tensors)

@@ -44,15 +44,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     tokens = int64(tokens, (rows,), "tokens")
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
-    floats = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
-    whole = torch.empty(rows * (1 + top), dtype=torch.int64, device=dev)
-    out = TokenLogprobs(floats[:rows], whole[:rows], floats[rows:2 * rows],
-                        floats[2 * rows:].view(rows, top), whole[rows:].view(rows, top))
+    f32, i64 = torch.float32, torch.int64
+    out = TokenLogprobs(torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=i64, device=dev),
+                        torch.empty(rows, dtype=f32, device=dev),
+                        torch.empty(rows, top, dtype=f32, device=dev),
+                        torch.empty(rows, top, dtype=i64, device=dev))
     if not rows:
         return out
     size = _lib.workspace_size("pe_token_logprobs_workspace_size", rows, vocab, top)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     call("pe_token_logprobs", dev, logits.data_ptr(), code, rows,
          logits.stride(0) if rows > 1 else vocab, vocab, tokens.data_ptr(), top,
-         *(t.data_ptr() for t in out), _lib.ptr(ws), size)
+         out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(),
+         _lib.ptr(ws), size)
     return out

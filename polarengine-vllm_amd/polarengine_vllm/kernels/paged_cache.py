@@ -110,23 +110,22 @@ def _block_size(t: int) -> None:
 def _cache(cache: PagedCache):
     """(the library's arguments of a cache up to its sizes, shape of the keys)."""
     k, v, ks, vs = cache
-    shape = k.shape
-    if k.dim() != 4 or v.dim() != 4 or v.shape != (shape[0], shape[1], shape[3], shape[2]):
+    shape, pair = k.shape, ks.shape
+    if len(shape) != 4 or v.shape != (shape[0], shape[1], shape[3], shape[2]):
         raise ValueError(f"codes must be [blocks, kv_heads, block_size, head_dim] and [.., head_dim, "
                          f"block_size], got {list(shape)} and {list(v.shape)}")
-    if ks.shape != shape[:2] or vs.shape != shape[:2]:
-        raise ValueError(f"scales must be {list(shape[:2])}, got {list(ks.shape)} and {list(vs.shape)}")
-    if k.dtype is not F8 or v.dtype is not F8 or ks.dtype is not E8 or vs.dtype is not E8:
+    blocks, heads, t, d = shape
+    if pair != (blocks, heads) or vs.shape != pair:
+        raise ValueError(f"scales must be {list(shape[:2])}, got {list(pair)} and {list(vs.shape)}")
+    if not (k.dtype is v.dtype is F8 and ks.dtype is vs.dtype is E8):
         raise TypeError(f"codes must be {F8} and scales {E8}, got {k.dtype}, {v.dtype}, {ks.dtype} "
                         f"and {vs.dtype}")
-    blocks, heads, t, d = shape
     _block_size(t)
     if not blocks or not heads:
         raise ValueError(f"a cache has at least one block and KV head, got {list(shape)}")
-    part = heads * t * d
-    sk, sv, ss = k.stride(), v.stride(), ks.stride()
-    if (sk[1:] != (t * d, d, 1) or sv[1:] != (t * d, t, 1) or ss[1] != 1 or ss != vs.stride()
-            or sk[0] < part or sv[0] < part or ss[0] < heads):
+    sk, sv, ss, head = k.stride(), v.stride(), ks.stride(), t * d
+    if (sk[1:] != (head, d, 1) or sv[1:] != (head, t, 1) or ss[1] != 1 or ss != vs.stride()
+            or sk[0] < heads * head or sv[0] < heads * head or ss[0] < heads):
         # a stride along one element says nothing
         sk, sv, ss = _block_stride(k), _block_stride(v), _block_stride(ks)
         if ss != _block_stride(vs):
@@ -195,7 +194,7 @@ def plan_step(lengths: torch.Tensor, counts: torch.Tensor, tables: torch.Tensor,
         raise ValueError(f"rows must be at least 0, got {rows}")
     lengths, counts = int64(lengths, (batch,), "lengths"), int64(counts, (batch,), "counts")
     out = torch.empty(2 * batch + 1 + 2 * rows, dtype=torch.int64, device=dev)
-    positions, slots, starts, after = out.split((rows, rows, batch + 1, batch))
+    positions, slots, starts, after = out.split_with_sizes((rows, rows, batch + 1, batch))
     if not batch:
         positions.fill_(-1), slots.fill_(-1), starts.zero_()
         return StepPlan(starts, positions, slots, after)
@@ -291,7 +290,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
         return torch.zeros(rows, heads, dim, dtype=q.dtype, device=dev)
     if q.stride(1) != dim or q.stride(2) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty(rows, heads, dim, dtype=q.dtype, device=dev)
+    out = q.new_empty((rows, heads, dim))
     width = tables.shape[1]
     size = _lib.workspace_size("pe_paged_attention_workspace_size", rows, batch, heads, shape[1], dim,
                                width * shape[2])
