@@ -176,6 +176,17 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
           __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48)));
 }
 
+// running sum over the 64 lanes: DPP row_shr within 16 lanes, then the rows
+__device__ __forceinline__ int wave_scan_i32(int v, int lane) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31);
+  const int r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+  return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
+}
+
 // ---------------------------------------------------------------------------
 // FWHT-128 on a 16-lane group: each lane holds 8 consecutive values
 // (positions 8q..8q+7, q = lane & 15). Stages 1, 2, 4 are in-lane, 8..64 use

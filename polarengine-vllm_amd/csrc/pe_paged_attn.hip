@@ -108,18 +108,10 @@ __device__ __forceinline__ PaSpan pa_span(const PagedAttnArgs& a, const PaSeq& s
 }
 // tiles of all row blocks of a sequence, one KV head
 template <int RB, int TILE>
-__device__ __forceinline__ int64_t pa_tiles(const PagedAttnArgs& a, const PaSeq& s) {
-  int64_t sum = 0;
+__device__ __forceinline__ int pa_tiles(const PagedAttnArgs& a, const PaSeq& s) {
+  int sum = 0;
   for (int qb = 0; qb < s.blocks; ++qb) sum += pa_span<RB, TILE>(a, s, qb).tiles;
   return sum;
-}
-__device__ __forceinline__ int64_t pa_scan(int64_t v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t u = __shfl_up((long long)v, off, 64);
-    if (lane >= off) v += u;
-  }
-  return v;
 }
 // a row block's place in the line
 struct PaPlace {
@@ -131,62 +123,63 @@ struct PaPlace {
 template <int RB>
 struct PaChunk {
   PaSeq seq;
-  int64_t tiles;
+  int tiles, scan;  // and their running sum
 };
 template <int RB, int TILE>
 __device__ __forceinline__ PaChunk<RB> pa_chunk(const PagedAttnArgs& a, int b0, int lane) {
   PaChunk<RB> c;
   c.seq = pa_seq<RB>(a, b0 + lane);
   c.tiles = pa_tiles<RB, TILE>(a, c.seq);
+  c.scan = wave_scan_i32(c.tiles, lane);
   return c;
 }
-__device__ __forceinline__ int64_t pa_from(int64_t v, int lane) { return __shfl((long long)v, lane, 64); }
+__device__ __forceinline__ int pa_from(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 // one wave: the length of the line; c: the first chunk
 template <int RB, int TILE>
 __device__ __forceinline__ int64_t pa_total(const PagedAttnArgs& a, const PaChunk<RB>& c, int lane) {
-  int64_t sum = c.tiles;
-  for (int b0 = 64; b0 <= a.batch; b0 += 64) sum += pa_chunk<RB, TILE>(a, b0, lane).tiles;
-#pragma unroll
-  for (int m = 32; m; m >>= 1) sum += __shfl_xor((long long)sum, m, 64);
-  return sum * a.c.kv_heads;
+  int sum = pa_from(c.scan, 63);
+  for (int b0 = 64; b0 <= a.batch; b0 += 64) sum += pa_from(pa_chunk<RB, TILE>(a, b0, lane).scan, 63);
+  return (int64_t)sum * a.c.kv_heads;
 }
 // one wave: what holds place `at` of the line (all lanes; at below the total)
 template <int RB, int TILE>
 __device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, PaChunk<RB> c, int64_t at, int lane) {
   PaPlace r{-1, 0, 0, 0, 0, {}};
-  int64_t before = 0;
+  int before = 0;
   for (int b0 = 0; b0 <= a.batch; b0 += 64) {
     if (b0) c = pa_chunk<RB, TILE>(a, b0, lane);
-    const int64_t scan = pa_scan(c.tiles, lane);
-    const uint64_t hit = __ballot((before + scan) * a.c.kv_heads > at);
+    const uint64_t hit = __ballot((int64_t)(before + c.scan) * a.c.kv_heads > at);
     if (!hit) {
-      before += pa_from(scan, 63);
+      before += pa_from(c.scan, 63);
       continue;
     }
     const int l = __builtin_ctzll(hit);
-    const int64_t tiles = pa_from(c.tiles, l);
-    at -= (before + pa_from(scan, l) - tiles) * a.c.kv_heads;
-    r.kvh = (int)(at / tiles);
-    at -= r.kvh * tiles;
+    const int tiles = pa_from(c.tiles, l);
+    const int64_t in_seq = at - (int64_t)(before + pa_from(c.scan, l) - tiles) * a.c.kv_heads;
+    // below tiles kv_heads; KV heads are at most 4096, so that 64 bits are seldom needed
+    r.kvh = in_seq <= UINT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)tiles) : (int)(in_seq / tiles);
+    int left = (int)(in_seq - (int64_t)r.kvh * tiles);
     PaSeq& s = r.seq;
-    s.first = __shfl(c.seq.first, l, 64);
-    s.n = __shfl(c.seq.n, l, 64);
-    s.lead = __shfl(c.seq.lead, l, 64);
-    s.p0 = pa_from(c.seq.p0, l);
-    s.blocks = __shfl(c.seq.blocks, l, 64);
+    s.first = pa_from(c.seq.first, l);
+    s.n = pa_from(c.seq.n, l);
+    s.lead = pa_from(c.seq.lead, l);
+    const uint32_t lo = pa_from((int)(uint32_t)c.seq.p0, l);
+    const uint32_t hi = pa_from((int)(uint32_t)((uint64_t)c.seq.p0 >> 32), l);
+    s.p0 = (int64_t)((uint64_t)hi << 32 | lo);
+    s.blocks = pa_from(c.seq.blocks, l);
     for (int q0 = 0; q0 < s.blocks; q0 += 64) {
-      const int64_t t = q0 + lane < s.blocks ? pa_span<RB, TILE>(a, s, q0 + lane).tiles : 0;
-      const int64_t sc = pa_scan(t, lane);
-      const uint64_t in = __ballot(sc > at);
+      const int t = q0 + lane < s.blocks ? pa_span<RB, TILE>(a, s, q0 + lane).tiles : 0;
+      const int sc = wave_scan_i32(t, lane);
+      const uint64_t in = __ballot(sc > left);
       if (in) {
         const int k = __builtin_ctzll(in);
         r.b = b0 + l;
         r.qb = q0 + k;
-        r.tiles = (int)pa_from(t, k);
-        r.t0 = (int)(at - (pa_from(sc, k) - r.tiles));
+        r.tiles = pa_from(t, k);
+        r.t0 = left - (pa_from(sc, k) - r.tiles);
         return r;
       }
-      at -= pa_from(sc, 63);
+      left -= pa_from(sc, 63);
     }
     return r;
   }
@@ -273,6 +266,7 @@ struct PaRun {
   int64_t run, at, end, size;  // at >= end: none
 };
 __device__ __forceinline__ PaRun pa_run(const PagedAttnArgs& a, int64_t total) {
+  total = max(total, (int64_t)1);  // less only for starts that do not rise
   const int64_t size = (total + a.runs - 1) / a.runs;
   const int64_t active = (total + size - 1) / size, per = (active + 7) / 8;
   const int64_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
@@ -991,22 +985,46 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
   }
 }
 
+// The form, by the rows of a KV head that a sequence has in the mean: 16 rows a workgroup
+// up to 32 (two row blocks cost no more than one of 32), 32 rows up to 64 (not for heads
+// of 256, where they do not fit the registers), 128 beyond. That form's steps are dearer
+// where there are few of them: up to 128 rows it needs 64 (sequence, KV head) pairs.
+// Microseconds by 16, 32 and 128 rows, from a graph, one sequence of 8000 and of 30,000
+// and 16 of 4000 positions, 8 KV heads:
+//   head    rows      1 x 8000      1 x 30,000       16 x 4000
+//    64       32    23  24  30      25   33   44     29   32   50
+//             64    21  22  35      30   35   48     43   40   56
+//            128    23  24  39      42   48   57     74   77   62
+//            256    29  29  38      64   73   63    121  133   98
+//   128       32    26  28  37      34   42   58     42   43   73
+//             64    26  27  43      46   47   61     69   58   81
+//            128    31  32  47      76   67   73    137  113   89
+//            256    43  39  45     120  104   84    242  196  134
+//   256       32    29   -  73      60    -  131     78    -  207
+//             64    36   -  76      89    -  126    153    -  213
+//            128    48   -  83     154    -  144    271    -  231
+//            256    73   -  92     223    -  214    495    -  392
+// Workgroups a CU: two of 16 or 128 rows (one with heads of 256: 16 rows, 16 x 4000, 59
+// us, two 72), one of 32 (64 rows, 16 x 4000, 58 us, two 76).
 struct PaPlan {
-  int rb;      // rows of a row block: 16 and 32 in the form for few rows, else 128
+  int rb;      // rows of a row block
   int runs;
   bool split;  // a row block may be divided
+  bool fits;   // the tiles of a KV head can be counted in 32 bits
 };
 static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int dim, int64_t positions) {
   PaPlan p;
   const int group = heads / kv_heads;
-  // rows of a KV head that a sequence has in the mean
   const int64_t mean = (rows + batch - 1) / batch * group;
-  p.rb = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+  if (mean > 128 || (mean > 64 && batch * kv_heads >= 64)) p.rb = 128;
+  else p.rb = mean > 32 && dim != 256 ? 32 : 16;
   const int tile = p.rb == 128 ? 64 : 256;
   const int64_t tiles = (positions + tile - 1) / tile;
-  const int64_t most = (rows * group / p.rb + batch + 1) * kv_heads * tiles;
-  const int64_t wanted = (int64_t)num_cus() * ((p.rb == 16 || p.rb == 128) && dim != 256 ? 2 : 1);
-  p.runs = (int)(wanted < most ? wanted : most);
+  const int64_t blocks = rows * group / p.rb + batch + 1;  // row blocks of a KV head, at most
+  p.fits = (double)blocks * (double)tiles < 1e9;
+  const double most = p.fits ? (double)blocks * tiles * kv_heads : 1e9;
+  const int64_t wanted = (int64_t)num_cus() * (p.rb != 32 && dim != 256 ? 2 : 1);
+  p.runs = (int)((double)wanted < most ? (double)wanted : most);
   p.split = tiles > 1 && p.runs > 1;
   return p;
 }
@@ -1024,14 +1042,18 @@ static int launch_pa(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
   const dim3 join((unsigned)p.runs, (unsigned)p.rb / 4);
   switch (p.rb) {
     case 16: paged_attn_kernel<D, BF, 1><<<grid, 256, 0, st>>>(a); break;
-    case 32: paged_attn_kernel<D, BF, 2><<<grid, 256, 0, st>>>(a); break;
+    case 32:
+      if constexpr (D != 256) paged_attn_kernel<D, BF, 2><<<grid, 256, 0, st>>>(a);
+      break;
     default: paged_chunk_kernel<D, BF, 2><<<grid, 256, 0, st>>>(a); break;
   }
   const int rc = launch_status();
   if (rc != PE_OK || !p.split) return rc;
   switch (p.rb) {
     case 16: paged_join_kernel<D, BF, 16><<<join, 256, 0, st>>>(a); break;
-    case 32: paged_join_kernel<D, BF, 32><<<join, 256, 0, st>>>(a); break;
+    case 32:
+      if constexpr (D != 256) paged_join_kernel<D, BF, 32><<<join, 256, 0, st>>>(a);
+      break;
     default: paged_join_kernel<D, BF, 128><<<join, 256, 0, st>>>(a); break;
   }
   return launch_status();
@@ -1071,6 +1093,7 @@ extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t
   if (rows == 0) return PE_OK;
   if (batch == 0) return PE_ERR_DIMS;
   const PaPlan p = pa_plan(rows, batch, heads, kv_heads, head_dim, width * block_size);
+  if (!p.fits) return PE_ERR_DIMS;
   const size_t need = pe_paged_attention_workspace_size(rows, batch, heads, kv_heads, head_dim,
                                                         width * block_size);
   if (need && (!workspace || workspace_bytes < need)) return PE_ERR_WORKSPACE;

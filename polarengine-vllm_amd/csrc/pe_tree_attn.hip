@@ -73,16 +73,6 @@ __host__ __device__ inline int64_t part_words(int rb, int dim) { return (int64_t
 // launches find their way from the lengths alone, in a workgroup that works together
 // one wave for all.
 // ---------------------------------------------------------------------------
-// running sum over the 64 lanes: DPP row_shr within 16 lanes, then the rows
-__device__ __forceinline__ int wave_scan_i32(int v, int lane) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31);
-  const int r2 = r1 + __builtin_amdgcn_readlane(v, 47);
-  return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
-}
 __device__ __forceinline__ bool tree_active(const TreeAttnArgs& a, int64_t len) {
   return len >= 0 && len <= a.cap - a.n;
 }
