@@ -529,7 +529,7 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  * layer's cache: keys e4m3 [blocks, kv_heads, block_size, head_dim], values e4m3
  * [blocks, kv_heads, head_dim, block_size], each block and head with a power of two
  * as scale (e8m0 [blocks, kv_heads]: 2^(byte - 127)); a block's parts are contiguous
- * and 16-byte aligned, k_b, v_b and s_b are the strides of blocks in bytes.
+ * and 16-byte aligned, k_b, v_b and s_b (below 2^31) the strides of blocks in bytes.
  * head_dim 64, 128 or 256. tables int32 [batch, width] (row stride t_b): the blocks
  * of each sequence in order of position, below 0 where it has none. All sizes that
  * differ between sequences are read on the device.

@@ -31,6 +31,7 @@ inline int paged_cache(PagedCache& c, const void* k, int64_t k_b, const void* v,
   if (kv_heads < 1 || kv_heads > 4096 || blocks < 1 || blocks > INT32_MAX) return PE_ERR_DIMS;
   const int64_t part = (int64_t)kv_heads * block_size * head_dim;
   if (k_b < part || v_b < part || s_b < kv_heads) return PE_ERR_DIMS;
+  if (k_b > INT32_MAX || v_b > INT32_MAX || s_b > INT32_MAX) return PE_ERR_DIMS;
   if (!aligned16(k) || !aligned16(v) || k_b % 16 || v_b % 16) return PE_ERR_ALIGN;
   c.k = const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(k));
   c.v = const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(v));

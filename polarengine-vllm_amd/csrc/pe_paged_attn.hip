@@ -494,20 +494,36 @@ __device__ __forceinline__ PaBlocks pa_blocks(const PagedAttnArgs& a, const int3
   if (iv >= a.width || r.v >= a.c.blocks) r.v = -1;
   return r;
 }
-// the lane's part of the keys (rows 4 t and 16-byte chunks 4 j behind it) and values
-// (16 dimensions behind it) of 64 positions from p on
+// The lane's part of the keys (rows 4 t and 16-byte chunks 4 j behind it) and values
+// (16 dimensions behind it) of 64 positions from p on: what does not change within a KV
+// head once, then a multiply-add a step (strides of blocks are below 2^31 bytes).
 template <int D>
-__device__ __forceinline__ const uint8_t* pa_keys(const PagedAttnArgs& a, int kvh, int p, int block, int li,
-                                                  int lg) {
-  return a.c.k + (int64_t)max(block, 0) * a.c.k_b +
-         (((int64_t)kvh << a.c.log_t) + ((p + 16 * (li >> 2)) & ((1 << a.c.log_t) - 1)) + (li & 3)) * D + 16 * lg;
-}
-template <int D>
-__device__ __forceinline__ const uint8_t* pa_values(const PagedAttnArgs& a, int kvh, int p, int block, int li,
-                                                    int lg) {
-  return a.c.v + (int64_t)max(block, 0) * a.c.v_b +
-         ((((int64_t)kvh * D + li) << a.c.log_t) + ((p + 16 * lg) & ((1 << a.c.log_t) - 1)));
-}
+struct PaLanes {
+  const uint8_t *k, *v, *ks, *vs;
+  uint32_t k_b, v_b, s_b;
+  int t_mask, k_off, v_off;  // the lane's 16 positions among the 64
+  __device__ __forceinline__ PaLanes(const PagedAttnArgs& a, int kvh, int li, int lg) {
+    k = a.c.k + (((int64_t)kvh << a.c.log_t) + (li & 3)) * D + 16 * lg;
+    v = a.c.v + (((int64_t)kvh * D + li) << a.c.log_t);
+    ks = a.c.ks + kvh;
+    vs = a.c.vs + kvh;
+    k_b = (uint32_t)a.c.k_b;
+    v_b = (uint32_t)a.c.v_b;
+    s_b = (uint32_t)a.c.s_b;
+    t_mask = (1 << a.c.log_t) - 1;
+    k_off = 16 * (li >> 2);
+    v_off = 16 * lg;
+  }
+  __device__ __forceinline__ const uint8_t* keys(int p, int block) const {
+    return k + ((uint64_t)(uint32_t)max(block, 0) * k_b + (uint32_t)(((p + k_off) & t_mask) * D));
+  }
+  __device__ __forceinline__ const uint8_t* values(int p, int block) const {
+    return v + ((uint64_t)(uint32_t)max(block, 0) * v_b + (uint32_t)((p + v_off) & t_mask));
+  }
+  __device__ __forceinline__ uint64_t scale(int block) const {
+    return (uint64_t)(uint32_t)max(block, 0) * s_b;
+  }
+};
 // bits of the lane's 16 positions from x on that some row of the block sees
 __device__ __forceinline__ uint32_t pa_any(const PaSpan& span, int x, uint32_t there) {
   return pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
@@ -558,6 +574,7 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     w.begin(a, seq, kvh, qb * RB, li, lg);
     const float c = a.scale * kPaLog2e;
 
+    const PaLanes<D> at_lane(a, kvh, li, lg);
     // the wave's 64 positions of tile i of the row block, and whether any row sees one
     auto first_pos = [&](int i) {
       return (i < span.sink_tiles ? i : span.first_tile + i - span.sink_tiles) * TILE + wave * 64;
@@ -572,20 +589,19 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     u32x4v kr[4][KL], vr[DT];
     uint32_t ksb, vsb;
     auto load_k = [&](int p, PaBlocks bl) {
-      const uint8_t* k = pa_keys<D>(a, kvh, p, bl.k, li, lg);
+      const uint8_t* k = at_lane.keys(p, bl.k);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int j = 0; j < KL; ++j)
           kr[t][j] = *reinterpret_cast<const u32x4v*>(k + 4 * t * D + 64 * j);
-      ksb = a.c.ks[(int64_t)max(bl.v, 0) * a.c.s_b + kvh];
+      ksb = at_lane.ks[at_lane.scale(bl.v)];
     };
     auto load_v = [&](int p, PaBlocks bl) {
-      const uint8_t* v = pa_values<D>(a, kvh, p, bl.v, li, lg);
+      const uint8_t* v = at_lane.values(p, bl.v);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        vr[dt] = *reinterpret_cast<const u32x4v*>(v + ((int64_t)(16 * dt) << a.c.log_t));
-      vsb = a.c.vs[(int64_t)max(bl.v, 0) * a.c.s_b + kvh];
+      for (int dt = 0; dt < DT; ++dt) vr[dt] = *reinterpret_cast<const u32x4v*>(v + ((16 * dt) << a.c.log_t));
+      vsb = at_lane.vs[at_lane.scale(bl.v)];
     };
 
     int i = next_tile(t0);
@@ -770,6 +786,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
       while (i < t1 && !in_sight(i)) ++i;
       return i;
     };
+    const PaLanes<D> at_lane(a, kvh, li, lg);
     // a step on its way: the wave's part of it, the scales of the lane's 16 positions
     u32x4v raw[PER];
     uint32_t rk, rv;
@@ -777,21 +794,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
     PaBlocks nb;
     auto load = [&](int p, PaBlocks bl) {
       if (wave < 2) {
-        const uint8_t* k = pa_keys<D>(a, kvh, p, bl.k, li, lg);
+        const uint8_t* k = at_lane.keys(p, bl.k);
 #pragma unroll
         for (int n = 0; n < PER; ++n) {
           const int f = wave * PER + n;
           raw[n] = *reinterpret_cast<const u32x4v*>(k + 4 * (f / KL) * D + 64 * (f % KL));
         }
       } else {
-        const uint8_t* v = pa_values<D>(a, kvh, p, bl.v, li, lg) + ((int64_t)((wave - 2) * PER * 16) << a.c.log_t);
+        const uint8_t* v = at_lane.values(p, bl.v) + (((wave - 2) * PER * 16) << a.c.log_t);
 #pragma unroll
-        for (int n = 0; n < PER; ++n)
-          raw[n] = *reinterpret_cast<const u32x4v*>(v + ((int64_t)(16 * n) << a.c.log_t));
+        for (int n = 0; n < PER; ++n) raw[n] = *reinterpret_cast<const u32x4v*>(v + ((16 * n) << a.c.log_t));
       }
-      const int64_t sc = (int64_t)max(bl.v, 0) * a.c.s_b + kvh;
-      rk = a.c.ks[sc];
-      rv = a.c.vs[sc];
+      const uint64_t sc = at_lane.scale(bl.v);
+      rk = at_lane.ks[sc];
+      rv = at_lane.vs[sc];
       rblock = bl.v;
     };
     // of the step that is worked on
@@ -857,6 +873,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
       // them all at once, for which there are no registers
       constexpr int A = 4;
       float4v s[RT][4];
+      __builtin_amdgcn_s_setprio(1);  // the other workgroup's wave has vector work meanwhile
       {
         u32x4v g[A];
 #pragma unroll
@@ -871,6 +888,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
           if (f & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       // above 0: a masked -inf stays one
       const float kc = fmaxf(e8m0(kb) * c, 1e-37f);
       const uint32_t there = block >= 0 ? 0xFFFFu : 0u;
@@ -903,6 +921,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
         }
       } else {
         u32x4v v[A];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int f = 0; f < A; ++f) v[f] = vf[f * 64];
 #pragma unroll
@@ -914,6 +933,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
             if (f + h + A < KF) v[(f + h) % A] = vf[(f + h + A) * 64];
           __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
     };
     while (i < t1) {

@@ -50,7 +50,8 @@ CACHE_BAD = [({k: None}, NULL) for k in ("kc", "vc", "ks", "vs")] + [
     (dict(k_b=16368), DIMS), (dict(v_b=16368), DIMS), (dict(s_b=1), DIMS), (dict(blocks=0), DIMS),
     (dict(blocks=1 << 31), DIMS), (dict(kvh=0), DIMS), (dict(kvh=4097), DIMS), (dict(block=40), DIMS),
     (dict(dim=96), DIMS), (dict(dim=512), DIMS), (dict(kc=P + 8), ALIGN), (dict(vc=P + 8), ALIGN),
-    (dict(k_b=16392), ALIGN), (dict(v_b=16392), ALIGN)]
+    (dict(k_b=16392), ALIGN), (dict(v_b=16392), ALIGN), (dict(k_b=1 << 31), DIMS), (dict(v_b=1 << 31), DIMS),
+    (dict(s_b=1 << 31), DIMS)]
 
 
 def test_write_blocks():
