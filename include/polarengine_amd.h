@@ -528,7 +528,8 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  * lengths share a pool of blocks of block_size positions (16, 32, 64 or 128). A
  * layer's cache: keys e4m3 [blocks, kv_heads, block_size, head_dim], values e4m3
  * [blocks, kv_heads, head_dim, block_size], each block and head with a power of two
- * as scale (e8m0 [blocks, kv_heads]: 2^(byte - 127)); a block's parts are contiguous
+ * as scale (e8m0 [blocks, kv_heads]: 2^(byte - 127), bytes 1 to 254); a block's parts
+ * are contiguous
  * and 16-byte aligned, k_b, v_b and s_b (below 2^31) the strides of blocks in bytes.
  * head_dim 64, 128 or 256. tables int32 [batch, width] (row stride t_b): the blocks
  * of each sequence in order of position, below 0 where it has none. All sizes that
@@ -573,7 +574,8 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  *       many tokens come before t (larger logit, or as large and of a lower number),
  *       entropy float32 of softmax(x), and the `top` likeliest tokens in order
  *       (top_logprobs float32, top_tokens int64, [rows, top], ties by number).
- *       A token outside the vocabulary: logprob 0, rank -1. top <= 64, vocab >= top.
+ *       A token outside the vocabulary: logprob 0, rank -1; a NaN logit counts as ruled
+ *       out. top <= 64, vocab >= top, rows < 2^24.
  */
 int pe_plan_step(const int64_t* lengths, const int64_t* counts, int32_t* tables, int64_t t_b,
                  int64_t batch, int64_t width, const int32_t* free_blocks, int64_t free_cap,

@@ -379,7 +379,7 @@ static size_t lp_bytes(const LpPlan& p, int64_t rows, int top) {
   return p.pieces == 1 ? 0 : (size_t)rows * p.pieces * (sizeof(LpSums) + (size_t)top * sizeof(LpKey));
 }
 static bool lp_shape_ok(int64_t rows, int64_t vocab, int top) {
-  return rows >= 0 && rows <= (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && top >= 0 && top <= kTopMax &&
+  return rows >= 0 && rows < (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && top >= 0 && top <= kTopMax &&
          top <= vocab;
 }
 

@@ -137,6 +137,10 @@ def test_rows_without_a_distribution():
     tokens = torch.arange(6, device=DEV)
     want = _lp().token_logprobs(x, tokens, 8)
     x[1, 77], x[3] = float("nan"), -math.inf
+    x[5, 3::7] = float("nan")  # ruled out
+    ruled = x.clone()
+    ruled[5, 3::7] = -math.inf
+    want = [torch.cat([w[:5], o[5:]]) for w, o in zip(want, _lp().token_logprobs(ruled, tokens, 8))]
     x[4, 4000] = math.inf
     got = _lp().token_logprobs(x, tokens, 8)
     for w, o in zip(want, got):

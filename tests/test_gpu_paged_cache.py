@@ -562,6 +562,28 @@ def test_attention_strided_queries_and_empty_batches():
     tab[:, ::2] = rest[1]
     assert torch.equal(pc.paged_attention(q.to(DEV), dev, tab[:, ::2], *rest[2:]), want)
     assert not pc.paged_attention(q.to(DEV), dev, rest[1], torch.zeros_like(rest[2]), rest[3]).any()
+    # every second block of a larger pool, whose others hold NaN
+    def wide(x):
+        big = torch.full((2 * x.shape[0], *x.shape[1:]), 0x7F, dtype=torch.uint8, device=DEV).view(x.dtype)
+        big.view(torch.uint8)[::2] = x.view(torch.uint8)
+        return big[::2]
+    assert torch.equal(pc.paged_attention(q.to(DEV), pc.PagedCache(*(wide(x) for x in dev)), *rest[1:]), want)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_rows_outside_all_sequences(n):
+    """Rows before the first sequence's, too, and batches of which nothing is left."""
+    say(f"attention rows outside n={n}")
+    rng, g = random.Random(19), torch.Generator().manual_seed(19)
+    q, cache, tables, starts, lengths = _attend_case(g, rng, 3, 2, 4, 64, 16, torch.float16, [n], 400)
+    lengths = [max(x, n) for x in lengths]
+    rows = starts[-1] + 9
+    q = torch.randn(rows, 8, 64, generator=g).half()
+    got = _attend_compare((q, cache, tables, [s + 5 for s in starts], lengths))
+    assert not got[:5].any() and not got[-4:].any() and got[5:-4].any()
+    assert not _attend_gpu(q, cache, tables, starts, [-1, -1, -1]).any()
+    # more rows than positions: those before position 0 see nothing
+    _attend_compare((q, cache, tables, starts, [min(x, 1 + n // 2) for x in lengths]), 3, 1)
 
 
 def test_attention_and_write_past_32_bits():

@@ -97,7 +97,8 @@ def test_token_logprobs():
     f = L.pe_token_logprobs
     assert f(*_change(a, rows=0)) == OK
     for new, rc in [({k: None}, NULL) for k in ("logits", "tokens", "lp", "rank", "ent", "tl", "tt")] + [
-            (dict(dtype=3), DTYPE), (dict(rows=-1), DIMS), (dict(vocab=0), DIMS), (dict(ld=999), DIMS),
+            (dict(dtype=3), DTYPE), (dict(rows=-1), DIMS), (dict(rows=1 << 24), DIMS), (dict(logits=P + 2), ALIGN),
+            (dict(vocab=0), DIMS), (dict(ld=999), DIMS),
             (dict(vocab=(1 << 24) + 1, ld=1 << 25), DIMS), (dict(top=-1), DIMS), (dict(top=65), DIMS),
             (dict(top=5, vocab=4), DIMS)]:
         assert f(*_change(a, **new)) == rc, new
