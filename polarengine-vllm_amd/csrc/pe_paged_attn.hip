@@ -51,6 +51,7 @@ struct PagedAttnArgs {
   int window;  // 0: none
   int sinks;
   float scale;
+  int whole;     // row blocks are not divided: each counts as one tile of the line
   int runs;
   float* parts;  // [runs][2]: a run divides at most its first and its last row block
   struct PaCut* cuts;  // [runs], behind the parts
@@ -109,6 +110,7 @@ __device__ __forceinline__ PaSpan pa_span(const PagedAttnArgs& a, const PaSeq& s
 // tiles of all row blocks of a sequence, one KV head
 template <int RB, int TILE>
 __device__ __forceinline__ int pa_tiles(const PagedAttnArgs& a, const PaSeq& s) {
+  if (a.whole) return s.blocks;
   int sum = 0;
   for (int qb = 0; qb < s.blocks; ++qb) sum += pa_span<RB, TILE>(a, s, qb).tiles;
   return sum;
@@ -167,6 +169,12 @@ __device__ __forceinline__ PaPlace pa_find(const PagedAttnArgs& a, PaChunk<RB> c
     const uint32_t hi = pa_from((int)(uint32_t)((uint64_t)c.seq.p0 >> 32), l);
     s.p0 = (int64_t)((uint64_t)hi << 32 | lo);
     s.blocks = pa_from(c.seq.blocks, l);
+    if (a.whole) {
+      r.b = b0 + l;
+      r.qb = left;
+      r.tiles = pa_span<RB, TILE>(a, s, left).tiles;
+      return r;
+    }
     for (int q0 = 0; q0 < s.blocks; q0 += 64) {
       const int t = q0 + lane < s.blocks ? pa_span<RB, TILE>(a, s, q0 + lane).tiles : 0;
       const int sc = wave_scan_i32(t, lane);
@@ -562,8 +570,8 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     const PaPlace here = pa_place(place);
     const int b = here.b, kvh = here.kvh, qb = here.qb, t0 = here.t0;
     if (b < 0) return;
-    const int t1 = (int)min((int64_t)here.tiles, t0 + (run.end - at));
-    at += t1 - t0;
+    const int t1 = a.whole ? here.tiles : (int)min((int64_t)here.tiles, t0 + (run.end - at));
+    at += a.whole ? 1 : t1 - t0;
     const PaSeq seq = here.seq;
     const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
@@ -760,8 +768,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
     const PaPlace here = pa_place(place);
     const int b = here.b, kvh = here.kvh, qb = here.qb, t0 = here.t0;
     if (b < 0) return;
-    const int t1 = (int)min((int64_t)here.tiles, t0 + (run.end - at));
-    at += t1 - t0;
+    const int t1 = a.whole ? here.tiles : (int)min((int64_t)here.tiles, t0 + (run.end - at));
+    at += a.whole ? 1 : t1 - t0;
     const PaSeq seq = here.seq;
     const PaSpan span = pa_span<RB, TILE>(a, seq, qb);
     const int32_t* table = a.tables + (int64_t)min(b, a.batch - 1) * a.t_b;
@@ -1026,9 +1034,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 //            256    73   -  92     223    -  214    495    -  392
 // Workgroups a CU: two of 16 or 128 rows (one with heads of 256: 16 rows, 16 x 4000, 59
 // us, two 72), one of 32 (64 rows, 16 x 4000, 58 us, two 76).
+//
+// Row blocks of up to four tiles (1024 positions that the tables have room for) are not
+// divided: no second launch. Microseconds divided and whole, heads of 128, one row block
+// a sequence, graph and eager: one sequence of 700 14.5 14.1 and 17.3 13.5, of 1400 14.0
+// 19.1 and 17.2 18.0; 16 of 959 16.9 15.6 and 17.2 14.5; 64 of 959 28.7 26.7 and 27.3
+// 25.4. Heads of 256 lose more by a whole block's steps (one sequence of 700: 18.4 21.5
+// eager), 128 rows by their fewer workgroups (700 positions: 34.3 41.2).
+constexpr int kPaWhole = 4;
 struct PaPlan {
   int rb;      // rows of a row block
   int runs;
+  bool whole;  // row blocks of so few tiles that they are not divided
   bool split;  // a row block may be divided
   bool fits;   // the tiles of a KV head can be counted in 32 bits
 };
@@ -1042,10 +1059,11 @@ static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int 
   const int64_t tiles = (positions + tile - 1) / tile;
   const int64_t blocks = rows * group / p.rb + batch + 1;  // row blocks of a KV head, at most
   p.fits = (double)blocks * (double)tiles < 1e9;
-  const double most = p.fits ? (double)blocks * tiles * kv_heads : 1e9;
+  p.whole = tiles <= (p.rb != 128 && dim != 256 ? kPaWhole : 1);
+  const double most = p.fits ? (double)blocks * (p.whole ? 1 : tiles) * kv_heads : 1e9;
   const int64_t wanted = (int64_t)num_cus() * (p.rb != 32 && dim != 256 ? 2 : 1);
   p.runs = (int)((double)wanted < most ? (double)wanted : most);
-  p.split = tiles > 1 && p.runs > 1;
+  p.split = !p.whole && p.runs > 1;
   return p;
 }
 
@@ -1133,6 +1151,7 @@ extern "C" int pe_paged_attention(const void* q, int dtype, int64_t q_r, int64_t
   a.window = (int)(window < kPagedMaxPositions ? window : 0);
   a.sinks = a.window ? (int)(sinks < kPagedMaxPositions ? sinks : kPagedMaxPositions) : 0;
   a.scale = scale;
+  a.whole = p.whole;
   a.runs = p.runs;
   a.parts = reinterpret_cast<float*>(workspace);
   a.cuts = p.split ? reinterpret_cast<PaCut*>(a.parts + (int64_t)p.runs * 2 * pa_part_words(p.rb, head_dim))
