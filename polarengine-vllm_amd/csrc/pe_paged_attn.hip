@@ -961,11 +961,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(cons
 // ---------------------------------------------------------------------------
 template <int D, bool BF, int RB>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
-  constexpr int E = D / 64, U = 8;
+  // rows of a wave: of 128 its workgroups would be many, most of them with nothing to do
+  // (1024 tokens behind 30,000: 27 us by one row)
+  constexpr int ROWS = RB == 128 ? 4 : 1;
+  constexpr int E = D / 64, U = ROWS == 1 ? 8 : 4;
   typedef float floatE __attribute__((ext_vector_type(E)));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t run = blockIdx.x;
-  const int local = blockIdx.y * 4 + wave;
   const PaCut cut = a.cuts[run];
   const int parts = cut.parts;
   if (!parts) return;
@@ -973,40 +975,60 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
   const float* base = a.parts + run * 2 * words;
   // the first part is its run's last, the others are their runs' first
   auto part = [&](int s) { return base + s * 2 * words + (s == 0 ? words : 0); };
-  {
-    const int r = cut.qb * RB + local;
-    const int token = r / a.group, g = r - token * a.group;
-    if (token >= cut.n) return;
-    float m = -__builtin_inff(), l = 0.f;
-    floatE o = 0.f;
-    for (int s0 = 0; s0 < parts; s0 += 64) {
-      const int here = min(64, parts - s0);
-      const float* p = part(s0 + min(lane, here - 1)) + RB * D + local;
-      const float pm = lane < here ? p[0] : -__builtin_inff(), pl = p[RB];
+  const int first = (blockIdx.y * 4 + wave) * ROWS;
+  if ((cut.qb * RB + first) / a.group >= cut.n) return;
+  float m[ROWS], l[ROWS];
+  floatE o[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    m[i] = -__builtin_inff();
+    l[i] = 0.f;
+    o[i] = 0.f;
+  }
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    const int here = min(64, parts - s0);
+    float w[ROWS];
+    const float* p = part(s0 + min(lane, here - 1)) + RB * D + first;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const float pm = lane < here ? p[i] : -__builtin_inff(), pl = p[RB + i];
       float mn = pm;
 #pragma unroll
       for (int off = 32; off >= 1; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off, 64));
-      mn = fmaxf(mn, m);
+      mn = fmaxf(mn, m[i]);
       const float shift = mn == -__builtin_inff() ? 0.f : mn;
-      const float w = __builtin_amdgcn_exp2f(pm - shift), al = __builtin_amdgcn_exp2f(m - shift);
-      m = mn;
-      o *= al;
-      l = l * al + wave_sum(lane < here ? w * pl : 0.f);
-      for (int s = 0; s < here; s += U) {
-        floatE t[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          t[u] = reinterpret_cast<const floatE*>(part(s0 + min(s + u, here - 1)) + local * D)[lane];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (s + u < here)
-            o += t[u] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + u));
-      }
+      const float al = __builtin_amdgcn_exp2f(m[i] - shift);
+      w[i] = __builtin_amdgcn_exp2f(pm - shift);
+      m[i] = mn;
+      o[i] *= al;
+      l[i] = l[i] * al + wave_sum_dpp(lane < here ? w[i] * pl : 0.f);
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    for (int s = 0; s < here; s += U) {
+      floatE t[U][ROWS];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float* q = part(s0 + min(s + u, here - 1)) + first * D;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) t[u][i] = reinterpret_cast<const floatE*>(q + i * D)[lane];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s + u < here)
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i)
+            o[i] += t[u][i] *
+                    __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[i]), s + u));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = cut.qb * RB + first + i;
+    const int token = r / a.group, g = r - token * a.group;
+    if (token >= cut.n) return;
+    const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
     uint16_t h[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = to16(o[e] * inv, BF);
+    for (int e = 0; e < E; ++e) h[e] = to16(o[i][e] * inv, BF);
     uint16_t* dst = a.out + ((int64_t)(cut.first + token) * a.c.kv_heads * a.group + cut.kvh * a.group + g) * D +
                     lane * E;
     __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
@@ -1077,7 +1099,7 @@ static bool pa_shape_ok(int64_t rows, int64_t batch, int heads, int kv_heads, in
 template <int D, bool BF>
 static int launch_pa(const PaPlan& p, const PagedAttnArgs& a, hipStream_t st) {
   const unsigned grid = (unsigned)((p.runs + 7) / 8 * 8);
-  const dim3 join((unsigned)p.runs, (unsigned)p.rb / 4);
+  const dim3 join((unsigned)p.runs, (unsigned)(p.rb == 128 ? p.rb / 16 : p.rb / 4));
   switch (p.rb) {
     case 16: paged_attn_kernel<D, BF, 1><<<grid, 256, 0, st>>>(a); break;
     case 32:
