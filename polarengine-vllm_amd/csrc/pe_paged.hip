@@ -35,11 +35,13 @@ __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t* waves, uint3
 // The plan, one workgroup: a thread a sequence, then a thread a row. What bounds it is
 // the chain of loads: lengths, table entries, free blocks, the rows' entries. A
 // sequence's first kPlanShort entries are its thread's, at once; of longer ones a wave
-// takes 64 at a time.
+// takes 64 at a time (a thread alone: 27.6 us for 496 users beside four chunks of up to
+// 2800 rows, this way 13.4; their release 17.2 -> 5.9). 64 users' step: 4.7 us, 3.4 for
+// its release.
 // ---------------------------------------------------------------------------
 constexpr int kPlanShort = 4;
 
-// sequences of a round that have more than kPlanShort entries to look at
+// sequences of a pass that have more than kPlanShort entries to look at
 struct PlanLong {
   uint32_t count;
   uint16_t of[kPlanThreads];
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_step_kernel(
     starts[0] = 0;
     used = 0;
   }
-  uint32_t row0 = 0, need0 = 0;  // of the sequences before this round's
+  uint32_t row0 = 0, need0 = 0;  // of the sequences before these
   for (int b0 = 0; b0 < batch; b0 += threads) {
     const int b = b0 + tid;
     const int64_t len = b < batch ? lengths[b] : -1;
@@ -261,7 +263,9 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(
 // dimensions: the run is read once, its largest |x| gives the scale, then codes go out.
 // Threads of a wave run over dimensions first for keys (rows of the block) and over
 // slots first for values (which the block stores by dimension), so that either writes
-// neighbouring bytes.
+// neighbouring bytes. What bounds it is the chain of slots, rows, largest value and codes
+// of a run: 32 rows of 8 heads of 128 6.4 us, 4 x 2048 rows 17 us (50 MB, 2.9 TB/s; with
+// a workgroup for every row 628).
 // ---------------------------------------------------------------------------
 // four codes; NaN where a value is not finite (the conversion itself would saturate)
 __device__ __forceinline__ uint32_t f8_codes(float a, float b, float c, float d) {
