@@ -745,8 +745,12 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 // worked on, the next one's operands are written and the loads of the one behind it are
 // under way; one barrier a step.
 // ---------------------------------------------------------------------------
+// workgroups a CU: as many as the registers hold (heads of 64, microseconds by two and
+// three: 1024 tokens behind 30,000 479 409, 16 x 64 behind 4000 89 85, 2048 tokens of a
+// prompt 82 90)
+constexpr int pa_chunk_wgs(int dim) { return dim == 256 ? 1 : dim == 64 ? 3 : 2; }
 template <int D, bool BF, int RT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_chunk_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const PagedAttnArgs a) {
   constexpr int RB = 64 * RT, TILE = 64;
   constexpr int KL = D / 64, DT = D / 16;
   constexpr int PER = DT / 2;          // 16-byte loads of a wave; 4 KL = DT of keys and of values
@@ -1047,7 +1051,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 // of 256, where they do not fit the registers), 128 beyond. That form's steps are dearer
 // where there are few of them: up to 128 rows it needs 64 (sequence, KV head) pairs.
 // Microseconds by 16, 32 and 128 rows, from a graph, one sequence of 8000 and of 30,000
-// and 16 of 4000 positions, 8 KV heads:
+// and 16 of 4000 positions, 8 KV heads (128 rows of heads of 64 by two workgroups a CU):
 //   head    rows      1 x 8000      1 x 30,000       16 x 4000
 //    64       32    23  24  30      25   33   44     29   32   50
 //             64    21  22  35      30   35   48     43   40   56
@@ -1061,8 +1065,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 //             64    36   -  76      89    -  126    153    -  213
 //            128    48   -  83     154    -  144    271    -  231
 //            256    73   -  92     223    -  214    495    -  392
-// Workgroups a CU: two of 16 or 128 rows (one with heads of 256: 16 rows, 16 x 4000, 59
-// us, two 72), one of 32 (64 rows, 16 x 4000, 58 us, two 76).
+// Workgroups a CU: two of 16 rows (one with heads of 256: 16 rows, 16 x 4000, 59 us, two
+// 72), one of 32 (64 rows, 16 x 4000, 58 us, two 76); of 128 as above.
 //
 // Row blocks of up to four tiles (1024 positions that the tables have room for) are not
 // divided: no second launch. Microseconds divided and whole, heads of 128, one row block
@@ -1090,7 +1094,7 @@ static PaPlan pa_plan(int64_t rows, int64_t batch, int heads, int kv_heads, int 
   p.fits = (double)blocks * (double)tiles < 1e9;
   p.whole = tiles <= (p.rb != 128 && dim != 256 ? kPaWhole : 1);
   const double most = p.fits ? (double)blocks * (p.whole ? 1 : tiles) * kv_heads : 1e9;
-  const int64_t wanted = (int64_t)num_cus() * (p.rb != 32 && dim != 256 ? 2 : 1);
+  const int64_t wanted = (int64_t)num_cus() * (p.rb == 128 ? pa_chunk_wgs(dim) : p.rb == 16 && dim != 256 ? 2 : 1);
   p.runs = (int)((double)wanted < most ? (double)wanted : most);
   p.split = !p.whole && p.runs > 1;
   return p;

@@ -313,8 +313,9 @@ class DecodeRunner:
                window: Optional[int], sinks: int):
         """A paged step's plan and its attention, as a function of (layer, qkv rows)."""
         c = self.cfg
-        if tokens.dim() != 1 or tokens.dtype != torch.int64:
-            raise ValueError(f"tokens must be int64 [rows], got {tokens.dtype} of {list(tokens.shape)}")
+        if tokens.dim() != 1 or tokens.dtype != torch.int64 or not tokens.numel():
+            raise ValueError(f"tokens must be int64 [rows], at least one, got {tokens.dtype} of "
+                             f"{list(tokens.shape)}")
         if len(pool.caches) != c.layers:
             raise ValueError(f"the pool has {len(pool.caches)} layers, the model {c.layers}")
         if pool.tables.shape[1] * pool.block_size > self.max_len:

@@ -297,6 +297,6 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     call("pe_paged_attention", dev, q.data_ptr(), code, q.stride(0), rows, heads, *args,
          tables.data_ptr(), _row_stride(tables), batch, width, starts.data_ptr(), lengths.data_ptr(),
-         window or 0, sinks, 1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(),
+         min(window or 0, 1 << 40), min(sinks, 1 << 40), 1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(),
          _lib.ptr(ws), size)
     return out

@@ -562,6 +562,8 @@ def test_attention_strided_queries_and_empty_batches():
     tab[:, ::2] = rest[1]
     assert torch.equal(pc.paged_attention(q.to(DEV), dev, tab[:, ::2], *rest[2:]), want)
     assert not pc.paged_attention(q.to(DEV), dev, rest[1], torch.zeros_like(rest[2]), rest[3]).any()
+    # a window and first positions past everything
+    assert torch.equal(pc.paged_attention(q.to(DEV), *rest, window=1 << 70, sinks=1 << 70), want)
     # every second block of a larger pool, whose others hold NaN
     def wide(x):
         big = torch.full((2 * x.shape[0], *x.shape[1:]), 0x7F, dtype=torch.uint8, device=DEV).view(x.dtype)

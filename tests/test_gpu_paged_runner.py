@@ -177,6 +177,8 @@ def test_refusals():
     with pytest.raises(ValueError):
         run.paged_step(_tokens((2,), 0).int(), counts, pool)
     with pytest.raises(ValueError):
+        run.paged_step(_tokens((0,), 0), counts, pool)
+    with pytest.raises(ValueError):
         _runner(1, 32).paged_step(_tokens((2,), 0), counts, pool)
     with pytest.raises(ValueError):
         _runner(1, 64, layers=1).paged_step(_tokens((2,), 0), counts, pool)
