@@ -574,8 +574,9 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  *       many tokens come before t (larger logit, or as large and of a lower number),
  *       entropy float32 of softmax(x), and the `top` likeliest tokens in order
  *       (top_logprobs float32, top_tokens int64, [rows, top], ties by number).
- *       A token outside the vocabulary: logprob 0, rank -1; a NaN logit counts as ruled
- *       out. top <= 64, vocab >= top, rows < 2^24.
+ *       A token outside the vocabulary: logprob 0, rank -1; a NaN logit counts as -inf,
+ *       in the given token, ranks and alternatives alike. top <= 64, vocab >= top, rows
+ *       < 2^24.
  */
 int pe_plan_step(const int64_t* lengths, const int64_t* counts, int32_t* tables, int64_t t_b,
                  int64_t batch, int64_t width, const int32_t* free_blocks, int64_t free_cap,

@@ -11,8 +11,8 @@
 // likeliest tokens so far lie sorted across its lanes; a chunk is looked through only
 // if one of its values passes the last of them, which is rare behind the first chunks.
 //
-// 2048 rows of 151,936 fp32: 224 us, 5.6 TB/s (bf16: 148 us, 4.2 TB/s, about eleven
-// vector instructions a value); one row with 20 alternatives 8 us and 6 us for the join,
+// 2048 rows of 151,936 fp32: 230 us, 5.4 TB/s (bf16: 159 us, 3.9 TB/s, about twelve
+// vector instructions a value, one of them for signalling NaN: 227 and 155 without); one row with 20 alternatives 8 us and 6 us for the join,
 // 7.4 us without alternatives; 48 rows of 100,003 bf16 with 5: 14 + 5 us, of which the
 // read would be 2.
 
@@ -51,13 +51,16 @@ __device__ __forceinline__ float lp_logit(const void* p, int64_t i) {
   else return f16or_bf(reinterpret_cast<const uint16_t*>(p)[i], DT == PE_DTYPE_BF16);
 }
 
+// A NaN logit is one of -inf: the token is ruled out.
+__device__ __forceinline__ float lp_ruled(float x) { return x != x ? -__builtin_inff() : x; }
+
 // A token as one number: the larger the logit the larger, of equal logits the lower
 // token; 0: none.
 typedef uint64_t LpKey;
 __device__ __forceinline__ LpKey lp_key(float x, int i) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);  // -0 is 0
   const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-  return x != x ? 0 : (uint64_t)o << 32 | ~(uint32_t)i;
+  return (uint64_t)o << 32 | ~(uint32_t)i;
 }
 __device__ __forceinline__ float lp_value(LpKey k) {
   const uint32_t o = (uint32_t)(k >> 32);
@@ -211,7 +214,7 @@ __device__ __forceinline__ void lp_answer(const LogprobArgs& a, int row, const L
     float lp = 0.f;
     int64_t rank = -1;
     if (tok >= 0 && tok < a.vocab) {
-      const float xt = lp_logit<DT>(a.logits, row * a.ld + tok);
+      const float xt = lp_ruled(lp_logit<DT>(a.logits, row * a.ld + tok));
       lp = (float)((double)(xt - s.m) - lz);
       rank = s.rank;
     }
@@ -239,7 +242,10 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
   const int64_t tok64 = a.tokens[row];
   const bool there = tok64 >= 0 && tok64 < a.vocab;
   const int tok = there ? (int)tok64 : 0;
-  const float xt = there ? lp_logit<DT>(a.logits, row * a.ld + tok) : __builtin_nanf("");
+  const float xt = there ? lp_ruled(lp_logit<DT>(a.logits, row * a.ld + tok)) : __builtin_nanf("");
+  // Among ruled-out tokens NaN and -inf tie: such a token's rank is counted apart, so that
+  // a comparison for which NaN does not hold serves all others.
+  const bool ruled = xt == -__builtin_inff();
 
   LpList list;
   list.begin();
@@ -268,14 +274,20 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         x[j] = __builtin_bit_cast(float, j & 1 ? w & 0xFFFF0000u : w << 16);
       else x[j] = h2f((uint16_t)(w >> (16 * (j & 1))));
     }
+    // a signalling NaN would take the maximum's other operand with it (fp16's are quiet
+    // after their conversion)
+    if constexpr (DT != PE_DTYPE_F16)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_canonicalizef(x[j]);
     auto index = [&](int j) { return (c + (j / PER) * 64 + lane) * PER + j % PER - off; };
     // outside the row and past the piece: NaN, which no comparison holds for
-    if (c == 0 || c + 64 * U > g1 || c + 64 * U >= all) {
+    auto outside = [&](int j) {
+      return ((uint32_t)index(j) >= (uint32_t)a.vocab) | (c + (j / PER) * 64 + lane >= g1);
+    };
+    const bool edge = c == 0 || c + 64 * U > g1 || c + 64 * U >= all;
+    if (edge) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool out = ((uint32_t)index(j) >= (uint32_t)a.vocab) | (c + (j / PER) * 64 + lane >= g1);
-        x[j] = out ? __builtin_nanf("") : x[j];
-      }
+      for (int j = 0; j < 8; ++j) x[j] = outside(j) ? __builtin_nanf("") : x[j];
     }
     float cm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     if (__any(cm > m)) {
@@ -300,6 +312,11 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     z += zs;
     e += es;
     // ties count where they come before the token; its own granule is looked at below
+    if (__builtin_expect(ruled, 0)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        rank += __builtin_popcountll(__ballot(x[j] > xt || (!outside(j) && index(j) < tok)));
+    } else
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint64_t before = __ballot((c + u * 64 + lane) * PER + PER - 1 - off < tok);
@@ -308,15 +325,18 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         rank += __builtin_popcountll(__ballot(x[j] > xt) | (__ballot(x[j] == xt) & before));
     }
     if constexpr (TOP)
-      if (__any(cm > list.last_x) || (list.last == 0 && __any(cm == list.last_x))) {
+      if (__any(cm > list.last_x) || list.last == 0) {
         LpKey k[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = lp_key(x[j], index(j));
+        for (int j = 0; j < 8; ++j) k[j] = lp_key(lp_ruled(x[j]), index(j));
+        if (edge)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) k[j] = outside(j) ? 0 : k[j];
         list.offer(k, lane, a.top);
       }
   }
   rank = lane == 0 ? rank : 0;
-  if (there && piece == 0 && wave == 0 && lane < PER) {
+  if (there && !ruled && piece == 0 && wave == 0 && lane < PER) {
     // ties before the token in its granule
     const int i = (tok + off) / PER * PER - off + lane;
     rank += i >= 0 && i < tok && lp_logit<DT>(a.logits, row * a.ld + i) == xt;

@@ -29,9 +29,9 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Of logits [rows, vocab] (fp32, fp16 or bf16; -inf where a token is ruled out) and
     tokens int64 [rows] (outside the vocabulary: none, with logprob 0 and rank -1).
-    Equal logits rank by number. ``top``: 0 to 64, at most the vocabulary (-1 where a row
-    has no more). A NaN counts as ruled out. A row with +inf, or without a finite logit,
-    has no distribution: its numbers say nothing."""
+    Equal logits rank by number. ``top``: 0 to 64, at most the vocabulary. A NaN counts as
+    -inf; ruled-out tokens have logprob -inf and follow the others by number. A row with
+    +inf, or without a finite logit, has no distribution: its numbers say nothing."""
     dev = inputs(logits, tokens)
     code = _DTYPES.get(logits.dtype)
     if code is None:
