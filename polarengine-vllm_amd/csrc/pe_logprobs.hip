@@ -12,9 +12,9 @@
 // if one of its values passes the last of them, which is rare behind the first chunks.
 //
 // 2048 rows of 151,936 fp32: 230 us, 5.4 TB/s (bf16: 159 us, 3.9 TB/s, about twelve
-// vector instructions a value, one of them for signalling NaN: 227 and 155 without); one row with 20 alternatives 8 us and 6 us for the join,
-// 7.4 us without alternatives; 48 rows of 100,003 bf16 with 5: 14 + 5 us, of which the
-// read would be 2.
+// vector instructions a value, one of them for signalling NaN: 227 and 155 without); one
+// row with 20 alternatives 8 us and 6 us for the join, 7.4 us without alternatives; 48
+// rows of 100,003 bf16 with 5: 14 + 5 us, of which the read would be 2.
 
 #include "pe_internal.h"
 
@@ -175,7 +175,7 @@ __device__ __forceinline__ LpSums lp_join(LpSums s, LpSums* shared, int lane, in
   auto onto = [](LpSums v, float to) {  // relative to `to`
     const float d = v.m - to;
     const double f = v.z > 0 ? (double)__builtin_amdgcn_exp2f(d * kLpLog2e) : 0.0;
-    v.e = v.z > 0 ? f * (v.e + d * v.z) : 0.0;
+    v.e = f > 0 ? f * (v.e + d * v.z) : 0.0;  // d may be -inf, also of finite logits
     v.z *= f;
     v.m = to;
     return v;
@@ -294,8 +294,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
       const float mn = fmaxf(m, cm);
       if (mn > m) {
         const float d = m - mn;
-        const double f = m == -__builtin_inff() ? 0.0 : (double)__builtin_amdgcn_exp2f(d * kLpLog2e);
-        e = m == -__builtin_inff() ? 0.0 : f * (e + d * z);
+        const double f = __builtin_amdgcn_exp2f(d * kLpLog2e);
+        e = f > 0 ? f * (e + d * z) : 0.0;  // d may be -inf, also of finite logits
         z *= f;
         m = mn;
       }
