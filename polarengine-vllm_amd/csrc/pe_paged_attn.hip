@@ -12,16 +12,20 @@
 //  * the probabilities, in fp16, are the B operand of O^T = V^T P^T just as the scores'
 //    products left them, and the lane's part of V^T is 16 neighbouring bytes of the
 //    block's values, which are stored by dimension. Nothing goes through LDS;
-//  * e4m3 values are exact in fp16 and bf16 (v_cvt_scalef32_pk, two a instruction).
-//    The keys' scale multiplies the fp32 scores; the values' is applied by the
-//    conversion, relative to the largest that the wave has seen (er: sums are rescaled
-//    when it grows), 2^7 times as large: codes of a scale down to 2^-22 of the largest
-//    stay exact.
-//  * one pass with running maximum and sum in fp32. Probabilities are 2^7 times as
-//    large and relative to a base that moves only when they would pass 2^15, so that
-//    fp16 keeps what is 2^-21 of the largest whole and what is above 2^-32 of it in
-//    part. Rounding them costs half an fp16 step of each (in the sum that divides
-//    alike): less than the rounding of a bf16 result, about that of an fp16 one.
+//  * e4m3 codes are exact in fp16 and bf16 (v_cvt_scalef32_pk, two a instruction).
+//    The keys' scale multiplies the fp32 scores, the values' the probabilities: what
+//    goes through the second product with the codes is probability times scale;
+//  * one pass with running maxima and sums in fp32, both by row: of the scores, for the
+//    sum that divides, and of probability times scale. So a row's result depends on
+//    what that row sees alone, whatever scales others' positions, positions behind the
+//    sequence's end or hidden by a window have. A product is 2^7 times as large and
+//    relative to a base that moves only when it would pass 2^15, so that fp16 keeps
+//    what is 2^-20 of the row's largest whole and what is above 2^-31 of it in part.
+//    Rounding them costs half an fp16 step of each: less than the rounding of a bf16
+//    result, about that of an fp16 one. The sum that divides is that of the unrounded
+//    ones, since a block's share of it does not go by its scale;
+//  * NaN codes are zeros for the products, in steps that some row does not see whole; a
+//    map of where they are says which sums become NaN.
 // The tiles of all sequences, KV heads and row blocks form one line, cut into equal
 // runs, one a workgroup, by the lengths read on the device; a second launch joins the
 // parts of a row block that a cut divides.
@@ -39,8 +43,11 @@ namespace pe {
 
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaSlack = 8.f;    // powers of two that an exponent may exceed its base by
-constexpr float kPaLift = 7.f;     // and by which probabilities are larger
-constexpr int kPaVLift = 7;        // and values
+constexpr float kPaLift = 7.f;     // and by which products of probability and scale are larger
+// A value's scale is taken for at least 2^-60 of what the row's largest product implies:
+// what is smaller vanishes in fp16 either way, and the probability can be had back from
+// the product in fp32.
+constexpr float kPaLeast = -60.f;
 
 struct PagedAttnArgs {
   const uint16_t* q;
@@ -220,9 +227,10 @@ __device__ __forceinline__ float4v pa_mfma(u32x4v a, u32x4v b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, a),
                                                   __builtin_bit_cast(half8v, b), c, 0, 0, 0);
 }
-// eight e4m3 values times a power of two, as bf16 or fp16
+// eight e4m3 codes as bf16 or fp16
 template <bool BF>
-__device__ __forceinline__ u32x4v pa_unpack(uint32_t lo, uint32_t hi, float s) {
+__device__ __forceinline__ u32x4v pa_unpack(uint32_t lo, uint32_t hi) {
+  constexpr float s = 1.f;
   if constexpr (BF)
     return u32x4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false)),
                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true)),
@@ -257,9 +265,17 @@ __device__ __forceinline__ float pa_rows_max(float v) {
 __device__ __forceinline__ uint32_t pa_nan(uint32_t w) {
   return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
-// bit 15 of each fp16 value that is not finite (converted codes: NaN)
-__device__ __forceinline__ uint32_t pa_nan16(uint32_t w) {
-  return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+__device__ __forceinline__ uint32_t pa_nan(u32x4v w) { return pa_nan(w[0]) | pa_nan(w[1]) | pa_nan(w[2]) | pa_nan(w[3]); }
+// NaN among 16 codes made zeros; a bit for each
+__device__ __forceinline__ uint32_t pa_clean(u32x4v& w) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t n = pa_nan(w[i]) >> 7;  // bits 0, 8, 16 and 24
+    bits |= ((n * 0x10204080u) >> 28) << (4 * i);
+    w[i] = w[i] & ~(n * 0xFFu);
+  }
+  return bits;
 }
 
 // the bits of positions below n, of 16
@@ -301,22 +317,6 @@ __device__ __forceinline__ float* pa_part(const PagedAttnArgs& a, const PaRun& r
   return a.parts + (run.run * 2 + (p.t0 == 0)) * words;
 }
 
-// The largest exponent byte of values so far: vb is that of the lane's 16 positions (0:
-// none there).
-__device__ __forceinline__ int pa_largest(int er, int vb) {
-  if (__any(vb > er)) {
-    int top = vb;
-#pragma unroll
-    for (int k = 32; k; k >>= 1) top = max(top, __shfl_xor(top, k, 64));
-    er = __builtin_amdgcn_readfirstlane(max(top, er));
-  }
-  return er;
-}
-// and the factor that the conversion gives the lane's values
-__device__ __forceinline__ float pa_factor(int vb, int er) {
-  return e8m0((uint32_t)max(127 + kPaVLift + vb - er, 1));
-}
-
 // What a wave keeps of RT products of 16 rows.
 template <int D, int RT>
 struct PaRows {
@@ -324,13 +324,14 @@ struct PaRows {
   u32x4v q[RT][KS];  // B operand: lane = row li, dimensions 64 j + 16 lg + 8 h of product 2 j + h
   int pos[RT];       // of the lane's rows, below 0: sees nothing
   float4v o[RT][DT];
-  float m[RT], l[RT];
-  int er;            // the values' scale (exponent byte) that o is relative to
+  // bases, whole numbers, so that their powers of two are exact: scores are relative to
+  // m (-inf: none seen yet), scores plus the values' exponent bytes, and o, to m + d
+  float m[RT], d[RT];
+  float l[RT];
 
   // rows first .. first + 16 RT - 1 of the row block
   __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PaSeq& seq, int kvh, int first, int li,
                                         int lg) {
-    er = 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = first + rt * 16 + li;
@@ -346,6 +347,7 @@ struct PaRows {
         if (there) q[rt][ks] = *reinterpret_cast<const u32x4v*>(src + 64 * (ks >> 1) + 8 * (ks & 1));
       }
       m[rt] = -__builtin_inff();
+      d[rt] = 0.f;
       l[rt] = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -367,18 +369,11 @@ struct PaRows {
           s[rt][t][e] = seen[rt] & (1u << (4 * t + e)) ? s[rt][t][e] : -__builtin_inff();
     }
   }
-  // sums relative to another scale of values, `to`, that is larger
-  __device__ __forceinline__ void rescale(int to) {
-    const float f = __builtin_ldexpf(1.f, max(er - to, -200));
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-    er = to;
-  }
   // p: B operands of two products, 8 neighbouring positions each. kc: what the scores
-  // of the lane are multiplied by
-  __device__ __forceinline__ void softmax(const float4v (&s)[RT][4], float kc, u32x4v (&p)[RT][2]) {
+  // of the lane are multiplied by; vb: exponent byte of its values
+  __device__ __forceinline__ void softmax(float4v (&s)[RT][4], float kc, float vb, u32x4v (&p)[RT][2]) {
+    // the base is a rounded product, and what is compared with it has to be
+#pragma clang fp contract(off)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float top = -__builtin_inff();
@@ -387,61 +382,64 @@ struct PaRows {
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[rt][t][e]);
       top *= kc;
-      if (__any(top > m[rt] + kPaSlack)) {
-        const float mn = fmaxf(m[rt], pa_rows_max(top));
-        const float al = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
-        l[rt] *= al;
+      // the larger of the score's and the product's exponent (NaN where nothing is seen)
+      if (__any(top - m[rt] + fmaxf(vb - d[rt], 0.f) > kPaSlack)) {
+        const float mn = fmaxf(m[rt], ceilf(pa_rows_max(top)));
+        const float to = mn == -__builtin_inff() ? 0.f : mn;
+        const float dm = m[rt] - to;
+        const float dn = fmaxf(d[rt] + dm, ceilf(pa_rows_max(top - to + vb)));
+        const float dz = dn == -__builtin_inff() ? 0.f : dn;
+        const float al = __builtin_amdgcn_exp2f(d[rt] + dm - dz);
+        l[rt] *= __builtin_amdgcn_exp2f(dm);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= al;
         m[rt] = mn;
+        d[rt] = dz;
       }
-      const float base = (m[rt] == -__builtin_inff() ? 0.f : m[rt]) - kPaLift;
+      const float base = m[rt] == -__builtin_inff() ? 0.f : m[rt];
+      const float lift = fmaxf(vb - d[rt], kPaLeast) + kPaLift;
+      float mul = kc, add = lift - base;
+      // beside a base of that size the lift would be rounded, and an exponent that is
+      // rounded once could pass the base, which is a rounded product, by its rounding
+      if (__builtin_expect(__any(fabsf(base) > 0x1p22f), 0)) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[rt][t][e] = s[rt][t][e] * kc - base;
+        mul = 1.f;
+        add = lift;
+      }
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][e], kc, -base));
-        const uint32_t w0 = pa_pack(w[0], w[1]), w1 = pa_pack(w[2], w[3]);
-        // the sum is that of the rounded probabilities
-        const half2v ones{(_Float16)1.f, (_Float16)1.f};
-        l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w0), ones, l[rt], false);
-        l[rt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w1), ones, l[rt], false);
-        p[rt][t >> 1][2 * (t & 1)] = w0;
-        p[rt][t >> 1][2 * (t & 1) + 1] = w1;
+        for (int e = 0; e < 4; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][e], mul, add));
+          sum[e & 1] += w[e];
+        }
+        p[rt][t >> 1][2 * (t & 1)] = pa_pack(w[0], w[1]);
+        p[rt][t >> 1][2 * (t & 1) + 1] = pa_pack(w[2], w[3]);
       }
+      l[rt] = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_exp2f(-lift), l[rt]);
     }
   }
-  // fp16 values of 16 dimensions, positions 8 h .. 8 h + 7 of the lane's 16, where some
-  // are NaN. NaN must not reach, as 0 x NaN, the rows that do not see it: for the product
-  // it is a zero, and a product of where it is with what each row sees says which sums
-  // are NaN. `any`: positions that some row of the block sees; the others hold anything.
-  static __device__ __forceinline__ uint32_t pairs(uint32_t bits, int h, int w) {
-    return (bits >> (8 * h + 2 * w) & 1u) * 0xFFFFu | (bits >> (8 * h + 2 * w + 1) & 1u) * 0xFFFF0000u;
-  }
-  static __device__ __forceinline__ u32x4v clean(u32x4v v) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t u = v[w];
-      v[w] = u & ~((pa_nan16(u) >> 15) * 0xFFFFu);
-    }
-    return v;
-  }
-  __device__ __forceinline__ void nan_values(u32x4v v, int dt, int h, const uint32_t (&seen)[RT], uint32_t any) {
-    u32x4v nf;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t u = v[w];
-      nf[w] = (pa_nan16(u) >> 15) * 0xFFFFu & pairs(any, h, w) & 0x3C003C00u;  // 1.0
-    }
+  // A NaN among the values must not reach, as 0 x NaN, the rows that do not see it: for
+  // the products it is a zero (pa_clean), and the sums of rows that see it are made NaN
+  // here. map: the step's 64 positions, a bit each, of every dimension; FROM, TO: 16
+  // dimensions each; seen: as mask() has it.
+  template <int FROM, int TO>
+  __device__ __forceinline__ void nan_values(const uint64_t* map, const uint32_t (&seen)[RT], int lg) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      u32x4v sf;
+      unsigned long long all = (unsigned long long)seen[rt] << (16 * lg);
+      all |= __shfl_xor(all, 16, 64);
+      all |= __shfl_xor(all, 32, 64);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sf[w] = pairs(seen[rt], h, w) & 0x3C003C00u;
-      const float4v hit = pa_mfma<false>(nf, sf, float4v{0.f, 0.f, 0.f, 0.f});
+      for (int dt = FROM; dt < TO; ++dt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[rt][dt][e] = hit[e] > 0.f ? __builtin_nanf("") : o[rt][dt][e];
+        for (int e = 0; e < 4; ++e)
+          if (map[16 * dt + 4 * lg + e] & all) o[rt][dt][e] = __builtin_nanf("");
     }
   }
   __device__ __forceinline__ void values(u32x4v v, int dt, int h, const u32x4v (&p)[RT][2]) {
@@ -450,9 +448,9 @@ struct PaRows {
   }
   // the row's whole sum in all of its lanes, sums in units of 1
   __device__ __forceinline__ void finish() {
-    const float unit = __builtin_ldexpf(1.f, er - 127 - kPaVLift);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+      const float unit = __builtin_amdgcn_exp2f(d[rt] - 127.f - kPaLift);
       l[rt] += __shfl_xor(l[rt], 16, 64);
       l[rt] += __shfl_xor(l[rt], 32, 64);
 #pragma unroll
@@ -536,11 +534,6 @@ struct PaLanes {
     return (uint64_t)(uint32_t)max(block, 0) * s_b;
   }
 };
-// bits of the lane's 16 positions from x on that some row of the block sees
-__device__ __forceinline__ uint32_t pa_any(const PaSpan& span, int x, uint32_t there) {
-  return pa_below(span.hi - x) & (~pa_below(span.lo - x) | pa_below(span.sink - x)) & there;
-}
-
 // ---------------------------------------------------------------------------
 // Few rows: the four waves of a workgroup take 64 positions each of a tile of 256,
 // straight from memory to registers, and join their sums in LDS at the end of a row
@@ -552,7 +545,7 @@ template <int D, bool BF, int RT>
 __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
   constexpr int RB = 16 * RT, TILE = 256;
   constexpr int KS = D / 32, KL = D / 64, DT = D / 16;
-  __shared__ __align__(16) float4v join[2][RT * DT * 64];
+  __shared__ __align__(16) float4v join[2][RT * DT * 64];  // and, until then, each wave's map of NaN
   __shared__ float join_m[4][RB], join_l[4][RB];
   __shared__ PaPlace place;
   __shared__ int64_t line;
@@ -602,6 +595,7 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     };
     u32x4v kr[4][KL], vr[DT];
     uint32_t ksb, vsb;
+    uint16_t* const nan_map = reinterpret_cast<uint16_t*>(&join[0][0]) + wave * D * 4;
     auto load_k = [&](int p, PaBlocks bl) {
       const uint8_t* k = at_lane.keys(p, bl.k);
 #pragma unroll
@@ -639,7 +633,7 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
         for (int rt = 0; rt < RT; ++rt) s[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const u32x4v kf = pa_unpack<BF>(kr[t][ks >> 1][2 * (ks & 1)], kr[t][ks >> 1][2 * (ks & 1) + 1], 1.f);
+          const u32x4v kf = pa_unpack<BF>(kr[t][ks >> 1][2 * (ks & 1)], kr[t][ks >> 1][2 * (ks & 1) + 1]);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[rt][t] = pa_mfma<BF>(kf, w.q[rt][ks], s[rt][t]);
         }
@@ -648,38 +642,27 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
       const float kc = fmaxf(e8m0(ksb) * c, 1e-37f);
       if (in < t1) load_k(first_pos(in), nxt);
       uint32_t seen[RT];
-      bool slow = false;
+      bool some_nan = false;
       if (!full) {
-        const uint32_t there = cur.v >= 0 ? 0xFFFFu : 0u;
-        w.mask(a, s, seen, p + 16 * lg, there);
-        // NaN codes of positions that a row does not see must not reach it as 0 x NaN
+        w.mask(a, s, seen, p + 16 * lg, cur.v >= 0 ? 0xFFFFu : 0u);
         uint32_t bad = 0;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          bad |= pa_nan(vr[dt][0]) | pa_nan(vr[dt][1]) | pa_nan(vr[dt][2]) | pa_nan(vr[dt][3]);
-        slow = __any(bad != 0);
+        for (int dt = 0; dt < DT; ++dt) bad |= pa_nan(vr[dt]);
+        some_nan = __any(bad != 0);
+        if (__builtin_expect(some_nan, 0))
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) nan_map[(16 * dt + li) * 4 + lg] = (uint16_t)pa_clean(vr[dt]);
       }
-      const int vb = cur.v >= 0 ? (int)vsb : 0, er = pa_largest(w.er, vb);
-      if (er != w.er) w.rescale(er);
-      const float vscale = pa_factor(vb, er);
       u32x4v pf[RT][2];
-      w.softmax(s, kc, pf);
-      auto unpack = [&](int dt, int h) { return pa_unpack<false>(vr[dt][2 * h], vr[dt][2 * h + 1], vscale); };
-      if (__builtin_expect(!slow, 1)) {
+      w.softmax(s, kc, (float)vsb, pf);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) w.values(unpack(dt, h), dt, h, pf);
-      } else {
-        const uint32_t any = pa_any(span, p + 16 * lg, cur.v >= 0 ? 0xFFFFu : 0u);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x4v v = unpack(dt, h);
-            w.values(w.clean(v), dt, h, pf);
-            w.nan_values(v, dt, h, seen, any);
-          }
+        for (int h = 0; h < 2; ++h)
+          w.values(pa_unpack<false>(vr[dt][2 * h], vr[dt][2 * h + 1]), dt, h, pf);
+      if (__builtin_expect(some_nan, 0)) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // other lanes' bits
+        w.template nan_values<0, DT>(reinterpret_cast<const uint64_t*>(nan_map), seen, lg);
       }
       if (in < t1) load_v(first_pos(in), nxt);
       cur = nxt;
@@ -757,6 +740,9 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
   constexpr int KF = 2 * DT;           // operands of keys, 1 KB each, then as many of values
   __shared__ __align__(16) u32x4v buf0[2 * KF * 64];
   __shared__ __align__(16) u32x4v buf1[2 * KF * 64];
+  // positions of NaN by dimension, and whether a wave that brings values had any
+  __shared__ uint64_t nan0[D], nan1[D];
+  __shared__ uint32_t some0[2], some1[2];
   __shared__ PaPlace place;
   __shared__ int64_t line;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -790,6 +776,9 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
     const int64_t p_low = seq.lead ? -1 : seq.p0 + token0;
     const int64_t p_high = seq.p0 + min(token1, seq.n - 1);
     const bool idle = token0 >= seq.n;
+    // and of the row block's
+    const int64_t block_low = seq.lead ? -1 : seq.p0 + qb * RB / a.group;
+    const int64_t block_high = seq.p0 + min((qb * RB + RB - 1) / a.group, seq.n - 1);
     PaRows<D, RT> w;
     w.begin(a, seq, kvh, first, li, lg);
     const float c = a.scale * kPaLog2e;
@@ -829,43 +818,48 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
       rv = at_lane.vs[sc];
       rblock = bl.v;
     };
-    // of the step that is worked on
-    int block = -1, er = 0;
-    uint32_t kb = 0;
-    // and of the one whose operands are in LDS next
-    int nblock = -1, ner = 0;
-    uint32_t nkb = 0;
-    auto convert = [&](u32x4v* to) {
-      const int vb = rblock >= 0 ? (int)rv : 0;
-      nblock = rblock;
-      nkb = rk;
-      ner = pa_largest(er, vb);
-      const float f = pa_factor(vb, ner);
+    // of the step that is worked on, and of the one whose operands are in LDS next
+    uint32_t sc = 0, nsc = 0;
+    auto convert = [&](u32x4v* to, uint64_t* nan_map, uint32_t* some_nan, int p) {
+      nsc = rk | rv << 8 | (rblock >= 0 ? 1u << 16 : 0u);
+      if (wave >= 2) {
+        // a NaN that all rows see makes them all NaN as it is
+        uint32_t bad = 0;
+        if (p + 63 > block_low || __any(rblock < 0) ||
+            (a.window && p <= block_high - a.window && p + 64 > a.sinks)) {
+#pragma unroll
+          for (int n = 0; n < PER; ++n) bad |= pa_nan(raw[n]);
+        }
+        const bool some = __any(bad != 0);
+        if (__builtin_expect(some, 0))
+#pragma unroll
+          for (int n = 0; n < PER; ++n)
+            reinterpret_cast<uint16_t*>(nan_map)[(((wave - 2) * PER + n) * 16 + li) * 4 + lg] =
+                (uint16_t)pa_clean(raw[n]);
+        if (lane == 0) some_nan[wave - 2] = some;
+      }
       u32x4v* dst = to + (wave * PER * 2) * 64 + lane;
 #pragma unroll
       for (int n = 0; n < PER; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          dst[(2 * n + h) * 64] = BF && wave < 2 ? pa_unpack<true>(raw[n][2 * h], raw[n][2 * h + 1], 1.f)
-                                                 : pa_unpack<false>(raw[n][2 * h], raw[n][2 * h + 1],
-                                                                    wave < 2 ? 1.f : f);
+          dst[(2 * n + h) * 64] = BF && wave < 2 ? pa_unpack<true>(raw[n][2 * h], raw[n][2 * h + 1])
+                                                 : pa_unpack<false>(raw[n][2 * h], raw[n][2 * h + 1]);
     };
     int i = next_tile(t0), in = next_tile(i + 1), after = next_tile(in + 1);
     if (i < t1) {
       load(first_pos(i), pa_blocks(a, table, first_pos(i), li, lg));
-      convert(buf0);
+      convert(buf0, nan0, some0, first_pos(i));
       if (in < t1) load(first_pos(in), pa_blocks(a, table, first_pos(in), li, lg));
       if (after < t1) nb = pa_blocks(a, table, first_pos(after), li, lg);
     }
-    auto step = [&](const u32x4v* from, u32x4v* to) {
+    auto step = [&](const u32x4v* from, const uint64_t* nan_map, const uint32_t* some_nan, u32x4v* to,
+                    uint64_t* nan_to, uint32_t* some_to) {
       const int p = first_pos(i);
-      block = nblock;
-      kb = nkb;
-      er = ner;
-      if (er != w.er) w.rescale(er);
+      sc = nsc;
       __syncthreads();  // the operands are there, and `to` is done with
       if (in < t1) {
-        convert(to);
+        convert(to, nan_to, some_to, first_pos(in));
         if (after < t1) {
           load(first_pos(after), nb);
           const int behind = next_tile(after + 1);
@@ -884,7 +878,7 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
       const bool none = idle || p > p_high ||
                         (a.window && p + 63 <= max(p_low, (int64_t)-1) - a.window && p >= a.sinks);
       if (none) return;
-      const bool full = p + 63 <= p_low && !__any(block < 0) &&
+      const bool full = p + 63 <= p_low && !__any(!(sc >> 16)) &&
                         (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
       const u32x4v* kf = from + lane;
       const u32x4v* vf = kf + KF * 64;
@@ -909,36 +903,15 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
       }
       __builtin_amdgcn_s_setprio(0);
       // above 0: a masked -inf stays one
-      const float kc = fmaxf(e8m0(kb) * c, 1e-37f);
-      const uint32_t there = block >= 0 ? 0xFFFFu : 0u;
+      const float kc = fmaxf(e8m0(sc & 0xFFu) * c, 1e-37f);
+      const uint32_t there = sc >> 16 ? 0xFFFFu : 0u;
       uint32_t seen[RT];
-      bool slow = false;
-      if (!full) {
-        w.mask(a, s, seen, p + 16 * lg, there);
-        uint32_t bad = 0;
 #pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          const u32x4v v = vf[f * 64];
-          bad |= pa_nan16(v[0]) | pa_nan16(v[1]) | pa_nan16(v[2]) | pa_nan16(v[3]);
-          if ((f & 3) == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-        slow = __any(bad != 0);
-      }
+      for (int rt = 0; rt < RT; ++rt) seen[rt] = 0xFFFFu;
+      if (!full) w.mask(a, s, seen, p + 16 * lg, there);
       u32x4v pf[RT][2];
-      w.softmax(s, kc, pf);
-      if (__builtin_expect(slow, 0)) {
-#pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          w.values(w.clean(vf[f * 64]), f >> 1, f & 1, pf);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        const uint32_t any = pa_any(span, p + 16 * lg, there);
-#pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          w.nan_values(vf[f * 64], f >> 1, f & 1, seen, any);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
+      w.softmax(s, kc, (float)(sc >> 8 & 0xFFu), pf);
+      {
         u32x4v v[A];
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -954,10 +927,12 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
         }
         __builtin_amdgcn_s_setprio(0);
       }
+      if (__builtin_expect(pa_uniform(some_nan[0]), 0)) w.template nan_values<0, DT / 2>(nan_map, seen, lg);
+      if (__builtin_expect(pa_uniform(some_nan[1]), 0)) w.template nan_values<DT / 2, DT>(nan_map, seen, lg);
     };
     while (i < t1) {
-      step(buf0, buf1);
-      if (i < t1) step(buf1, buf0);
+      step(buf0, nan0, some0, buf1, nan1, some1);
+      if (i < t1) step(buf1, nan1, some1, buf0, nan0, some0);
     }
     w.finish();
     float* part = pa_part(a, run, here, t1, pa_part_words(RB, D));

@@ -270,7 +270,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
 
     Zeros for rows outside all sequences, of a sequence with ``lengths[b] < 0`` and
     where nothing is in sight; positions whose block is none of the cache's are not
-    seen."""
+    seen. Scores, softmax statistics and sums in fp32; a probability times its value's
+    scale is rounded to fp16 once, relative to the row's largest such product: 2^-20 of
+    that keeps all of its bits, what is below 2^-31 of it may be dropped."""
     dev = inputs(q, tables, starts, lengths, *cache)
     code = _lib.act_dtype(q)
     args, shape = _cache(cache)
