@@ -48,6 +48,7 @@ constexpr float kPaLift = 7.f;     // and by which products of probability and s
 // what is smaller vanishes in fp16 either way, and the probability can be had back from
 // the product in fp32.
 constexpr float kPaLeast = -60.f;
+constexpr float kPaUnit = 16.f;    // of a row's mean until it is rounded to the result
 
 struct PagedAttnArgs {
   const uint16_t* q;
@@ -68,7 +69,7 @@ struct PagedAttnArgs {
   struct PaCut* cuts;  // [runs], behind the parts
 };
 
-// fp32 words of one part: RB x D sums, RB maxima, RB sums
+// fp32 words of one part: RB x D means, RB maxima, RB sums
 __host__ __device__ inline int64_t pa_part_words(int rb, int dim) { return (int64_t)rb * (dim + 2); }
 
 // ---------------------------------------------------------------------------
@@ -304,7 +305,7 @@ __device__ __forceinline__ PaRun pa_run(const PagedAttnArgs& a, int64_t total) {
   if (run >= active) return PaRun{run, 0, 0, size};
   return PaRun{run, run * size, min(total, (run + 1) * size), size};
 }
-// where the row block at tiles t0 .. t1 of `tiles` puts its sums: null if it is whole.
+// where the row block at tiles t0 .. t1 of `tiles` puts its means: null if it is whole.
 // A part: the run's first row block, begun before it, or its last, which goes on.
 __device__ __forceinline__ float* pa_part(const PagedAttnArgs& a, const PaRun& run, const PaPlace& p, int t1,
                                           int64_t words) {
@@ -316,6 +317,9 @@ __device__ __forceinline__ float* pa_part(const PagedAttnArgs& a, const PaRun& r
   }
   return a.parts + (run.run * 2 + (p.t0 == 0)) * words;
 }
+
+// 1 / l, and 0 for a row that has seen nothing
+__device__ __forceinline__ float pa_inverse(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
 
 // What a wave keeps of RT products of 16 rows.
 template <int D, int RT>
@@ -446,15 +450,18 @@ struct PaRows {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(v, p[rt][h], o[rt][dt]);
   }
-  // the row's whole sum in all of its lanes, sums in units of 1
+  // the row's whole sum in all of its lanes, and the mean of its values, in units of
+  // kPaUnit: finite also where values are near the largest that bf16 has, or rounded past
+  // it to a code (256 * 2^120), which their sums are not
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float unit = __builtin_amdgcn_exp2f(d[rt] - 127.f - kPaLift);
+      const float unit = __builtin_amdgcn_exp2f(d[rt] - (127.f + kPaLift)) * (1.f / kPaUnit);
       l[rt] += __shfl_xor(l[rt], 16, 64);
       l[rt] += __shfl_xor(l[rt], 32, 64);
+      const float inv = pa_inverse(l[rt]);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= unit;
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = o[rt][dt] * inv * unit;
     }
   }
   // result or part (of RB rows) of rows first .. of the row block
@@ -468,14 +475,13 @@ struct PaRows {
         const int r = qb * RB + local;
         const int token = r / a.group, g = r - token * a.group;
         if (token >= seq.n) continue;
-        const float inv = l[rt] > 0.f || l[rt] != l[rt] ? 1.f / l[rt] : 0.f;
         uint16_t* dst = a.out + ((int64_t)(seq.first + token) * (a.c.kv_heads * a.group) + kvh * a.group + g) * D +
                         4 * lg;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          *reinterpret_cast<uint2*>(dst + 16 * dt) =
-              make_uint2(pa_pack16<BF>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
-                         pa_pack16<BF>(o[rt][dt][2] * inv, o[rt][dt][3] * inv));
+        for (int dt = 0; dt < DT; ++dt) {
+          const float4v v = o[rt][dt] * kPaUnit;
+          *reinterpret_cast<uint2*>(dst + 16 * dt) = make_uint2(pa_pack16<BF>(v[0], v[1]), pa_pack16<BF>(v[2], v[3]));
+        }
       } else {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -669,20 +675,27 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
       i = in;
     }
 
-    // the four waves' sums, in the order (0 + 2) + (1 + 3)
+    // the four waves' means, each by its share of the sum, in the order (0 + 2) + (1 + 3)
+    w.finish();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
-      if (lg == 0) join_m[wave][rt * 16 + li] = w.m[rt];
-    w.finish();
+      if (lg == 0) {
+        join_m[wave][rt * 16 + li] = w.m[rt];
+        join_l[wave][rt * 16 + li] = w.l[rt];
+      }
     __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = rt * 16 + li;
       const float top = fmaxf(fmaxf(join_m[0][r], join_m[1][r]), fmaxf(join_m[2][r], join_m[3][r]));
-      const float al = __builtin_amdgcn_exp2f(w.m[rt] - (top == -__builtin_inff() ? 0.f : top));
+      const float base = top == -__builtin_inff() ? 0.f : top;
+      float sum[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] = join_l[k][r] * __builtin_amdgcn_exp2f(join_m[k][r] - base);
+      const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float al = w.l[rt] * __builtin_amdgcn_exp2f(w.m[rt] - base) * pa_inverse(all);
       w.m[rt] = top;
-      w.l[rt] *= al;
-      if (lg == 0) join_l[wave][r] = w.l[rt];
+      w.l[rt] = all;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         w.o[rt][dt] *= al;
@@ -705,8 +718,6 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
     if (wave == 0) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int r = rt * 16 + li;
-        w.l[rt] = (join_l[0][r] + join_l[1][r]) + (join_l[2][r] + join_l[3][r]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) w.o[rt][dt] += join[0][(rt * DT + dt) * 64 + lane];
       }
@@ -942,8 +953,9 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
 }
 
 // ---------------------------------------------------------------------------
-// The row block that begins in a run and goes on behind it: out = sum of its parts,
-// each weighted exp2(m_part - m) / l, in order. A wave a row, lane = dimensions.
+// The row block that begins in a run and goes on behind it: out = sum of its parts'
+// means, each weighted l_part exp2(m_part - m) / l, in order. A wave a row, lane =
+// dimensions.
 // ---------------------------------------------------------------------------
 template <int D, bool BF, int RB>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
@@ -983,11 +995,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
       for (int off = 32; off >= 1; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off, 64));
       mn = fmaxf(mn, m[i]);
       const float shift = mn == -__builtin_inff() ? 0.f : mn;
-      const float al = __builtin_amdgcn_exp2f(m[i] - shift);
-      w[i] = __builtin_amdgcn_exp2f(pm - shift);
+      w[i] = lane < here ? pl * __builtin_amdgcn_exp2f(pm - shift) : 0.f;
+      const float before = l[i] * __builtin_amdgcn_exp2f(m[i] - shift);
       m[i] = mn;
-      o[i] *= al;
-      l[i] = l[i] * al + wave_sum_dpp(lane < here ? w[i] * pl : 0.f);
+      l[i] = before + wave_sum_dpp(w[i]);
+      const float inv = pa_inverse(l[i]);
+      o[i] *= before * inv;
+      w[i] *= inv;
     }
     for (int s = 0; s < here; s += U) {
       floatE t[U][ROWS];
@@ -1011,10 +1025,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     const int r = cut.qb * RB + first + i;
     const int token = r / a.group, g = r - token * a.group;
     if (token >= cut.n) return;
-    const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
     uint16_t h[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = to16(o[i][e] * inv, BF);
+    for (int e = 0; e < E; ++e) h[e] = to16(o[i][e] * kPaUnit, BF);
     uint16_t* dst = a.out + ((int64_t)(cut.first + token) * a.c.kv_heads * a.group + cut.kvh * a.group + g) * D +
                     lane * E;
     __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);
