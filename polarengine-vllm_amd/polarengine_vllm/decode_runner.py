@@ -39,7 +39,7 @@ from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
 from polarengine_vllm.kernels import paged_cache, tree_decode
-from polarengine_vllm.kernels.logprobs import TokenLogprobs, token_logprobs
+from polarengine_vllm.kernels.logprobs import TokenLogprobs, check_top, token_logprobs
 from polarengine_vllm.linear_method import PolarQuantLinearMethod
 
 
@@ -300,6 +300,7 @@ class DecodeRunner:
         """``paged_step`` with the log probability of each row's next token (logprob 0 and
         rank -1 in a sequence's last row of the step, of no meaning in rows that found no
         room), entropy and ``top`` likeliest tokens of every row."""
+        check_top(top, self.cfg.vocab)
         plan, attend = self._paged(tokens, counts, pool, window, sinks)
         rows = tokens.shape[0]
         follow = torch.cat([tokens[1:], tokens[:1]])
@@ -311,13 +312,20 @@ class DecodeRunner:
 
     def _paged(self, tokens: torch.Tensor, counts: torch.Tensor, pool: paged_cache.PagedPool,
                window: Optional[int], sinks: int):
-        """A paged step's plan and its attention, as a function of (layer, qkv rows)."""
+        """A paged step's plan and its attention, as a function of (layer, qkv rows).
+        What a step refuses is refused here, before the plan changes the pool."""
         c = self.cfg
+        _lib.require_device(self.embed, tokens, counts, pool.tables)
+        paged_cache.check_sight(window, sinks)
         if tokens.dim() != 1 or tokens.dtype != torch.int64 or not tokens.numel():
             raise ValueError(f"tokens must be int64 [rows], at least one, got {tokens.dtype} of "
                              f"{list(tokens.shape)}")
         if len(pool.caches) != c.layers:
             raise ValueError(f"the pool has {len(pool.caches)} layers, the model {c.layers}")
+        for cache in pool.caches[:1]:
+            if (cache.k.shape[1], cache.k.shape[3]) != (c.kv_heads, c.head_dim):
+                raise ValueError(f"the pool has {cache.k.shape[1]} KV heads of {cache.k.shape[3]}, the model "
+                                 f"{c.kv_heads} of {c.head_dim}")
         if pool.tables.shape[1] * pool.block_size > self.max_len:
             raise ValueError(f"the pool's sequences pass the {self.max_len} positions of the model")
         plan = pool.plan(counts, tokens.shape[0])

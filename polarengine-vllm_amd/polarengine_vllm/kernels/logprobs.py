@@ -26,6 +26,12 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor    # int64 [rows, top]
 
 
+def check_top(top: int, vocab: int) -> None:
+    """Refuses a number of alternatives that ``token_logprobs`` has none for."""
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Of logits [rows, vocab] (fp32, fp16 or bf16; -inf where a token is ruled out) and
     tokens int64 [rows] (outside the vocabulary: none, with logprob 0 and rank -1).
@@ -39,8 +45,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if logits.dim() != 2 or not logits.shape[1]:
         raise ValueError(f"logits must be [rows, vocab], got {list(logits.shape)}")
     rows, vocab = logits.shape
-    if not 0 <= top <= min(MAX_TOP, vocab):
-        raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
+    check_top(top, vocab)
     tokens = int64(tokens, (rows,), "tokens")
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()

@@ -223,6 +223,14 @@ def release_blocks(tables: torch.Tensor, keep: torch.Tensor, free: torch.Tensor,
     written(tables, free, free_count)
 
 
+def check_sight(window: Optional[int], sinks: int) -> None:
+    """Refuses what ``paged_attention`` takes for no window and first positions."""
+    if window is not None and window < 1:
+        raise ValueError(f"a window holds at least one position, got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must be at least 0, got {sinks}")
+
+
 def _rows16(x: torch.Tensor) -> torch.Tensor:
     """Rows of heads that the kernels read 16 bytes at a time."""
     st = x.stride()
@@ -281,10 +289,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
                          f"{list(q.shape)}")
     if lengths.dim() != 1:
         raise ValueError(f"lengths must be [batch], got {list(lengths.shape)}")
-    if window is not None and window < 1:
-        raise ValueError(f"a window holds at least one position, got {window}")
-    if sinks < 0:
-        raise ValueError(f"sinks must be at least 0, got {sinks}")
+    check_sight(window, sinks)
     (rows, heads, dim), batch = q.shape, lengths.shape[0]
     tables = _tables(tables, batch, False)
     starts, lengths = int64(starts, (batch + 1,), "starts"), int64(lengths, (batch,), "lengths")
