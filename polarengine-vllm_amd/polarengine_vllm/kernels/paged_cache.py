@@ -97,9 +97,10 @@ class PagedPool:
     def keep(self, lengths: torch.Tensor) -> None:
         """Each sequence's first ``lengths[b]`` positions stay (int64 [batch]), as many as
         it has, and its other blocks are free again: 0 begins a new sequence, below 0
-        leaves an empty slot."""
+        leaves an empty slot. An empty slot stays one unless it is given 0."""
         release_blocks(self.tables, lengths.clamp(min=0), self.free, self.free_count, self.block_size)
-        torch.minimum(lengths, self.lengths.clamp(min=0), out=self.lengths)
+        # of an empty slot, -1, the smaller of both but for a 0
+        self.lengths.copy_(torch.minimum(lengths, self.lengths).masked_fill_(lengths == 0, 0))
 
 
 def _block_size(t: int) -> None:
