@@ -32,7 +32,8 @@ import torch
 from polarengine_vllm import _lib
 from polarengine_vllm.kernels._calls import call, inputs, int64, written
 
-F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+# None in a torch that is too old for them: importing the package does not need them
+F8, E8 = (getattr(torch, name, None) for name in ("float8_e4m3fn", "float8_e8m0fnu"))
 BLOCK_SIZES = (16, 32, 64, 128)
 
 
@@ -57,6 +58,8 @@ class StepPlan(NamedTuple):
 
 def new_cache(blocks: int, kv_heads: int, block_size: int, head_dim: int, device) -> PagedCache:
     """A layer's cache for ``blocks`` blocks."""
+    if F8 is None or E8 is None:
+        raise RuntimeError("the paged cache needs a torch with float8_e4m3fn and float8_e8m0fnu")
     _block_size(block_size)
     if blocks < 1 or kv_heads < 1 or head_dim not in (64, 128, 256):
         raise ValueError(f"a cache has at least one block and KV head of 64, 128 or 256 dimensions, "
