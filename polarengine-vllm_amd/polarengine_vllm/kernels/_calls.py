@@ -11,6 +11,15 @@ from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
 
+try:
+    increment_version(())  # several at once, 0.9 against 2.2 us for four
+    _count = increment_version
+except TypeError:  # an older torch takes one tensor
+
+    def _count(tensors) -> None:
+        for t in tensors:
+            increment_version(t)
+
 
 def call(name: str, dev: torch.device, *args) -> None:
     """One call into the library on the device's current stream, the device made the
@@ -59,4 +68,4 @@ def written(*tensors: torch.Tensor) -> None:
     """Counts writes through raw pointers (inference tensors keep no count)."""
     if any(t.is_inference() for t in tensors):
         tensors = tuple(t for t in tensors if not t.is_inference())
-    increment_version(tensors)
+    _count(tensors)

@@ -1,5 +1,5 @@
-"""The package without the 8-bit types: they came to torch later than what the quantized
-linears need, whose import must not ask for them."""
+"""The package with a torch older than this one: without the 8-bit types, which only the
+paged cache needs, and with one tensor at a time for increment_version."""
 
 import os
 import subprocess
@@ -25,4 +25,27 @@ else:
 def test_import_without_the_scales_type():
     env = dict(os.environ, PYTHONPATH=os.path.join(ROOT, "polarengine-vllm_amd"))
     got = subprocess.run([sys.executable, "-c", CODE], env=env, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0, got.stderr[-2000:]
+
+OLD = """
+import torch, torch.autograd.graph as graph
+real = graph.increment_version
+def one(tensor):
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError("a tensor")
+    real(tensor)
+graph.increment_version = one
+from polarengine_vllm.kernels._calls import written
+x, y = torch.zeros(2), torch.zeros(2)
+with torch.inference_mode():
+    z = torch.zeros(2)
+before = x._version, y._version
+written(x, z, y)
+assert (x._version, y._version) == (before[0] + 1, before[1] + 1)
+"""
+
+
+def test_writes_count_where_torch_takes_one_tensor_at_a_time():
+    env = dict(os.environ, PYTHONPATH=os.path.join(ROOT, "polarengine-vllm_amd"))
+    got = subprocess.run([sys.executable, "-c", OLD], env=env, capture_output=True, text=True, timeout=300)
     assert got.returncode == 0, got.stderr[-2000:]
