@@ -39,6 +39,7 @@ from torch.autograd.graph import increment_version
 
 from polarengine_vllm import _lib
 from polarengine_vllm.kernels import paged_cache, tree_decode
+from polarengine_vllm.kernels._calls import int64
 from polarengine_vllm.kernels.logprobs import TokenLogprobs, check_top, token_logprobs
 from polarengine_vllm.linear_method import PolarQuantLinearMethod
 
@@ -296,19 +297,29 @@ class DecodeRunner:
         return self._layers(tokens.clamp(0, self.cfg.vocab - 1), attend, (plan.starts[1:] - 1).clamp(min=0))
 
     def score(self, tokens: torch.Tensor, counts: torch.Tensor, pool: paged_cache.PagedPool, top: int = 0,
-              window: Optional[int] = None, sinks: int = 0) -> TokenLogprobs:
-        """``paged_step`` with the log probability of each row's next token (logprob 0 and
-        rank -1 in a sequence's last row of the step, of no meaning in rows that found no
-        room), entropy and ``top`` likeliest tokens of every row."""
+              window: Optional[int] = None, sinks: int = 0,
+              follow: Optional[torch.Tensor] = None) -> TokenLogprobs:
+        """``paged_step`` with the log probability of each row's next token, entropy and
+        ``top`` likeliest tokens of every row (of no meaning in rows that found no room).
+        What follows a sequence's last row of the step is ``follow[b]`` (int64 [batch]), as
+        the next chunk of a prompt begins; without it, or outside the vocabulary, that row
+        has logprob 0 and rank -1."""
         check_top(top, self.cfg.vocab)
+        if follow is not None:
+            _lib.require_device(self.embed, follow)
+            follow = int64(follow, (pool.lengths.shape[0],), "follow")
         plan, attend = self._paged(tokens, counts, pool, window, sinks)
         rows = tokens.shape[0]
-        follow = torch.cat([tokens[1:], tokens[:1]])
+        after = torch.cat([tokens[1:], tokens[:1]])
         # rows before another sequence's first, and behind the last sequence
         last = torch.zeros(rows + 1, dtype=torch.bool, device=self.dev).index_fill_(0, plan.starts, True)[1:]
         last |= torch.arange(rows, device=self.dev) >= plan.starts[-1]
+        after = torch.where(last, -1, after)
+        if follow is not None:  # sequences without rows write behind the last row
+            ends = torch.where(plan.starts[1:] > plan.starts[:-1], plan.starts[1:] - 1, rows)
+            after = torch.cat([after, after[:1]]).scatter_(0, ends, follow)[:rows]
         logits = self._layers(tokens.clamp(0, self.cfg.vocab - 1), attend)
-        return token_logprobs(logits, torch.where(last, -1, follow), top)
+        return token_logprobs(logits, after, top)
 
     def _paged(self, tokens: torch.Tensor, counts: torch.Tensor, pool: paged_cache.PagedPool,
                window: Optional[int], sinks: int):
