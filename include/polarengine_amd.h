@@ -570,8 +570,9 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  *       whose block is none of the cache's are not seen. Scores, softmax statistics
  *       and sums in fp32; a probability times its value's scale is rounded to fp16 once,
  *       in units in which the row's largest such product is 2^6 to 2^15 (what is below
- *       2^-31 of it may count as 0 in the sum of values, not in the sum that divides). Keys,
- *       values and scales that a row does not see have no effect on it.
+ *       2^-31 of it may count as 0 in the sum of values; in the sum that divides, only
+ *       what is below 2^-27 of the largest probability). Keys, values and scales that a
+ *       row does not see have no effect on it.
  *   pe_token_logprobs: of logits [rows, vocab] (PE_DTYPE_F32 too; row stride ld) and
  *       tokens int64 [rows]: logprob float32 = x[t] - log sum exp x, rank int64 = how
  *       many tokens come before t (larger logit, or as large and of a lower number),
