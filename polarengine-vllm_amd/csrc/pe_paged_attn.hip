@@ -53,7 +53,7 @@ constexpr float kPaLeast = -60.f;
 // probability): errors that numerator and denominator have in common cancel (relative error
 // of fp16 results with a window of 4000, heads of 256, 2.4e-4, of unrounded sums 2.9e-4).
 constexpr float kPaNear = -4.f;
-constexpr float kPaUnit = 16.f;    // of a row's mean until it is rounded to the result
+constexpr int kPaUnit = 4;         // a row's mean is in units of 2^4 until it is rounded to the result
 
 struct PagedAttnArgs {
   const uint16_t* q;
@@ -475,17 +475,19 @@ struct PaRows {
     for (int rt = 0; rt < RT; ++rt) o[rt][dt] = pa_mfma<false>(v, p[rt][h], o[rt][dt]);
   }
   // the row's whole sum in all of its lanes, and the mean of its values, in units of
-  // kPaUnit: finite also where values are near the largest that bf16 has, or rounded past
+  // 2^kPaUnit: finite also where values are near the largest that bf16 has, or rounded past
   // it to a code (256 * 2^120), which their sums are not
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float unit = __builtin_amdgcn_exp2f(d[rt] - (127.f + kPaLift)) * (1.f / kPaUnit);
+      const int unit = (int)d[rt] - 127 - (int)kPaLift - kPaUnit;
       l[rt] += __shfl_xor(l[rt], 16, 64);
       l[rt] += __shfl_xor(l[rt], 32, 64);
       const float inv = pa_inverse(l[rt]);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = o[rt][dt] * inv * unit;
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[rt][dt][e] = __builtin_ldexpf(o[rt][dt][e] * inv, unit);
     }
   }
   // result or part (of RB rows) of rows first .. of the row block
@@ -503,7 +505,7 @@ struct PaRows {
                         4 * lg;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const float4v v = o[rt][dt] * kPaUnit;
+          const float4v v = o[rt][dt] * (float)(1 << kPaUnit);
           *reinterpret_cast<uint2*>(dst + 16 * dt) = make_uint2(pa_pack16<BF>(v[0], v[1]), pa_pack16<BF>(v[2], v[3]));
         }
       } else {
@@ -1051,7 +1053,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     if (token >= cut.n) return;
     uint16_t h[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = to16(o[i][e] * kPaUnit, BF);
+    for (int e = 0; e < E; ++e) h[e] = to16(o[i][e] * (float)(1 << kPaUnit), BF);
     uint16_t* dst = a.out + ((int64_t)(cut.first + token) * a.c.kv_heads * a.group + cut.kvh * a.group + g) * D +
                     lane * E;
     __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E), h, 2 * E);

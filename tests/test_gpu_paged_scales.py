@@ -217,3 +217,15 @@ def test_long_sequences(d, t, new, length):
     _bytes(case[1].v_scale).copy_(torch.randint(60, 160, case[1].v_scale.shape, generator=torch.Generator().manual_seed(1)))
     _compare(case)
     _compare(case, length // 3, 5)
+
+
+@pytest.mark.parametrize("new,group,d", FORMS)
+def test_smallest_scales(new, group, d):
+    """Scales that no write gives, down to the type's smallest."""
+    say(f"smallest scales {new} x {group} x {d}")
+    for length in (70, 900):
+        case = _case(d * 2 + new, 1, 2, group, d, 16, torch.bfloat16, [new], [length])
+        scale = _bytes(case[1].v_scale)
+        for low, high in ((1, 2), (1, 27), (9, 14)):
+            scale.copy_(torch.randint(low, high, scale.shape, generator=torch.Generator().manual_seed(low)))
+            _compare(case)
