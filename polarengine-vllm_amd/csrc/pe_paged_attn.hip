@@ -917,6 +917,7 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
       if (none) return;
       const bool full = p + 63 <= p_low && !__any(!(sc >> 16)) &&
                         (!a.window || p > p_high - a.window || p + 64 <= a.sinks);
+      const uint32_t nan_low = some_nan[0], nan_high = some_nan[1];  // under way until they are needed
       const u32x4v* kf = from + lane;
       const u32x4v* vf = kf + KF * 64;
       // operands A ahead of their products; the fences keep the compiler from bringing
@@ -964,8 +965,10 @@ __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const
         }
         __builtin_amdgcn_s_setprio(0);
       }
-      if (__builtin_expect(pa_uniform(some_nan[0]), 0)) w.template nan_values<0, DT / 2>(nan_map, seen, lg);
-      if (__builtin_expect(pa_uniform(some_nan[1]), 0)) w.template nan_values<DT / 2, DT>(nan_map, seen, lg);
+      if (__builtin_expect(pa_uniform(nan_low | nan_high), 0)) {
+        if (pa_uniform(nan_low)) w.template nan_values<0, DT / 2>(nan_map, seen, lg);
+        if (pa_uniform(nan_high)) w.template nan_values<DT / 2, DT>(nan_map, seen, lg);
+      }
     };
     while (i < t1) {
       step(buf0, nan0, some0, buf1, nan1, some1);
