@@ -563,8 +563,8 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  *       call may go to a block.
  *   pe_paged_attention: q [rows, heads, head_dim] (row stride q_r) of sequences whose
  *       rows begin at starts (int64 [batch + 1]), the last of a sequence at position
- *       lengths[b] - 1. out [rows, heads, head_dim] = softmax(scale q K^T) V over the
- *       positions j <= p of a row's position p with j > p - window or j < sinks
+ *       lengths[b] - 1. out [rows, heads, head_dim] = softmax(scale q K^T) V, scale >= 0,
+ *       over the positions j <= p of a row's position p with j > p - window or j < sinks
  *       (window 0: all). Rows of a sequence with lengths[b] < 0, before position 0,
  *       without a block in sight, and outside all sequences get zeros; positions
  *       whose block is none of the cache's are not seen. Scores, softmax statistics
@@ -579,8 +579,9 @@ int pe_keep_accepted(void* cache, int64_t layers, int64_t batch, int heads, int6
  *       entropy float32 of softmax(x), and the `top` likeliest tokens in order
  *       (top_logprobs float32, top_tokens int64, [rows, top], ties by number).
  *       A token outside the vocabulary: logprob 0, rank -1; a NaN logit counts as -inf,
- *       in the given token, ranks and alternatives alike. top <= 64, vocab >= top, rows
- *       < 2^24.
+ *       in the given token, ranks and alternatives alike. Rows are read in aligned words
+ *       of 16 bytes: up to 14 bytes before a row and behind it are read and not used.
+ *       top <= 64, vocab >= top, rows < 2^24.
  */
 int pe_plan_step(const int64_t* lengths, const int64_t* counts, int32_t* tables, int64_t t_b,
                  int64_t batch, int64_t width, const int32_t* free_blocks, int64_t free_cap,

@@ -6,7 +6,6 @@
 namespace pe {
 
 constexpr int kMinExp = -100;      // the smallest exponent of a block's scale
-constexpr float kF8Max = 448.f;    // the largest e4m3 value
 constexpr int64_t kPagedMaxBatch = 4096;
 constexpr int64_t kPagedMaxRows = (int64_t)1 << 24;
 constexpr int64_t kPagedMaxPositions = (int64_t)1 << 30;  // of a sequence

@@ -50,9 +50,10 @@ def inputs(*tensors: Optional[torch.Tensor]) -> torch.device:
                 _lib.require_device(*tensors)
             if (grad and t.requires_grad) or (
                     dual and not t.is_inference() and fwAD.unpack_dual(t).tangent is not None):
-                raise RuntimeError("this kernel has no backward pass: call it under "
+                raise RuntimeError("the kernels of drafted tokens, the paged cache and log "
+                                   "probabilities have no backward pass: call them under "
                                    "torch.no_grad(), without forward-mode tangents, or detach "
-                                   "its inputs")
+                                   "their inputs")
     return tensors[0].device
 
 

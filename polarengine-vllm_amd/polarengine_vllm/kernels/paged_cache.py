@@ -278,7 +278,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
     over the cache: the rows of sequence b begin at ``starts[b]`` (int64 [batch + 1]),
     its last one is at position ``lengths[b] - 1`` (int64 [batch]). A row sees the
     positions up to its own; with a ``window`` the last ``window`` of them and the
-    first ``sinks`` of the sequence. scale: 1 / sqrt(head_dim) if not given.
+    first ``sinks`` of the sequence. scale: at least 0, 1 / sqrt(head_dim) if not given.
 
     Zeros for rows outside all sequences, of a sequence with ``lengths[b] < 0`` and
     where nothing is in sight; positions whose block is none of the cache's are not
