@@ -229,3 +229,16 @@ def test_smallest_scales(new, group, d):
         for low, high in ((1, 2), (1, 27), (9, 14)):
             scale.copy_(torch.randint(low, high, scale.shape, generator=torch.Generator().manual_seed(low)))
             _compare(case)
+
+
+@pytest.mark.parametrize("d,t,new,group,length", [(64, 128, 1, 4, 40000), (128, 64, 2, 8, 20000), (256, 128, 1, 2, 17000),
+                                                  (64, 64, 40, 8, 9000), (128, 128, 50, 8, 6000)])
+def test_parts_past_a_wave(d, t, new, group, length):
+    """One KV head, so that a row block is divided into more parts than a wave has lanes."""
+    say(f"parts past a wave d={d} new={new} length={length}")
+    case = _case(length, 1, 1, group, d, t, torch.bfloat16, [new], [length])
+    _compare(case)
+    scale = _bytes(case[1].v_scale)
+    scale.copy_(torch.randint(60, 160, scale.shape, generator=torch.Generator().manual_seed(2)))
+    _compare(case)
+    _compare(case, length - 700, 9)
