@@ -11,10 +11,10 @@
 // likeliest tokens so far lie sorted across its lanes; a chunk is looked through only
 // if one of its values passes the last of them, which is rare behind the first chunks.
 //
-// 2048 rows of 151,936 fp32: 230 us, 5.4 TB/s (bf16: 159 us, 3.9 TB/s, about twelve
-// vector instructions a value, one of them for signalling NaN: 227 and 155 without); one
-// row with 20 alternatives 8 us and 6 us for the join, 7.4 us without alternatives; 48
-// rows of 100,003 bf16 with 5: 14 + 5 us, of which the read would be 2.
+// 2048 rows of 151,936 fp32: 227 us, 5.5 TB/s (bf16: 151 us, 4.1 TB/s, about twelve
+// vector instructions a value, one of them for signalling NaN, 2% of either); one row
+// with 20 alternatives 8 us and 6 us for the join, 7.4 us without alternatives; 48 rows of
+// 100,003 bf16 with 5: 15 + 5 us, of which the read would be 2.
 
 #include "pe_internal.h"
 

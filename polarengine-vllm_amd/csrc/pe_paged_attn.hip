@@ -31,11 +31,12 @@
 // parts of a row block that a cut divides.
 //
 // Bound by HBM where a KV head has few rows: 32 sequences of up to 16,000 positions, 4
-// rows, 134 + 5 us, 5.3 TB/s in the first launch; 16 windows of 4000 with heads of 256,
-// one wave a SIMD, 112 + 5 us, 4.7 TB/s. 1024 tokens behind 30,000 (4096 rows): 660 us
-// for both launches, 0.78 PFLOP/s, the matrix cores busy about 35% of the time. One
-// sequence of 778, one row: 15 us in one launch, a chain of loads (lengths, tables, keys
-// and values of four tiles).
+// rows, 135 + 5 us, 5.2 TB/s in the first launch; 16 windows of 4000 with heads of 256,
+// one wave a SIMD, 111 + 5 us, 4.7 TB/s. 1024 tokens behind 30,000 (4096 rows): 657 us
+// for both launches, 0.78 PFLOP/s, the matrix cores busy about a third of the time; heads
+// of 64 426 us (operations: 213), 512 tokens with heads of 256 930 us (423). One sequence
+// of 778, one row: 15 us in one launch, a chain of loads (lengths, tables, keys and values
+// of four tiles).
 
 #include "pe_paged.h"
 
@@ -760,14 +761,17 @@ __global__ __launch_bounds__(256, RT == 1 && D != 256 ? 2 : 1) void paged_attn_k
 // and put them to LDS in the order in which lanes read them (64 lanes x 16 bytes an
 // operand, from the addresses that the other form loads), so that a code is converted
 // once for all rows: the conversions, one instruction for two codes, would otherwise be
-// a third of the vector instructions beside the products (749 us for 1024 tokens behind
-// 30,000, this way 676). Two buffers: while a step is
+// a third of the vector instructions beside the products (1024 tokens behind 30,000 were
+// 749 us that way and 676 this way, before later changes). Two buffers: while a step is
 // worked on, the next one's operands are written and the loads of the one behind it are
-// under way; one barrier a step.
+// under way; one barrier a step. The waves that bring values look for NaN in them, in
+// steps that some row of the block does not see whole, for all waves: looked for behind
+// the barrier by every wave, with the products of the rare path in its code, the steps
+// had no registers left (1024 tokens behind 30,000: 992 us, with spills).
 // ---------------------------------------------------------------------------
 // workgroups a CU: as many as the registers hold (heads of 64, microseconds by two and
-// three: 1024 tokens behind 30,000 479 409, 16 x 64 behind 4000 89 85, 2048 tokens of a
-// prompt 82 90)
+// three: 1024 tokens behind 30,000 507 426, 16 x 64 behind 4000 91 85, 2048 tokens of a
+// prompt 87 78)
 constexpr int pa_chunk_wgs(int dim) { return dim == 256 ? 1 : dim == 64 ? 3 : 2; }
 template <int D, bool BF, int RT>
 __global__ __launch_bounds__(256, pa_chunk_wgs(D)) void paged_chunk_kernel(const PagedAttnArgs a) {
@@ -1066,31 +1070,35 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 // The form, by the rows of a KV head that a sequence has in the mean: 16 rows a workgroup
 // up to 32 (two row blocks cost no more than one of 32), 32 rows up to 64 (not for heads
 // of 256, where they do not fit the registers), 128 beyond. That form's steps are dearer
-// where there are few of them: up to 128 rows it needs 64 (sequence, KV head) pairs.
+// where there are few of them: up to 128 rows it needs 64 (sequence, KV head) pairs. The
+// mean is over what the call has on the host, empty slots and padding among it; a step of
+// long chunks beside single tokens has one form for both.
 // Microseconds by 16, 32 and 128 rows, from a graph, one sequence of 8000 and of 30,000
-// and 16 of 4000 positions, 8 KV heads (128 rows of heads of 64 by two workgroups a CU):
+// and 16 of 4000 positions, 8 KV heads, equal counts:
 //   head    rows      1 x 8000      1 x 30,000       16 x 4000
-//    64       32    23  24  30      25   33   44     29   32   50
-//             64    21  22  35      30   35   48     43   40   56
-//            128    23  24  39      42   48   57     74   77   62
-//            256    29  29  38      64   73   63    121  133   98
-//   128       32    26  28  37      34   42   58     42   43   73
-//             64    26  27  43      46   47   61     69   58   81
-//            128    31  32  47      76   67   73    137  113   89
-//            256    43  39  45     120  104   84    242  196  134
-//   256       32    29   -  73      60    -  131     78    -  207
-//             64    36   -  76      89    -  126    153    -  213
-//            128    48   -  83     154    -  144    271    -  231
-//            256    73   -  92     223    -  214    495    -  392
-// Workgroups a CU: two of 16 rows (one with heads of 256: 16 rows, 16 x 4000, 59 us, two
-// 72), one of 32 (64 rows, 16 x 4000, 58 us, two 76); of 128 as above.
+//    64       32    23  24  29      24   32   46      28   32   42
+//             64    21  22  34      29   35   50      42   41   47
+//            128    22  24  45      41   49   67      72   78   56
+//            256    28  29  43      62   74   63     118  135   85
+//   128       32    25  27  49      33   41   66      43   42   68
+//             64    26  27  60      44   46   74      69   54   77
+//            128    32  31  75      73   64   91     135  106   85
+//            256    43  38  58     120   98   92     236  182  122
+//   256       32    27   -  52      59    -   97      76    -  160
+//             64    35   -  64      87    -  107     153    -  165
+//            128    48   -  75     154    -  121     276    -  175
+//            256    73   -  77     224    -  166     501    -  302
+// Not the fewest by this rule: 256 rows behind 8000 (heads of 64 43 for 28, of 128 58 for
+// 38) and 128 rows of heads of 256 behind 30,000 (154 for 121).
+// Workgroups a CU: two of 16 rows (one with heads of 256: 16 rows, 16 x 4000, 58 us, two
+// 70), one of 32 (64 rows, 16 x 4000, 56 us, two 72); of 128 as above.
 //
 // Row blocks of up to four tiles (1024 positions that the tables have room for) are not
 // divided: no second launch. Microseconds divided and whole, heads of 128, one row block
-// a sequence, graph and eager: one sequence of 700 14.5 14.1 and 17.3 13.5, of 1400 14.0
-// 19.1 and 17.2 18.0; 16 of 959 16.9 15.6 and 17.2 14.5; 64 of 959 28.7 26.7 and 27.3
-// 25.4. Heads of 256 lose more by a whole block's steps (one sequence of 700: 18.4 21.5
-// eager), 128 rows by their fewer workgroups (700 positions: 34.3 41.2).
+// a sequence, graph and eager: one sequence of 700 14.1 13.7 and 17.6 13.7, of 1400 13.7
+// 18.8 and 17.4 17.5; 16 of 959 17.3 16.7 and 17.4 15.8; 64 of 959 29.6 27.1 and 28.0
+// 25.7. Heads of 256 lose more by a whole block's steps (one sequence of 700: 18.0 20.5
+// eager), 128 rows by their fewer workgroups (256 rows of 64 tokens behind 700: 30.1 36.3).
 constexpr int kPaWhole = 4;
 struct PaPlan {
   int rb;      // rows of a row block
