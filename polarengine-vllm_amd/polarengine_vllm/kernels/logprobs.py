@@ -6,6 +6,7 @@ There is no backward pass: inputs that autograd follows are refused.
 
 from __future__ import annotations
 
+from operator import index
 from typing import NamedTuple
 
 import torch
@@ -28,7 +29,7 @@ class TokenLogprobs(NamedTuple):
 
 def check_top(top: int, vocab: int) -> None:
     """Refuses a number of alternatives that ``token_logprobs`` has none for."""
-    if not 0 <= top <= min(MAX_TOP, vocab):
+    if not 0 <= index(top) <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
 
 

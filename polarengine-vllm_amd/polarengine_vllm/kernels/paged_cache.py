@@ -25,6 +25,7 @@ There is no backward pass: inputs that autograd follows are refused.
 from __future__ import annotations
 
 import math
+from operator import index
 from typing import NamedTuple, Optional
 
 import torch
@@ -229,9 +230,9 @@ def release_blocks(tables: torch.Tensor, keep: torch.Tensor, free: torch.Tensor,
 
 def check_sight(window: Optional[int], sinks: int) -> None:
     """Refuses what ``paged_attention`` takes for no window and first positions."""
-    if window is not None and window < 1:
+    if window is not None and index(window) < 1:
         raise ValueError(f"a window holds at least one position, got {window}")
-    if sinks < 0:
+    if index(sinks) < 0:
         raise ValueError(f"sinks must be at least 0, got {sinks}")
 
 

@@ -54,3 +54,21 @@ def test_a_refused_step_leaves_the_pool():
                 assert torch.equal(a, b), name
     run.paged_step(tokens, counts, pool)  # and the pool goes on
     assert pool.lengths.tolist() == [8, 10]
+
+
+def test_numbers_that_are_not_whole_leave_the_pool():
+    run = _runner(1, 64)
+    pool = run.paged_pool(blocks=8, batch=2, block_size=16)
+    pool.keep(_i64([0, 0]).to(DEV))
+    tokens, counts = _tokens((9,), 1), _i64([4, 5]).to(DEV)
+    run.paged_step(tokens, counts, pool)
+    before = _state(pool)
+    for name, call in {"window": lambda: run.paged_step(tokens, counts, pool, window=8.0),
+                       "sinks": lambda: run.paged_step(tokens, counts, pool, window=8, sinks=1.0),
+                       "top": lambda: run.score(tokens, counts, pool, top=3.0)}.items():
+        say(f"refused: {name} as a float")
+        with pytest.raises(TypeError):
+            call()
+        torch.cuda.synchronize()
+        for a, b in zip(_state(pool), before):
+            assert torch.equal(a, b), name
